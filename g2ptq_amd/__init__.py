@@ -13,6 +13,8 @@ from .gptaq_utils import GPTAQ
 from .gptq_guided_utils import GPTQGuided
 from .gptq_utils import GPTQ
 from .graph_utils import clear_graph_cache, run_graph, validate_tensors
+from .int8_utils import Int8Linear, int8_matmul, quantize_tokens
+from .kv_cache_utils import PagedKVCache, paged_attention
 from .quant_utils import WeightQuantizer
 from .shared import SharedInputHessian
 
@@ -20,6 +22,7 @@ __all__ = [
     "GPTQ", "GPTAQ", "G2PTQ", "GPTQGuided", "WeightQuantizer", "ChunkSpec", "build_chunk_specs",
     "make_group_quantizers", "merge_group_quantizers", "fake_quantize_grouped", "run_graph",
     "validate_tensors", "clear_graph_cache", "SharedInputHessian",
+    "Int8Linear", "int8_matmul", "quantize_tokens", "PagedKVCache", "paged_attention",
 ]
 
 

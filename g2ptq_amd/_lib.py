@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libg2ptq_hi
 FLAG_BAD_SCALE = 1
 FLAG_NAN_OUTPUT = 2
 FLAG_GROUP_SCALE = 4
+FLAG_BAD_INDEX = 8
 VARIANT_GPTQ, VARIANT_GPTAQ, VARIANT_G2PTQ = 0, 1, 2
 
 _p = ctypes.c_void_p
@@ -21,6 +22,14 @@ _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 _szp = ctypes.POINTER(ctypes.c_size_t)
+
+
+class KvCacheStruct(ctypes.Structure):
+    """``g2ptq_kv_cache`` of include/g2ptq_hip.h."""
+    _fields_ = [("k_codes", _p), ("v_codes", _p), ("k_scale", _p), ("v_scale", _p),
+                ("k_zero", _p), ("v_zero", _p), ("flags", _p), ("pages", _i64), ("heads", _i64),
+                ("page", _i64), ("dim", _i64), ("bits", _i32), ("sym", _i32)]
+
 
 # name -> argtypes (all functions return int status except the two string ones)
 SIGNATURES = {
@@ -78,6 +87,20 @@ SIGNATURES = {
     "g2ptq_running_mean_update": [_p, _p, _p, _i32, _i64, _f32, _f32, _i32],
     "g2ptq_gemm_f32": [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64,
                        _p, _i64, _i64, _f32, _f32],
+    "g2ptq_quantize_tokens": [_p, _p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _p],
+    "g2ptq_int8_gemm_workspace": [_i64, _i64, _i64, _szp],
+    "g2ptq_int8_gemm": [_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i32, _i64,
+                        _p, _sz],
+    "g2ptq_int8_linear_workspace": [_i64, _i64, _i64, _szp],
+    "g2ptq_int8_linear": [_p, _p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _p, _p, _i64, _p, _i64,
+                          _p, _sz],
+    "g2ptq_kv_write": [_p, ctypes.POINTER(KvCacheStruct), _p, _i64, _i64, _p, _i64, _i64, _i32,
+                       _i64, _p],
+    "g2ptq_kv_read": [_p, ctypes.POINTER(KvCacheStruct), _p, _i64, _i64, _i64, _p, _i64, _p, _p,
+                      _i32],
+    "g2ptq_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _szp],
+    "g2ptq_paged_attention": [_p, ctypes.POINTER(KvCacheStruct), _p, _i64, _i64, _i32, _i64, _i64,
+                              _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _f32, _p, _p, _sz],
 }
 STRING_FUNCS = ("g2ptq_status_string", "g2ptq_last_error")
 
@@ -207,6 +230,29 @@ def workspace(nbytes, device):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _WORKSPACES[key] = buf
     return buf
+
+
+def scratch(nbytes, device):
+    """A buffer for one call on the current stream: ``workspace``, or while a
+    graph is captured a buffer of the graph's own (a cached one may be replaced
+    by a larger one while the graph still uses it)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return workspace(nbytes, device)
+
+
+def require_current(t, what):
+    """Kernels run on the current device: refuse a tensor of another one."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: a GPU tensor is needed, got one on {t.device}")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: a tensor on {t.device} while device "
+                         f"{torch._C._cuda_getDevice()} is current")
+
+
+def require_no_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: inference only (no gradient); call under torch.no_grad()")
 
 
 def release_workspaces():

@@ -1,0 +1,217 @@
+// Paged cache of quantized keys and values: writing and reading back.
+//
+// Layout (pages of `page` slots, H heads of D channels, b bits; keys and values
+// apart):
+//   codes  [pages][H][page][D·b/8] bytes: unsigned codes q + 2^(b−1), at 4 bits
+//          two channels a byte, the first in the low half
+//   scale  [pages][H][page] fp32
+//   zero   [pages][H][page] bytes: z + 2^(b−1) (asymmetric grid only)
+// A code u of a slot stands for scale·(u − zero), zero = 2^(b−1) in the
+// symmetric grid.  A sequence's token p lives in slot p % page of page
+// table[p / page].
+#include <algorithm>
+
+#include "grid8.hpp"
+#include "kvcache.hpp"
+
+namespace g2ptq {
+namespace {
+
+struct WriteArgs {
+  const void* x[2];        // keys, values: T × H × D, channels contiguous
+  int64_t st[2], sh[2];    // strides of token and head (elements)
+  const int64_t* slots;    // page·(page size) + offset; negative: not written
+  int64_t T;
+  KvCache c;
+  bool vec[2];
+};
+
+// L lanes hold one token's head, eight channels each (lanes past D idle).
+// grid.y: 0 keys, 1 values.
+template <int DT, bool SYM, int L>
+__global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
+  const int w = blockIdx.y;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const int d = (threadIdx.x % L) * 8;
+  if (item >= a.T * a.c.H) return;
+  const int64_t t = item / a.c.H, h = item - t * a.c.H;
+  const int64_t slot = a.slots[t];
+  if (slot < 0) return;
+  if (slot >= a.c.pages << a.c.shift) {
+    if (d == 0) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+    return;
+  }
+  const bool on = d < a.c.D;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (on) load8<DT>(a.x[w], t * a.st[w] + h * a.sh[w] + d, a.vec[w], 8, v);
+  Range r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.add(v[i]);
+  reduce_range<L>(r);
+  const Grid g = make_grid<SYM>(r, a.c.bits);
+  const int64_t at = a.c.row(slot, h);
+  if (d == 0) {
+    a.c.scale[w][at] = g.s;
+    if (!SYM) a.c.zero[w][at] = (uint8_t)((int)g.z + (1 << (a.c.bits - 1)));
+  }
+  if (!on) return;
+  uint32_t u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = (uint32_t)(to_code(g, v[i]) + (1 << (a.c.bits - 1)));
+  if (a.c.bits == 8) {
+    uint2 o = make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24,
+                         u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
+    *reinterpret_cast<uint2*>(a.c.codes[w] + at * a.c.D + d) = o;
+  } else {
+    uint32_t o = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o |= u[i] << (4 * i);
+    *reinterpret_cast<uint32_t*>(a.c.codes[w] + at * (a.c.D / 2) + d / 2) = o;
+  }
+}
+
+struct ReadArgs {
+  KvCache c;
+  const int32_t* table;
+  int64_t ldt, B, width;
+  const int32_t* cu;  // B + 1 offsets of the sequences in the output
+  int64_t total;
+  void* out[2];       // total × H × D
+};
+
+// One output token's head per L lanes, as in kv_write_kernel.  Output rows
+// outside every sequence, and tokens whose page is not in the cache, are zero.
+template <int DT, bool SYM, int L>
+__global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
+  const int w = blockIdx.y;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const int d = (threadIdx.x % L) * 8;
+  if (item >= a.total * a.c.H || d >= a.c.D) return;
+  const int64_t t = item / a.c.H, h = item - t * a.c.H;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int64_t slot = a.c.find(a.table, a.ldt, a.width, a.cu, a.B, t);
+  if (slot >= 0) {
+    const int64_t at = a.c.row(slot, h);
+    const float s = a.c.scale[w][at];
+    const int z = SYM ? 1 << (a.c.bits - 1) : a.c.zero[w][at];
+    if (a.c.bits == 8) {
+      const uint2 o = *reinterpret_cast<const uint2*>(a.c.codes[w] + at * a.c.D + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = s * (float)((int)((i < 4 ? o.x : o.y) >> (8 * (i & 3)) & 0xffu) - z);
+    } else {
+      const uint32_t o =
+          *reinterpret_cast<const uint32_t*>(a.c.codes[w] + at * (a.c.D / 2) + d / 2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = s * (float)((int)(o >> (4 * i) & 15u) - z);
+    }
+  } else if (slot == -2 && d == 0) {
+    atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+  }
+  store8<DT>(a.out[w], item * a.c.D + d, true, 8, v);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename F>
+int by_lanes(int64_t D, F f) {
+  if (D <= 16) return f(std::integral_constant<int, 2>());
+  if (D <= 32) return f(std::integral_constant<int, 4>());
+  if (D <= 64) return f(std::integral_constant<int, 8>());
+  if (D <= 128) return f(std::integral_constant<int, 16>());
+  return f(std::integral_constant<int, 32>());
+}
+
+}  // namespace
+
+int check_cache(const char* who, const g2ptq_kv_cache* c, KvCache& k) {
+  G2PTQ_CHECK(c, "%s: null cache", who);
+  G2PTQ_CHECK(c->bits == 4 || c->bits == 8, "%s: %d bits (4 or 8)", who, c->bits);
+  G2PTQ_CHECK(c->pages >= 0 && c->pages < (1ll << 31) && c->heads >= 1 && c->heads <= 65535,
+              "%s: %lld pages of %lld heads", who, (long long)c->pages, (long long)c->heads);
+  G2PTQ_CHECK(c->dim >= 16 && c->dim <= 256 && c->dim % 16 == 0,
+              "%s: head dimension %lld (a multiple of 16 up to 256)", who, (long long)c->dim);
+  G2PTQ_CHECK(c->page >= 1 && c->page <= 4096 && (c->page & (c->page - 1)) == 0,
+              "%s: pages of %lld slots (a power of two up to 4096)", who, (long long)c->page);
+  G2PTQ_CHECK(c->flags, "%s: null flags", who);
+  G2PTQ_CHECK(c->pages == 0 || (c->k_codes && c->v_codes && c->k_scale && c->v_scale),
+              "%s: null cache buffer", who);
+  G2PTQ_CHECK(aligned16(c->k_codes) && aligned16(c->v_codes),
+              "%s: codes not 16-byte aligned", who);
+  G2PTQ_CHECK(c->sym || c->pages == 0 || (c->k_zero && c->v_zero), "%s: null zero points", who);
+  k.codes[0] = c->k_codes, k.codes[1] = c->v_codes;
+  k.scale[0] = c->k_scale, k.scale[1] = c->v_scale;
+  k.zero[0] = c->sym ? nullptr : c->k_zero, k.zero[1] = c->sym ? nullptr : c->v_zero;
+  k.pages = c->pages, k.H = c->heads, k.D = c->dim;
+  k.shift = __builtin_ctzll((unsigned long long)c->page);
+  k.bits = c->bits;
+  k.flags = c->flags;
+  return G2PTQ_OK;
+}
+
+}  // namespace g2ptq
+
+using namespace g2ptq;
+
+extern "C" int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const void* k,
+                              int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, int dtype, int64_t T, const int64_t* slots) {
+  WriteArgs a;
+  G2PTQ_TRY(check_cache("kv_write", cache, a.c));
+  G2PTQ_CHECK(dtype >= 0 && dtype <= 2, "kv_write: dtype code %d", dtype);
+  G2PTQ_CHECK(T >= 0 && T * a.c.H < (1ll << 31), "kv_write: %lld tokens of %lld heads",
+              (long long)T, (long long)a.c.H);
+  if (T == 0) return G2PTQ_OK;
+  G2PTQ_CHECK(k && v && slots, "kv_write: null pointer");
+  const int e = dtype == 2 ? 4 : 2;
+  a.x[0] = k, a.x[1] = v;
+  a.st[0] = k_token, a.sh[0] = k_head, a.st[1] = v_token, a.sh[1] = v_head;
+  a.vec[0] = aligned16(k) && k_token * e % 16 == 0 && k_head * e % 16 == 0;
+  a.vec[1] = aligned16(v) && v_token * e % 16 == 0 && v_head * e % 16 == 0;
+  a.slots = slots;
+  a.T = T;
+  hipStream_t st = as_stream(stream);
+  const bool sym = cache->sym != 0;
+  return by_lanes(a.c.D, [&](auto lanes) -> int {
+    constexpr int L = decltype(lanes)::value;
+    const dim3 grid((unsigned)cdiv(T * a.c.H * L, 256), 2);
+#define G2_WR(DT, SYM) \
+  hipLaunchKernelGGL((kv_write_kernel<DT, SYM, L>), grid, dim3(256), 0, st, a)
+    if (dtype == 0) { if (sym) G2_WR(0, true); else G2_WR(0, false); }
+    else if (dtype == 1) { if (sym) G2_WR(1, true); else G2_WR(1, false); }
+    else { if (sym) G2_WR(2, true); else G2_WR(2, false); }
+#undef G2_WR
+    G2PTQ_LAUNCHED();
+    return G2PTQ_OK;
+  });
+}
+
+extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const int32_t* table,
+                             int64_t ldt, int64_t B, int64_t width, const int32_t* cu,
+                             int64_t total, void* k, void* v, int dtype) {
+  ReadArgs a;
+  G2PTQ_TRY(check_cache("kv_read", cache, a.c));
+  G2PTQ_CHECK(dtype >= 0 && dtype <= 2, "kv_read: dtype code %d", dtype);
+  G2PTQ_CHECK(B >= 0 && width >= 0 && ldt >= width, "kv_read: bad page table");
+  G2PTQ_CHECK(total >= 0 && total * a.c.H < (1ll << 31), "kv_read: %lld tokens of %lld heads",
+              (long long)total, (long long)a.c.H);
+  if (total == 0) return G2PTQ_OK;
+  G2PTQ_CHECK(k && v && cu && (table || B * width == 0), "kv_read: null pointer");
+  G2PTQ_CHECK(aligned16(k) && aligned16(v), "kv_read: outputs not 16-byte aligned");
+  a.table = table, a.ldt = ldt, a.B = B, a.width = width, a.cu = cu, a.total = total;
+  a.out[0] = k, a.out[1] = v;
+  hipStream_t st = as_stream(stream);
+  const bool sym = cache->sym != 0;
+  return by_lanes(a.c.D, [&](auto lanes) -> int {
+    constexpr int L = decltype(lanes)::value;
+    const dim3 grid((unsigned)cdiv(total * a.c.H * L, 256), 2);
+#define G2_RD(DT, SYM) \
+  hipLaunchKernelGGL((kv_read_kernel<DT, SYM, L>), grid, dim3(256), 0, st, a)
+    if (dtype == 0) { if (sym) G2_RD(0, true); else G2_RD(0, false); }
+    else if (dtype == 1) { if (sym) G2_RD(1, true); else G2_RD(1, false); }
+    else { if (sym) G2_RD(2, true); else G2_RD(2, false); }
+#undef G2_RD
+    G2PTQ_LAUNCHED();
+    return G2PTQ_OK;
+  });
+}

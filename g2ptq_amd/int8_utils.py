@@ -1,0 +1,204 @@
+"""Linears that run in 8-bit integers: what an 8-bit per-channel quantization
+made (``W_int`` and one scale per output channel) multiplied with tokens
+quantized on the fly, one scale (and zero point) per token.
+
+    Y[t, n] = s_t · w_n · (Σ_k c[t, k]·W[n, k] − z_t·Σ_k W[n, k]) + b_n
+
+The integer sums are exact; scales are applied in fp32 and the result is
+rounded once.  The token grid is the weight quantizer's (``quant_utils``) at
+8 bits with one group per token.  Inference only: nothing here has a
+gradient.
+"""
+import torch
+
+from . import _lib
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_COLUMNS = 65536  # longer rows could overflow the 32-bit sums
+
+
+def _rows(x, columns, what):
+    """``x`` (..., columns) as a (T, columns) GPU tensor with contiguous rows."""
+    if x.dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"{what} takes bf16, fp16 or fp32 tokens, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] != columns:
+        raise ValueError(f"{what}: tokens of shape {tuple(x.shape)} where the last dimension "
+                         f"should be {columns}")
+    _lib.require_current(x, what)
+    _lib.require_no_grad(what, x)
+    x2 = x if x.dim() == 2 else x.reshape(-1, columns)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < columns):
+        x2 = x2.contiguous()
+    return x2
+
+
+def _row_stride(x2):
+    """The row stride of a (T, K) tensor; a single row's is arbitrary in torch."""
+    return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
+
+
+def _padded(n):
+    return (n + 15) // 16 * 16
+
+
+def quantize_tokens(x, sym=True):
+    """Codes (int8, shape of ``x``), scale and zero point (fp32, shape of ``x``
+    without its last dimension; the zero point is None in the symmetric grid)
+    of every token.  A token's value is ``scale · (code − zero)``.
+
+    Codes come as a view of rows padded to 16 bytes, as ``int8_matmul`` reads
+    them."""
+    columns = x.shape[-1] if x.dim() else 0
+    if not 1 <= columns <= MAX_COLUMNS:
+        raise ValueError(f"quantize_tokens: rows of 1 to {MAX_COLUMNS} values, got {columns}")
+    x2 = _rows(x, columns, "quantize_tokens")
+    rows, ldc = x2.shape[0], _padded(columns)
+    codes = torch.empty(rows, ldc, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, device=x.device)
+    zero = None if sym else torch.empty(rows, device=x.device)
+    _lib.call("g2ptq_quantize_tokens", _lib.stream_ptr(x.device), _lib.ptr(x2),
+              _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), int(bool(sym)),
+              _lib.ptr(codes), ldc, _lib.ptr(scale), _lib.ptr(zero))
+    lead = x.shape[:-1]
+    codes = codes[:, :columns].unflatten(0, lead) if len(lead) != 1 else codes[:, :columns]
+    return codes, scale.view(lead), (None if zero is None else zero.view(lead))
+
+
+class Int8Linear(torch.nn.Module):
+    """``y = x̂ · Ŵᵀ + b`` with x̂ the tokens quantized to 8 bits and Ŵ = scale · codes.
+
+    ``codes``: (out, in) int8 GPU tensor; ``scale``: one per output channel;
+    ``bias``: (out,) or None; ``sym``: the tokens' grid.  ``y`` has ``x``'s
+    dtype.  Columns are laid out once in rows of a multiple of 16 bytes."""
+
+    def __init__(self, codes, scale, bias=None, sym=True):
+        super().__init__()
+        if codes.dtype is not torch.int8 or codes.dim() != 2:
+            raise ValueError(f"Int8Linear takes (out, in) int8 codes, got {codes.dtype} of shape "
+                             f"{tuple(codes.shape)}")
+        self.out_features, self.in_features = codes.shape
+        if not 1 <= self.in_features <= MAX_COLUMNS:
+            raise ValueError(f"Int8Linear takes 1 to {MAX_COLUMNS} columns, got "
+                             f"{self.in_features}")
+        if scale.numel() != self.out_features:
+            raise ValueError(f"Int8Linear takes one scale per output channel "
+                             f"({self.out_features}), got shape {tuple(scale.shape)}")
+        if bias is not None and tuple(bias.shape) != (self.out_features,):
+            raise ValueError(f"Int8Linear: bias of shape {tuple(bias.shape)}, expected "
+                             f"({self.out_features},)")
+        if not codes.is_cuda:
+            raise RuntimeError("Int8Linear requires GPU tensors")
+        self.sym = bool(sym)
+        dev = codes.device
+        weight = torch.zeros(self.out_features, _padded(self.in_features), dtype=torch.int8,
+                             device=dev)
+        weight[:, :self.in_features] = codes
+        self.register_buffer("weight", weight)
+        self.register_buffer("weight_scale", scale.detach().reshape(-1).to(
+            device=dev, dtype=torch.float32, copy=True))
+        self.register_buffer("weight_sum", None if self.sym else
+                             codes.sum(dim=1, dtype=torch.int32))
+        self.register_buffer("bias", None if bias is None else bias.detach().to(
+            device=dev, dtype=torch.float32, copy=True))
+
+    @classmethod
+    def from_export(cls, qparams, bias=None, sym=True):
+        """From a layer's exported tensors (``layer._export_qparams`` of an 8-bit
+        ``fasterquant(..., export_compressed_tensors=True)`` with one group per
+        row, or the buffers that ``register_qparam_buffers`` made of them)."""
+        if isinstance(qparams, torch.nn.Module):
+            layer = qparams
+            qparams = layer.__dict__.get("_export_qparams") or {
+                k: b for k, b in layer.named_buffers(recurse=False)}
+            bias = getattr(layer, "bias", None) if bias is None else bias
+        try:
+            packed, scale = qparams["weight_packed"], qparams["weight_scale"]
+            rows, columns = (int(n) for n in qparams["weight_shape"])
+        except KeyError as e:
+            raise ValueError(f"Int8Linear.from_export: no {e} among the exported tensors") from None
+        if packed.shape != (rows, (columns + 3) // 4):
+            raise ValueError(f"Int8Linear.from_export: packed words of shape "
+                             f"{tuple(packed.shape)} are no 8-bit codes of a {rows}x{columns} "
+                             "weight")
+        if scale.numel() != rows:
+            raise ValueError(f"Int8Linear.from_export: scales of shape {tuple(scale.shape)}; "
+                             "one group per row (groupsize -1) is needed")
+        codes = packed.contiguous().view(torch.uint8)[:, :columns]
+        return cls((codes ^ 0x80).view(torch.int8), scale, bias=bias, sym=sym)
+
+    @classmethod
+    def from_linear(cls, linear, quantizer, sym=True):
+        """Round-to-nearest codes of ``linear.weight`` on a fitted symmetric
+        per-channel ``WeightQuantizer`` of at most 8 bits."""
+        if not quantizer.ready() or quantizer.bits > 8 or not quantizer.sym \
+                or quantizer.weight_groupsize > 0:
+            raise ValueError("Int8Linear.from_linear needs a fitted symmetric per-channel "
+                             "quantizer of at most 8 bits")
+        weight = linear.weight.detach()
+        _, codes, scale = quantizer.fake_quantize(weight)
+        if scale.numel() == 1:
+            scale = scale.reshape(1).expand(weight.shape[0])
+        return cls(codes.to(torch.int8), scale, bias=linear.bias, sym=sym)
+
+    def forward(self, x):
+        x2 = _rows(x, self.in_features, "Int8Linear")
+        rows, columns, out = x2.shape[0], self.in_features, self.out_features
+        if self.weight.device != x.device:
+            raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {self.weight.device}")
+        y = torch.empty(rows, out, dtype=x.dtype, device=x.device)
+        if rows:
+            need = _lib.query_size("g2ptq_int8_linear_workspace", rows, out, columns)
+            ws = _lib.scratch(need, x.device)
+            _lib.call("g2ptq_int8_linear", _lib.stream_ptr(x.device), _lib.ptr(x2),
+                      _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), int(self.sym),
+                      _lib.ptr(self.weight), self.weight.stride(0), _lib.ptr(self.weight_scale),
+                      _lib.ptr(self.weight_sum), _lib.ptr(self.bias), out, _lib.ptr(y), out,
+                      _lib.ptr(ws), ws.numel())
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], out)
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, sym={self.sym}")
+
+
+def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
+    """The product alone, for tokens that several linears share: ``codes``,
+    ``scale`` and ``zero`` from ``quantize_tokens``, ``linear`` an
+    ``Int8Linear``; the result is what ``linear`` gives for the tokens, in
+    ``dtype``."""
+    if codes.dtype is not torch.int8 or codes.dim() == 0 \
+            or codes.shape[-1] != linear.in_features:
+        raise ValueError(f"int8_matmul: codes of {codes.dtype} and shape {tuple(codes.shape)} for "
+                         f"{linear.in_features} columns")
+    if dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"int8_matmul gives bf16, fp16 or fp32, not {dtype}")
+    _lib.require_current(codes, "int8_matmul")
+    lead, columns, out = codes.shape[:-1], linear.in_features, linear.out_features
+    for name, t in (("scale", scale), ("zero", zero)):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != lead):
+            raise ValueError(f"int8_matmul: {name} of {t.dtype} and shape {tuple(t.shape)}, "
+                             f"expected fp32 {tuple(lead)}")
+    if zero is not None and linear.weight_sum is None:
+        raise ValueError("int8_matmul: tokens with zero points need a linear made with sym=False")
+    c2 = codes if codes.dim() == 2 else codes.flatten(0, -2) if codes.dim() > 2 \
+        else codes.unsqueeze(0)
+    rows, need = c2.shape[0], _padded(columns)
+    # rows have to be readable in 16-byte steps to their end
+    room = c2.untyped_storage().nbytes() - c2.storage_offset()
+    if (c2.stride(1) != 1 or c2.stride(0) % 16 or c2.stride(0) < need or c2.data_ptr() % 16
+            or (rows - 1) * c2.stride(0) + need > room):
+        padded = torch.zeros(rows, need, dtype=torch.int8, device=codes.device)
+        padded[:, :columns] = c2
+        c2 = padded
+    y = torch.empty(rows, out, dtype=dtype, device=codes.device)
+    if rows:
+        scale, zero = scale.contiguous(), None if zero is None else zero.contiguous()
+        ws = _lib.scratch(_lib.query_size("g2ptq_int8_gemm_workspace", rows, out, columns),
+                          codes.device)
+        _lib.call("g2ptq_int8_gemm", _lib.stream_ptr(codes.device), _lib.ptr(c2), c2.stride(0),
+                  _lib.ptr(scale), _lib.ptr(zero), _lib.ptr(linear.weight),
+                  linear.weight.stride(0), _lib.ptr(linear.weight_scale),
+                  _lib.ptr(linear.weight_sum if zero is not None else None),
+                  _lib.ptr(linear.bias), rows, out, columns, _lib.ptr(y), _DTYPE_CODE[dtype], out,
+                  _lib.ptr(ws), ws.numel())
+    return y.view(*lead, out)

@@ -1,0 +1,178 @@
+"""A paged cache of quantized keys and values, and attention over it.
+
+Keys and values are quantized as they are written, with 4 or 8 bits on the
+weight quantizer's grid (``quant_utils``), one scale (and zero point) per token
+and head.  A slot is ``page number · page_size + offset``; a sequence's token p
+lives in slot ``table[b, p // page_size] · page_size + p % page_size``.
+
+    cache = PagedKVCache(num_pages, page_size=64, kv_heads=8, head_dim=128, bits=4, sym=False)
+    cache.write(k, v, slots)                       # this step's tokens
+    out = paged_attention(q, cache, table, cu_q, kv_lens)
+    k, v = cache.read(table, cu_tokens, total)     # what the cache stands for
+
+Page tables, offsets and lengths are device tensors: nothing here waits for
+the GPU, and a step can be captured into a graph.  Indices outside the cache
+are never followed; they are flagged, and ``cache.check()`` raises for them at
+a point of the caller's choosing.  Inference only: nothing has a gradient.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _heads(x, heads, dim, what):
+    """``x`` (tokens, heads, dim) with contiguous channels on the GPU."""
+    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim:
+        raise ValueError(f"{what} of shape {tuple(x.shape)}, expected (tokens, {heads}, {dim})")
+    _lib.require_current(x, what)
+    _lib.require_no_grad(what, x)
+    return x if x.stride(2) == 1 and x.stride(0) >= 0 and x.stride(1) >= 0 else x.contiguous()
+
+
+def _index(t, dtype, dims, what, device):
+    if t.dtype is not dtype or t.dim() != dims:
+        raise ValueError(f"{what}: a {dims}-dimensional {dtype} tensor is needed, got "
+                         f"{t.dtype} of shape {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} on {t.device}, the cache on {device}")
+    rows = dims == 1 or t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+    return t if rows and (t.stride(-1) == 1 or t.shape[-1] <= 1) else t.contiguous()
+
+
+class PagedKVCache:
+    """``num_pages`` pages of ``page_size`` slots for ``kv_heads`` heads of
+    ``head_dim`` channels, keys and values, ``bits`` 4 or 8.
+
+    ``k_codes``, ``v_codes`` (num_pages, kv_heads, page_size, head_dim·bits/8)
+    uint8, ``k_scale``, ``v_scale`` (num_pages, kv_heads, page_size) fp32 and,
+    with ``sym=False``, ``k_zero``, ``v_zero`` uint8 hold the cache; a code u
+    stands for ``scale · (u − zero)`` with ``zero = 2^(bits − 1)`` in the
+    symmetric grid.  Slots never written stand for zeros."""
+
+    def __init__(self, num_pages, page_size, kv_heads, head_dim, bits=8, sym=True, device="cuda"):
+        if bits not in (4, 8):
+            raise ValueError(f"PagedKVCache holds 4 or 8 bits, not {bits}")
+        if page_size < 1 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError(f"PagedKVCache: pages of {page_size} slots (a power of two up to "
+                             "4096 is needed)")
+        if head_dim % 16 or not 16 <= head_dim <= 256:
+            raise ValueError(f"PagedKVCache: head dimension {head_dim} (a multiple of 16 up to "
+                             "256 is needed)")
+        if num_pages < 0 or not 1 <= kv_heads <= 65535:
+            raise ValueError(f"PagedKVCache: {num_pages} pages of {kv_heads} heads")
+        self.num_pages, self.page_size = num_pages, page_size
+        self.kv_heads, self.head_dim, self.bits, self.sym = kv_heads, head_dim, bits, bool(sym)
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise RuntimeError("PagedKVCache lives on the GPU")
+        shape = (num_pages, kv_heads, page_size)
+        self.k_codes, self.v_codes = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8,
+                                                  device=dev) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.zeros(shape, device=dev) for _ in range(2))
+        self.k_zero, self.v_zero = (None if self.sym else torch.zeros(
+            shape, dtype=torch.uint8, device=dev) for _ in range(2))
+        self.flags = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.device = self.flags.device
+        self._struct = _lib.KvCacheStruct(
+            *(_lib.ptr(t) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale,
+                                    self.k_zero, self.v_zero, self.flags)),
+            num_pages, kv_heads, page_size, head_dim, bits, int(self.sym))
+        self._ref = ctypes.byref(self._struct)
+
+    def write(self, k, v, slots):
+        """Quantize tokens' keys and values (tokens, kv_heads, head_dim; bf16, fp16
+        or fp32, any strides of token and head) into their slots (int64).
+        Negative slots are skipped (padding of a batch); slots must not repeat
+        within a call."""
+        k = _heads(k, self.kv_heads, self.head_dim, "keys")
+        v = _heads(v, self.kv_heads, self.head_dim, "values")
+        if k.dtype not in _DTYPE_CODE or v.dtype is not k.dtype:
+            raise NotImplementedError(f"PagedKVCache.write takes bf16, fp16 or fp32 keys and "
+                                      f"values, got {k.dtype} and {v.dtype}")
+        slots = _index(slots, torch.int64, 1, "slots", self.device)
+        if k.shape[0] != v.shape[0] or k.shape[0] != slots.shape[0]:
+            raise ValueError(f"{k.shape[0]} keys, {v.shape[0]} values, {slots.shape[0]} slots")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError(f"keys on {k.device}, values on {v.device}, the cache on "
+                             f"{self.device}")
+        _lib.call("g2ptq_kv_write", _lib.stream_ptr(self.device), self._ref, _lib.ptr(k),
+                  k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1),
+                  _DTYPE_CODE[k.dtype], k.shape[0], _lib.ptr(slots))
+
+    def read(self, table, cu_tokens, total, dtype=torch.bfloat16):
+        """``(k, v)``, each (total, kv_heads, head_dim) of ``dtype``: rows
+        ``cu_tokens[b]`` to ``cu_tokens[b + 1]`` hold the first positions of the
+        sequence whose pages are ``table[b]`` (both int32).  Rows outside every
+        sequence, and positions without a page, are zero."""
+        if dtype not in _DTYPE_CODE:
+            raise NotImplementedError(f"PagedKVCache.read gives bf16, fp16 or fp32, not {dtype}")
+        table = _index(table, torch.int32, 2, "table", self.device)
+        cu = _index(cu_tokens, torch.int32, 1, "cu_tokens", self.device)
+        if cu.shape[0] != table.shape[0] + 1:
+            raise ValueError(f"cu_tokens has {cu.shape[0]} entries for {table.shape[0]} sequences")
+        if total < 0:
+            raise ValueError(f"total is {total}")
+        _lib.require_current(self.flags, "PagedKVCache.read")
+        k = torch.empty(total, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        _lib.call("g2ptq_kv_read", _lib.stream_ptr(self.device), self._ref, _lib.ptr(table),
+                  max(table.stride(0), table.shape[1]), table.shape[0], table.shape[1],
+                  _lib.ptr(cu), total, _lib.ptr(k), _lib.ptr(v), _DTYPE_CODE[dtype])
+        return k, v
+
+    def check(self):
+        """Raise if a slot or page outside the cache was met since the last check
+        (waits for the GPU)."""
+        v = int(self.flags.item())
+        self.flags.zero_()
+        if v & _lib.FLAG_BAD_INDEX:
+            raise IndexError("a slot or page outside the cache was given to a PagedKVCache")
+
+
+def paged_attention(q, cache, table, cu_q, kv_lens, scale=None, max_q=None, max_kv=None):
+    """Causal attention of each sequence's new tokens over its keys and values in
+    the cache (the new tokens' own among them: write before attending).
+
+    ``q`` (tokens, heads, head_dim) bf16 or fp16, any strides of token and
+    head: rows ``cu_q[b]`` to ``cu_q[b + 1]`` are the last tokens of sequence b,
+    which has ``kv_lens[b]`` in the cache, in pages ``table[b]`` (all int32).
+    ``heads`` is a multiple of the cache's; neighbouring heads share one of them.
+    ``scale`` defaults to 1/sqrt(head_dim).  Returns (tokens, heads, head_dim) in
+    ``q``'s dtype; rows without a key, and rows outside every sequence, are zero.
+
+    ``max_q`` and ``max_kv``, the batch's most new tokens and longest sequence
+    where the caller knows them, size the launch (default: all tokens, the whole
+    table); lengths beyond them are still computed."""
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"paged_attention takes bf16 or fp16 queries, got {q.dtype}")
+    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"queries of shape {tuple(q.shape)} over {cache.kv_heads} heads of the "
+                         "cache")
+    q = _heads(q, q.shape[1], cache.head_dim, "queries")
+    if q.device != cache.device:
+        raise ValueError(f"queries on {q.device}, the cache on {cache.device}")
+    table = _index(table, torch.int32, 2, "table", cache.device)
+    cu_q = _index(cu_q, torch.int32, 1, "cu_q", cache.device)
+    kv_lens = _index(kv_lens, torch.int32, 1, "kv_lens", cache.device)
+    (T, heads, dim), (B, width) = q.shape, table.shape
+    if cu_q.shape[0] != B + 1 or kv_lens.shape[0] != B:
+        raise ValueError(f"cu_q has {cu_q.shape[0]} and kv_lens {kv_lens.shape[0]} entries for "
+                         f"{B} sequences")
+    max_q = T if max_q is None else max(0, min(int(max_q), T))
+    room = width * cache.page_size
+    max_kv = room if max_kv is None else max(0, min(int(max_kv), room))
+    out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
+    need = _lib.query_size("g2ptq_paged_attention_workspace", T, heads, cache.kv_heads, dim, B,
+                           max_q, max_kv)
+    ws = _lib.scratch(need, q.device)
+    _lib.call("g2ptq_paged_attention", _lib.stream_ptr(q.device), cache._ref, _lib.ptr(q),
+              q.stride(0), q.stride(1), _DTYPE_CODE[q.dtype], T, heads, _lib.ptr(table),
+              max(table.stride(0), width), B, width, _lib.ptr(cu_q), _lib.ptr(kv_lens), max_q,
+              max_kv, 1.0 / math.sqrt(dim) if scale is None else float(scale), _lib.ptr(out),
+              _lib.ptr(ws), ws.numel())
+    return out

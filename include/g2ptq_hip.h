@@ -36,6 +36,7 @@ extern "C" {
 #define G2PTQ_FLAG_BAD_SCALE 1   /* a scale was <= 0 or NaN (quant_utils.py:432 assert) */
 #define G2PTQ_FLAG_NAN_OUTPUT 2  /* NaN in quantized weights (gptq_utils.py:346-350) */
 #define G2PTQ_FLAG_GROUP_SCALE 4 /* scales differ within a group (compressed_tensors_utils.py:35 assert) */
+#define G2PTQ_FLAG_BAD_INDEX 8   /* a cache slot or page outside the cache */
 
 /* Compensation variants. */
 #define G2PTQ_VARIANT_GPTQ 0
@@ -392,6 +393,98 @@ int g2ptq_gemm_f32(void* stream, int64_t M, int64_t N, int64_t K, int64_t batch,
                    int64_t lda, int64_t sA, const float* B, int64_t ldb, int64_t sB, int b_trans,
                    const float* C, int64_t ldc, int64_t sC, float* D, int64_t ldd, int64_t sD,
                    float alpha, float beta);
+
+/* ------------------------------------------------------------------------
+ * Running a quantized layer: 8-bit linears, the paged cache, attention over it
+ *
+ * No counterpart in the reference, which fake-quantizes activations in torch.
+ * The grid is the weight quantizer's (utils/quant_utils.py:8-68) with one
+ * group per token (and head):
+ *   sym:  s = max|x| / ((2^b − 1)/2), z = 0
+ *   else: s = (max(x,0) − min(x,0)) / (2^b − 1), z = clamp(round(minq − min(x,0)/s))
+ *   q = clamp(round(x/s) + z), x̂ = s·(q − z)
+ * with every quotient rounded to fp32.  A group of zeros has s = 0 and codes 0;
+ * a group with a NaN or an infinity has a NaN or infinite s, codes 0 and so
+ * x̂ = NaN.
+ * ---------------------------------------------------------------------- */
+
+/* Tokens x (T × K, ld ldx, dtype 0 bf16, 1 fp16, 2 fp32) to 8-bit codes (rows
+ * of ldc bytes: 16-byte aligned, ldc a multiple of 16; columns from K to the
+ * next multiple of 16 are written as zeros), scale (T) and, with sym == 0,
+ * zero (T).  K at most 65536. */
+int g2ptq_quantize_tokens(void* stream, const void* x, int dtype, int64_t T, int64_t K,
+                          int64_t ldx, int sym, int8_t* codes, int64_t ldc, float* scale,
+                          float* zero);
+
+/* out[t][n] = scale[t]·wscale[n]·(Σ_k codes[t][k]·W[n][k] − zero[t]·wsum[n]) + bias[n]
+ * (dtype as above, ld ldo).  codes as written by g2ptq_quantize_tokens; W: N
+ * rows of ldw bytes, 16-byte aligned, ldw a multiple of 16, zero in the columns
+ * from K to the next multiple of 16; wsum[n] = Σ_k W[n][k].  zero (with wsum)
+ * and bias are nullable.  Sums are exact integers. */
+int g2ptq_int8_gemm_workspace(int64_t T, int64_t N, int64_t K, size_t* bytes);
+int g2ptq_int8_gemm(void* stream, const int8_t* codes, int64_t ldc, const float* scale,
+                    const float* zero, const int8_t* W, int64_t ldw, const float* wscale,
+                    const int32_t* wsum, const float* bias, int64_t T, int64_t N, int64_t K,
+                    void* out, int dtype, int64_t ldo, void* ws, size_t ws_bytes);
+
+/* Both in one call: out = the product of x's quantized tokens (out has x's
+ * dtype; wsum is needed with sym == 0 only).  ws is 16-byte aligned. */
+int g2ptq_int8_linear_workspace(int64_t T, int64_t N, int64_t K, size_t* bytes);
+int g2ptq_int8_linear(void* stream, const void* x, int dtype, int64_t T, int64_t K, int64_t ldx,
+                      int sym, const int8_t* W, int64_t ldw, const float* wscale,
+                      const int32_t* wsum, const float* bias, int64_t N, void* out, int64_t ldo,
+                      void* ws, size_t ws_bytes);
+
+/* A paged cache of keys and values (the struct is host memory, its pointers
+ * device memory).  codes: [pages][heads][page][dim·bits/8] bytes, q + 2^(bits−1)
+ * unsigned, at 4 bits two channels a byte with the first in the low half,
+ * 16-byte aligned; scale: [pages][heads][page]; zero: the same in bytes,
+ * z + 2^(bits−1), with sym == 0 only.  bits: 4 or 8; dim: a multiple of 16 up to
+ * 256; page: a power of two up to 4096.  flags: one int32 (G2PTQ_FLAG_BAD_INDEX). */
+typedef struct g2ptq_kv_cache {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  uint8_t* k_zero;
+  uint8_t* v_zero;
+  int* flags;
+  int64_t pages, heads, page, dim;
+  int bits, sym;
+} g2ptq_kv_cache;
+
+/* Quantizes T tokens' keys and values (dtype 0 bf16, 1 fp16, 2 fp32; strides of
+ * token and head in elements, channels contiguous) into the cache, token t at
+ * slot slots[t] = page number·page + offset.  Negative slots are skipped; a slot
+ * outside the cache is skipped and flagged.  Slots must not repeat. */
+int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const void* k, int64_t k_token,
+                   int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int dtype,
+                   int64_t T, const int64_t* slots);
+
+/* Reads sequences back: row cu[b] + p of k and v (total × heads × dim of the given
+ * dtype, 16-byte aligned) is position p of sequence b, whose pages are table[b][0 ..]
+ * (B rows of width entries, ld ldt).  cu: B + 1 non-decreasing offsets.  Rows
+ * outside every sequence are zero; so are positions whose page is not in the
+ * cache, which are flagged. */
+int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const int32_t* table, int64_t ldt,
+                  int64_t B, int64_t width, const int32_t* cu, int64_t total, void* k, void* v,
+                  int dtype);
+
+/* Causal attention over the cache: query rows cu_q[b] .. cu_q[b + 1] − 1 of q
+ * (T × Hq × dim, dtype 0 or 1, strides of token and head) are the last tokens of
+ * sequence b's kv_lens[b] in the cache; out (T × Hq × dim, contiguous) gets
+ *   out[i] = Σ_j softmax_j(scale·q_i·k̂_j)·v̂_j,  j ≤ kv_lens[b] − q_len + i.
+ * Query head h reads the cache's head h / (Hq / heads).  Rows without keys and rows
+ * outside every sequence are zero; keys whose page is not in the cache are left
+ * out and flagged.  max_q and max_kv size the launch: the result does not depend
+ * on them beyond rounding. */
+int g2ptq_paged_attention_workspace(int64_t T, int64_t Hq, int64_t kv_heads, int64_t dim,
+                                    int64_t B, int64_t max_q, int64_t max_kv, size_t* bytes);
+int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, const void* q,
+                          int64_t q_token, int64_t q_head, int dtype, int64_t T, int64_t Hq,
+                          const int32_t* table, int64_t ldt, int64_t B, int64_t width,
+                          const int32_t* cu_q, const int32_t* kv_lens, int64_t max_q,
+                          int64_t max_kv, float scale, void* out, void* ws, size_t ws_bytes);
 
 #ifdef __cplusplus
 }
