@@ -5,6 +5,26 @@
 // over the keys j ≤ p_i of the query's sequence, p_i = kv_len − q_len + i the
 // position of its i-th new token.  k̂ = s(u − z) and v̂ are what the cache holds
 // (kvcache.hip).  A query without keys (kv_len < q_len) gets zeros.
+//
+// Rows.  The G query heads that share a head of the cache read the same keys and
+// values, so the rows of a product are (token, head of the group) pairs: row r
+// of a sequence and cache head is token r / G, head r % G.
+//
+// Numbers.  u − z is an integer of at most 255, exact in fp16 (formed as
+// (u − z)·2^-9 from the subnormal fp16 whose bits are u).  A query row is scaled
+// by a power of two so that its largest element is in [1, 2) and rounded to fp16
+// (exact for fp16 and, above 2^-14 of the largest element, for bf16).  Both
+// products run on the fp16 matrix cores with fp32 accumulators; scales, softmax
+// statistics and sums are fp32:
+//   s_j = (Σ q·(u − z)2^-9)·(2^9·scale·log2 e·sk_j),  p_j = exp2(C·(s_j − max) + e),
+//   l = Σ p_j,  o = 2^9·Σ fp16(p_j·sv_j)·(u − z)2^-9 / l,
+// C the row's power of two (so C·max is exact), e = 15 − log2(ref), ref
+// a power of two above the scales sv of the values that the row has seen: the
+// weights p·sv reach up to 2^15 and keep their 11 bits down to 2^-29 of that.
+// One pass over the keys: when the maximum or ref grows, the row's sums are
+// scaled back.  Scales are the only numbers of the cache that can be NaN or
+// infinite, and a key that a row does not see enters neither its maximum, its
+// ref nor its sums.
 #include <algorithm>
 
 #include "grid8.hpp"
@@ -13,92 +33,873 @@
 namespace g2ptq {
 namespace {
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kFewRows = 16;  // rows of a sequence and head up to which attend_rows_kernel runs
+
 struct AttnArgs {
   KvCache c;
   const void* q;
   int64_t qt, qh;  // strides of query token and head
   void* out;       // T × Hq × D, contiguous
-  int64_t T, Hq, B, ldt, width;
+  int64_t ldt;
   const int32_t *table, *cu, *kv;
+  int T, Hq, B, G, width;
+  int dtype;
+  bool vec;        // 16-byte loads of queries
   float scale;
+  float kscale;    // |scale|·log2 e·2^9: multiplies the keys' scales
+  int tiles;       // row tiles a launch provides for a sequence and head (attend_tiles_kernel)
+  int split, few_split;  // shares of the keys (tiles; few rows)
+  bool by_rows, by_tiles;  // kernels that run; with both, sequences of at most kFewRows rows
+                           // go to attend_rows_kernel
+  float *part, *few_part;  // partial results of the shares, or null
 };
 
-// One wave per (query token, head): lanes share a block of 64 keys for the
-// products with the query, then the head's channels for the products with the
-// values.
-template <int DT>
-__global__ __launch_bounds__(64) void attention_simple_kernel(AttnArgs a) {
-  __shared__ float qs[256], ps[64];
-  const int64_t t = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
-  const int lane = threadIdx.x, D = (int)a.c.D;
-  const int64_t h = hq / (a.Hq / a.c.H);
-  const int64_t b = KvCache::sequence(a.cu, a.B, t);
-  int64_t last = -1;  // the last key that the query sees
-  if (b >= 0) last = (int64_t)a.kv[b] - (a.cu[b + 1] - t);
-  const int half = 1 << (a.c.bits - 1), per = a.c.bits == 8 ? 1 : 2;
-  for (int d = lane * 8; d < D; d += 512) {
-    float v[8];
-    load8<DT>(a.q, t * a.qt + hq * a.qh + d, false, 8, v);
-    for (int i = 0; i < 8; ++i) qs[d + i] = v[i];
+// A sequence's rows of the query and its keys.
+struct Span {
+  int q0, qlen;  // first query row, query rows
+  int pos0;      // position of the first new token (negative: queries without keys)
+  int n;         // keys that the page table has
+};
+
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
+  Span s;
+  s.q0 = min(max(a.cu[b], 0), a.T);
+  s.qlen = min(max(a.cu[b + 1], s.q0), a.T) - s.q0;
+  const int kv = a.kv[b];
+  s.pos0 = kv - s.qlen;
+  const int64_t room = (int64_t)a.width << a.c.shift;
+  s.n = a.c.pages == 0 ? 0 : (int)min<int64_t>(max(kv, 0), room);
+  if (kv > s.n && s.qlen > 0 && threadIdx.x == 0) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+  return s;
+}
+
+// Keys of one of `split` shares of n keys, in multiples of `step`.
+__device__ __forceinline__ int share_of(int n, int split, int step) {
+  const int each = (n + split - 1) / split;
+  return max(step, (each + step - 1) / step * step);
+}
+
+__device__ __forceinline__ f16x2 as_h2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+
+// (u − z)·2^-9 of two codes held as 16-bit integers; zc = −z·2^-9 twice.
+__device__ __forceinline__ f16x2 centred(uint32_t two, f16x2 zc) {
+  const f16x2 up = {(_Float16)32768.f, (_Float16)32768.f};
+  return __builtin_elementwise_fma(as_h2(two), up, zc);
+}
+__device__ __forceinline__ f16x2 centre(int z0, int z1) {
+  return f16x2{(_Float16)((float)-z0 * 0x1p-9f), (_Float16)((float)-z1 * 0x1p-9f)};
+}
+
+// Eight channels of one key, in the order channel_of gives.
+template <int BITS>
+__device__ __forceinline__ f16x8 key_codes(const uint32_t* w, f16x2 zc) {
+  f16x2 h[4];
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[2 * i] = centred(__builtin_amdgcn_perm(0, w[i], 0x0c010c00), zc);
+      h[2 * i + 1] = centred(__builtin_amdgcn_perm(0, w[i], 0x0c030c02), zc);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = centred((w[0] >> (4 * i)) & 0x000f000fu, zc);
   }
-  __syncthreads();
-  float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.f;
-  int bad = 0;
-  const int32_t* table = a.table + (b < 0 ? 0 : b) * a.ldt;
-  for (int64_t j0 = 0; j0 <= last; j0 += 64) {
-    const int64_t j = j0 + lane;
-    float s = -INFINITY;
-    int64_t at = -1;
-    if (j <= last) {
-      const int64_t slot = a.c.slot(table, a.width, j);
-      if (slot >= 0) {
-        at = a.c.row(slot, h);
-        const uint8_t* k = a.c.codes[0] + at * (D / per);
-        const int z = a.c.zero[0] ? a.c.zero[0][at] : half;
-        float x = 0.f;
-        for (int d = 0; d < D; ++d) {
-          const int u = per == 1 ? k[d] : (k[d >> 1] >> (4 * (d & 1))) & 15;
-          x += qs[d] * (float)(u - z);
+  return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+// Position i of key_codes' eight channels (4-bit codes: i and i + 4 side by side).
+template <int BITS>
+__device__ __forceinline__ constexpr int channel_of(int i) {
+  return BITS == 8 ? i : (i >> 1) + 4 * (i & 1);
+}
+
+// Channel e (of eight) of two tokens' values.
+template <int BITS>
+__device__ __forceinline__ f16x2 value_codes(const uint32_t* a, const uint32_t* b, int e,
+                                             f16x2 zc) {
+  if constexpr (BITS == 8) {
+    const uint32_t k = e & 3;
+    return centred(__builtin_amdgcn_perm(b[e >> 2], a[e >> 2], 0x0c000c00u | (4 + k) << 16 | k), zc);
+  } else {
+    const uint32_t k = e >> 1;
+    const uint32_t two = __builtin_amdgcn_perm(b[0], a[0], 0x0c000c00u | (4 + k) << 16 | k);
+    return centred((two >> (4 * (e & 1))) & 0x000f000fu, zc);
+  }
+}
+
+// Power of two just above the finite scale x, from 2^-90 up.
+__device__ __forceinline__ float above(float x) {
+  const uint32_t e = (__float_as_uint(x) & 0x7f800000u) + 0x00800000u;
+  return __uint_as_float(max(e, (uint32_t)(127 - 90) << 23));
+}
+__device__ __forceinline__ int exponent(float p) { return (int)(__float_as_uint(p) >> 23) - 127; }
+
+// Power of two that brings a query row with largest |q| = m into [1, 2), and its
+// inverse.
+struct RowScale {
+  float down, up;
+};
+__device__ __forceinline__ RowScale row_scale(float m) {
+  uint32_t e = __float_as_uint(m) >> 23;
+  e = e >= 255 ? 127 : min(max(e, 1u), 253u);  // a NaN or infinite row stays one as it is
+  return {__uint_as_float((254 - e) << 23), __uint_as_float(e << 23)};
+}
+
+// Output row of sequence row r, or -1 past the sequence's rows.
+struct RowAt {
+  int token, head;
+};
+__device__ __forceinline__ RowAt row_at(const AttnArgs& a, const Span& s, int h, int r) {
+  const uint32_t t = (uint32_t)r / (uint32_t)a.G;
+  return {s.q0 + (int)t, h * a.G + (r - (int)t * a.G)};
+}
+
+template <int N>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, const float (&y)[N]) {
+  uint16_t w[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    w[i] = a.dtype == 0 ? __builtin_bit_cast(uint16_t, (__bf16)y[i])
+                        : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
+  uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+  if constexpr (N == 8)
+    *reinterpret_cast<uint4*>(o) = make_uint4(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16,
+                                              w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
+  else
+    *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+}
+
+__device__ __forceinline__ void load_q8(const AttnArgs& a, int64_t at, float (&v)[8]) {
+  if (a.dtype == 0) load8<0>(a.q, at, a.vec, 8, v);
+  else load8<1>(a.q, at, a.vec, 8, v);
+}
+
+// A partial result: the row's output over a share of the keys (D floats), its
+// maximum (log2 units) and its sum.
+__device__ __forceinline__ int64_t part_size(const AttnArgs& a) { return a.c.D + 4; }
+
+// Query rows outside every sequence.
+__device__ void clear_outside(const AttnArgs& a) {
+  const int lo = a.B ? min(max(a.cu[0], 0), a.T) : a.T;
+  const int hi = a.B ? min(max(a.cu[a.B], 0), a.T) : a.T;
+  const int64_t row = a.Hq * a.c.D / 8;
+  uint4* o = static_cast<uint4*>(a.out);
+  for (int64_t i = threadIdx.x; i < lo * row; i += blockDim.x) o[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = hi * row + threadIdx.x; i < a.T * row; i += blockDim.x)
+    o[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (decoding): the keys' and values' bytes are what counts.  A wave takes
+// 32 keys at a time straight into registers, laid out so that neither operand
+// needs a shuffle: with v_mfma_f32_16x16x32_f16,
+//   S^T (16 keys × 16 rows) = K·Q^T: lane (key, g) loads a quarter g of the key's
+//     channels in one piece, the query's channels are laid out alike;
+//   O^T (channels × 16 rows) += V^T·P^T: lane (n, g) loads channels n·DV .. of the
+//     eight tokens whose weights lie in its own registers after the softmax
+//     (4g .. 4g + 3 and 16 + 4g ..), so P^T needs no exchange; channel n·DV + e is
+//     row n of the e-th product.
+// Row statistics are per lane (row = lane % 16).  Four waves interleave blocks of 32
+// keys and join through LDS; `few_split` workgroups share a sequence's keys.
+// DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
+// ---------------------------------------------------------------------------
+template <int BITS, int DP, bool FULL>
+__global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
+  constexpr int DG = DP / 4;                  // channels of a lane's share of a key
+  constexpr int KW = DG * BITS / 32;          // its words
+  constexpr int KS = DP / 32;                 // products of 32 channels
+  constexpr int DV = DP / 16;                 // channels of a lane's share of a value
+  constexpr int VW = (DV * BITS + 31) / 32;   // its words
+  constexpr int PITCH = DP + 4;
+  __shared__ uint32_t rowL[4][32];
+  __shared__ __attribute__((aligned(16))) float skL[4][32], svL[4][32];
+  __shared__ __attribute__((aligned(16))) int zvL[4][32];
+  __shared__ int zkL[4][32];
+  __shared__ __attribute__((aligned(16))) float oL[4][16 * PITCH];
+  __shared__ float mL[4][16], lL[4][16];
+
+  const int b = blockIdx.z, h = blockIdx.y, split = blockIdx.x;
+  if (b == a.B) {
+    if (h == 0 && split == 0) clear_outside(a);
+    return;
+  }
+  const Span sp = span_of(a, b);
+  const int rows = sp.qlen * a.G;
+  if (rows == 0 || (a.by_tiles && rows > kFewRows)) return;
+  const int shares = rows > kFewRows ? 1 : a.few_split;
+  if (split >= shares) return;
+  const int share = share_of(sp.n, shares, 128);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int D = FULL ? DP : (int)a.c.D;
+  const int rowb = D * BITS / 8;
+  const int half = 1 << (BITS - 1);
+  const int32_t* table = a.table + b * a.ldt;
+
+  for (int r0 = 0; r0 < rows; r0 += 16) {
+    const RowAt at = row_at(a, sp, h, min(r0 + n, rows - 1));
+    // the last key that the lane's row sees, and that any of the block's rows sees
+    const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
+    const int last_all = min(sp.pos0 + (min(r0 + 15, rows - 1)) / a.G, sp.n - 1);
+    const int k0 = split * share, k1 = min(last_all + 1, k0 + share);
+
+    // query: channels g·DG + 8s .. of row n, scaled into fp16
+    f16x8 qf[KS];
+    float C;
+    {
+      float v[KS][8], m = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = g * DG + 8 * s;
+        if (FULL || d < D) {
+          load_q8(a, at.token * a.qt + at.head * a.qh + d, v[s]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
         }
-        s = x * a.c.scale[0][at] * a.scale;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[s][i]) & 0x7fffffffu));
+      }
+      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 16))));
+      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 32))));
+      const RowScale rs = row_scale(m);
+      const float sign = a.scale < 0.f ? -rs.down : rs.down;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)(v[s][channel_of<BITS>(i)] * sign);
+      C = rs.up;
+    }
+
+    f32x4 acc[DV];
+#pragma unroll
+    for (int e = 0; e < DV; ++e) acc[e] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
+    int bad = 0;
+
+    for (int j0 = k0 + 32 * wave; j0 < k1; j0 += 128) {
+      // ---- the 32 keys' rows in the cache, scales and zero points ----
+      {
+        const int key = j0 + (lane & 31), kv = lane >> 5;
+        int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
+        bad |= slot == -2;
+        const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
+        const float s = slot < 0 ? 0.f : a.c.scale[kv][row];
+        const int z = a.c.zero[0] ? a.c.zero[kv][row] : half;
+        if (kv == 0) {
+          rowL[wave][lane] = row;
+          skL[wave][lane] = s * a.kscale;
+          zkL[wave][lane] = z;
+        } else {
+          svL[wave][lane - 32] = s;
+          zvL[wave][lane - 32] = z;
+        }
+        const uint32_t ok = (uint32_t)__builtin_amdgcn_ballot_w64(slot >= 0);
+        __builtin_amdgcn_wave_barrier();
+        // ---- their codes ----
+        uint32_t kw[2][KW], vw[8][VW];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint8_t* p =
+              a.c.codes[0] + (int64_t)rowL[wave][16 * kb + n] * rowb + g * (DG * BITS / 8);
+          if constexpr (FULL && KW % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < KW / 4; ++i) {
+              const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+              kw[kb][4 * i] = v.x, kw[kb][4 * i + 1] = v.y;
+              kw[kb][4 * i + 2] = v.z, kw[kb][4 * i + 3] = v.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < KW / 2; ++i) {  // 8 bytes: 8 or 16 channels
+              uint2 v = make_uint2(0, 0);
+              if (FULL || g * DG + i * (64 / BITS) < D) v = reinterpret_cast<const uint2*>(p)[i];
+              kw[kb][2 * i] = v.x, kw[kb][2 * i + 1] = v.y;
+            }
+          }
+        }
+        const bool von = FULL || n * DV < D;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);
+          const uint8_t* p =
+              a.c.codes[1] + (int64_t)rowL[wave][t] * rowb + n * (DV * BITS / 8);
+          if (!von) p = a.c.codes[1];
+          if constexpr (DV * BITS == 16) {
+            vw[j][0] = *reinterpret_cast<const uint16_t*>(p);
+          } else if constexpr (VW == 1) {
+            vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
+          } else if constexpr (VW == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            vw[j][0] = v.x, vw[j][1] = v.y;
+          } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            vw[j][0] = v.x, vw[j][1] = v.y, vw[j][2] = v.z, vw[j][3] = v.w;
+          }
+        }
+        // ---- logits ----
+        float p[8], sv[8];
+        float mx = m, vx = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const int zk = zkL[wave][16 * kb + n];
+          const f16x2 zc = centre(zk, zk);
+          f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                key_codes<BITS>(&kw[kb][s * BITS / 4], zc), qf[s], x, 0, 0, 0);
+          const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[wave][16 * kb + 4 * g]);
+          const f32x4 s4 = *reinterpret_cast<const f32x4*>(&svL[wave][16 * kb + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = 16 * kb + 4 * g + i;
+            const bool see = (ok >> t & 1) && j0 + t <= last;
+            p[4 * kb + i] = x[i] * sk[i];
+            sv[4 * kb + i] = s4[i];
+            if (see) {
+              mx = fmaxf(mx, p[4 * kb + i]);
+              if (s4[i] < __builtin_inff()) vx = fmaxf(vx, s4[i]);
+            }
+          }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        vx = fmaxf(vx, __shfl_xor(vx, 16));
+        vx = fmaxf(vx, __shfl_xor(vx, 32));
+        // ---- the row's units ----
+        if (__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0) {
+          const float nref = vx >= ref ? above(vx) : ref;
+          float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
+          if (m == mx) f = 1.f;
+          f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
+          m = mx, ref = nref;
+          l *= f;
+#pragma unroll
+          for (int e = 0; e < DV; ++e) acc[e] *= f;
+        }
+        const float e0 = (float)(15 - exponent(ref)), m0 = m == -INFINITY ? 0.f : m;
+        f16x8 w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int t = 16 * (i >> 2) + 4 * g + (i & 3);
+          const bool see = (ok >> t & 1) && j0 + t <= last;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
+          l += see ? x : 0.f;
+          w[i] = (_Float16)(see ? x * sv[i] : 0.f);
+        }
+        // ---- values ----
+        f16x2 zc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = (i < 2 ? 4 * g + 2 * i : 16 + 4 * g + 2 * i - 4);
+          zc[i] = centre(zvL[wave][t], zvL[wave][t + 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < DV; ++e) {
+          f16x2 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = value_codes<BITS>(&vw[2 * i][e / 8 * (BITS / 4)],
+                                     &vw[2 * i + 1][e / 8 * (BITS / 4)], e & 7, zc[i]);
+          const f16x8 vf = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+          acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, w, acc[e], 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+
+    // ---- join the four waves: units of the block's maximum, true scale ----
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    l = __builtin_amdgcn_ldexpf(l, exponent(ref) - 15);
+    if (g == 0) mL[wave][n] = m, lL[wave][n] = l;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(mL[0][n], mL[1][n]), fmaxf(mL[2][n], mL[3][n]));
+    {
+      // (a wave without keys has m = -inf and sums of zero)
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * C);
+      const float back = __builtin_amdgcn_ldexpf(f, exponent(ref) - 15 + 9);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < DV; ++e)
+          oL[wave][n * PITCH + (4 * g + i) * DV + e] = acc[e][i] * back;
+      if (g == 0) lL[wave][n] = l * f;
+    }
+    __syncthreads();
+    const float MC = M * C;  // of row n, as every wave has it
+    for (int i = threadIdx.x; i < 16 * (D / 8); i += 256) {
+      // lanes of a row block are spread over rows: row = i % 16
+      const int r = i & 15, d = (i >> 4) * 8;
+      if (r0 + r >= rows) continue;
+      const float L = lL[0][r] + lL[1][r] + lL[2][r] + lL[3][r];
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      float y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        y[k] = (oL[0][r * PITCH + d + k] + oL[1][r * PITCH + d + k] + oL[2][r * PITCH + d + k] +
+                oL[3][r * PITCH + d + k]) * inv;
+      if (shares > 1) {
+        // row n of this lane is row r: i % 16 == threadIdx.x % 16
+        float* o = a.few_part +
+                   ((((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split + split) * part_size(a);
+        *reinterpret_cast<float4*>(o + d) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(o + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        if (d == 0) o[D] = M == -INFINITY ? -INFINITY : MC, o[D + 1] = L;
       } else {
-        bad = 1;
+        const RowAt ra = row_at(a, sp, h, r0 + r);
+        store_out(a, ((int64_t)ra.token * a.Hq + ra.head) * D + d, y);
       }
     }
-    float mj = s;
-    for (int w = 32; w > 0; w >>= 1) mj = fmaxf(mj, __shfl_xor(mj, w));
-    const float mn = fmaxf(m, mj);
-    const float shift = mn == -INFINITY ? 0.f : mn;
-    const float p = at >= 0 ? expf(s - shift) : 0.f, alpha = expf(m - shift);
-    m = mn;
-    float pl = p;
-    for (int w = 32; w > 0; w >>= 1) pl += __shfl_xor(pl, w);
-    l = l * alpha + pl;
-    for (int r = 0; r < 4; ++r) o[r] *= alpha;
-    const float pv = at >= 0 ? p * a.c.scale[1][at] : 0.f;
-    for (int i = 0; i < 64; ++i) {
-      const int64_t ai = __shfl(at, i);
-      const float pi = __shfl(pv, i);
-      if (ai < 0) continue;
-      const uint8_t* v = a.c.codes[1] + ai * (D / per);
-      const int z = a.c.zero[1] ? a.c.zero[1][ai] : half;
-      for (int r = 0; r < 4; ++r) {
-        const int d = lane + 64 * r;
-        if (d >= D) break;
-        const int u = per == 1 ? v[d] : (v[d >> 1] >> (4 * (d & 1))) & 15;
-        o[r] += pi * (float)(u - z);
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (chunks of prompts): matrix cores.  A workgroup of NW waves takes 32·NW
+// rows, 32 per wave, through 64 keys at a time.  The keys and values of a step are
+// converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
+// transposed as [channel][key]; the codes of the next step are loaded meanwhile (two
+// buffers, one barrier a step).  v_mfma_f32_32x32x16_f16:
+//   S^T (32 keys × 32 rows) = K·Q^T, so that a lane holds one row's logits (row =
+//     lane % 32, the other half of the keys in lane + 32) and its statistics;
+//   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
+//     a lane's operand are 16t + 4h .. and 16t + 8 + 4h .. (h = lane / 32), and V^T is
+//     stored with its keys in that order.
+// 16-byte chunks of LDS rows are placed at chunk ^ f(row), which keeps fragment
+// reads (8 consecutive rows, one chunk) and writes free of bank conflicts.
+// ---------------------------------------------------------------------------
+template <int BITS, int DP, bool FULL, int NW>
+__global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
+  constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
+  constexpr int KP = BN * (DP / 16), KC = (KP + NT - 1) / NT;      // 16-channel pieces of keys
+  constexpr int VP = BN / 4 * (DP / 8), VQ = (VP + NT - 1) / NT;   // 4-key × 8-channel of values
+  constexpr int KW = BITS / 2, VW = BITS / 4;   // words of 16 and of 8 channels
+  __shared__ __attribute__((aligned(16))) _Float16 kL[2][BN * DP], vL[2][DP * BN];
+  __shared__ __attribute__((aligned(16))) float skL[2][BN], svL[2][BN];
+  __shared__ float vmaxL[2];
+  __shared__ uint64_t okL[2];
+
+  // Workgroups go round the 8 XCDs; number them so that an XCD takes a contiguous
+  // range: the row tiles of one sequence and head share its keys in one L2.
+  const int total = a.B * (int)a.c.H * a.split * a.tiles;
+  if ((int)blockIdx.x == total) {
+    clear_outside(a);
+    return;
+  }
+  int id;
+  {
+    const int q8 = total >> 3, r8 = total & 7, xcd = blockIdx.x & 7;
+    id = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
+  }
+  const int tile0 = id % a.tiles;
+  id /= a.tiles;
+  const int split = id % a.split;
+  id /= a.split;
+  const int h = id % (int)a.c.H, b = id / (int)a.c.H;
+  const Span sp = span_of(a, b);
+  const int rows = sp.qlen * a.G;
+  if (rows == 0 || (a.by_rows && rows <= kFewRows)) return;
+  const int share = share_of(sp.n, a.split, BN);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+  const int D = FULL ? DP : (int)a.c.D;
+  const int rowb = D * BITS / 8;
+  const int half = 1 << (BITS - 1);
+  const int32_t* table = a.table + b * a.ldt;
+  const int ntile = (rows + BM - 1) / BM;
+
+  // the longest tiles (the last rows) first
+  for (int tile = ntile - 1 - tile0; tile >= 0; tile -= a.tiles) {
+    const int r0 = tile * BM, r = r0 + wave * 32 + lr;
+    const RowAt at = row_at(a, sp, h, min(r, rows - 1));
+    const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
+    const int first_all = min(sp.pos0 + r0 / a.G, sp.n - 1);  // seen by every row of the tile
+    const int last_all = min(sp.pos0 + (min(r0 + BM, rows) - 1) / a.G, sp.n - 1);
+    const int k0 = split * share, k1 = min(last_all + 1, k0 + share);
+    const int steps = k1 > k0 ? (k1 - k0 + BN - 1) / BN : 0;
+
+    // query fragments: chunk c = 2s + lh of keys' LDS rows holds channels 16c .. + 7
+    // for c < DP/16 and 16(c − DP/16) + 8 .. above
+    f16x8 qf[DP / 16];
+    float C;
+    {
+      float m = 0.f;
+      float v[8];
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const int c = 2 * s + lh, d = c < DP / 16 ? 16 * c : 16 * (c - DP / 16) + 8;
+        if (FULL || d < D) {
+          load_q8(a, at.token * a.qt + at.head * a.qh + d, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7fffffffu));
+        }
+      }
+      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 32))));
+      const RowScale rs = row_scale(m);
+      const float sign = a.scale < 0.f ? -rs.down : rs.down;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const int c = 2 * s + lh, d = c < DP / 16 ? 16 * c : 16 * (c - DP / 16) + 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        if (FULL || d < D) load_q8(a, at.token * a.qt + at.head * a.qh + d, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)(v[channel_of<BITS>(i)] * sign);
+      }
+      C = rs.up;
+    }
+
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[e][v] = 0.f;
+    float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
+    int bad = 0;
+
+    // Pieces of a step that a thread loads.  Keys: piece p = tid + i·NT, key p / (DP/16),
+    // 16 channels.  Values: bits of p from low to high: 3 of the 8-channel group, 1 half
+    // of the chunk, the group's other bits, 3 of the chunk (8 keys); with fewer pieces than
+    // threads the upper half of the workgroup takes them.
+    const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
+    uint32_t kw[KC][KW], vw[VQ][4][VW];
+    int kz[KC], vz[VQ][4];
+    float ssk = 0.f, ssv = 0.f;
+    bool sok = false;
+    constexpr int OH = DP / 64;  // 8-channel groups over 8
+    auto value_piece = [&](int i, int& o, int& key) __attribute__((always_inline)) {
+      const int p = tv + i * NT;
+      const int lo = p & 7, hf = (p >> 3) & 1, hi = (p >> 4) % OH, ch = (p >> 4) / OH;
+      o = lo + 8 * hi;
+      // chunk ch: keys 16(ch/2) + 4(ch%2) .. (first half) and + 8 (second half)
+      key = 16 * (ch >> 1) + 4 * (ch & 1) + 8 * hf;
+      return (ch << 1) | hf;
+    };
+    auto fetch = [&](int step) __attribute__((always_inline)) {
+      const int j0 = k0 + step * BN;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int p = tid + i * NT, key = j0 + p / (DP / 16), c = p % (DP / 16);
+        if (KP % NT && p >= KP) break;
+        const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
+        const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
+        const uint8_t* src = a.c.codes[0] + (int64_t)row * rowb + c * (2 * BITS);
+        if (!FULL && c * 16 >= D) src = a.c.codes[0];
+        if constexpr (BITS == 8) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          kw[i][0] = v.x, kw[i][1] = v.y, kw[i][2] = v.z, kw[i][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(src);
+          kw[i][0] = v.x, kw[i][1] = v.y;
+        }
+        kz[i] = a.c.zero[0] ? a.c.zero[0][row] : half;
+      }
+#pragma unroll
+      for (int i = 0; i < VQ; ++i) {
+        int o, k;
+        value_piece(i, o, k);
+        if (VP % NT && tv + i * NT >= VP) break;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int key = j0 + k + t;
+          const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
+          const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
+          const uint8_t* src = a.c.codes[1] + (int64_t)row * rowb + o * BITS;
+          if (!FULL && o * 8 >= D) src = a.c.codes[1];
+          if constexpr (BITS == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            vw[i][t][0] = v.x, vw[i][t][1] = v.y;
+          } else {
+            vw[i][t][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+          vz[i][t] = a.c.zero[1] ? a.c.zero[1][row] : half;
+        }
+      }
+      if (wave == 0) {
+        const int key = j0 + lane;
+        const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
+        bad |= slot == -2;
+        sok = slot >= 0;
+        const uint32_t row = sok ? (uint32_t)a.c.row(slot, h) : 0;
+        ssk = sok ? a.c.scale[0][row] * a.kscale : 0.f;
+        ssv = sok ? a.c.scale[1][row] : 0.f;
+      }
+    };
+    auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int p = tid + i * NT, key = p / (DP / 16), c = p % (DP / 16);
+        if (KP % NT && p >= KP) break;
+        const f16x2 zc = centre(kz[i], kz[i]);
+        _Float16* row = &kL[buf][key * DP];
+        *reinterpret_cast<f16x8*>(row + ((c ^ (key & 7)) << 3)) = key_codes<BITS>(&kw[i][0], zc);
+        *reinterpret_cast<f16x8*>(row + (((c + DP / 16) ^ (key & 7)) << 3)) =
+            key_codes<BITS>(&kw[i][KW / 2], zc);
+      }
+#pragma unroll
+      for (int i = 0; i < VQ; ++i) {
+        int o, k;
+        const int piece = value_piece(i, o, k), ch = piece >> 1, hf = piece & 1;
+        if (VP % NT && tv + i * NT >= VP) break;
+        const f16x2 z0 = centre(vz[i][0], vz[i][1]), z1 = centre(vz[i][2], vz[i][3]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const f16x2 x = value_codes<BITS>(vw[i][0], vw[i][1], e, z0);
+          const f16x2 y = value_codes<BITS>(vw[i][2], vw[i][3], e, z1);
+          const int d = o * 8 + e;
+          *reinterpret_cast<f16x4*>(&vL[buf][d * BN + ((ch ^ ((d ^ (d >> 3)) & 7)) << 3) + 4 * hf]) =
+              f16x4{x[0], x[1], y[0], y[1]};
+        }
+      }
+      if (wave == 0) {
+        skL[buf][lane] = ssk;
+        svL[buf][lane] = ssv;
+        float vx = ssv < __builtin_inff() ? ssv : 0.f;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) vx = fmaxf(vx, __shfl_xor(vx, o));
+        const uint64_t ok = __builtin_amdgcn_ballot_w64(sok);
+        if (lane == 0) vmaxL[buf] = vx, okL[buf] = ok;
+      }
+    };
+
+    if (steps > 0) fetch(0);
+    for (int step = 0; step < steps; ++step) {
+      const int buf = step & 1, j0 = k0 + step * BN;
+      put(buf);
+      if (step + 1 < steps) fetch(step + 1);
+      __syncthreads();
+      f32x16 x[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const int key = kb * 32 + lr;
+          const f16x8 kf = *reinterpret_cast<const f16x8*>(
+              &kL[buf][key * DP + (((2 * s + lh) ^ (key & 7)) << 3)]);
+          x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], x[kb], 0, 0, 0);
+        }
+      // element v of block kb: key 32kb + 8(v/4) + 4lh + v%4
+      const uint64_t ok = okL[buf];
+      const bool whole = ok == ~0ull && j0 + BN - 1 <= first_all;
+      float mx = m, vx = vmaxL[buf];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[buf][32 * kb + 8 * q + 4 * lh]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= sk[i];
+        }
+      if (whole) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, x[kb][v]);
+      } else {
+        vx = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int t = 32 * kb + 8 * (v >> 2) + 4 * lh + (v & 3);
+            const float sv = svL[buf][t];
+            if ((ok >> t & 1) && j0 + t <= last) {
+              mx = fmaxf(mx, x[kb][v]);
+              if (sv < __builtin_inff()) vx = fmaxf(vx, sv);
+            }
+          }
+        vx = fmaxf(vx, __shfl_xor(vx, 32));
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      if (__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0) {
+        const float nref = vx >= ref ? above(vx) : ref;
+        float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
+        if (m == mx) f = 1.f;
+        f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
+        m = mx, ref = nref;
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[e][v] *= f;
+      }
+      const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
+      f16x8 w[4];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 sv = *reinterpret_cast<const f32x4*>(&svL[buf][32 * kb + 8 * q + 4 * lh]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
+            float pv = p * sv[i];
+            if (!whole) {
+              const int t = 32 * kb + 8 * q + 4 * lh + i;
+              const bool see = (ok >> t & 1) && j0 + t <= last;
+              p = see ? p : 0.f;
+              pv = see ? pv : 0.f;
+            }
+            l += p;
+            w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)pv;
+          }
+        }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) {
+          const int d = e * 32 + lr;
+          const f16x8 vf = *reinterpret_cast<const f16x8*>(
+              &vL[buf][d * BN + (((2 * t + lh) ^ ((d ^ (d >> 3)) & 7)) << 3)]);
+          acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[t], acc[e], 0, 0, 0);
+        }
+    }
+    if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.f ? 0.f : 512.f / l;
+    if (r < rows) {
+      const int64_t row = (int64_t)at.token * a.Hq + at.head;
+      float* o = a.part + (row * a.split + split) * part_size(a);
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = e * 32 + 8 * q + 4 * lh;
+          if (!FULL && d >= D) continue;
+          const float y[4] = {acc[e][4 * q] * inv, acc[e][4 * q + 1] * inv,
+                              acc[e][4 * q + 2] * inv, acc[e][4 * q + 3] * inv};
+          if (a.split > 1)
+            *reinterpret_cast<float4*>(o + d) = make_float4(y[0], y[1], y[2], y[3]);
+          else
+            store_out(a, row * D + d, y);
+        }
+      if (a.split > 1 && lh == 0) {
+        o[D] = m == -INFINITY ? -INFINITY : m * C;
+        o[D + 1] = __builtin_amdgcn_ldexpf(l, exponent(ref) - 15);
       }
     }
+    __syncthreads();
   }
-  if (__any(bad) && lane == 0) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
-  for (int r = 0; r < 4; ++r) {
-    const int d = lane + 64 * r;
-    if (d >= D) break;
-    const float y = l == 0.f ? 0.f : o[r] / l;
-    const int64_t e = (t * a.Hq + hq) * D + d;
-    if (DT == 0) static_cast<uint16_t*>(a.out)[e] = __builtin_bit_cast(uint16_t, (__bf16)y);
-    else static_cast<_Float16*>(a.out)[e] = (_Float16)y;
+}
+
+// Joins the shares of a query row: one wave per (token, head).
+__global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.T * a.Hq) return;
+  const int lane = threadIdx.x & 63, t = (int)(row / a.Hq), hq = (int)(row % a.Hq);
+  const int b = (int)KvCache::sequence(a.cu, a.B, t);
+  if (b < 0) return;
+  Span sp;
+  sp.q0 = min(max(a.cu[b], 0), a.T);
+  sp.qlen = min(max(a.cu[b + 1], sp.q0), a.T) - sp.q0;
+  sp.pos0 = a.kv[b] - sp.qlen;
+  sp.n = a.c.pages == 0 ? 0 : (int)min<int64_t>(max(a.kv[b], 0), (int64_t)a.width << a.c.shift);
+  const int rows = sp.qlen * a.G, h = hq / a.G;
+  // which kernel had the row, and in how many shares
+  const bool by_rows = a.by_rows && (rows <= kFewRows || !a.by_tiles);
+  const int split = by_rows ? (rows <= kFewRows ? a.few_split : 1) : a.split;
+  if (split == 1) return;
+  const int r = (t - sp.q0) * a.G + hq - h * a.G;
+  const float* p = by_rows
+      ? a.few_part + (((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split * part_size(a)
+      : a.part + row * a.split * part_size(a);
+  const int D = (int)a.c.D;
+  const int64_t pitch = part_size(a);
+  float M = -INFINITY;
+  for (int s = 0; s < split; ++s) M = fmaxf(M, p[s * pitch + D]);
+  const int d = lane * 4;
+  float L = 0.f, y[4] = {0, 0, 0, 0};
+  for (int s = 0; s < split; ++s) {
+    const float m = p[s * pitch + D];
+    if (m == -INFINITY) {
+      // a share without keys adds nothing, unless its sum is NaN
+      L += p[s * pitch + D + 1];
+      continue;
+    }
+    const float w = __builtin_amdgcn_exp2f(m - M) * p[s * pitch + D + 1];
+    L += w;
+    if (d < D) {
+      const float4 o = *reinterpret_cast<const float4*>(p + s * pitch + d);
+      y[0] += w * o.x, y[1] += w * o.y, y[2] += w * o.z, y[3] += w * o.w;
+    }
   }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] *= inv;
+  if (d < D) store_out(a, row * D + d, y);
+}
+
+// ---------------------------------------------------------------------------
+// Launch
+// ---------------------------------------------------------------------------
+constexpr int64_t kCUs = 256;
+
+struct Plan {
+  bool few, tiles;     // which kernels run
+  int nw;              // waves of a tile's workgroup
+  int64_t ntiles, split, few_split;
+  int64_t part, few_part;  // bytes of partial results
+  Plan(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t max_q, int64_t max_kv) {
+    const int64_t G = Hq / H, rows = max_q * G, pairs = std::max<int64_t>(1, B * H);
+    tiles = rows > kFewRows;
+    // a batch of chunks only has sequences of few rows if some are shorter than the rest
+    few = !tiles || B > 1;
+    const int64_t keys = std::max<int64_t>(1, max_kv);
+    // few rows: two workgroups per CU, shares of 256 keys at least
+    few_split = std::max<int64_t>(1, std::min(cdiv(4 * kCUs, pairs), keys / 256));
+    few_split = std::min<int64_t>(few_split, 64);
+    nw = rows > 192 ? 8 : rows > 64 ? 4 : 2;
+    if (D > 128) nw = rows > 64 ? 4 : 2;
+    ntiles = std::max<int64_t>(1, cdiv(rows, 32 * nw));
+    split = std::max<int64_t>(1, std::min(2 * kCUs / (pairs * ntiles), keys / 256));
+    split = std::min<int64_t>(split, 32);
+    part = tiles && split > 1 ? cdiv(T * Hq * split * (D + 4) * 4, 256) * 256 : 0;
+    few_part = few && few_split > 1
+                   ? cdiv(B * H * kFewRows * few_split * (D + 4) * 4, 256) * 256 : 0;
+  }
+};
+
+template <int BITS, int DP, bool FULL>
+int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
+  if (p.few) {
+    hipLaunchKernelGGL((attend_rows_kernel<BITS, DP, FULL>),
+                       dim3((unsigned)p.few_split, (unsigned)a.c.H, (unsigned)a.B + 1), dim3(256),
+                       0, st, a);
+    G2PTQ_LAUNCHED();
+  }
+  if (p.tiles) {
+    const dim3 grid((unsigned)(a.B * a.c.H * a.split * a.tiles + 1));
+#define G2_AT(NW)                                                                             \
+  hipLaunchKernelGGL((attend_tiles_kernel<BITS, DP, FULL, NW>), grid, dim3(64 * NW), 0, st, a)
+    if constexpr (DP <= 128) {
+      if (p.nw == 8) G2_AT(8);
+      else if (p.nw == 4) G2_AT(4);
+      else G2_AT(2);
+    } else {
+      if (p.nw == 4) G2_AT(4);
+      else G2_AT(2);
+    }
+#undef G2_AT
+    G2PTQ_LAUNCHED();
+  }
+  if (a.part || a.few_part) {
+    hipLaunchKernelGGL(attend_join_kernel, dim3((unsigned)cdiv((int64_t)a.T * a.Hq, 4)), dim3(256),
+                       0, st, a);
+    G2PTQ_LAUNCHED();
+  }
+  return G2PTQ_OK;
 }
 
 }  // namespace
@@ -112,7 +913,8 @@ extern "C" int g2ptq_paged_attention_workspace(int64_t T, int64_t Hq, int64_t kv
   G2PTQ_CHECK(bytes && T >= 0 && Hq >= 1 && kv_heads >= 1 && Hq % kv_heads == 0 && dim >= 16 &&
                   B >= 0 && max_q >= 0 && max_kv >= 0,
               "paged_attention_workspace: bad sizes");
-  *bytes = 0;
+  const Plan p(T, Hq, kv_heads, dim, B, max_q, max_kv);
+  *bytes = (size_t)(p.part + p.few_part);
   return G2PTQ_OK;
 }
 
@@ -130,18 +932,45 @@ extern "C" int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, 
               (long long)a.c.H);
   G2PTQ_CHECK(T >= 0 && T * Hq < (1ll << 31), "paged_attention: %lld tokens of %lld heads",
               (long long)T, (long long)Hq);
-  G2PTQ_CHECK(B >= 0 && B <= 65535 && width >= 0 && ldt >= width && max_q >= 0 && max_kv >= 0,
-              "paged_attention: bad page table");
+  G2PTQ_CHECK(B >= 0 && B < 65535 && width >= 0 && width < (1ll << 31) && ldt >= width &&
+                  max_q >= 0 && max_q <= T && max_kv >= 0,
+              "paged_attention: bad page table or sizes");
   if (T == 0) return G2PTQ_OK;
+  G2PTQ_CHECK(width << a.c.shift <= 1ll << 30,
+              "paged_attention: sequences of up to %lld keys (at most 2^30)",
+              (long long)(width << a.c.shift));
   G2PTQ_CHECK(q && out && (B == 0 || (cu_q && kv_lens)) && (table || B * width == 0),
               "paged_attention: null pointer");
-  a.q = q, a.qt = q_token, a.qh = q_head, a.out = out, a.T = T, a.Hq = Hq, a.B = B, a.ldt = ldt;
-  a.width = width, a.table = table, a.cu = cu_q, a.kv = kv_lens, a.scale = scale;
-  const dim3 grid((unsigned)(T * Hq));
-  if (dtype == 0)
-    hipLaunchKernelGGL(attention_simple_kernel<0>, grid, dim3(64), 0, as_stream(stream), a);
-  else
-    hipLaunchKernelGGL(attention_simple_kernel<1>, grid, dim3(64), 0, as_stream(stream), a);
-  G2PTQ_LAUNCHED();
-  return G2PTQ_OK;
+  G2PTQ_CHECK((reinterpret_cast<uintptr_t>(out) & 15) == 0,
+              "paged_attention: output not 16-byte aligned");
+  const Plan p(T, Hq, a.c.H, a.c.D, B, max_q, max_kv);
+  G2PTQ_CHECK(B * a.c.H * p.split * p.ntiles < (1ll << 31) - 1, "paged_attention: batch too large");
+  const size_t need = (size_t)(p.part + p.few_part);
+  if (need && (!ws || ws_bytes < need)) {
+    set_error("paged_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    return G2PTQ_ERR_WORKSPACE;
+  }
+  G2PTQ_CHECK(!need || (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
+              "paged_attention: workspace not 16-byte aligned");
+  a.q = q, a.qt = q_token, a.qh = q_head, a.out = out, a.ldt = ldt;
+  a.table = table, a.cu = cu_q, a.kv = kv_lens;
+  a.T = (int)T, a.Hq = (int)Hq, a.B = (int)B, a.G = (int)(Hq / a.c.H), a.width = (int)width;
+  a.dtype = dtype;
+  a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_token % 8 == 0 && q_head % 8 == 0;
+  a.scale = scale, a.kscale = fabsf(scale) * 1.44269504088896340736f * 512.f;
+  a.tiles = (int)p.ntiles, a.split = (int)p.split, a.few_split = (int)p.few_split;
+  a.by_rows = p.few, a.by_tiles = p.tiles;
+  a.part = p.part ? static_cast<float*>(ws) : nullptr;
+  a.few_part = p.few_part ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.part) : nullptr;
+  hipStream_t st = as_stream(stream);
+  const int64_t D = a.c.D;
+#define G2_DIM(BITS)                                        \
+  if (D == 64) return launch<BITS, 64, true>(st, a, p);     \
+  if (D < 64) return launch<BITS, 64, false>(st, a, p);     \
+  if (D == 128) return launch<BITS, 128, true>(st, a, p);   \
+  if (D < 128) return launch<BITS, 128, false>(st, a, p);   \
+  return launch<BITS, 256, false>(st, a, p)
+  if (a.c.bits == 8) { G2_DIM(8); }
+  G2_DIM(4);
+#undef G2_DIM
 }

@@ -133,6 +133,9 @@ int check_cache(const char* who, const g2ptq_kv_cache* c, KvCache& k) {
               "%s: head dimension %lld (a multiple of 16 up to 256)", who, (long long)c->dim);
   G2PTQ_CHECK(c->page >= 1 && c->page <= 4096 && (c->page & (c->page - 1)) == 0,
               "%s: pages of %lld slots (a power of two up to 4096)", who, (long long)c->page);
+  G2PTQ_CHECK(c->pages * c->heads * c->page < (1ll << 31),
+              "%s: %lld pages of %lld heads of %lld slots (fewer than 2^31 in all)", who,
+              (long long)c->pages, (long long)c->heads, (long long)c->page);
   G2PTQ_CHECK(c->flags, "%s: null flags", who);
   G2PTQ_CHECK(c->pages == 0 || (c->k_codes && c->v_codes && c->k_scale && c->v_scale),
               "%s: null cache buffer", who);
