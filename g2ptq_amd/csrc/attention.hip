@@ -139,13 +139,15 @@ __device__ __forceinline__ float above(float x) {
 }
 __device__ __forceinline__ int exponent(float p) { return (int)(__float_as_uint(p) >> 23) - 127; }
 
-// Power of two that brings a query row with largest |q| = m into [1, 2), and its
-// inverse.
+// Power of two that brings a query row into [1, 2) and its inverse, from the row's
+// largest |q| (16 bits of the query's type in the high half of m).
 struct RowScale {
   float down, up;
 };
-__device__ __forceinline__ RowScale row_scale(float m) {
-  uint32_t e = __float_as_uint(m) >> 23;
+__device__ __forceinline__ RowScale row_scale(int dtype, uint32_t m) {
+  const float x = dtype == 0 ? __uint_as_float(m)
+                             : (float)__builtin_bit_cast(_Float16, (uint16_t)(m >> 16));
+  uint32_t e = __float_as_uint(x) >> 23;
   e = e >= 255 ? 127 : min(max(e, 1u), 253u);  // a NaN or infinite row stays one as it is
   return {__uint_as_float((254 - e) << 23), __uint_as_float(e << 23)};
 }
@@ -174,9 +176,53 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, const f
     *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
 }
 
-__device__ __forceinline__ void load_q8(const AttnArgs& a, int64_t at, float (&v)[8]) {
-  if (a.dtype == 0) load8<0>(a.q, at, a.vec, 8, v);
-  else load8<1>(a.q, at, a.vec, 8, v);
+// Pieces of eight channels of a query row as they are, piece s from channel
+// channel(s) (zeros from channel D up).
+template <int N, typename F>
+__device__ __forceinline__ void load_query(const AttnArgs& a, int64_t at, uint4 (&raw)[N], int D,
+                                           F channel) {
+  const uint16_t* x = static_cast<const uint16_t*>(a.q) + at;
+#pragma unroll
+  for (int s = 0; s < N; ++s) raw[s] = make_uint4(0, 0, 0, 0);
+  if (a.vec) {
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+      if (channel(s) < D) raw[s] = *reinterpret_cast<const uint4*>(x + channel(s));
+  } else {
+#pragma nounroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int s = 0; s < N; ++s)
+        if (channel(s) < D) {
+          const uint16_t* y = x + channel(s) + 2 * i;
+          const uint32_t w = y[0] | (uint32_t)y[1] << 16;
+          raw[s].x = i == 0 ? w : raw[s].x, raw[s].y = i == 1 ? w : raw[s].y;
+          raw[s].z = i == 2 ? w : raw[s].z, raw[s].w = i == 3 ? w : raw[s].w;
+        }
+    }
+  }
+}
+
+// Scaled (and negated for a negative scale of the logits) to fp16, in the order of
+// key_codes.
+template <int BITS>
+__device__ __forceinline__ f16x8 scaled_query(const AttnArgs& a, uint4 raw, float down) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  const float f = a.scale < 0.f ? -down : down;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (a.dtype == 0) {
+      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+      v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+    }
+  }
+  f16x8 h;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = (_Float16)(v[channel_of<BITS>(i)] * f);
+  return h;
 }
 
 // A partial result: the row's output over a share of the keys (D floats), its
@@ -251,28 +297,22 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
     f16x8 qf[KS];
     float C;
     {
-      float v[KS][8], m = 0.f;
+      uint4 raw[KS];
+      uint32_t top = 0;
+      load_query<KS>(a, at.token * a.qt + at.head * a.qh, raw, D,
+                     [&](int s) { return g * DG + 8 * s; });
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const int d = g * DG + 8 * s;
-        if (FULL || d < D) {
-          load_q8(a, at.token * a.qt + at.head * a.qh + d, v[s]);
-        } else {
+        const uint32_t w[4] = {raw[s].x, raw[s].y, raw[s].z, raw[s].w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[s][i]) & 0x7fffffffu));
+        for (int i = 0; i < 4; ++i)
+          top = max(top, max(w[i] << 16 & 0x7fff0000u, w[i] & 0x7fff0000u));
       }
-      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 16))));
-      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 32))));
-      const RowScale rs = row_scale(m);
-      const float sign = a.scale < 0.f ? -rs.down : rs.down;
+      top = max(top, __shfl_xor(top, 16));
+      top = max(top, __shfl_xor(top, 32));
+      const RowScale rs = row_scale(a.dtype, top);
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)(v[s][channel_of<BITS>(i)] * sign);
+      for (int s = 0; s < KS; ++s) qf[s] = scaled_query<BITS>(a, raw[s], rs.down);
       C = rs.up;
     }
 
@@ -362,10 +402,8 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
             const bool see = (ok >> t & 1) && j0 + t <= last;
             p[4 * kb + i] = x[i] * sk[i];
             sv[4 * kb + i] = s4[i];
-            if (see) {
-              mx = fmaxf(mx, p[4 * kb + i]);
-              if (s4[i] < __builtin_inff()) vx = fmaxf(vx, s4[i]);
-            }
+            mx = fmaxf(mx, see ? p[4 * kb + i] : -INFINITY);
+            vx = fmaxf(vx, see && s4[i] < __builtin_inff() ? s4[i] : 0.f);
           }
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -467,7 +505,8 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // rows, 32 per wave, through 64 keys at a time.  The keys and values of a step are
 // converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
 // transposed as [channel][key]; the codes of the next step are loaded meanwhile (two
-// buffers, one barrier a step).  v_mfma_f32_32x32x16_f16:
+// buffers, one barrier a step).  The first wave looks up a step's pages, scales and
+// zero points two steps ahead (three buffers).  v_mfma_f32_32x32x16_f16:
 //   S^T (32 keys × 32 rows) = K·Q^T, so that a lane holds one row's logits (row =
 //     lane % 32, the other half of the keys in lane + 32) and its statistics;
 //   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
@@ -482,10 +521,14 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   constexpr int KP = BN * (DP / 16), KC = (KP + NT - 1) / NT;      // 16-channel pieces of keys
   constexpr int VP = BN / 4 * (DP / 8), VQ = (VP + NT - 1) / NT;   // 4-key × 8-channel of values
   constexpr int KW = BITS / 2, VW = BITS / 4;   // words of 16 and of 8 channels
-  __shared__ __attribute__((aligned(16))) _Float16 kL[2][BN * DP], vL[2][DP * BN];
-  __shared__ __attribute__((aligned(16))) float skL[2][BN], svL[2][BN];
-  __shared__ float vmaxL[2];
-  __shared__ uint64_t okL[2];
+  constexpr int KB = BN * DP * 2;               // bytes of a step's keys, and of its values
+  __shared__ __attribute__((aligned(16))) char kvL[4 * KB];  // keys 0, keys 1, values 0, values 1
+  __shared__ __attribute__((aligned(16))) float skL[3][BN], svL[3][BN];
+  __shared__ __attribute__((aligned(16))) uint32_t rowL[3][BN];
+  __shared__ uint32_t zkL[3][BN];  // −z·2^-9 in fp16, twice
+  __shared__ __attribute__((aligned(16))) _Float16 zvL[3][BN];
+  __shared__ float vmaxL[3];
+  __shared__ uint64_t okL[3];
 
   // Workgroups go round the 8 XCDs; number them so that an XCD takes a contiguous
   // range: the row tiles of one sequence and head share its keys in one L2.
@@ -508,12 +551,20 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   const int rows = sp.qlen * a.G;
   if (rows == 0 || (a.by_rows && rows <= kFewRows)) return;
   const int share = share_of(sp.n, a.split, BN);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = FULL ? DP : (int)a.c.D;
-  const int rowb = D * BITS / 8;
+  const uint32_t rowb = D * BITS / 8;
   const int half = 1 << (BITS - 1);
   const int32_t* table = a.table + b * a.ldt;
   const int ntile = (rows + BM - 1) / BM;
+
+  // Keys: piece p = tid + i·NT is 16 channels c of key p / (DP/16).  Values: bits of a
+  // piece from low to high: 3 of the 8-channel group, 1 half of the chunk (8 keys), the
+  // group's other bits, 3 of the chunk; with fewer pieces than threads the upper half
+  // of the workgroup takes them.
+  const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
+  constexpr int OH = DP / 64;  // 8-channel groups over 8
 
   // the longest tiles (the last rows) first
   for (int tile = ntile - 1 - tile0; tile >= 0; tile -= a.tiles) {
@@ -530,30 +581,22 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     f16x8 qf[DP / 16];
     float C;
     {
-      float m = 0.f;
-      float v[8];
+      uint4 raw[DP / 16];
+      uint32_t m = 0;
+      load_query<DP / 16>(a, at.token * a.qt + at.head * a.qh, raw, D, [&](int s) {
+        const int c = 2 * s + lh;
+        return c < DP / 16 ? 16 * c : 16 * (c - DP / 16) + 8;
+      });
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
-        const int c = 2 * s + lh, d = c < DP / 16 ? 16 * c : 16 * (c - DP / 16) + 8;
-        if (FULL || d < D) {
-          load_q8(a, at.token * a.qt + at.head * a.qh + d, v);
+        const uint32_t w[4] = {raw[s].x, raw[s].y, raw[s].z, raw[s].w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7fffffffu));
-        }
+        for (int i = 0; i < 4; ++i) m = max(m, max(w[i] << 16 & 0x7fff0000u, w[i] & 0x7fff0000u));
       }
-      m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(__shfl_xor(m, 32))));
-      const RowScale rs = row_scale(m);
-      const float sign = a.scale < 0.f ? -rs.down : rs.down;
+      m = max(m, __shfl_xor(m, 32));
+      const RowScale rs = row_scale(a.dtype, m);
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        const int c = 2 * s + lh, d = c < DP / 16 ? 16 * c : 16 * (c - DP / 16) + 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        if (FULL || d < D) load_q8(a, at.token * a.qt + at.head * a.qh + d, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)(v[channel_of<BITS>(i)] * sign);
-      }
+      for (int s = 0; s < DP / 16; ++s) qf[s] = scaled_query<BITS>(a, raw[s], rs.down);
       C = rs.up;
     }
 
@@ -565,117 +608,133 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
     int bad = 0;
 
-    // Pieces of a step that a thread loads.  Keys: piece p = tid + i·NT, key p / (DP/16),
-    // 16 channels.  Values: bits of p from low to high: 3 of the 8-channel group, 1 half
-    // of the chunk, the group's other bits, 3 of the chunk (8 keys); with fewer pieces than
-    // threads the upper half of the workgroup takes them.
-    const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
-    uint32_t kw[KC][KW], vw[VQ][4][VW];
-    int kz[KC], vz[VQ][4];
-    float ssk = 0.f, ssv = 0.f;
+    // first wave: page of key `lane` of a step (−1: none), then its row and numbers
+    int page = -1;
+#define G2_PAGE(step)                                                          \
+  do {                                                                         \
+    const int key_ = k0 + (step) * BN + lane;                                  \
+    page = -1;                                                                 \
+    if (key_ < k1) page = table[key_ >> a.c.shift];                            \
+  } while (0)
     bool sok = false;
-    constexpr int OH = DP / 64;  // 8-channel groups over 8
-    auto value_piece = [&](int i, int& o, int& key) __attribute__((always_inline)) {
-      const int p = tv + i * NT;
-      const int lo = p & 7, hf = (p >> 3) & 1, hi = (p >> 4) % OH, ch = (p >> 4) / OH;
-      o = lo + 8 * hi;
-      // chunk ch: keys 16(ch/2) + 4(ch%2) .. (first half) and + 8 (second half)
-      key = 16 * (ch >> 1) + 4 * (ch & 1) + 8 * hf;
-      return (ch << 1) | hf;
-    };
-    auto fetch = [&](int step) __attribute__((always_inline)) {
-      const int j0 = k0 + step * BN;
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int p = tid + i * NT, key = j0 + p / (DP / 16), c = p % (DP / 16);
-        if (KP % NT && p >= KP) break;
-        const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
-        const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
-        const uint8_t* src = a.c.codes[0] + (int64_t)row * rowb + c * (2 * BITS);
-        if (!FULL && c * 16 >= D) src = a.c.codes[0];
-        if constexpr (BITS == 8) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src);
-          kw[i][0] = v.x, kw[i][1] = v.y, kw[i][2] = v.z, kw[i][3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(src);
-          kw[i][0] = v.x, kw[i][1] = v.y;
-        }
-        kz[i] = a.c.zero[0] ? a.c.zero[0][row] : half;
-      }
-#pragma unroll
-      for (int i = 0; i < VQ; ++i) {
-        int o, k;
-        value_piece(i, o, k);
-        if (VP % NT && tv + i * NT >= VP) break;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int key = j0 + k + t;
-          const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
-          const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
-          const uint8_t* src = a.c.codes[1] + (int64_t)row * rowb + o * BITS;
-          if (!FULL && o * 8 >= D) src = a.c.codes[1];
-          if constexpr (BITS == 8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(src);
-            vw[i][t][0] = v.x, vw[i][t][1] = v.y;
-          } else {
-            vw[i][t][0] = *reinterpret_cast<const uint32_t*>(src);
-          }
-          vz[i][t] = a.c.zero[1] ? a.c.zero[1][row] : half;
-        }
-      }
-      if (wave == 0) {
-        const int key = j0 + lane;
-        const int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
-        bad |= slot == -2;
-        sok = slot >= 0;
-        const uint32_t row = sok ? (uint32_t)a.c.row(slot, h) : 0;
-        ssk = sok ? a.c.scale[0][row] * a.kscale : 0.f;
-        ssv = sok ? a.c.scale[1][row] : 0.f;
-      }
-    };
-    auto put = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int p = tid + i * NT, key = p / (DP / 16), c = p % (DP / 16);
-        if (KP % NT && p >= KP) break;
-        const f16x2 zc = centre(kz[i], kz[i]);
-        _Float16* row = &kL[buf][key * DP];
-        *reinterpret_cast<f16x8*>(row + ((c ^ (key & 7)) << 3)) = key_codes<BITS>(&kw[i][0], zc);
-        *reinterpret_cast<f16x8*>(row + (((c + DP / 16) ^ (key & 7)) << 3)) =
-            key_codes<BITS>(&kw[i][KW / 2], zc);
-      }
-#pragma unroll
-      for (int i = 0; i < VQ; ++i) {
-        int o, k;
-        const int piece = value_piece(i, o, k), ch = piece >> 1, hf = piece & 1;
-        if (VP % NT && tv + i * NT >= VP) break;
-        const f16x2 z0 = centre(vz[i][0], vz[i][1]), z1 = centre(vz[i][2], vz[i][3]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const f16x2 x = value_codes<BITS>(vw[i][0], vw[i][1], e, z0);
-          const f16x2 y = value_codes<BITS>(vw[i][2], vw[i][3], e, z1);
-          const int d = o * 8 + e;
-          *reinterpret_cast<f16x4*>(&vL[buf][d * BN + ((ch ^ ((d ^ (d >> 3)) & 7)) << 3) + 4 * hf]) =
-              f16x4{x[0], x[1], y[0], y[1]};
-        }
-      }
-      if (wave == 0) {
-        skL[buf][lane] = ssk;
-        svL[buf][lane] = ssv;
-        float vx = ssv < __builtin_inff() ? ssv : 0.f;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) vx = fmaxf(vx, __shfl_xor(vx, o));
-        const uint64_t ok = __builtin_amdgcn_ballot_w64(sok);
-        if (lane == 0) vmaxL[buf] = vx, okL[buf] = ok;
-      }
-    };
+    uint32_t srow = 0;
+    float ssk = 0.f, ssv = 0.f;
+    int szk = half, szv = half;
+#define G2_META(step)                                                          \
+  do {                                                                         \
+    const int key_ = k0 + (step) * BN + lane;                                  \
+    sok = key_ < k1 && page >= 0 && page < a.c.pages;                          \
+    bad |= key_ < k1 && !sok;                                                  \
+    srow = sok ? (uint32_t)a.c.row((int64_t)page << a.c.shift |                \
+                                   (key_ & ((1 << a.c.shift) - 1)), h) : 0;    \
+    ssk = sok ? a.c.scale[0][srow] : 0.f;                                      \
+    ssv = sok ? a.c.scale[1][srow] : 0.f;                                      \
+    if (a.c.zero[0]) szk = a.c.zero[0][srow], szv = a.c.zero[1][srow];         \
+  } while (0)
+#define G2_SHOW(at3)                                                           \
+  do {                                                                         \
+    skL[at3][lane] = ssk * a.kscale;                                           \
+    svL[at3][lane] = ssv;                                                      \
+    rowL[at3][lane] = srow;                                                    \
+    zkL[at3][lane] = __builtin_bit_cast(uint32_t, centre(szk, szk));           \
+    zvL[at3][lane] = centre(szv, szv)[0];                                      \
+    float vx_ = ssv < __builtin_inff() ? ssv : 0.f;                            \
+    _Pragma("unroll") for (int o_ = 32; o_ > 0; o_ >>= 1)                      \
+      vx_ = fmaxf(vx_, __shfl_xor(vx_, o_));                                   \
+    const uint64_t ok_ = __builtin_amdgcn_ballot_w64(sok);                     \
+    if (lane == 0) vmaxL[at3] = vx_, okL[at3] = ok_;                           \
+  } while (0)
+    uint32_t kw[KC][KW], vw[VQ][4][VW];
+#define G2_FETCH(at3)                                                                        \
+  do {                                                                                       \
+    _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
+      const int p_ = tid + i * NT, c_ = p_ % (DP / 16);                                      \
+      if (KP % NT && p_ >= KP) break;                                                        \
+      const uint8_t* s_ = a.c.codes[0];                                                      \
+      if (FULL || c_ * 16 < D)                                                               \
+        s_ += (uint64_t)rowL[at3][p_ / (DP / 16)] * rowb + c_ * (2 * BITS);                  \
+      if constexpr (BITS == 8) {                                                             \
+        const uint4 v_ = *reinterpret_cast<const uint4*>(s_);                                \
+        kw[i][0] = v_.x, kw[i][1] = v_.y, kw[i][2] = v_.z, kw[i][3] = v_.w;                  \
+      } else {                                                                               \
+        const uint2 v_ = *reinterpret_cast<const uint2*>(s_);                                \
+        kw[i][0] = v_.x, kw[i][1] = v_.y;                                                    \
+      }                                                                                      \
+    }                                                                                        \
+    _Pragma("unroll") for (int i = 0; i < VQ; ++i) {                                         \
+      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH; \
+      if (VP % NT && p_ >= VP) break;                                                        \
+      const uint4 r_ = *reinterpret_cast<const uint4*>(                                      \
+          &rowL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * ((p_ >> 3) & 1)]);                \
+      const uint32_t row_[4] = {r_.x, r_.y, r_.z, r_.w};                                     \
+      _Pragma("unroll") for (int t = 0; t < 4; ++t) {                                        \
+        const uint8_t* s_ = a.c.codes[1];                                                    \
+        if (FULL || o_ * 8 < D) s_ += (uint64_t)row_[t] * rowb + o_ * BITS;                  \
+        if constexpr (BITS == 8) {                                                           \
+          const uint2 v_ = *reinterpret_cast<const uint2*>(s_);                              \
+          vw[i][t][0] = v_.x, vw[i][t][1] = v_.y;                                            \
+        } else {                                                                             \
+          vw[i][t][0] = *reinterpret_cast<const uint32_t*>(s_);                              \
+        }                                                                                    \
+      }                                                                                      \
+    }                                                                                        \
+  } while (0)
+#define G2_PUT(kbase, vbase, at3)                                                            \
+  do {                                                                                       \
+    _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
+      const int p_ = tid + i * NT, key_ = p_ / (DP / 16), c_ = p_ % (DP / 16);               \
+      if (KP % NT && p_ >= KP) break;                                                        \
+      const f16x2 zc_ = as_h2(zkL[at3][key_]);                                               \
+      char* row_ = (kbase) + key_ * (DP * 2);                                                \
+      *reinterpret_cast<f16x8*>(row_ + ((c_ ^ (key_ & 7)) << 4)) =                           \
+          key_codes<BITS>(&kw[i][0], zc_);                                                   \
+      *reinterpret_cast<f16x8*>(row_ + (((c_ + DP / 16) ^ (key_ & 7)) << 4)) =               \
+          key_codes<BITS>(&kw[i][KW / 2], zc_);                                              \
+    }                                                                                        \
+    _Pragma("unroll") for (int i = 0; i < VQ; ++i) {                                         \
+      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH; \
+      const int hf_ = (p_ >> 3) & 1;                                                         \
+      if (VP % NT && p_ >= VP) break;                                                        \
+      const f16x4 z_ = *reinterpret_cast<const f16x4*>(                                      \
+          &zvL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * hf_]);                             \
+      const f16x2 z0_ = {z_[0], z_[1]}, z1_ = {z_[2], z_[3]};                                \
+      _Pragma("unroll") for (int e = 0; e < 8; ++e) {                                        \
+        const f16x2 x_ = value_codes<BITS>(vw[i][0], vw[i][1], e, z0_);                      \
+        const f16x2 y_ = value_codes<BITS>(vw[i][2], vw[i][3], e, z1_);                      \
+        const int d_ = o_ * 8 + e;                                                           \
+        *reinterpret_cast<f16x4*>((vbase) + d_ * (BN * 2) + 8 * hf_ +                        \
+                                  ((ch_ ^ ((d_ ^ (d_ >> 3)) & 7)) << 4)) =                   \
+            f16x4{x_[0], x_[1], y_[0], y_[1]};                                               \
+      }                                                                                      \
+    }                                                                                        \
+  } while (0)
 
-    if (steps > 0) fetch(0);
-    for (int step = 0; step < steps; ++step) {
-      const int buf = step & 1, j0 = k0 + step * BN;
-      put(buf);
-      if (step + 1 < steps) fetch(step + 1);
+    if (steps > 0) {
+      if (wave == 0) {
+        G2_PAGE(0);
+        G2_META(0);
+        G2_SHOW(0);
+        G2_PAGE(1);
+        G2_META(1);
+        G2_SHOW(1);
+        G2_PAGE(2);
+      }
       __syncthreads();
+      G2_FETCH(0);
+    }
+    int at3 = 0;  // step % 3
+    for (int step = 0; step < steps; ++step) {
+      const int j0 = k0 + step * BN;
+      const int next3 = at3 == 2 ? 0 : at3 + 1, last3 = next3 == 2 ? 0 : next3 + 1;
+      char* kbase = kvL + (step & 1) * KB;
+      char* vbase = kvL + (2 + (step & 1)) * KB;
+      G2_PUT(kbase, vbase, at3);
+      __syncthreads();
+      if (step + 1 < steps) G2_FETCH(next3);
+      if (wave == 0) {
+        G2_META(step + 2);
+        G2_PAGE(step + 3);
+      }
       f32x16 x[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -685,40 +744,47 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const int key = kb * 32 + lr;
           const f16x8 kf = *reinterpret_cast<const f16x8*>(
-              &kL[buf][key * DP + (((2 * s + lh) ^ (key & 7)) << 3)]);
+              kbase + kb * 32 * (DP * 2) + (lr * (DP * 2) + (((2 * s + lh) ^ (lr & 7)) << 4)));
           x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], x[kb], 0, 0, 0);
         }
+      __builtin_amdgcn_sched_barrier(0);
       // element v of block kb: key 32kb + 8(v/4) + 4lh + v%4
-      const uint64_t ok = okL[buf];
+      const float* sk = &skL[at3][4 * lh];
+      const float* sv = &svL[at3][4 * lh];
+      const uint64_t ok = okL[at3];
       const bool whole = ok == ~0ull && j0 + BN - 1 <= first_all;
-      float mx = m, vx = vmaxL[buf];
+      float mx = m, vx = vmaxL[at3];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[buf][32 * kb + 8 * q + 4 * lh]);
+          const f32x4 s4 = *reinterpret_cast<const f32x4*>(sk + 32 * kb + 8 * q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= sk[i];
+          for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
         }
+      // keys that the lane's row sees, bit 8q + i of word kb: element 4q + i of block kb
+      uint32_t see[2] = {~0u, ~0u};
       if (whole) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int v = 0; v < 16; ++v) mx = fmaxf(mx, x[kb][v]);
       } else {
+        const int n = last - j0;  // the last key seen
+        const uint64_t seen = n < 0 ? 0 : n >= 63 ? ok : ok & ((2ull << n) - 1);
+        see[0] = (uint32_t)seen >> (4 * lh);
+        see[1] = (uint32_t)(seen >> 32) >> (4 * lh);
         vx = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int t = 32 * kb + 8 * (v >> 2) + 4 * lh + (v & 3);
-            const float sv = svL[buf][t];
-            if ((ok >> t & 1) && j0 + t <= last) {
-              mx = fmaxf(mx, x[kb][v]);
-              if (sv < __builtin_inff()) vx = fmaxf(vx, sv);
-            }
+            const int t = 8 * (v >> 2) + (v & 3);
+            const float s1 = sv[32 * kb + t];
+            const bool on = see[kb] >> t & 1;
+            mx = fmaxf(mx, on ? x[kb][v] : -INFINITY);
+            vx = fmaxf(vx, on && s1 < __builtin_inff() ? s1 : 0.f);
           }
         vx = fmaxf(vx, __shfl_xor(vx, 32));
       }
@@ -737,35 +803,52 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       }
       const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
       f16x8 w[4];
+      if (whole) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 sv = *reinterpret_cast<const f32x4*>(&svL[buf][32 * kb + 8 * q + 4 * lh]);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
-            float pv = p * sv[i];
-            if (!whole) {
-              const int t = 32 * kb + 8 * q + 4 * lh + i;
-              const bool see = (ok >> t & 1) && j0 + t <= last;
-              p = see ? p : 0.f;
-              pv = see ? pv : 0.f;
+            for (int i = 0; i < 4; ++i) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
+              l += p;
+              w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
             }
-            l += p;
-            w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)pv;
           }
-        }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool on = see[kb] >> (8 * q + i) & 1;
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
+              l += on ? p : 0.f;
+              w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
+            }
+          }
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) {
-          const int d = e * 32 + lr;
-          const f16x8 vf = *reinterpret_cast<const f16x8*>(
-              &vL[buf][d * BN + (((2 * t + lh) ^ ((d ^ (d >> 3)) & 7)) << 3)]);
+          // f(d) of d = 32e + lr is f(lr) ^ 4(e % 2)
+          const int c = (2 * t + lh) ^ ((lr ^ (lr >> 3)) & 7) ^ (4 * (e & 1));
+          const f16x8 vf =
+              *reinterpret_cast<const f16x8*>(vbase + e * 32 * (BN * 2) + (lr * (BN * 2) + (c << 4)));
           acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[t], acc[e], 0, 0, 0);
         }
+      if (wave == 0) G2_SHOW(last3);
+      at3 = next3;
     }
+#undef G2_PAGE
+#undef G2_META
+#undef G2_SHOW
+#undef G2_FETCH
+#undef G2_PUT
     if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
     l += __shfl_xor(l, 32);
     const float inv = l == 0.f ? 0.f : 512.f / l;
