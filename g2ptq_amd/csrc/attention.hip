@@ -515,6 +515,19 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // 16-byte chunks of LDS rows are placed at chunk ^ f(row), which keeps fragment
 // reads (8 consecutive rows, one chunk) and writes free of bank conflicts.
 // ---------------------------------------------------------------------------
+// Schedule of N products with one LDS fragment each: four reads ahead of them.
+template <int N>
+__device__ __forceinline__ void ahead_of_products() {
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - 4; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int BITS, int DP, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
@@ -724,6 +737,11 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     }
     int at3 = 0;  // step % 3
     for (int step = 0; step < steps; ++step) {
+      // (opaque: addresses kept over the whole loop cost more registers than there are)
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+      const int lane = tid & 63, lr = lane & 31, lh = lane >> 5;
+      const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
       const int j0 = k0 + step * BN;
       const int next3 = at3 == 2 ? 0 : at3 + 1, last3 = next3 == 2 ? 0 : next3 + 1;
       char* kbase = kvL + (step & 1) * KB;
@@ -740,6 +758,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
@@ -748,7 +767,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               kbase + kb * 32 * (DP * 2) + (lr * (DP * 2) + (((2 * s + lh) ^ (lr & 7)) << 4)));
           x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], x[kb], 0, 0, 0);
         }
-      __builtin_amdgcn_sched_barrier(0);
+      ahead_of_products<DP / 8>();
       // element v of block kb: key 32kb + 8(v/4) + 4lh + v%4
       const float* sk = &skL[at3][4 * lh];
       const float* sv = &svL[at3][4 * lh];
@@ -762,6 +781,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
           const f32x4 s4 = *reinterpret_cast<const f32x4*>(sk + 32 * kb + 8 * q);
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
+          if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
       // keys that the lane's row sees, bit 8q + i of word kb: element 4q + i of block kb
       uint32_t see[2] = {~0u, ~0u};
@@ -815,6 +835,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               l += p;
               w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
       } else {
 #pragma unroll
@@ -829,8 +850,10 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               l += on ? p : 0.f;
               w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -841,6 +864,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               *reinterpret_cast<const f16x8*>(vbase + e * 32 * (BN * 2) + (lr * (BN * 2) + (c << 4)));
           acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[t], acc[e], 0, 0, 0);
         }
+      ahead_of_products<DP / 8>();
       if (wave == 0) G2_SHOW(last3);
       at3 = next3;
     }
@@ -852,7 +876,10 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
     l += __shfl_xor(l, 32);
     const float inv = l == 0.f ? 0.f : 512.f / l;
-    if (r < rows) {
+    int r_end = r;
+    asm volatile("" : "+v"(r_end));
+    if (r_end < rows) {
+      const RowAt at = row_at(a, sp, h, r_end);
       const int64_t row = (int64_t)at.token * a.Hq + at.head;
       float* o = a.part + (row * a.split + split) * part_size(a);
 #pragma unroll
