@@ -512,30 +512,19 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 //   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
 //     a lane's operand are 16t + 4h .. and 16t + 8 + 4h .. (h = lane / 32), and V^T is
 //     stored with its keys in that order.
-// 16-byte chunks of LDS rows are placed at chunk ^ f(row), which keeps fragment
-// reads (8 consecutive rows, one chunk) and writes free of bank conflicts.
+// LDS rows are 16 bytes longer than their data, so that fragment reads (8 consecutive
+// rows, one 16-byte chunk) touch all banks; values' rows also hold chunk c at
+// c ^ (channel / 8), which spreads the writes (8 rows 8 channels apart, one chunk).
 // ---------------------------------------------------------------------------
-// Schedule of N products with one LDS fragment each: four reads ahead of them.
-template <int N>
-__device__ __forceinline__ void ahead_of_products() {
-  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
-#pragma unroll
-  for (int i = 0; i < N - 4; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 template <int BITS, int DP, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
   constexpr int KP = BN * (DP / 16), KC = (KP + NT - 1) / NT;      // 16-channel pieces of keys
   constexpr int VP = BN / 4 * (DP / 8), VQ = (VP + NT - 1) / NT;   // 4-key × 8-channel of values
   constexpr int KW = BITS / 2, VW = BITS / 4;   // words of 16 and of 8 channels
-  constexpr int KB = BN * DP * 2;               // bytes of a step's keys, and of its values
-  __shared__ __attribute__((aligned(16))) char kvL[4 * KB];  // keys 0, keys 1, values 0, values 1
+  constexpr int KPITCH = DP * 2 + 16, VPITCH = BN * 2 + 16;  // bytes of an LDS row
+  constexpr int KB = BN * KPITCH, VB = DP * VPITCH;          // of a step's keys and values
+  __shared__ __attribute__((aligned(16))) char kL[2 * KB], vL[2 * VB];
   __shared__ __attribute__((aligned(16))) float skL[3][BN], svL[3][BN];
   __shared__ __attribute__((aligned(16))) uint32_t rowL[3][BN];
   __shared__ uint32_t zkL[3][BN];  // −z·2^-9 in fp16, twice
@@ -698,11 +687,9 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       const int p_ = tid + i * NT, key_ = p_ / (DP / 16), c_ = p_ % (DP / 16);               \
       if (KP % NT && p_ >= KP) break;                                                        \
       const f16x2 zc_ = as_h2(zkL[at3][key_]);                                               \
-      char* row_ = (kbase) + key_ * (DP * 2);                                                \
-      *reinterpret_cast<f16x8*>(row_ + ((c_ ^ (key_ & 7)) << 4)) =                           \
-          key_codes<BITS>(&kw[i][0], zc_);                                                   \
-      *reinterpret_cast<f16x8*>(row_ + (((c_ + DP / 16) ^ (key_ & 7)) << 4)) =               \
-          key_codes<BITS>(&kw[i][KW / 2], zc_);                                              \
+      char* at_ = (kbase) + key_ * KPITCH + c_ * 16;                                         \
+      *reinterpret_cast<f16x8*>(at_) = key_codes<BITS>(&kw[i][0], zc_);                      \
+      *reinterpret_cast<f16x8*>(at_ + DP) = key_codes<BITS>(&kw[i][KW / 2], zc_);            \
     }                                                                                        \
     _Pragma("unroll") for (int i = 0; i < VQ; ++i) {                                         \
       const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH; \
@@ -711,13 +698,11 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       const f16x4 z_ = *reinterpret_cast<const f16x4*>(                                      \
           &zvL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * hf_]);                             \
       const f16x2 z0_ = {z_[0], z_[1]}, z1_ = {z_[2], z_[3]};                                \
+      char* at_ = (vbase) + o_ * (8 * VPITCH) + ((ch_ ^ (o_ & 7)) << 4) + 8 * hf_;           \
       _Pragma("unroll") for (int e = 0; e < 8; ++e) {                                        \
         const f16x2 x_ = value_codes<BITS>(vw[i][0], vw[i][1], e, z0_);                      \
         const f16x2 y_ = value_codes<BITS>(vw[i][2], vw[i][3], e, z1_);                      \
-        const int d_ = o_ * 8 + e;                                                           \
-        *reinterpret_cast<f16x4*>((vbase) + d_ * (BN * 2) + 8 * hf_ +                        \
-                                  ((ch_ ^ ((d_ ^ (d_ >> 3)) & 7)) << 4)) =                   \
-            f16x4{x_[0], x_[1], y_[0], y_[1]};                                               \
+        *reinterpret_cast<f16x4*>(at_ + e * VPITCH) = f16x4{x_[0], x_[1], y_[0], y_[1]};     \
       }                                                                                      \
     }                                                                                        \
   } while (0)
@@ -740,12 +725,12 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       // (opaque: addresses kept over the whole loop cost more registers than there are)
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));
-      const int lane = tid & 63, lr = lane & 31, lh = lane >> 5;
+      const int lane = tid & 63;
       const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
       const int j0 = k0 + step * BN;
       const int next3 = at3 == 2 ? 0 : at3 + 1, last3 = next3 == 2 ? 0 : next3 + 1;
-      char* kbase = kvL + (step & 1) * KB;
-      char* vbase = kvL + (2 + (step & 1)) * KB;
+      char* kbase = kL + (step & 1) * KB;
+      char* vbase = vL + (step & 1) * VB;
       G2_PUT(kbase, vbase, at3);
       __syncthreads();
       if (step + 1 < steps) G2_FETCH(next3);
@@ -753,27 +738,51 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
         G2_META(step + 2);
         G2_PAGE(step + 3);
       }
+      // ---- logits; element v of block kb: key 32kb + 8(v/4) + 4lh + v%4.  Fragments are
+      // read one group of products ahead. ----
       f32x16 x[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
-      __builtin_amdgcn_sched_barrier(0);
+      {
+        const char* kp = kbase + lr * KPITCH + lh * 16;
+        f16x8 kf[2][2][2];
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const f16x8 kf = *reinterpret_cast<const f16x8*>(
-              kbase + kb * 32 * (DP * 2) + (lr * (DP * 2) + (((2 * s + lh) ^ (lr & 7)) << 4)));
-          x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], x[kb], 0, 0, 0);
+          for (int kb = 0; kb < 2; ++kb)
+            kf[0][s][kb] = *reinterpret_cast<const f16x8*>(kp + kb * (32 * KPITCH) + s * 32);
+#pragma unroll
+        for (int g = 0; g < DP / 32; ++g) {
+          if (g + 1 < DP / 32) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb)
+                kf[(g + 1) & 1][s][kb] = *reinterpret_cast<const f16x8*>(
+                    kp + kb * (32 * KPITCH) + (2 * g + 2 + s) * 32);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+              x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g & 1][s][kb], qf[2 * g + s],
+                                                             x[kb], 0, 0, 0);
         }
-      ahead_of_products<DP / 8>();
-      // element v of block kb: key 32kb + 8(v/4) + 4lh + v%4
+      }
+      const uint64_t ok = okL[at3];
       const float* sk = &skL[at3][4 * lh];
       const float* sv = &svL[at3][4 * lh];
-      const uint64_t ok = okL[at3];
+      const char* vp = vbase + lr * VPITCH;
+      const int vc = (lh ^ (lr >> 3)) << 4;  // chunk 2t + lh of row 32e + lr: vc ^ 32t ^ 64(e % 2)
+      f16x8 vf[2][DP / 32];
+      f16x8 w[4];
+      // ---- softmax of the step; whole: every row sees every key ----
       const bool whole = ok == ~0ull && j0 + BN - 1 <= first_all;
       float mx = m, vx = vmaxL[at3];
+      uint32_t see[2] = {~0u, ~0u};  // bit 8q + i of word kb: element 4q + i of block kb
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -783,8 +792,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
           for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
           if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
-      // keys that the lane's row sees, bit 8q + i of word kb: element 4q + i of block kb
-      uint32_t see[2] = {~0u, ~0u};
       if (whole) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -821,9 +828,12 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[e][v] *= f;
       }
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e)
+        vf[0][e] = *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (64 * (e & 1))));
       const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
-      f16x8 w[4];
       if (whole) {
+        asm volatile("");  // (keeps the branches apart: no selects here)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -835,7 +845,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               l += p;
               w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
           }
       } else {
 #pragma unroll
@@ -850,21 +860,23 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
               l += on ? p : 0.f;
               w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
           }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      // ---- values ----
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t) {
+        if (t < 3) {
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) {
-          // f(d) of d = 32e + lr is f(lr) ^ 4(e % 2)
-          const int c = (2 * t + lh) ^ ((lr ^ (lr >> 3)) & 7) ^ (4 * (e & 1));
-          const f16x8 vf =
-              *reinterpret_cast<const f16x8*>(vbase + e * 32 * (BN * 2) + (lr * (BN * 2) + (c << 4)));
-          acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[t], acc[e], 0, 0, 0);
+          for (int e = 0; e < DP / 32; ++e)
+            vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
+                vp + e * (32 * VPITCH) + (vc ^ (32 * (t + 1)) ^ (64 * (e & 1))));
         }
-      ahead_of_products<DP / 8>();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+          acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
+      }
       if (wave == 0) G2_SHOW(last3);
       at3 = next3;
     }
