@@ -772,7 +772,10 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
                                                              x[kb], 0, 0, 0);
         }
       }
-      const uint64_t ok = okL[at3];
+      const uint64_t ok_l = okL[at3];  // (the same in every lane: into scalar registers)
+      const uint64_t ok =
+          (uint64_t)__builtin_amdgcn_readfirstlane((int)(ok_l >> 32)) << 32 |
+          (uint32_t)__builtin_amdgcn_readfirstlane((int)ok_l);
       const float* sk = &skL[at3][4 * lh];
       const float* sv = &svL[at3][4 * lh];
       const char* vp = vbase + lr * VPITCH;
@@ -792,7 +795,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
           for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
           if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
-      if (whole) {
+      if (__builtin_expect(whole, 1)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -816,7 +819,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
         vx = fmaxf(vx, __shfl_xor(vx, 32));
       }
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
         const float nref = vx >= ref ? above(vx) : ref;
         float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
         if (m == mx) f = 1.f;
@@ -832,7 +835,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       for (int e = 0; e < DP / 32; ++e)
         vf[0][e] = *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (64 * (e & 1))));
       const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
-      if (whole) {
+      if (__builtin_expect(whole, 1)) {
         asm volatile("");  // (keeps the branches apart: no selects here)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
