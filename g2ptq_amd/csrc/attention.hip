@@ -505,17 +505,33 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // rows, 32 per wave, through 64 keys at a time.  The keys and values of a step are
 // converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
 // transposed as [channel][key]; the codes of the next step are loaded meanwhile (two
-// buffers, one barrier a step).  The first wave looks up a step's pages, scales and
-// zero points two steps ahead (three buffers).  v_mfma_f32_32x32x16_f16:
+// buffers, one barrier a step).  The first two waves look up a step's pages,
+// scales and zero points two steps ahead (three buffers).  v_mfma_f32_32x32x16_f16:
 //   S^T (32 keys × 32 rows) = K·Q^T, so that a lane holds one row's logits (row =
 //     lane % 32, the other half of the keys in lane + 32) and its statistics;
 //   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
 //     a lane's operand are 16t + 4h .. and 16t + 8 + 4h .. (h = lane / 32), and V^T is
 //     stored with its keys in that order.
-// LDS rows are 16 bytes longer than their data, so that fragment reads (8 consecutive
+// LDS rows are 16 bytes longer than their data, so that fragment reads (16 consecutive
 // rows, one 16-byte chunk) touch all banks; values' rows also hold chunk c at
-// c ^ (channel / 8), which spreads the writes (8 rows 8 channels apart, one chunk).
+// c ^ (channel / 16), which spreads the writes (8 rows 8 channels apart, one chunk).
 // ---------------------------------------------------------------------------
+// Largest of 64 lanes' non-negative x, in lane 63 (rows of 16 lanes, then across rows).
+__device__ __forceinline__ float wave_max(float x) {
+#define G2_DPP(ctrl, rows)                                                                   \
+  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                        \
+                                             0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, \
+                                             false)))
+  G2_DPP(0x111, 0xf);  // row_shr 1, 2, 4, 8
+  G2_DPP(0x112, 0xf);
+  G2_DPP(0x114, 0xf);
+  G2_DPP(0x118, 0xf);
+  G2_DPP(0x142, 0xa);  // row_bcast 15 into rows 1 and 3
+  G2_DPP(0x143, 0xc);  // row_bcast 31 into rows 2 and 3
+#undef G2_DPP
+  return x;
+}
+
 template <int BITS, int DP, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
@@ -610,7 +626,8 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
     int bad = 0;
 
-    // first wave: page of key `lane` of a step (−1: none), then its row and numbers
+    // first wave (keys) and second (values): page of key `lane` of a step (−1: none),
+    // then its row and numbers
     int page = -1;
 #define G2_PAGE(step)                                                          \
   do {                                                                         \
@@ -620,8 +637,8 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   } while (0)
     bool sok = false;
     uint32_t srow = 0;
-    float ssk = 0.f, ssv = 0.f;
-    int szk = half, szv = half;
+    float sc = 0.f;
+    int sz = half;
 #define G2_META(step)                                                          \
   do {                                                                         \
     const int key_ = k0 + (step) * BN + lane;                                  \
@@ -629,22 +646,24 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     bad |= key_ < k1 && !sok;                                                  \
     srow = sok ? (uint32_t)a.c.row((int64_t)page << a.c.shift |                \
                                    (key_ & ((1 << a.c.shift) - 1)), h) : 0;    \
-    ssk = sok ? a.c.scale[0][srow] : 0.f;                                      \
-    ssv = sok ? a.c.scale[1][srow] : 0.f;                                      \
-    if (a.c.zero[0]) szk = a.c.zero[0][srow], szv = a.c.zero[1][srow];         \
+    sc = a.c.scale[wave][srow];                                                \
+    if (a.c.zero[0]) sz = a.c.zero[wave][srow];                                \
   } while (0)
 #define G2_SHOW(at3)                                                           \
   do {                                                                         \
-    skL[at3][lane] = ssk * a.kscale;                                           \
-    svL[at3][lane] = ssv;                                                      \
-    rowL[at3][lane] = srow;                                                    \
-    zkL[at3][lane] = __builtin_bit_cast(uint32_t, centre(szk, szk));           \
-    zvL[at3][lane] = centre(szv, szv)[0];                                      \
-    float vx_ = ssv < __builtin_inff() ? ssv : 0.f;                            \
-    _Pragma("unroll") for (int o_ = 32; o_ > 0; o_ >>= 1)                      \
-      vx_ = fmaxf(vx_, __shfl_xor(vx_, o_));                                   \
-    const uint64_t ok_ = __builtin_amdgcn_ballot_w64(sok);                     \
-    if (lane == 0) vmaxL[at3] = vx_, okL[at3] = ok_;                           \
+    if (!sok) sc = 0.f;                                                        \
+    if (wave == 0) {                                                           \
+      skL[at3][lane] = sc * a.kscale;                                          \
+      rowL[at3][lane] = srow;                                                  \
+      zkL[at3][lane] = __builtin_bit_cast(uint32_t, centre(sz, sz));           \
+      const uint64_t ok_ = __builtin_amdgcn_ballot_w64(sok);                   \
+      if (lane == 0) okL[at3] = ok_;                                           \
+    } else {                                                                   \
+      svL[at3][lane] = sc;                                                     \
+      zvL[at3][lane] = centre(sz, sz)[0];                                      \
+      const float vx_ = wave_max(sc < __builtin_inff() ? sc : 0.f);            \
+      if (lane == 63) vmaxL[at3] = vx_;                                        \
+    }                                                                          \
   } while (0)
     uint32_t kw[KC][KW], vw[VQ][4][VW];
 #define G2_FETCH(at3)                                                                        \
@@ -698,7 +717,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       const f16x4 z_ = *reinterpret_cast<const f16x4*>(                                      \
           &zvL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * hf_]);                             \
       const f16x2 z0_ = {z_[0], z_[1]}, z1_ = {z_[2], z_[3]};                                \
-      char* at_ = (vbase) + o_ * (8 * VPITCH) + ((ch_ ^ (o_ & 7)) << 4) + 8 * hf_;           \
+      char* at_ = (vbase) + o_ * (8 * VPITCH) + ((ch_ ^ (o_ >> 1 & 7)) << 4) + 8 * hf_;           \
       _Pragma("unroll") for (int e = 0; e < 8; ++e) {                                        \
         const f16x2 x_ = value_codes<BITS>(vw[i][0], vw[i][1], e, z0_);                      \
         const f16x2 y_ = value_codes<BITS>(vw[i][2], vw[i][3], e, z1_);                      \
@@ -708,7 +727,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   } while (0)
 
     if (steps > 0) {
-      if (wave == 0) {
+      if (wave < 2) {
         G2_PAGE(0);
         G2_META(0);
         G2_SHOW(0);
@@ -722,11 +741,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     }
     int at3 = 0;  // step % 3
     for (int step = 0; step < steps; ++step) {
-      // (opaque: addresses kept over the whole loop cost more registers than there are)
-      int tid = threadIdx.x;
-      asm volatile("" : "+v"(tid));
-      const int lane = tid & 63;
-      const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
       const int j0 = k0 + step * BN;
       const int next3 = at3 == 2 ? 0 : at3 + 1, last3 = next3 == 2 ? 0 : next3 + 1;
       char* kbase = kL + (step & 1) * KB;
@@ -734,7 +748,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       G2_PUT(kbase, vbase, at3);
       __syncthreads();
       if (step + 1 < steps) G2_FETCH(next3);
-      if (wave == 0) {
+      if (wave < 2) {
         G2_META(step + 2);
         G2_PAGE(step + 3);
       }
@@ -779,7 +793,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       const float* sk = &skL[at3][4 * lh];
       const float* sv = &svL[at3][4 * lh];
       const char* vp = vbase + lr * VPITCH;
-      const int vc = (lh ^ (lr >> 3)) << 4;  // chunk 2t + lh of row 32e + lr: vc ^ 32t ^ 64(e % 2)
+      const int vc = (lh ^ (lr >> 4)) << 4;  // chunk 2t + lh of row 32e + lr: vc ^ 32(t ^ e % 4)
       f16x8 vf[2][DP / 32];
       f16x8 w[4];
       // ---- softmax of the step; whole: every row sees every key ----
@@ -833,7 +847,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e)
-        vf[0][e] = *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (64 * (e & 1))));
+        vf[0][e] = *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (32 * (e & 3))));
       const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
       if (__builtin_expect(whole, 1)) {
         asm volatile("");  // (keeps the branches apart: no selects here)
@@ -873,14 +887,14 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
 #pragma unroll
           for (int e = 0; e < DP / 32; ++e)
             vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
-                vp + e * (32 * VPITCH) + (vc ^ (32 * (t + 1)) ^ (64 * (e & 1))));
+                vp + e * (32 * VPITCH) + (vc ^ (32 * ((t + 1) ^ (e & 3)))));
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e)
           acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
       }
-      if (wave == 0) G2_SHOW(last3);
+      if (wave < 2) G2_SHOW(last3);
       at3 = next3;
     }
 #undef G2_PAGE
