@@ -504,9 +504,12 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // Many rows (chunks of prompts): matrix cores.  A workgroup of NW waves takes 32·NW
 // rows, 32 per wave, through 64 keys at a time.  The keys and values of a step are
 // converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
-// transposed as [channel][key]; the codes of the next step are loaded meanwhile (two
-// buffers, one barrier a step).  The first two waves look up a step's pages,
-// scales and zero points two steps ahead (three buffers).  v_mfma_f32_32x32x16_f16:
+// transposed as [channel][key] (two buffers each); the codes after them are loaded
+// meanwhile.  The first two waves look up pages, scales and zero points three steps
+// ahead (a ring of four).  With eight waves the two of a SIMD take turns: while the
+// second four do the products of a step (and the values' of the step before), the first
+// four do the softmax of theirs and move codes, with a barrier at each turn, so that
+// the matrix cores and the vector units both have work.  v_mfma_f32_32x32x16_f16:
 //   S^T (32 keys × 32 rows) = K·Q^T, so that a lane holds one row's logits (row =
 //     lane % 32, the other half of the keys in lane + 32) and its statistics;
 //   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // rows, one 16-byte chunk) touch all banks; values' rows also hold chunk c at
 // c ^ (channel / 16), which spreads the writes (8 rows 8 channels apart, one chunk).
 // ---------------------------------------------------------------------------
-// Largest of 64 lanes' non-negative x, in lane 63 (rows of 16 lanes, then across rows).
+// Largest of 64 lanes' non-negative x (rows of 16 lanes, then across rows, into lane 63).
 __device__ __forceinline__ float wave_max(float x) {
 #define G2_DPP(ctrl, rows)                                                                   \
   x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                        \
@@ -529,7 +532,7 @@ __device__ __forceinline__ float wave_max(float x) {
   G2_DPP(0x142, 0xa);  // row_bcast 15 into rows 1 and 3
   G2_DPP(0x143, 0xc);  // row_bcast 31 into rows 2 and 3
 #undef G2_DPP
-  return x;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 template <int BITS, int DP, bool FULL, int NW>
@@ -541,12 +544,12 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   constexpr int KPITCH = DP * 2 + 16, VPITCH = BN * 2 + 16;  // bytes of an LDS row
   constexpr int KB = BN * KPITCH, VB = DP * VPITCH;          // of a step's keys and values
   __shared__ __attribute__((aligned(16))) char kL[2 * KB], vL[2 * VB];
-  __shared__ __attribute__((aligned(16))) float skL[3][BN], svL[3][BN];
-  __shared__ __attribute__((aligned(16))) uint32_t rowL[3][BN];
-  __shared__ uint32_t zkL[3][BN];  // −z·2^-9 in fp16, twice
-  __shared__ __attribute__((aligned(16))) _Float16 zvL[3][BN];
-  __shared__ float vmaxL[3];
-  __shared__ uint64_t okL[3];
+  __shared__ __attribute__((aligned(16))) float skL[4][BN], svL[4][BN];
+  __shared__ __attribute__((aligned(16))) uint32_t rowL[4][BN];
+  __shared__ uint32_t zkL[4][BN];  // −z·2^-9 in fp16, twice
+  __shared__ __attribute__((aligned(16))) _Float16 zvL[4][BN];
+  __shared__ float vmaxL[4];
+  __shared__ uint64_t okL[4];
 
   // Workgroups go round the 8 XCDs; number them so that an XCD takes a contiguous
   // range: the row tiles of one sequence and head share its keys in one L2.
@@ -571,6 +574,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   const int share = share_of(sp.n, a.split, BN);
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool second = NW == 8 && wave >= 4;
   const int D = FULL ? DP : (int)a.c.D;
   const uint32_t rowb = D * BITS / 8;
   const int half = 1 << (BITS - 1);
@@ -582,6 +586,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   // group's other bits, 3 of the chunk; with fewer pieces than threads the upper half
   // of the workgroup takes them.
   const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
+  const int first = wave * 64, first_v = VP < NT ? (first + NT / 2) % NT : first;  // of the wave
   constexpr int OH = DP / 64;  // 8-channel groups over 8
 
   // the longest tiles (the last rows) first
@@ -629,51 +634,51 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     // first wave (keys) and second (values): page of key `lane` of a step (−1: none),
     // then its row and numbers
     int page = -1;
-#define G2_PAGE(step)                                                          \
-  do {                                                                         \
-    const int key_ = k0 + (step) * BN + lane;                                  \
-    page = -1;                                                                 \
-    if (key_ < k1) page = table[key_ >> a.c.shift];                            \
+#define G2_PAGE(step)                                                                        \
+  do {                                                                                       \
+    const int key_ = k0 + (step) * BN + lane;                                                \
+    page = table[min(key_, k1 - 1) >> a.c.shift];                                            \
   } while (0)
     bool sok = false;
     uint32_t srow = 0;
     float sc = 0.f;
     int sz = half;
-#define G2_META(step)                                                          \
-  do {                                                                         \
-    const int key_ = k0 + (step) * BN + lane;                                  \
-    sok = key_ < k1 && page >= 0 && page < a.c.pages;                          \
-    bad |= key_ < k1 && !sok;                                                  \
-    srow = sok ? (uint32_t)a.c.row((int64_t)page << a.c.shift |                \
-                                   (key_ & ((1 << a.c.shift) - 1)), h) : 0;    \
-    sc = a.c.scale[wave][srow];                                                \
-    if (a.c.zero[0]) sz = a.c.zero[wave][srow];                                \
+#define G2_META(step)                                                                        \
+  do {                                                                                       \
+    const int key_ = k0 + (step) * BN + lane;                                                \
+    const int64_t pages_ = a.c.pages;                                                        \
+    sok = (key_ < k1) & ((uint32_t)page < (uint64_t)pages_);                                 \
+    bad |= (key_ < k1) & !sok;                                                               \
+    const int pg_ = sok ? page : 0, of_ = sok ? key_ & ((1 << a.c.shift) - 1) : 0;           \
+    srow = ((uint32_t)(pg_ * (int)a.c.H + h) << a.c.shift) + of_;                            \
+    sc = a.c.scale[wave][srow];                                                              \
+    if (a.c.zero[0]) sz = a.c.zero[wave][srow];                                              \
   } while (0)
-#define G2_SHOW(at3)                                                           \
-  do {                                                                         \
-    if (!sok) sc = 0.f;                                                        \
-    if (wave == 0) {                                                           \
-      skL[at3][lane] = sc * a.kscale;                                          \
-      rowL[at3][lane] = srow;                                                  \
-      zkL[at3][lane] = __builtin_bit_cast(uint32_t, centre(sz, sz));           \
-      const uint64_t ok_ = __builtin_amdgcn_ballot_w64(sok);                   \
-      if (lane == 0) okL[at3] = ok_;                                           \
-    } else {                                                                   \
-      svL[at3][lane] = sc;                                                     \
-      zvL[at3][lane] = centre(sz, sz)[0];                                      \
-      const float vx_ = wave_max(sc < __builtin_inff() ? sc : 0.f);            \
-      if (lane == 63) vmaxL[at3] = vx_;                                        \
-    }                                                                          \
+#define G2_SHOW(at4)                                                                         \
+  do {                                                                                       \
+    if (!sok) sc = 0.f;                                                                      \
+    if (wave == 0) {                                                                         \
+      skL[at4][lane] = sc * a.kscale;                                                        \
+      rowL[at4][lane] = srow;                                                                \
+      zkL[at4][lane] = __builtin_bit_cast(uint32_t, centre(sz, sz));                         \
+      const uint64_t ok_ = __builtin_amdgcn_ballot_w64(sok);                                 \
+      okL[at4] = ok_;                                                                        \
+    } else {                                                                                 \
+      svL[at4][lane] = sc;                                                                   \
+      zvL[at4][lane] = centre(sz, sz)[0];                                                    \
+      const float vx_ = wave_max(sc < __builtin_inff() ? sc : 0.f);                          \
+      vmaxL[at4] = vx_;                                                                      \
+    }                                                                                        \
   } while (0)
     uint32_t kw[KC][KW], vw[VQ][4][VW];
-#define G2_FETCH(at3)                                                                        \
+#define G2_FETCH_K(at4)                                                                      \
   do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
       const int p_ = tid + i * NT, c_ = p_ % (DP / 16);                                      \
-      if (KP % NT && p_ >= KP) break;                                                        \
-      const uint8_t* s_ = a.c.codes[0];                                                      \
-      if (FULL || c_ * 16 < D)                                                               \
-        s_ += (uint64_t)rowL[at3][p_ / (DP / 16)] * rowb + c_ * (2 * BITS);                  \
+      if (KP % NT && first + i * NT >= KP) break;                                            \
+      uint64_t o_ = (uint64_t)rowL[at4][p_ / (DP / 16)] * rowb + c_ * (2 * BITS);            \
+      if (!FULL) o_ = c_ * 16 < D ? o_ : 0;                                                  \
+      const uint8_t* s_ = a.c.codes[0] + o_;                                                 \
       if constexpr (BITS == 8) {                                                             \
         const uint4 v_ = *reinterpret_cast<const uint4*>(s_);                                \
         kw[i][0] = v_.x, kw[i][1] = v_.y, kw[i][2] = v_.z, kw[i][3] = v_.w;                  \
@@ -682,15 +687,19 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
         kw[i][0] = v_.x, kw[i][1] = v_.y;                                                    \
       }                                                                                      \
     }                                                                                        \
+  } while (0)
+#define G2_FETCH_V(at4)                                                                      \
+  do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < VQ; ++i) {                                         \
-      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH; \
-      if (VP % NT && p_ >= VP) break;                                                        \
+      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH;\
+      if (VP % NT && first_v + i * NT >= VP) break;                                          \
       const uint4 r_ = *reinterpret_cast<const uint4*>(                                      \
-          &rowL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * ((p_ >> 3) & 1)]);                \
+          &rowL[at4][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * ((p_ >> 3) & 1)]);                \
       const uint32_t row_[4] = {r_.x, r_.y, r_.z, r_.w};                                     \
       _Pragma("unroll") for (int t = 0; t < 4; ++t) {                                        \
-        const uint8_t* s_ = a.c.codes[1];                                                    \
-        if (FULL || o_ * 8 < D) s_ += (uint64_t)row_[t] * rowb + o_ * BITS;                  \
+        uint64_t at_ = (uint64_t)row_[t] * rowb + o_ * BITS;                                 \
+        if (!FULL) at_ = o_ * 8 < D ? at_ : 0;                                               \
+        const uint8_t* s_ = a.c.codes[1] + at_;                                              \
         if constexpr (BITS == 8) {                                                           \
           const uint2 v_ = *reinterpret_cast<const uint2*>(s_);                              \
           vw[i][t][0] = v_.x, vw[i][t][1] = v_.y;                                            \
@@ -700,24 +709,28 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       }                                                                                      \
     }                                                                                        \
   } while (0)
-#define G2_PUT(kbase, vbase, at3)                                                            \
+#define G2_PUT_K(step)                                                                       \
   do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
       const int p_ = tid + i * NT, key_ = p_ / (DP / 16), c_ = p_ % (DP / 16);               \
-      if (KP % NT && p_ >= KP) break;                                                        \
-      const f16x2 zc_ = as_h2(zkL[at3][key_]);                                               \
-      char* at_ = (kbase) + key_ * KPITCH + c_ * 16;                                         \
+      if (KP % NT && first + i * NT >= KP) break;                                            \
+      const f16x2 zc_ = as_h2(zkL[(step) & 3][key_]);                                        \
+      char* at_ = kL + ((step) & 1) * KB + key_ * KPITCH + c_ * 16;                          \
       *reinterpret_cast<f16x8*>(at_) = key_codes<BITS>(&kw[i][0], zc_);                      \
       *reinterpret_cast<f16x8*>(at_ + DP) = key_codes<BITS>(&kw[i][KW / 2], zc_);            \
     }                                                                                        \
+  } while (0)
+#define G2_PUT_V(step)                                                                       \
+  do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < VQ; ++i) {                                         \
-      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH; \
+      const int p_ = tv + i * NT, o_ = (p_ & 7) + 8 * ((p_ >> 4) % OH), ch_ = (p_ >> 4) / OH;\
       const int hf_ = (p_ >> 3) & 1;                                                         \
-      if (VP % NT && p_ >= VP) break;                                                        \
+      if (VP % NT && first_v + i * NT >= VP) break;                                          \
       const f16x4 z_ = *reinterpret_cast<const f16x4*>(                                      \
-          &zvL[at3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * hf_]);                             \
+          &zvL[(step) & 3][16 * (ch_ >> 1) + 4 * (ch_ & 1) + 8 * hf_]);                      \
       const f16x2 z0_ = {z_[0], z_[1]}, z1_ = {z_[2], z_[3]};                                \
-      char* at_ = (vbase) + o_ * (8 * VPITCH) + ((ch_ ^ (o_ >> 1 & 7)) << 4) + 8 * hf_;           \
+      char* at_ = vL + ((step) & 1) * VB + o_ * (8 * VPITCH) +                               \
+                  ((ch_ ^ (o_ >> 1 & 7)) << 4) + 8 * hf_;                                    \
       _Pragma("unroll") for (int e = 0; e < 8; ++e) {                                        \
         const f16x2 x_ = value_codes<BITS>(vw[i][0], vw[i][1], e, z0_);                      \
         const f16x2 y_ = value_codes<BITS>(vw[i][2], vw[i][3], e, z1_);                      \
@@ -725,183 +738,212 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       }                                                                                      \
     }                                                                                        \
   } while (0)
+// The workgroup's next step: the codes loaded last go to LDS, the ones after them are loaded.
+#define G2_STAGE()             \
+  do {                         \
+    G2_PUT_K(stage);           \
+    G2_PUT_V(stage - 1);       \
+    G2_FETCH_K((stage + 1) & 3); \
+    G2_FETCH_V(stage & 3);     \
+    ++stage;                   \
+  } while (0)
 
+    f32x16 x[2];
+    f16x8 w[4];
+    // Products of a step's keys and the query; element v of block kb: key
+    // 32kb + 8(v/4) + 4lh + v%4.  Fragments are read one group of products ahead.
+    auto logits = [&](int step) __attribute__((always_inline)) {
+      #pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+      #pragma unroll
+                  for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
+                const char* kp = kL + (step & 1) * KB + lr * KPITCH + lh * 16;
+                f16x8 kf[2][2][2];
+      #pragma unroll
+                for (int s = 0; s < 2; ++s)
+      #pragma unroll
+                  for (int kb = 0; kb < 2; ++kb)
+                    kf[0][s][kb] = *reinterpret_cast<const f16x8*>(kp + kb * (32 * KPITCH) + s * 32);
+      #pragma unroll
+                for (int g = 0; g < DP / 32; ++g) {
+                  if (g + 1 < DP / 32) {
+      #pragma unroll
+                    for (int s = 0; s < 2; ++s)
+      #pragma unroll
+                      for (int kb = 0; kb < 2; ++kb)
+                        kf[(g + 1) & 1][s][kb] = *reinterpret_cast<const f16x8*>(
+                            kp + kb * (32 * KPITCH) + (2 * g + 2 + s) * 32);
+                  }
+                  __builtin_amdgcn_sched_barrier(0);
+      #pragma unroll
+                  for (int s = 0; s < 2; ++s)
+      #pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+                      x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g & 1][s][kb], qf[2 * g + s],
+                                                                     x[kb], 0, 0, 0);
+                }
+    };
+    int stage = 1;
     if (steps > 0) {
       if (wave < 2) {
-        G2_PAGE(0);
-        G2_META(0);
-        G2_SHOW(0);
-        G2_PAGE(1);
-        G2_META(1);
-        G2_SHOW(1);
-        G2_PAGE(2);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+          G2_PAGE(s);
+          G2_META(s);
+          G2_SHOW(s);
+        }
+        G2_PAGE(3);
+        G2_META(3);
+        G2_PAGE(4);
       }
       __syncthreads();
-      G2_FETCH(0);
-    }
-    int at3 = 0;  // step % 3
-    for (int step = 0; step < steps; ++step) {
-      const int j0 = k0 + step * BN;
-      const int next3 = at3 == 2 ? 0 : at3 + 1, last3 = next3 == 2 ? 0 : next3 + 1;
-      char* kbase = kL + (step & 1) * KB;
-      char* vbase = vL + (step & 1) * VB;
-      G2_PUT(kbase, vbase, at3);
+      G2_FETCH_K(0);
+      G2_PUT_K(0);
+      G2_FETCH_K(1);
+      G2_FETCH_V(0);
       __syncthreads();
-      if (step + 1 < steps) G2_FETCH(next3);
-      if (wave < 2) {
-        G2_META(step + 2);
-        G2_PAGE(step + 3);
+      if (second) {
+        G2_STAGE();
+        __syncthreads();
       }
-      // ---- logits; element v of block kb: key 32kb + 8(v/4) + 4lh + v%4.  Fragments are
-      // read one group of products ahead. ----
-      f32x16 x[2];
+      // (the logits past the last step are of finite numbers and not used)
+      logits(0);
+      if (NW == 8) __syncthreads();
+      for (int step = 0; step < steps; ++step) {
+        // ---- softmax of the step; whole: every row sees every key ----
+        const int at4 = step & 3, j0 = k0 + step * BN;
+        const uint64_t ok_l = okL[at4];  // (the same in every lane: into scalar registers)
+        const uint64_t ok = (uint64_t)__builtin_amdgcn_readfirstlane((int)(ok_l >> 32)) << 32 |
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)ok_l);
+        const float* sk = &skL[at4][4 * lh];
+        const float* sv = &svL[at4][4 * lh];
+        const bool whole = ok == ~0ull && j0 + BN - 1 <= first_all;
+        float mx = m, vx = vmaxL[at4];
+        uint32_t see[2] = {~0u, ~0u};  // bit 8q + i of word kb: element 4q + i of block kb
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
-      {
-        const char* kp = kbase + lr * KPITCH + lh * 16;
-        f16x8 kf[2][2][2];
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 s4 = *reinterpret_cast<const f32x4*>(sk + 32 * kb + 8 * q);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+            for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
+            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+          }
+        if (__builtin_expect(whole, 1)) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
-            kf[0][s][kb] = *reinterpret_cast<const f16x8*>(kp + kb * (32 * KPITCH) + s * 32);
 #pragma unroll
-        for (int g = 0; g < DP / 32; ++g) {
-          if (g + 1 < DP / 32) {
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, x[kb][v]);
+        } else {
+          const int n = last - j0;  // the last key seen
+          const uint64_t any = n < 0 ? 0 : ok;
+          const uint64_t seen = any & (~0ull >> (63 - min(max(n, 0), 63)));
+          see[0] = (uint32_t)seen >> (4 * lh);
+          see[1] = (uint32_t)(seen >> 32) >> (4 * lh);
+          vx = 0.f;
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-              for (int kb = 0; kb < 2; ++kb)
-                kf[(g + 1) & 1][s][kb] = *reinterpret_cast<const f16x8*>(
-                    kp + kb * (32 * KPITCH) + (2 * g + 2 + s) * 32);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-              x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g & 1][s][kb], qf[2 * g + s],
-                                                             x[kb], 0, 0, 0);
-        }
-      }
-      const uint64_t ok_l = okL[at3];  // (the same in every lane: into scalar registers)
-      const uint64_t ok =
-          (uint64_t)__builtin_amdgcn_readfirstlane((int)(ok_l >> 32)) << 32 |
-          (uint32_t)__builtin_amdgcn_readfirstlane((int)ok_l);
-      const float* sk = &skL[at3][4 * lh];
-      const float* sv = &svL[at3][4 * lh];
-      const char* vp = vbase + lr * VPITCH;
-      const int vc = (lh ^ (lr >> 4)) << 4;  // chunk 2t + lh of row 32e + lr: vc ^ 32(t ^ e % 4)
-      f16x8 vf[2][DP / 32];
-      f16x8 w[4];
-      // ---- softmax of the step; whole: every row sees every key ----
-      const bool whole = ok == ~0ull && j0 + BN - 1 <= first_all;
-      float mx = m, vx = vmaxL[at3];
-      uint32_t see[2] = {~0u, ~0u};  // bit 8q + i of word kb: element 4q + i of block kb
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 s4 = *reinterpret_cast<const f32x4*>(sk + 32 * kb + 8 * q);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
-          if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-        }
-      if (__builtin_expect(whole, 1)) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, x[kb][v]);
-      } else {
-        const int n = last - j0;  // the last key seen
-        const uint64_t seen = n < 0 ? 0 : n >= 63 ? ok : ok & ((2ull << n) - 1);
-        see[0] = (uint32_t)seen >> (4 * lh);
-        see[1] = (uint32_t)(seen >> 32) >> (4 * lh);
-        vx = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int t = 8 * (v >> 2) + (v & 3);
-            const float s1 = sv[32 * kb + t];
-            const bool on = see[kb] >> t & 1;
-            mx = fmaxf(mx, on ? x[kb][v] : -INFINITY);
-            vx = fmaxf(vx, on && s1 < __builtin_inff() ? s1 : 0.f);
-          }
-        vx = fmaxf(vx, __shfl_xor(vx, 32));
-      }
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
-        const float nref = vx >= ref ? above(vx) : ref;
-        float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
-        if (m == mx) f = 1.f;
-        f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
-        m = mx, ref = nref;
-        l *= f;
-#pragma unroll
-        for (int e = 0; e < DP / 32; ++e)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[e][v] *= f;
-      }
-#pragma unroll
-      for (int e = 0; e < DP / 32; ++e)
-        vf[0][e] = *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (32 * (e & 3))));
-      const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
-      if (__builtin_expect(whole, 1)) {
-        asm volatile("");  // (keeps the branches apart: no selects here)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
-              l += p;
-              w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
+            for (int v = 0; v < 16; ++v) {
+              const int t = 8 * (v >> 2) + (v & 3);
+              const float s1 = sv[32 * kb + t];
+              const bool on = see[kb] >> t & 1;
+              mx = fmaxf(mx, on ? x[kb][v] : -INFINITY);
+              vx = fmaxf(vx, on && s1 < __builtin_inff() ? s1 : 0.f);
             }
-            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-          }
-      } else {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool on = see[kb] >> (8 * q + i) & 1;
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
-              l += on ? p : 0.f;
-              w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
-            }
-            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-          }
-      }
-      // ---- values ----
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (t < 3) {
+          vx = fmaxf(vx, __shfl_xor(vx, 32));
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
+          const float nref = vx >= ref ? above(vx) : ref;
+          float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
+          if (m == mx) f = 1.f;
+          f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
+          m = mx, ref = nref;
+          l *= f;
 #pragma unroll
           for (int e = 0; e < DP / 32; ++e)
-            vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
-                vp + e * (32 * VPITCH) + (vc ^ (32 * ((t + 1) ^ (e & 3)))));
-        }
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e)
-          acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
+            for (int v = 0; v < 16; ++v) acc[e][v] *= f;
+        }
+        // (opaque: the rare branch stays a branch around, without a second copy of the sums)
+        asm volatile("" : "+v"(m), "+v"(ref));
+        const float off = (float)(15 - exponent(ref)) - (m == -INFINITY ? 0.f : m * C);
+        if (__builtin_expect(whole, 1)) {
+          asm volatile("");  // (keeps the branches apart: no selects here)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
+                l += p;
+                w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
+              }
+              if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 s4 = *reinterpret_cast<const f32x4*>(sv + 32 * kb + 8 * q);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool on = see[kb] >> (8 * q + i) & 1;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][4 * q + i], C, off));
+                l += on ? p : 0.f;
+                w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
+              }
+              if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // ---- the next steps' codes ----
+        G2_STAGE();
+        if (wave < 2) {
+          G2_SHOW((step + 3) & 3);
+          G2_META(step + 4);
+          G2_PAGE(step + 5);
+        }
+        __syncthreads();
+        // ---- products of this step's values and the next one's keys ----
+        __builtin_amdgcn_sched_barrier(0);
+                  const char* vp = vL + (step & 1) * VB + lr * VPITCH;
+                  // chunk 2t + lh of row 32e + lr: vc ^ 32(t ^ e % 4)
+                  const int vc = (lh ^ (lr >> 4)) << 4;
+                  f16x8 vf[2][DP / 32];
+        #pragma unroll
+                  for (int e = 0; e < DP / 32; ++e)
+                    vf[0][e] =
+                        *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (32 * (e & 3))));
+        #pragma unroll
+                  for (int t = 0; t < 4; ++t) {
+                    if (t < 3) {
+        #pragma unroll
+                      for (int e = 0; e < DP / 32; ++e)
+                        vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
+                            vp + e * (32 * VPITCH) + (vc ^ (32 * ((t + 1) ^ (e & 3)))));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+        #pragma unroll
+                    for (int e = 0; e < DP / 32; ++e)
+                      acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
+                  }
+        logits(step + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (NW == 8 && !(second && step == steps - 1)) __syncthreads();
       }
-      if (wave < 2) G2_SHOW(last3);
-      at3 = next3;
     }
+#undef G2_FETCH_K
+#undef G2_FETCH_V
+#undef G2_PUT_K
+#undef G2_PUT_V
+#undef G2_STAGE
 #undef G2_PAGE
 #undef G2_META
 #undef G2_SHOW
-#undef G2_FETCH
-#undef G2_PUT
     if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
     l += __shfl_xor(l, 32);
     const float inv = l == 0.f ? 0.f : 512.f / l;
@@ -1020,7 +1062,7 @@ int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
   }
   if (p.tiles) {
     const dim3 grid((unsigned)(a.B * a.c.H * a.split * a.tiles + 1));
-#define G2_AT(NW)                                                                             \
+#define G2_AT(NW)                                                                            \
   hipLaunchKernelGGL((attend_tiles_kernel<BITS, DP, FULL, NW>), grid, dim3(64 * NW), 0, st, a)
     if constexpr (DP <= 128) {
       if (p.nw == 8) G2_AT(8);
@@ -1103,11 +1145,11 @@ extern "C" int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, 
   a.few_part = p.few_part ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.part) : nullptr;
   hipStream_t st = as_stream(stream);
   const int64_t D = a.c.D;
-#define G2_DIM(BITS)                                        \
-  if (D == 64) return launch<BITS, 64, true>(st, a, p);     \
-  if (D < 64) return launch<BITS, 64, false>(st, a, p);     \
-  if (D == 128) return launch<BITS, 128, true>(st, a, p);   \
-  if (D < 128) return launch<BITS, 128, false>(st, a, p);   \
+#define G2_DIM(BITS)                                                                         \
+  if (D == 64) return launch<BITS, 64, true>(st, a, p);                                      \
+  if (D < 64) return launch<BITS, 64, false>(st, a, p);                                      \
+  if (D == 128) return launch<BITS, 128, true>(st, a, p);                                    \
+  if (D < 128) return launch<BITS, 128, false>(st, a, p);                                    \
   return launch<BITS, 256, false>(st, a, p)
   if (a.c.bits == 8) { G2_DIM(8); }
   G2_DIM(4);
