@@ -506,10 +506,8 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 // converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
 // transposed as [channel][key] (two buffers each); the codes after them are loaded
 // meanwhile.  The first two waves look up pages, scales and zero points three steps
-// ahead (a ring of four).  With eight waves the two of a SIMD take turns: while the
-// second four do the products of a step (and the values' of the step before), the first
-// four do the softmax of theirs and move codes, with a barrier at each turn, so that
-// the matrix cores and the vector units both have work.  v_mfma_f32_32x32x16_f16:
+// ahead (a ring of four).  A step is softmax and staging, a barrier, and the products
+// of its values and the next step's keys.  v_mfma_f32_32x32x16_f16:
 //   S^T (32 keys × 32 rows) = K·Q^T, so that a lane holds one row's logits (row =
 //     lane % 32, the other half of the keys in lane + 32) and its statistics;
 //   O^T (channels × rows) += V^T·P^T with the weights as they lie: the eight keys of
@@ -574,7 +572,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   const int share = share_of(sp.n, a.split, BN);
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool second = NW == 8 && wave >= 4;
   const int D = FULL ? DP : (int)a.c.D;
   const uint32_t rowb = D * BITS / 8;
   const int half = 1 << (BITS - 1);
@@ -802,13 +799,8 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
       G2_FETCH_K(1);
       G2_FETCH_V(0);
       __syncthreads();
-      if (second) {
-        G2_STAGE();
-        __syncthreads();
-      }
       // (the logits past the last step are of finite numbers and not used)
       logits(0);
-      if (NW == 8) __syncthreads();
       for (int step = 0; step < steps; ++step) {
         // ---- softmax of the step; whole: every row sees every key ----
         const int at4 = step & 3, j0 = k0 + step * BN;
@@ -827,7 +819,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
             const f32x4 s4 = *reinterpret_cast<const f32x4*>(sk + 32 * kb + 8 * q);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[kb][4 * q + i] *= s4[i];
-            if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
           }
         if (__builtin_expect(whole, 1)) {
 #pragma unroll
@@ -882,7 +873,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
                 l += p;
                 w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(p * s4[i]);
               }
-              if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
 #pragma unroll
@@ -897,7 +887,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
                 l += on ? p : 0.f;
                 w[2 * kb + (q >> 1)][4 * (q & 1) + i] = (_Float16)(on ? p * s4[i] : 0.f);
               }
-              if (q % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
         // ---- the next steps' codes ----
@@ -933,7 +922,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
                   }
         logits(step + 1);
         __builtin_amdgcn_sched_barrier(0);
-        if (NW == 8 && !(second && step == steps - 1)) __syncthreads();
       }
     }
 #undef G2_FETCH_K
