@@ -64,13 +64,13 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __rest
 }
 
 // ---------------------------------------------------------------------------
-// Product: one workgroup of four waves computes a 64 × 64 tile (tokens ×
-// channels), 32 × 32 per wave, in steps of 64 columns through LDS.
+// Products.  v_mfma_i32_*_i8: both operands' rows run along K, so that a lane's
+// 16 bytes of a row are its operand as they lie in memory.
 // ---------------------------------------------------------------------------
 struct GemmI8 {
   const int8_t* A;  // codes, T rows of lda bytes, readable to the next multiple of 16 columns
   int64_t lda;
-  const int8_t* W;  // weights, N rows of ldw bytes, zero from K to the next multiple of 16
+  const int8_t* W;  // weights, N rows of ldw bytes, zero from K to the next multiple of 256
   int64_t ldw;
   const float *sx, *zx, *sw, *bias;
   const int32_t* wsum;
@@ -80,47 +80,285 @@ struct GemmI8 {
 };
 
 // Y[t][n] from the integer sum.
-__device__ __forceinline__ void finish(const GemmI8& a, int64_t t, int64_t n, int acc) {
-  if (a.zx) acc = (int)((uint32_t)acc - (uint32_t)(int)a.zx[t] * (uint32_t)a.wsum[n]);
-  float y = __fmul_rn(__fmul_rn((float)acc, a.sx[t]), a.sw[n]);
-  if (a.bias) y = __fadd_rn(y, a.bias[n]);
-  const int64_t o = t * a.ldo + n;
+__device__ __forceinline__ float scaled(const GemmI8& a, float sx, int zx, int acc, float sw,
+                                        int wsum, float bias) {
+  acc = (int)((uint32_t)acc - (uint32_t)zx * (uint32_t)wsum);
+  return __fadd_rn(__fmul_rn(__fmul_rn((float)acc, sx), sw), bias);
+}
+__device__ __forceinline__ void store_y(const GemmI8& a, int64_t o, float y) {
   if (a.dtype == 0) static_cast<uint16_t*>(a.out)[o] = __builtin_bit_cast(uint16_t, (__bf16)y);
   else if (a.dtype == 1) static_cast<_Float16*>(a.out)[o] = (_Float16)y;
   else static_cast<float*>(a.out)[o] = y;
 }
 
-__global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8 a) {
-  __shared__ __attribute__((aligned(16))) int8_t As[64 * 80], Ws[64 * 80];
-  const int64_t t0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave >> 1, wn = wave & 1, lr = lane & 31, lh = lane >> 5;
-  const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-  const int64_t K16 = (a.K + 15) / 16 * 16;
-  i32x16 acc;
+// Tiles of BM tokens × BN channels by WM × WN waves, 32×32 products.  K advances 128
+// bytes a stage through two LDS buffers; the loads of a stage are issued two stages
+// ahead into registers and written to the other buffer during the products, one
+// barrier a stage.  LDS rows are 128 bytes, the 16-byte chunk c of row r at
+// c ^ f(r), f(r) = (r & 7) ^ ((r >> 3) & 1): fragment reads (16 consecutive rows, one
+// chunk) are free of bank conflicts.
+constexpr int KS = 128;
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm, int tn) {
+  constexpr int NT = 64 * WM * WN;
+  constexpr int MT = BM / WM / 32, NTL = BN / WN / 32;  // 32×32 tiles of a wave
+  constexpr int AL = BM * 8 / NT, BL = BN * 8 / NT;     // 16-byte loads of a thread per stage
+  __shared__ __attribute__((aligned(16))) int8_t Ls[2][(BM + BN) * KS];
+
+  // Workgroups go round the 8 XCDs: an XCD takes a contiguous range of tiles, in bands of
+  // eight token tiles walked channel tile by channel tile.
+  const int total = tm * tn;
+  int id;
+  {
+    const int q8 = total >> 3, r8 = total & 7, xcd = blockIdx.x & 7;
+    id = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
+  }
+  const int band = id / (8 * tn), in = id - band * 8 * tn, h = min(8, tm - band * 8);
+  const int64_t t0 = (int64_t)(band * 8 + in % h) * BM, n0 = (int64_t)(in / h) * BN;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  const int row = tid >> 3, c = tid & 7;  // load i: row + i·NT/8
+  const int8_t* Ab = a.A + t0 * a.lda;
+  const int8_t* Wb = a.W + n0 * a.ldw;
+  uint32_t aoff[AL], boff[BL];  // (rows past the end read the last row)
 #pragma unroll
-  for (int v = 0; v < 16; ++v) acc[v] = 0;
-  for (int64_t k = 0; k < K16; k += 64) {
-    uint4 av = make_uint4(0, 0, 0, 0), wv = av;
-    if (t0 + row < a.T && k + c < K16)
-      av = *reinterpret_cast<const uint4*>(a.A + (t0 + row) * a.lda + k + c);
-    if (n0 + row < a.N && k + c < K16)
-      wv = *reinterpret_cast<const uint4*>(a.W + (n0 + row) * a.ldw + k + c);
-    *reinterpret_cast<uint4*>(As + row * 80 + c) = av;
-    *reinterpret_cast<uint4*>(Ws + row * 80 + c) = wv;
+  for (int i = 0; i < AL; ++i)
+    aoff[i] = (uint32_t)min<int64_t>(row + i * (NT / 8), a.T - 1 - t0) * (uint32_t)a.lda;
+#pragma unroll
+  for (int i = 0; i < BL; ++i)
+    boff[i] = (uint32_t)min<int64_t>(row + i * (NT / 8), a.N - 1 - n0) * (uint32_t)a.ldw + c * 16;
+  const int lpos = row * KS + ((c ^ swz(row)) << 4);  // (NT/8 is a multiple of 16)
+  const uint32_t klast = (uint32_t)((a.K + 15) / 16 * 16 - 16);
+  const int nk = (int)((a.K + 255) / 256 * 2);  // even; weights are zero past K
+  i32x4 xa[AL], xb[BL], ya[AL], yb[BL];
+#define G2_LOAD(R, st)                                                              \
+  do {                                                                              \
+    const uint32_t k_ = (uint32_t)((st) < nk ? (st) : nk - 1) * KS;                 \
+    const uint32_t ka_ = min(k_ + c * 16, klast);                                   \
+    _Pragma("unroll") for (int i = 0; i < AL; ++i)                                  \
+      R##a[i] = *reinterpret_cast<const i32x4*>(Ab + (aoff[i] + ka_));              \
+    _Pragma("unroll") for (int i = 0; i < BL; ++i)                                  \
+      R##b[i] = *reinterpret_cast<const i32x4*>(Wb + (boff[i] + k_));               \
+  } while (0)
+#define G2_STORE(R, buf)                                                            \
+  do {                                                                              \
+    _Pragma("unroll") for (int i = 0; i < AL; ++i)                                  \
+      *reinterpret_cast<i32x4*>(&Ls[buf][lpos + i * (NT / 8) * KS]) = R##a[i];      \
+    _Pragma("unroll") for (int i = 0; i < BL; ++i)                                  \
+      *reinterpret_cast<i32x4*>(&Ls[buf][BM * KS + lpos + i * (NT / 8) * KS]) = R##b[i]; \
+  } while (0)
+  i32x16 acc[MT][NTL];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NTL; ++n)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[m][n][v] = 0;
+#define G2_MMA(buf)                                                                       \
+  do {                                                                                    \
+    const int8_t* As_ = Ls[buf];                                                          \
+    const int8_t* Bs_ = Ls[buf] + BM * KS;                                                \
+    _Pragma("unroll") for (int ks = 0; ks < KS / 32; ++ks) {                              \
+      const int c_ = ks * 2 + lh;                                                         \
+      i32x4 av[MT], bv[NTL];                                                              \
+      _Pragma("unroll") for (int m = 0; m < MT; ++m) {                                    \
+        const int r_ = wm * (BM / WM) + m * 32 + lr;                                      \
+        av[m] = *reinterpret_cast<const i32x4*>(As_ + r_ * KS + ((c_ ^ swz(r_)) << 4));   \
+      }                                                                                   \
+      _Pragma("unroll") for (int n = 0; n < NTL; ++n) {                                   \
+        const int r_ = wn * (BN / WN) + n * 32 + lr;                                      \
+        bv[n] = *reinterpret_cast<const i32x4*>(Bs_ + r_ * KS + ((c_ ^ swz(r_)) << 4));   \
+      }                                                                                   \
+      _Pragma("unroll") for (int m = 0; m < MT; ++m)                                      \
+      _Pragma("unroll") for (int n = 0; n < NTL; ++n)                                     \
+        acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[m], bv[n], acc[m][n], 0, 0, 0); \
+    }                                                                                     \
+  } while (0)
+  // Spreads a stage's LDS writes and loads over its products (256 × 256: 32 products, 8
+  // writes, 8 loads, 24 reads a wave).
+#define G2_PATTERN()                                                                      \
+  do {                                                                                    \
+    if constexpr (MT == 4 && NTL == 2) {                                                  \
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0); /* DS read  */                   \
+      _Pragma("unroll") for (int r_ = 0; r_ < 8; ++r_) {                                  \
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); /* MFMA */                     \
+        __builtin_amdgcn_sched_group_barrier(0x200, 1, 0); /* DS write */                 \
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                \
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); /* VMEM read */                \
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                \
+        if (r_ < 6) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);                    \
+      }                                                                                   \
+    }                                                                                     \
+    __builtin_amdgcn_sched_barrier(0);                                                    \
+  } while (0)
+  G2_LOAD(x, 0);
+  G2_STORE(x, 0);
+  G2_LOAD(x, 1);
+  G2_LOAD(y, 2);
+  __syncthreads();
+  for (int kt = 0; kt < nk; kt += 2) {
+    __builtin_amdgcn_sched_barrier(0);
+    G2_MMA(0);      // stage kt
+    G2_STORE(x, 1);  // stage kt + 1
+    G2_LOAD(x, kt + 3);
+    G2_PATTERN();
     __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const i32x4 x = *reinterpret_cast<const i32x4*>(As + (wm * 32 + lr) * 80 + ks * 32 + lh * 16);
-      const i32x4 w = *reinterpret_cast<const i32x4*>(Ws + (wn * 32 + lr) * 80 + ks * 32 + lh * 16);
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(x, w, acc, 0, 0, 0);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    G2_MMA(1);      // stage kt + 1
+    G2_STORE(y, 0);  // stage kt + 2
+    G2_LOAD(y, kt + 4);
+    G2_PATTERN();
     __syncthreads();
   }
+#undef G2_LOAD
+#undef G2_STORE
+#undef G2_MMA
+#undef G2_PATTERN
+  // 32×32 output: lane holds rows 8(v/4) + 4·(lane/32) + v%4 of column lane%32
+  float sw[NTL], bias[NTL];
+  int wsum[NTL];
 #pragma unroll
-  for (int v = 0; v < 16; ++v) {
-    const int64_t t = t0 + wm * 32 + 8 * (v >> 2) + 4 * lh + (v & 3), n = n0 + wn * 32 + lr;
-    if (t < a.T && n < a.N) finish(a, t, n, acc[v]);
+  for (int n = 0; n < NTL; ++n) {
+    const int64_t j = min<int64_t>(n0 + wn * (BN / WN) + n * 32 + lr, a.N - 1);
+    sw[n] = a.sw[j];
+    bias[n] = a.bias ? a.bias[j] : 0.f;
+    wsum[n] = a.zx ? a.wsum[j] : 0;
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int64_t i = t0 + wm * (BM / WM) + m * 32 + 8 * (v >> 2) + 4 * lh + (v & 3);
+      const int64_t ic = min<int64_t>(i, a.T - 1);
+      const float sx = a.sx[ic];
+      const int zx = a.zx ? (int)a.zx[ic] : 0;
+#pragma unroll
+      for (int n = 0; n < NTL; ++n) {
+        const int64_t j = n0 + wn * (BN / WN) + n * 32 + lr;
+        if (i < a.T && j < a.N)
+          store_y(a, i * a.ldo + j, scaled(a, sx, zx, acc[m][n][v], sw[n], wsum[n], bias[n]));
+      }
+    }
+}
+
+// Few tokens (TB blocks of 16): the weights' bytes are what counts.  A workgroup takes
+// 16·R channels; its eight waves take turns at blocks of 128 columns, with weights and
+// codes straight from memory into v_mfma_i32_16x16x64_i8 (channels × tokens: lane
+// (n, g) holds 16 bytes of row n at 16·g of 64 columns, so that a load covers 64
+// consecutive bytes of 16 rows).  The waves' integer sums are added in LDS.
+// FUSED: the tokens themselves are quantized here, by every workgroup, into LDS (one or
+// two tokens: cheaper than another launch before this one).
+template <int R, int TB, bool FUSED, int DT, bool SYM>
+__global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* __restrict__ x,
+                                                          int64_t ldx, bool vec) {
+  constexpr int NW = 8;
+  extern __shared__ __attribute__((aligned(16))) int8_t cL[];  // FUSED: T rows of K256 codes
+  __shared__ int sL[TB * 16][R * 16 + 1];
+  __shared__ float sxL[FUSED ? 16 : 1], zxL[FUSED ? 16 : 1];
+  __shared__ float rlo[NW], rhi[NW];
+  __shared__ uint32_t rtop[NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * R);
+  const int nb = (int)((a.K + 255) / 256 * 2);  // blocks of 128 columns; weights are zero past K
+  const int K256 = nb * 128;
+  const int8_t* wrow[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    wrow[r] = a.W + min<int64_t>(n0 + 16 * r + n, a.N - 1) * a.ldw + g * 16;
+  // the first weights are on their way while the tokens are prepared
+  i32x4 w0[R][2], w1[R][2];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w0[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + min(wave, nb - 1) * 128 + i * 64);
+      w1[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + min(wave + NW, nb - 1) * 128 + i * 64);
+    }
+  for (int i = tid; i < TB * 16 * (R * 16 + 1); i += 512) (&sL[0][0])[i] = 0;
+  if constexpr (FUSED) {
+    for (int t = 0; t < (int)a.T; ++t) {
+      Range r;
+      for (int k = tid * 8; k < a.K; k += 512 * 8) {
+        float v[8];
+        load8<DT>(x, t * ldx + k, vec, min(8, (int)a.K - k), v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.add(v[i]);
+      }
+      reduce_range<64>(r);
+      if (lane == 0) rlo[wave] = r.lo, rhi[wave] = r.hi, rtop[wave] = r.top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) r.merge(rlo[w], rhi[w], rtop[w]);
+      const Grid gr = make_grid<SYM>(r, 8);
+      if (tid == 0) sxL[t] = gr.s, zxL[t] = gr.z;
+      for (int k = tid * 8; k < K256; k += 512 * 8) {
+        float v[8];
+        const int m = min(8, (int)a.K - k);
+        load8<DT>(x, t * ldx + k, vec, m, v);
+        uint32_t o[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < m) o[i >> 2] |= ((uint32_t)to_code(gr, v[i]) & 0xffu) << (8 * (i & 3));
+        *reinterpret_cast<uint2*>(cL + t * K256 + k) = make_uint2(o[0], o[1]);
+      }
+      __syncthreads();
+    }
+  } else {
+    __syncthreads();
+  }
+  const int8_t* arow[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    const int64_t t = min<int64_t>(16 * b + n, a.T - 1);
+    arow[b] = FUSED ? cL + t * K256 + g * 16 : a.A + t * a.lda;
+  }
+  const int klast = (int)((a.K + 15) / 16 * 16 - 16);
+  i32x4 acc[R][TB];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[r][b] = i32x4{0, 0, 0, 0};
+#define G2_FEW(W, blk)                                                                         \
+  do {                                                                                         \
+    i32x4 x_[TB][2];                                                                           \
+    _Pragma("unroll") for (int b = 0; b < TB; ++b)                                             \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                              \
+      x_[b][i] = *reinterpret_cast<const i32x4*>(                                              \
+          arow[b] + (FUSED ? (blk) * 128 + i * 64 : min((blk) * 128 + i * 64 + g * 16, klast))); \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                              \
+    _Pragma("unroll") for (int r = 0; r < R; ++r)                                              \
+    _Pragma("unroll") for (int b = 0; b < TB; ++b)                                             \
+      acc[r][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(W[r][i], x_[b][i], acc[r][b], 0, 0, 0); \
+    const int nx_ = min((blk) + 2 * NW, nb - 1) * 128;                                         \
+    _Pragma("unroll") for (int r = 0; r < R; ++r)                                              \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                              \
+      W[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + nx_ + i * 64);                       \
+  } while (0)
+  for (int blk = wave; blk < nb; blk += 2 * NW) {
+    G2_FEW(w0, blk);
+    if (blk + NW < nb) G2_FEW(w1, blk + NW);
+  }
+#undef G2_FEW
+  // lane holds channels 4g + v of token n
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) atomicAdd(&sL[16 * b + n][16 * r + 4 * g + v], acc[r][b][v]);
+  __syncthreads();
+  for (int i = tid; i < (int)a.T * 16 * R; i += 512) {
+    const int t = i / (16 * R), j = i % (16 * R);
+    const int64_t ch = n0 + j;
+    if (ch >= a.N) continue;
+    const float sx = FUSED ? sxL[t] : a.sx[t];
+    const int zx = FUSED ? (int)zxL[t] : a.zx ? (int)a.zx[t] : 0;
+    store_y(a, t * a.ldo + ch,
+            scaled(a, sx, zx, sL[t][j], a.sw[ch], zx != 0 ? a.wsum[ch] : 0,
+                   a.bias ? a.bias[ch] : 0.f));
   }
 }
 
@@ -140,11 +378,63 @@ int quantize_tokens(hipStream_t st, const void* x, int dtype, int64_t T, int64_t
   return G2PTQ_OK;
 }
 
+constexpr int kFewTokens = 64;    // up to which the weights are streamed
+constexpr int64_t kFusedCodes = 16384;  // bytes of codes up to which they are made in that kernel
+
+template <int R, int TB>
+void launch_few(hipStream_t st, const GemmI8& a) {
+  hipLaunchKernelGGL((gemm_i8_few_kernel<R, TB, false, 0, true>),
+                     dim3((unsigned)cdiv(a.N, 16 * R)), dim3(512), 0, st, a, nullptr, 0, false);
+}
+
+template <int R>
+void launch_few(hipStream_t st, const GemmI8& a) {
+  if (a.T <= 16) launch_few<R, 1>(st, a);
+  else if (a.T <= 32) launch_few<R, 2>(st, a);
+  else if (a.T <= 48) launch_few<R, 3>(st, a);
+  else launch_few<R, 4>(st, a);
+}
+
+// Channels of a workgroup of few tokens: enough workgroups for every CU first, then
+// fewer workgroups that read the codes again.
+int few_rows(int64_t N) { return N >= 16 * 4 * 256 ? 4 : N >= 16 * 2 * 256 ? 2 : 1; }
+
+template <int BM, int BN, int WM, int WN>
+void launch_tiles(hipStream_t st, const GemmI8& a) {
+  const int64_t tm = cdiv(a.T, BM), tn = cdiv(a.N, BN);
+  hipLaunchKernelGGL((gemm_i8_kernel<BM, BN, WM, WN>), dim3((unsigned)(tm * tn)),
+                     dim3(64 * WM * WN), 0, st, a, (int)tm, (int)tn);
+}
+
 int gemm_i8(hipStream_t st, const GemmI8& a) {
-  hipLaunchKernelGGL(gemm_i8_kernel, dim3((unsigned)cdiv(a.N, 64), (unsigned)cdiv(a.T, 64)),
-                     dim3(256), 0, st, a);
+  if (a.T <= kFewTokens) {
+    const int r = few_rows(a.N);
+    if (r == 4) launch_few<4>(st, a);
+    else if (r == 2) launch_few<2>(st, a);
+    else launch_few<1>(st, a);
+  } else {
+    G2PTQ_CHECK(cdiv(a.T, 64) * cdiv(a.N, 64) < (1ll << 31), "int8_gemm: output too large");
+    if (cdiv(a.T, 256) * cdiv(a.N, 256) >= 192) launch_tiles<256, 256, 2, 4>(st, a);
+    else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 128) launch_tiles<128, 128, 2, 2>(st, a);
+    else launch_tiles<64, 64, 2, 2>(st, a);
+  }
   G2PTQ_LAUNCHED();
   return G2PTQ_OK;
+}
+
+// Tokens quantized and multiplied in one launch.
+bool fused(int64_t T, int64_t K) { return T <= 4 && T * (cdiv(K, 256) * 256) <= kFusedCodes; }
+template <int DT, bool SYM>
+void launch_fused(hipStream_t st, const GemmI8& a, const void* x, int64_t ldx, bool vec) {
+  const size_t lds = (size_t)(a.T * (cdiv(a.K, 256) * 256));
+  const int r = few_rows(a.N);
+#define G2_FU(R)                                                                             \
+  hipLaunchKernelGGL((gemm_i8_few_kernel<R, 1, true, DT, SYM>), dim3((unsigned)cdiv(a.N, 16 * R)), \
+                     dim3(512), lds, st, a, x, ldx, vec)
+  if (r == 4) G2_FU(4);
+  else if (r == 2) G2_FU(2);
+  else G2_FU(1);
+#undef G2_FU
 }
 
 int check_tokens(const char* who, const void* x, int dtype, int64_t T, int64_t K, int64_t ldx) {
@@ -165,9 +455,10 @@ int check_product(const char* who, const GemmI8& a) {
               (long long)a.K, (long long)a.N);
   if (a.T == 0 || a.N == 0) return G2PTQ_OK;
   G2PTQ_CHECK(a.W && a.sw && a.out && a.ldo >= a.N, "%s: null pointer or output stride", who);
-  const int64_t K16 = cdiv(a.K, 16) * 16;
-  G2PTQ_CHECK(a.ldw >= K16 && a.ldw % 16 == 0 && aligned16(a.W),
-              "%s: weights need 16-byte aligned rows of at least %lld bytes", who, (long long)K16);
+  const int64_t K256 = cdiv(a.K, 256) * 256;
+  G2PTQ_CHECK(a.ldw >= K256 && a.ldw % 16 == 0 && a.ldw < (1 << 20) && aligned16(a.W),
+              "%s: weights need 16-byte aligned rows of at least %lld bytes", who,
+              (long long)K256);
   return G2PTQ_OK;
 }
 
@@ -203,7 +494,7 @@ extern "C" int g2ptq_int8_gemm(void* stream, const int8_t* codes, int64_t ldc, c
   G2PTQ_TRY(check_product("int8_gemm", a));
   if (T == 0 || N == 0) return G2PTQ_OK;
   G2PTQ_CHECK(codes && scale && (!zero || wsum), "int8_gemm: null codes, scales or weight sums");
-  G2PTQ_CHECK(ldc % 16 == 0 && ldc >= cdiv(K, 16) * 16 && aligned16(codes),
+  G2PTQ_CHECK(ldc % 16 == 0 && ldc >= cdiv(K, 16) * 16 && ldc < (1 << 20) && aligned16(codes),
               "int8_gemm: codes need 16-byte aligned rows of at least %lld bytes",
               (long long)(cdiv(K, 16) * 16));
   return gemm_i8(as_stream(stream), a);
@@ -226,7 +517,7 @@ struct LinearWs {
 extern "C" int g2ptq_int8_linear_workspace(int64_t T, int64_t N, int64_t K, size_t* bytes) {
   G2PTQ_CHECK(T >= 0 && K >= 1, "int8_linear_workspace: bad sizes");
   G2PTQ_TRY(g2ptq_int8_gemm_workspace(T, N, K, bytes));
-  *bytes += (size_t)LinearWs(T, K).gemm;
+  if (!fused(T, K)) *bytes += (size_t)LinearWs(T, K).gemm;
   return G2PTQ_OK;
 }
 
@@ -239,9 +530,18 @@ extern "C" int g2ptq_int8_linear(void* stream, const void* x, int dtype, int64_t
   G2PTQ_TRY(check_product("int8_linear", a));
   if (T == 0 || N == 0) return G2PTQ_OK;
   G2PTQ_CHECK(sym || wsum, "int8_linear: asymmetric tokens need the weights' sums");
+  if (fused(T, K)) {
+    const bool vec = aligned16(x) && ldx * (dtype == 2 ? 4 : 2) % 16 == 0;
+    hipStream_t st = as_stream(stream);
+    if (dtype == 0) { if (sym) launch_fused<0, true>(st, a, x, ldx, vec); else launch_fused<0, false>(st, a, x, ldx, vec); }
+    else if (dtype == 1) { if (sym) launch_fused<1, true>(st, a, x, ldx, vec); else launch_fused<1, false>(st, a, x, ldx, vec); }
+    else { if (sym) launch_fused<2, true>(st, a, x, ldx, vec); else launch_fused<2, false>(st, a, x, ldx, vec); }
+    G2PTQ_LAUNCHED();
+    return G2PTQ_OK;
+  }
   size_t need;
   G2PTQ_TRY(g2ptq_int8_linear_workspace(T, N, K, &need));
-  if (!ws || ws_bytes < need) {
+  if (need && (!ws || ws_bytes < need)) {
     set_error("int8_linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
     return G2PTQ_ERR_WORKSPACE;
   }

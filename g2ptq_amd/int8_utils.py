@@ -37,8 +37,8 @@ def _row_stride(x2):
     return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
 
 
-def _padded(n):
-    return (n + 15) // 16 * 16
+def _padded(n, to=16):
+    return (n + to - 1) // to * to
 
 
 def quantize_tokens(x, sym=True):
@@ -69,7 +69,7 @@ class Int8Linear(torch.nn.Module):
 
     ``codes``: (out, in) int8 GPU tensor; ``scale``: one per output channel;
     ``bias``: (out,) or None; ``sym``: the tokens' grid.  ``y`` has ``x``'s
-    dtype.  Columns are laid out once in rows of a multiple of 16 bytes."""
+    dtype.  Columns are laid out once in rows of a multiple of 256 bytes."""
 
     def __init__(self, codes, scale, bias=None, sym=True):
         super().__init__()
@@ -90,7 +90,7 @@ class Int8Linear(torch.nn.Module):
             raise RuntimeError("Int8Linear requires GPU tensors")
         self.sym = bool(sym)
         dev = codes.device
-        weight = torch.zeros(self.out_features, _padded(self.in_features), dtype=torch.int8,
+        weight = torch.zeros(self.out_features, _padded(self.in_features, 256), dtype=torch.int8,
                              device=dev)
         weight[:, :self.in_features] = codes
         self.register_buffer("weight", weight)

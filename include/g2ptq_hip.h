@@ -419,7 +419,7 @@ int g2ptq_quantize_tokens(void* stream, const void* x, int dtype, int64_t T, int
 /* out[t][n] = scale[t]·wscale[n]·(Σ_k codes[t][k]·W[n][k] − zero[t]·wsum[n]) + bias[n]
  * (dtype as above, ld ldo).  codes as written by g2ptq_quantize_tokens; W: N
  * rows of ldw bytes, 16-byte aligned, ldw a multiple of 16, zero in the columns
- * from K to the next multiple of 16; wsum[n] = Σ_k W[n][k].  zero (with wsum)
+ * from K to the next multiple of 256; wsum[n] = Σ_k W[n][k].  zero (with wsum)
  * and bias are nullable.  Sums are exact integers. */
 int g2ptq_int8_gemm_workspace(int64_t T, int64_t N, int64_t K, size_t* bytes);
 int g2ptq_int8_gemm(void* stream, const int8_t* codes, int64_t ldc, const float* scale,

@@ -265,11 +265,15 @@ def test_refusals(dev):
     with pytest.raises(ValueError, match="scale"):
         int8_matmul(codes, scale[:2], lin)
     p = _lib.ptr
-    y = torch.empty(4, 8, device=dev)
-    wide = torch.zeros(4, 32, dtype=torch.int8, device=dev)
-    with pytest.raises(ValueError, match="16-byte aligned rows"):
-        _lib.call("g2ptq_int8_gemm", _lib.stream_ptr(), p(wide), 24, p(scale), None,
-                  p(lin.weight), 32, p(lin.weight_scale), None, None, 4, 8, 32, p(y), 2, 8, None, 0)
+    y = torch.empty(6, 8, device=dev)
+    wide = torch.zeros(6, 32, dtype=torch.int8, device=dev)
+    x, scale = torch.zeros(6, 32, device=dev), torch.zeros(6, device=dev)
+    ldw = lin.weight.stride(0)
+    for ldc, ldb in ((24, ldw), (32, 48)):
+        with pytest.raises(ValueError, match="16-byte aligned rows"):
+            _lib.call("g2ptq_int8_gemm", _lib.stream_ptr(), p(wide), ldc, p(scale), None,
+                      p(lin.weight), ldb, p(lin.weight_scale), None, None, 6, 8, 32, p(y), 2, 8,
+                      None, 0)
     with pytest.raises(RuntimeError, match="workspace"):
-        _lib.call("g2ptq_int8_linear", _lib.stream_ptr(), p(x), 2, 4, 32, 32, 1, p(lin.weight), 32,
-                  p(lin.weight_scale), None, None, 8, p(y), 8, None, 0)
+        _lib.call("g2ptq_int8_linear", _lib.stream_ptr(), p(x), 2, 6, 32, 32, 1, p(lin.weight),
+                  ldw, p(lin.weight_scale), None, None, 8, p(y), 8, None, 0)
