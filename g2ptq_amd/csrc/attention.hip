@@ -255,17 +255,18 @@ __device__ void clear_outside(const AttnArgs& a) {
 // DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
 // ---------------------------------------------------------------------------
 template <int BITS, int DP, bool FULL>
-__global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? (BITS == 4 ? 3 : 2) : 1) void
+attend_rows_kernel(AttnArgs a) {
   constexpr int DG = DP / 4;                  // channels of a lane's share of a key
   constexpr int KW = DG * BITS / 32;          // its words
   constexpr int KS = DP / 32;                 // products of 32 channels
   constexpr int DV = DP / 16;                 // channels of a lane's share of a value
   constexpr int VW = (DV * BITS + 31) / 32;   // its words
   constexpr int PITCH = DP + 4;
-  __shared__ uint32_t rowL[4][32];
-  __shared__ __attribute__((aligned(16))) float skL[4][32], svL[4][32];
-  __shared__ __attribute__((aligned(16))) int zvL[4][32];
-  __shared__ int zkL[4][32];
+  // a wave's steps: rows in the cache, scales, zero points (two buffers); then the join
+  __shared__ uint32_t rowL[4][2][32], zkL[4][2][32];
+  __shared__ __attribute__((aligned(16))) float skL[4][2][32], svL[4][2][32];
+  __shared__ __attribute__((aligned(8))) _Float16 zvL[4][2][32];
   __shared__ __attribute__((aligned(16))) float oL[4][16 * PITCH];
   __shared__ float mL[4][16], lL[4][16];
 
@@ -280,9 +281,10 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
   const int shares = rows > kFewRows ? 1 : a.few_split;
   if (split >= shares) return;
   const int share = share_of(sp.n, shares, 128);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int D = FULL ? DP : (int)a.c.D;
-  const int rowb = D * BITS / 8;
+  const uint32_t rowb = D * BITS / 8;
   const int half = 1 << (BITS - 1);
   const int32_t* table = a.table + b * a.ldt;
 
@@ -291,7 +293,87 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
     // the last key that the lane's row sees, and that any of the block's rows sees
     const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
     const int last_all = min(sp.pos0 + (min(r0 + 15, rows - 1)) / a.G, sp.n - 1);
-    const int k0 = split * share, k1 = min(last_all + 1, k0 + share);
+    const int k0 = split * share + 32 * wave, k1 = min(last_all + 1, (split + 1) * share);
+    const int steps = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;  // blocks of 32 keys, every 128
+
+    // A step's pages (P), rows and numbers (M, shown to the wave by S), codes (C): loaded
+    // three, two and one step ahead of the arithmetic.  Lanes 0 .. 31 are for keys, the
+    // others for values.
+    const int kv = lane >> 5;
+    int page = -1, sz = half, bad = 0;
+    uint32_t srow = 0;
+    float sc = 0.f;
+    bool sok = false;
+#define G2_P(step) page = table[max(min(k0 + (step) * 128 + (lane & 31), k1 - 1), 0) >> a.c.shift]
+#define G2_M(step)                                                                           \
+  do {                                                                                       \
+    const int key_ = k0 + (step) * 128 + (lane & 31);                                        \
+    sok = (key_ < k1) & ((uint32_t)page < (uint64_t)a.c.pages);                              \
+    bad |= (key_ < k1) & !sok;                                                               \
+    const int pg_ = sok ? page : 0, of_ = sok ? key_ & ((1 << a.c.shift) - 1) : 0;           \
+    srow = ((uint32_t)(pg_ * (int)a.c.H + h) << a.c.shift) + of_;                            \
+    sc = (kv ? a.c.scale[1] : a.c.scale[0])[srow];                                           \
+    if (a.c.zero[0]) sz = (kv ? a.c.zero[1] : a.c.zero[0])[srow];                            \
+  } while (0)
+#define G2_S(buf, ok)                                                                        \
+  do {                                                                                       \
+    if (!sok) sc = 0.f;                                                                      \
+    ok = (uint32_t)__builtin_amdgcn_ballot_w64(sok);                                         \
+    if (kv) {                                                                                \
+      svL[wave][buf][lane - 32] = sc;                                                        \
+      zvL[wave][buf][lane - 32] = centre(sz, sz)[0];                                         \
+    } else {                                                                                 \
+      rowL[wave][buf][lane] = srow;                                                          \
+      skL[wave][buf][lane] = sc * a.kscale;                                                  \
+      zkL[wave][buf][lane] = __builtin_bit_cast(uint32_t, centre(sz, sz));                   \
+    }                                                                                        \
+    __builtin_amdgcn_wave_barrier();                                                         \
+  } while (0)
+#define G2_C(buf, kw, vw)                                                                    \
+  do {                                                                                       \
+    _Pragma("unroll") for (int kb = 0; kb < 2; ++kb) {                                       \
+      const uint8_t* p_ = a.c.codes[0] + (uint64_t)rowL[wave][buf][16 * kb + n] * rowb +     \
+                          g * (DG * BITS / 8);                                               \
+      if constexpr (FULL && KW % 4 == 0) {                                                   \
+        _Pragma("unroll") for (int i = 0; i < KW / 4; ++i) {                                 \
+          const uint4 v_ = reinterpret_cast<const uint4*>(p_)[i];                            \
+          kw[kb][4 * i] = v_.x, kw[kb][4 * i + 1] = v_.y;                                    \
+          kw[kb][4 * i + 2] = v_.z, kw[kb][4 * i + 3] = v_.w;                                \
+        }                                                                                    \
+      } else {                                                                               \
+        _Pragma("unroll") for (int i = 0; i < KW / 2; ++i) { /* 8 or 16 channels */          \
+          uint2 v_ = make_uint2(0, 0);                                                       \
+          if (FULL || g * DG + i * (64 / BITS) < D)                                          \
+            v_ = reinterpret_cast<const uint2*>(p_)[i];                                      \
+          kw[kb][2 * i] = v_.x, kw[kb][2 * i + 1] = v_.y;                                    \
+        }                                                                                    \
+      }                                                                                      \
+    }                                                                                        \
+    _Pragma("unroll") for (int j = 0; j < 8; ++j) {                                          \
+      const int t_ = (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);                               \
+      uint64_t o_ = (uint64_t)rowL[wave][buf][t_] * rowb + n * (DV * BITS / 8);              \
+      if (!FULL) o_ = n * DV < D ? o_ : 0;                                                   \
+      const uint8_t* p_ = a.c.codes[1] + o_;                                                 \
+      if constexpr (DV * BITS == 16) {                                                       \
+        vw[j][0] = *reinterpret_cast<const uint16_t*>(p_);                                   \
+      } else if constexpr (VW == 1) {                                                        \
+        vw[j][0] = *reinterpret_cast<const uint32_t*>(p_);                                   \
+      } else if constexpr (VW == 2) {                                                        \
+        const uint2 v_ = *reinterpret_cast<const uint2*>(p_);                                \
+        vw[j][0] = v_.x, vw[j][1] = v_.y;                                                    \
+      } else {                                                                               \
+        const uint4 v_ = *reinterpret_cast<const uint4*>(p_);                                \
+        vw[j][0] = v_.x, vw[j][1] = v_.y, vw[j][2] = v_.z, vw[j][3] = v_.w;                  \
+      }                                                                                      \
+    }                                                                                        \
+  } while (0)
+    uint32_t ka[2][KW], va[8][VW], kb_[2][KW], vb[8][VW];
+    uint32_t oka = 0, okb = 0;
+    if (steps > 0) {
+      G2_P(0);
+      G2_M(0);
+      G2_P(1);
+    }
 
     // query: channels g·DG + 8s .. of row n, scaled into fp16
     f16x8 qf[KS];
@@ -320,137 +402,100 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < DV; ++e) acc[e] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
-    int bad = 0;
 
-    for (int j0 = k0 + 32 * wave; j0 < k1; j0 += 128) {
-      // ---- the 32 keys' rows in the cache, scales and zero points ----
+    auto arithmetic = [&](int j0, int buf, uint32_t ok, const uint32_t (&kw)[2][KW],
+                          const uint32_t (&vw)[8][VW]) __attribute__((always_inline)) {
+      float p[8], sv[8];
+      float mx = m, vx = 0.f;
+      uint32_t see = 0;  // bit i: element i = 4kb + i%4 is key 16kb + 4g + i%4 of the step
       {
-        const int key = j0 + (lane & 31), kv = lane >> 5;
-        int64_t slot = key < k1 ? a.c.slot(table, a.width, key) : -1;
-        bad |= slot == -2;
-        const uint32_t row = slot < 0 ? 0 : (uint32_t)a.c.row(slot, h);
-        const float s = slot < 0 ? 0.f : a.c.scale[kv][row];
-        const int z = a.c.zero[0] ? a.c.zero[kv][row] : half;
-        if (kv == 0) {
-          rowL[wave][lane] = row;
-          skL[wave][lane] = s * a.kscale;
-          zkL[wave][lane] = z;
-        } else {
-          svL[wave][lane - 32] = s;
-          zvL[wave][lane - 32] = z;
-        }
-        const uint32_t ok = (uint32_t)__builtin_amdgcn_ballot_w64(slot >= 0);
-        __builtin_amdgcn_wave_barrier();
-        // ---- their codes ----
-        uint32_t kw[2][KW], vw[8][VW];
+        const int c = last - j0;  // the last key seen
+        const uint32_t seen = (c < 0 ? 0u : ok) & (~0u >> (31 - min(max(c, 0), 31)));
+        see = (seen >> (4 * g) & 15u) | (seen >> (16 + 4 * g) & 15u) << 4;
+      }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const uint8_t* p =
-              a.c.codes[0] + (int64_t)rowL[wave][16 * kb + n] * rowb + g * (DG * BITS / 8);
-          if constexpr (FULL && KW % 4 == 0) {
+      for (int kb = 0; kb < 2; ++kb) {
+        const f16x2 zc = as_h2(zkL[wave][buf][16 * kb + n]);
+        f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < KW / 4; ++i) {
-              const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-              kw[kb][4 * i] = v.x, kw[kb][4 * i + 1] = v.y;
-              kw[kb][4 * i + 2] = v.z, kw[kb][4 * i + 3] = v.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < KW / 2; ++i) {  // 8 bytes: 8 or 16 channels
-              uint2 v = make_uint2(0, 0);
-              if (FULL || g * DG + i * (64 / BITS) < D) v = reinterpret_cast<const uint2*>(p)[i];
-              kw[kb][2 * i] = v.x, kw[kb][2 * i + 1] = v.y;
-            }
-          }
-        }
-        const bool von = FULL || n * DV < D;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);
-          const uint8_t* p =
-              a.c.codes[1] + (int64_t)rowL[wave][t] * rowb + n * (DV * BITS / 8);
-          if (!von) p = a.c.codes[1];
-          if constexpr (DV * BITS == 16) {
-            vw[j][0] = *reinterpret_cast<const uint16_t*>(p);
-          } else if constexpr (VW == 1) {
-            vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
-          } else if constexpr (VW == 2) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            vw[j][0] = v.x, vw[j][1] = v.y;
-          } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            vw[j][0] = v.x, vw[j][1] = v.y, vw[j][2] = v.z, vw[j][3] = v.w;
-          }
-        }
-        // ---- logits ----
-        float p[8], sv[8];
-        float mx = m, vx = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const int zk = zkL[wave][16 * kb + n];
-          const f16x2 zc = centre(zk, zk);
-          f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-          for (int s = 0; s < KS; ++s)
-            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                key_codes<BITS>(&kw[kb][s * BITS / 4], zc), qf[s], x, 0, 0, 0);
-          const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[wave][16 * kb + 4 * g]);
-          const f32x4 s4 = *reinterpret_cast<const f32x4*>(&svL[wave][16 * kb + 4 * g]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int t = 16 * kb + 4 * g + i;
-            const bool see = (ok >> t & 1) && j0 + t <= last;
-            p[4 * kb + i] = x[i] * sk[i];
-            sv[4 * kb + i] = s4[i];
-            mx = fmaxf(mx, see ? p[4 * kb + i] : -INFINITY);
-            vx = fmaxf(vx, see && s4[i] < __builtin_inff() ? s4[i] : 0.f);
-          }
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        vx = fmaxf(vx, __shfl_xor(vx, 16));
-        vx = fmaxf(vx, __shfl_xor(vx, 32));
-        // ---- the row's units ----
-        if (__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0) {
-          const float nref = vx >= ref ? above(vx) : ref;
-          float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
-          if (m == mx) f = 1.f;
-          f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
-          m = mx, ref = nref;
-          l *= f;
-#pragma unroll
-          for (int e = 0; e < DV; ++e) acc[e] *= f;
-        }
-        const float e0 = (float)(15 - exponent(ref)), m0 = m == -INFINITY ? 0.f : m;
-        f16x8 w;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int t = 16 * (i >> 2) + 4 * g + (i & 3);
-          const bool see = (ok >> t & 1) && j0 + t <= last;
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
-          l += see ? x : 0.f;
-          w[i] = (_Float16)(see ? x * sv[i] : 0.f);
-        }
-        // ---- values ----
-        f16x2 zc[4];
+        for (int s = 0; s < KS; ++s)
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes<BITS>(&kw[kb][s * BITS / 4], zc),
+                                                     qf[s], x, 0, 0, 0);
+        const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[wave][buf][16 * kb + 4 * g]);
+        const f32x4 s4 = *reinterpret_cast<const f32x4*>(&svL[wave][buf][16 * kb + 4 * g]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int t = (i < 2 ? 4 * g + 2 * i : 16 + 4 * g + 2 * i - 4);
-          zc[i] = centre(zvL[wave][t], zvL[wave][t + 1]);
+          const bool on = see >> (4 * kb + i) & 1;
+          p[4 * kb + i] = x[i] * sk[i];
+          sv[4 * kb + i] = s4[i];
+          mx = fmaxf(mx, on ? p[4 * kb + i] : -INFINITY);
+          vx = fmaxf(vx, on && s4[i] < __builtin_inff() ? s4[i] : 0.f);
         }
-#pragma unroll
-        for (int e = 0; e < DV; ++e) {
-          f16x2 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = value_codes<BITS>(&vw[2 * i][e / 8 * (BITS / 4)],
-                                     &vw[2 * i + 1][e / 8 * (BITS / 4)], e & 7, zc[i]);
-          const f16x8 vf = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
-          acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, w, acc[e], 0, 0, 0);
-        }
-        __builtin_amdgcn_wave_barrier();
       }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      vx = fmaxf(vx, __shfl_xor(vx, 16));
+      vx = fmaxf(vx, __shfl_xor(vx, 32));
+      // ---- the row's units ----
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
+        const float nref = vx >= ref ? above(vx) : ref;
+        float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
+        if (m == mx) f = 1.f;
+        f = __builtin_amdgcn_ldexpf(f, exponent(ref) - exponent(nref));
+        m = mx, ref = nref;
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < DV; ++e) acc[e] *= f;
+      }
+      asm volatile("" : "+v"(m), "+v"(ref));  // (as in attend_tiles_kernel)
+      const float e0 = (float)(15 - exponent(ref)), m0 = m == -INFINITY ? 0.f : m;
+      f16x8 w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool on = see >> i & 1;
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
+        l += on ? x : 0.f;
+        w[i] = (_Float16)(on ? x * sv[i] : 0.f);
+      }
+      // ---- values ----
+      const f16x4 z0 = *reinterpret_cast<const f16x4*>(&zvL[wave][buf][4 * g]);
+      const f16x4 z1 = *reinterpret_cast<const f16x4*>(&zvL[wave][buf][16 + 4 * g]);
+      const f16x2 zc[4] = {{z0[0], z0[1]}, {z0[2], z0[3]}, {z1[0], z1[1]}, {z1[2], z1[3]}};
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        f16x2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = value_codes<BITS>(&vw[2 * i][e / 8 * (BITS / 4)],
+                                   &vw[2 * i + 1][e / 8 * (BITS / 4)], e & 7, zc[i]);
+        const f16x8 vf = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, w, acc[e], 0, 0, 0);
+      }
+      __builtin_amdgcn_wave_barrier();
+    };
+    if (steps > 0) {
+      G2_S(0, oka);
+      G2_C(0, ka, va);
+      G2_M(1);
+      G2_P(2);
     }
+    for (int step = 0; step < steps; step += 2) {
+      G2_S(1, okb);
+      G2_C(1, kb_, vb);
+      G2_M(step + 2);
+      G2_P(step + 3);
+      arithmetic(k0 + step * 128, 0, oka, ka, va);
+      if (step + 1 == steps) break;
+      G2_S(0, oka);
+      G2_C(0, ka, va);
+      G2_M(step + 3);
+      G2_P(step + 4);
+      arithmetic(k0 + step * 128 + 128, 1, okb, kb_, vb);
+    }
+#undef G2_P
+#undef G2_M
+#undef G2_S
+#undef G2_C
     if (bad) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
 
     // ---- join the four waves: units of the block's maximum, true scale ----
@@ -474,7 +519,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
     __syncthreads();
     const float MC = M * C;  // of row n, as every wave has it
     for (int i = threadIdx.x; i < 16 * (D / 8); i += 256) {
-      // lanes of a row block are spread over rows: row = i % 16
+      // i % 16 == lane % 16: row n of this lane is row r
       const int r = i & 15, d = (i >> 4) * 8;
       if (r0 + r >= rows) continue;
       const float L = lL[0][r] + lL[1][r] + lL[2][r] + lL[3][r];
@@ -485,7 +530,6 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttnArgs a) {
         y[k] = (oL[0][r * PITCH + d + k] + oL[1][r * PITCH + d + k] + oL[2][r * PITCH + d + k] +
                 oL[3][r * PITCH + d + k]) * inv;
       if (shares > 1) {
-        // row n of this lane is row r: i % 16 == threadIdx.x % 16
         float* o = a.few_part +
                    ((((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split + split) * part_size(a);
         *reinterpret_cast<float4*>(o + d) = make_float4(y[0], y[1], y[2], y[3]);
@@ -986,25 +1030,34 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
       : a.part + row * a.split * part_size(a);
   const int D = (int)a.c.D;
   const int64_t pitch = part_size(a);
-  float M = -INFINITY;
-  for (int s = 0; s < split; ++s) M = fmaxf(M, p[s * pitch + D]);
+  // lane s has share s's maximum and sum (at most 64 shares); a share without keys has a
+  // maximum of -inf and adds nothing, unless its sum is NaN
+  float m = -INFINITY, L = 0.f;
+  if (lane < split) m = p[lane * pitch + D], L = p[lane * pitch + D + 1];
+  float M = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+  if (m != -INFINITY) L *= __builtin_amdgcn_exp2f(m - M);
+  const float w = m == -INFINITY ? 0.f : L;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   const int d = lane * 4;
-  float L = 0.f, y[4] = {0, 0, 0, 0};
-  for (int s = 0; s < split; ++s) {
-    const float m = p[s * pitch + D];
-    if (m == -INFINITY) {
-      // a share without keys adds nothing, unless its sum is NaN
-      L += p[s * pitch + D + 1];
-      continue;
-    }
-    const float w = __builtin_amdgcn_exp2f(m - M) * p[s * pitch + D + 1];
-    L += w;
-    if (d < D) {
-      const float4 o = *reinterpret_cast<const float4*>(p + s * pitch + d);
-      y[0] += w * o.x, y[1] += w * o.y, y[2] += w * o.z, y[3] += w * o.w;
+  float y[4] = {0, 0, 0, 0};
+  const float* pd = p + (d < D ? d : 0);
+  for (int s0 = 0; s0 < split; s0 += 8) {  // eight loads under way
+    float4 o[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      o[s] = *reinterpret_cast<const float4*>(pd + min(s0 + s, split - 1) * pitch);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float ws = s0 + s < split ? __shfl(w, s0 + s) : 0.f;
+      if (ws != 0.f) {  // (also where ws is NaN)
+        y[0] += ws * o[s].x, y[1] += ws * o[s].y, y[2] += ws * o[s].z, y[3] += ws * o[s].w;
+      }
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int k = 0; k < 4; ++k) y[k] *= inv;
   if (d < D) store_out(a, row * D + d, y);
@@ -1026,9 +1079,10 @@ struct Plan {
     // a batch of chunks only has sequences of few rows if some are shorter than the rest
     few = !tiles || B > 1;
     const int64_t keys = std::max<int64_t>(1, max_kv);
-    // few rows: two workgroups per CU, shares of 256 keys at least
-    few_split = std::max<int64_t>(1, std::min(cdiv(4 * kCUs, pairs), keys / 256));
-    few_split = std::min<int64_t>(few_split, 64);
+    // few rows: shares of 128 keys (a step of every wave) or more, some eight workgroups
+    // per CU (sequences of a batch differ in length), at most 64 shares
+    const int64_t want = std::min<int64_t>(64, cdiv(8 * kCUs, pairs));
+    few_split = cdiv(keys, cdiv(cdiv(keys, want), 128) * 128);
     nw = rows > 192 ? 8 : rows > 64 ? 4 : 2;
     if (D > 128) nw = rows > 64 ? 4 : 2;
     ntiles = std::max<int64_t>(1, cdiv(rows, 32 * nw));
