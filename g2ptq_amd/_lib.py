@@ -157,7 +157,7 @@ _FAST = None
 
 
 def fastcall():
-    """The CPython fast-call module of the per-batch staging entry points
+    """The CPython fast-call module of the per-batch and per-token entry points
     (``g2ptq_amd/_fastcall``, built with the library), or None when it is
     not built; it calls the same entry points as ``call``, without ctypes'
     per-argument conversions."""
@@ -170,6 +170,31 @@ def fastcall():
         except ImportError:
             _FAST = False
     return _FAST or None
+
+
+def call_fast(name, *args):
+    """``call`` through the fast-call module where it is built.  Pointers and
+    streams are addresses, a host struct its ctypes object."""
+    fast = _FAST if _FAST is not None else fastcall()
+    if fast:
+        status = getattr(fast, name)(*args)
+        if status != 0:
+            raise_status("g2ptq_" + name, status)
+        return status
+    args = [ctypes.byref(KvCacheStruct.from_address(a)) if i == 1 and name != "int8_linear" else a
+            for i, a in enumerate(args)]
+    return call("g2ptq_" + name, *args)
+
+
+def workspace_fast(name, *args):
+    """The bytes of ``g2ptq_<name>`` through the fast-call module where it is built."""
+    fast = _FAST if _FAST is not None else fastcall()
+    if fast:
+        nbytes = getattr(fast, name)(*args)
+        if nbytes < 0:
+            raise_status("g2ptq_" + name, nbytes)
+        return nbytes
+    return query_size("g2ptq_" + name, *args)
 
 
 def query_size(name, *args):
@@ -236,7 +261,7 @@ def scratch(nbytes, device):
     """A buffer for one call on the current stream: ``workspace``, or while a
     graph is captured a buffer of the graph's own (a cached one may be replaced
     by a larger one while the graph still uses it)."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
     return workspace(nbytes, device)
 
@@ -245,13 +270,18 @@ def require_current(t, what):
     """Kernels run on the current device: refuse a tensor of another one."""
     if not t.is_cuda:
         raise RuntimeError(f"{what}: a GPU tensor is needed, got one on {t.device}")
-    if t.device.index != torch._C._cuda_getDevice():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: a tensor on {t.device} while device "
                          f"{torch._C._cuda_getDevice()} is current")
 
 
+def current_stream():
+    """The current stream of the current device as an integer handle."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 def require_no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if any(t.requires_grad for t in tensors) and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: inference only (no gradient); call under torch.no_grad()")
 
 

@@ -248,7 +248,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm,
 // 16·R channels; its eight waves take turns at blocks of 128 columns, with weights and
 // codes straight from memory into v_mfma_i32_16x16x64_i8 (channels × tokens: lane
 // (n, g) holds 16 bytes of row n at 16·g of 64 columns, so that a load covers 64
-// consecutive bytes of 16 rows).  The waves' integer sums are added in LDS.
+// consecutive bytes of 16 rows).  The waves' integer sums meet in LDS.
 // FUSED: the tokens themselves are quantized here, by every workgroup, into LDS (one or
 // two tokens: cheaper than another launch before this one).
 template <int R, int TB, bool FUSED, int DT, bool SYM>
@@ -256,11 +256,12 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
                                                           int64_t ldx, bool vec) {
   constexpr int NW = 8;
   extern __shared__ __attribute__((aligned(16))) int8_t cL[];  // FUSED: T rows of K256 codes
-  __shared__ int sL[TB * 16][R * 16 + 1];
+  __shared__ __attribute__((aligned(16))) int sL[NW][TB * 16][R * 16 + 4];
   __shared__ float sxL[FUSED ? 16 : 1], zxL[FUSED ? 16 : 1];
   __shared__ float rlo[NW], rhi[NW];
   __shared__ uint32_t rtop[NW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * R);
   const int nb = (int)((a.K + 255) / 256 * 2);  // blocks of 128 columns; weights are zero past K
   const int K256 = nb * 128;
@@ -277,7 +278,6 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
       w0[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + min(wave, nb - 1) * 128 + i * 64);
       w1[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + min(wave + NW, nb - 1) * 128 + i * 64);
     }
-  for (int i = tid; i < TB * 16 * (R * 16 + 1); i += 512) (&sL[0][0])[i] = 0;
   if constexpr (FUSED) {
     for (int t = 0; t < (int)a.T; ++t) {
       Range r;
@@ -306,8 +306,6 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
       }
       __syncthreads();
     }
-  } else {
-    __syncthreads();
   }
   const int8_t* arow[TB];
 #pragma unroll
@@ -332,33 +330,39 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
     _Pragma("unroll") for (int r = 0; r < R; ++r)                                              \
     _Pragma("unroll") for (int b = 0; b < TB; ++b)                                             \
       acc[r][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(W[r][i], x_[b][i], acc[r][b], 0, 0, 0); \
-    const int nx_ = min((blk) + 2 * NW, nb - 1) * 128;                                         \
-    _Pragma("unroll") for (int r = 0; r < R; ++r)                                              \
-    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                              \
-      W[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + nx_ + i * 64);                       \
+    if ((blk) + 2 * NW < nb) {                                                                 \
+      _Pragma("unroll") for (int r = 0; r < R; ++r)                                            \
+      _Pragma("unroll") for (int i = 0; i < 2; ++i)                                            \
+        W[r][i] = *reinterpret_cast<const i32x4*>(wrow[r] + ((blk) + 2 * NW) * 128 + i * 64);  \
+    }                                                                                          \
   } while (0)
   for (int blk = wave; blk < nb; blk += 2 * NW) {
     G2_FEW(w0, blk);
     if (blk + NW < nb) G2_FEW(w1, blk + NW);
   }
 #undef G2_FEW
-  // lane holds channels 4g + v of token n
+  // lane holds channels 4g .. 4g + 3 of token n
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int b = 0; b < TB; ++b)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) atomicAdd(&sL[16 * b + n][16 * r + 4 * g + v], acc[r][b][v]);
+      *reinterpret_cast<i32x4*>(&sL[wave][16 * b + n][16 * r + 4 * g]) = acc[r][b];
   __syncthreads();
-  for (int i = tid; i < (int)a.T * 16 * R; i += 512) {
-    const int t = i / (16 * R), j = i % (16 * R);
-    const int64_t ch = n0 + j;
-    if (ch >= a.N) continue;
+  for (int i = tid; i < (int)a.T * 4 * R; i += 512) {
+    const int t = i / (4 * R), j = i % (4 * R) * 4;
+    i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s += *reinterpret_cast<const i32x4*>(&sL[w][t][j]);
     const float sx = FUSED ? sxL[t] : a.sx[t];
     const int zx = FUSED ? (int)zxL[t] : a.zx ? (int)a.zx[t] : 0;
-    store_y(a, t * a.ldo + ch,
-            scaled(a, sx, zx, sL[t][j], a.sw[ch], zx != 0 ? a.wsum[ch] : 0,
-                   a.bias ? a.bias[ch] : 0.f));
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int64_t ch = n0 + j + v;
+      if (ch < a.N)
+        store_y(a, t * a.ldo + ch,
+                scaled(a, sx, zx, s[v], a.sw[ch], zx != 0 ? a.wsum[ch] : 0,
+                       a.bias ? a.bias[ch] : 0.f));
+    }
   }
 }
 
@@ -397,7 +401,7 @@ void launch_few(hipStream_t st, const GemmI8& a) {
 
 // Channels of a workgroup of few tokens: enough workgroups for every CU first, then
 // fewer workgroups that read the codes again.
-int few_rows(int64_t N) { return N >= 16 * 4 * 256 ? 4 : N >= 16 * 2 * 256 ? 2 : 1; }
+int few_rows(int64_t N) { return N >= 16 * 4 * 192 ? 4 : N >= 16 * 2 * 192 ? 2 : 1; }
 
 template <int BM, int BN, int WM, int WN>
 void launch_tiles(hipStream_t st, const GemmI8& a) {

@@ -143,17 +143,20 @@ class Int8Linear(torch.nn.Module):
     def forward(self, x):
         x2 = _rows(x, self.in_features, "Int8Linear")
         rows, columns, out = x2.shape[0], self.in_features, self.out_features
-        if self.weight.device != x.device:
-            raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {self.weight.device}")
-        y = torch.empty(rows, out, dtype=x.dtype, device=x.device)
+        held = self._buffers  # (attribute access of a module's buffers is slow)
+        weight, total, bias = held["weight"], held["weight_sum"], held["bias"]
+        if weight.get_device() != x.get_device():
+            raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {weight.device}")
+        y = x.new_empty((rows, out))
         if rows:
-            need = _lib.query_size("g2ptq_int8_linear_workspace", rows, out, columns)
-            ws = _lib.scratch(need, x.device)
-            _lib.call("g2ptq_int8_linear", _lib.stream_ptr(x.device), _lib.ptr(x2),
-                      _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), int(self.sym),
-                      _lib.ptr(self.weight), self.weight.stride(0), _lib.ptr(self.weight_scale),
-                      _lib.ptr(self.weight_sum), _lib.ptr(self.bias), out, _lib.ptr(y), out,
-                      _lib.ptr(ws), ws.numel())
+            need = _lib.workspace_fast("int8_linear_workspace", rows, out, columns)
+            ws = _lib.scratch(need, x.device) if need else None
+            _lib.call_fast("int8_linear", _lib.current_stream(), x2.data_ptr(),
+                           _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), self.sym,
+                           weight.data_ptr(), weight.stride(0), held["weight_scale"].data_ptr(),
+                           None if total is None else total.data_ptr(),
+                           None if bias is None else bias.data_ptr(), out, y.data_ptr(), out,
+                           None if ws is None else ws.data_ptr(), need)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], out)
 
     def extra_repr(self):

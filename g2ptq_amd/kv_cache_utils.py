@@ -31,14 +31,14 @@ def _heads(x, heads, dim, what):
         raise ValueError(f"{what} of shape {tuple(x.shape)}, expected (tokens, {heads}, {dim})")
     _lib.require_current(x, what)
     _lib.require_no_grad(what, x)
-    return x if x.stride(2) == 1 and x.stride(0) >= 0 and x.stride(1) >= 0 else x.contiguous()
+    return x if x.stride(2) == 1 else x.contiguous()
 
 
 def _index(t, dtype, dims, what, device):
     if t.dtype is not dtype or t.dim() != dims:
         raise ValueError(f"{what}: a {dims}-dimensional {dtype} tensor is needed, got "
                          f"{t.dtype} of shape {tuple(t.shape)}")
-    if t.device != device:
+    if not t.is_cuda or t.get_device() != device.index:
         raise ValueError(f"{what} on {t.device}, the cache on {device}")
     rows = dims == 1 or t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
     return t if rows and (t.stride(-1) == 1 or t.shape[-1] <= 1) else t.contiguous()
@@ -82,7 +82,7 @@ class PagedKVCache:
             *(_lib.ptr(t) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale,
                                     self.k_zero, self.v_zero, self.flags)),
             num_pages, kv_heads, page_size, head_dim, bits, int(self.sym))
-        self._ref = ctypes.byref(self._struct)
+        self._address = ctypes.addressof(self._struct)
 
     def write(self, k, v, slots):
         """Quantize tokens' keys and values (tokens, kv_heads, head_dim; bf16, fp16
@@ -97,12 +97,11 @@ class PagedKVCache:
         slots = _index(slots, torch.int64, 1, "slots", self.device)
         if k.shape[0] != v.shape[0] or k.shape[0] != slots.shape[0]:
             raise ValueError(f"{k.shape[0]} keys, {v.shape[0]} values, {slots.shape[0]} slots")
-        if k.device != self.device or v.device != self.device:
-            raise ValueError(f"keys on {k.device}, values on {v.device}, the cache on "
-                             f"{self.device}")
-        _lib.call("g2ptq_kv_write", _lib.stream_ptr(self.device), self._ref, _lib.ptr(k),
-                  k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1),
-                  _DTYPE_CODE[k.dtype], k.shape[0], _lib.ptr(slots))
+        if k.get_device() != self.device.index:
+            raise ValueError(f"keys on {k.device}, the cache on {self.device}")
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+        _lib.call_fast("kv_write", _lib.current_stream(), self._address, k.data_ptr(), kt, kh,
+                       v.data_ptr(), vt, vh, _DTYPE_CODE[k.dtype], k.shape[0], slots.data_ptr())
 
     def read(self, table, cu_tokens, total, dtype=torch.bfloat16):
         """``(k, v)``, each (total, kv_heads, head_dim) of ``dtype``: rows
@@ -120,9 +119,10 @@ class PagedKVCache:
         _lib.require_current(self.flags, "PagedKVCache.read")
         k = torch.empty(total, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        _lib.call("g2ptq_kv_read", _lib.stream_ptr(self.device), self._ref, _lib.ptr(table),
-                  max(table.stride(0), table.shape[1]), table.shape[0], table.shape[1],
-                  _lib.ptr(cu), total, _lib.ptr(k), _lib.ptr(v), _DTYPE_CODE[dtype])
+        B, width = table.shape
+        _lib.call_fast("kv_read", _lib.current_stream(), self._address, table.data_ptr(),
+                       max(table.stride(0), width), B, width, cu.data_ptr(), total, k.data_ptr(),
+                       v.data_ptr(), _DTYPE_CODE[dtype])
         return k, v
 
     def check(self):
@@ -154,7 +154,7 @@ def paged_attention(q, cache, table, cu_q, kv_lens, scale=None, max_q=None, max_
         raise ValueError(f"queries of shape {tuple(q.shape)} over {cache.kv_heads} heads of the "
                          "cache")
     q = _heads(q, q.shape[1], cache.head_dim, "queries")
-    if q.device != cache.device:
+    if q.get_device() != cache.device.index:
         raise ValueError(f"queries on {q.device}, the cache on {cache.device}")
     table = _index(table, torch.int32, 2, "table", cache.device)
     cu_q = _index(cu_q, torch.int32, 1, "cu_q", cache.device)
@@ -166,13 +166,14 @@ def paged_attention(q, cache, table, cu_q, kv_lens, scale=None, max_q=None, max_
     max_q = T if max_q is None else max(0, min(int(max_q), T))
     room = width * cache.page_size
     max_kv = room if max_kv is None else max(0, min(int(max_kv), room))
-    out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
-    need = _lib.query_size("g2ptq_paged_attention_workspace", T, heads, cache.kv_heads, dim, B,
-                           max_q, max_kv)
-    ws = _lib.scratch(need, q.device)
-    _lib.call("g2ptq_paged_attention", _lib.stream_ptr(q.device), cache._ref, _lib.ptr(q),
-              q.stride(0), q.stride(1), _DTYPE_CODE[q.dtype], T, heads, _lib.ptr(table),
-              max(table.stride(0), width), B, width, _lib.ptr(cu_q), _lib.ptr(kv_lens), max_q,
-              max_kv, 1.0 / math.sqrt(dim) if scale is None else float(scale), _lib.ptr(out),
-              _lib.ptr(ws), ws.numel())
+    out = q.new_empty((T, heads, dim))
+    need = _lib.workspace_fast("paged_attention_workspace", T, heads, cache.kv_heads, dim, B,
+                               max_q, max_kv)
+    ws = _lib.scratch(need, q.device) if need else None
+    q_token, q_head, _ = q.stride()
+    _lib.call_fast("paged_attention", _lib.current_stream(), cache._address, q.data_ptr(),
+                   q_token, q_head, _DTYPE_CODE[q.dtype], T, heads, table.data_ptr(),
+                   max(table.stride(0), width), B, width, cu_q.data_ptr(), kv_lens.data_ptr(),
+                   max_q, max_kv, 1.0 / math.sqrt(dim) if scale is None else float(scale),
+                   out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out
