@@ -267,22 +267,20 @@ def scratch(nbytes, device):
 
 
 def require_current(t, what):
-    """Kernels run on the current device: refuse a tensor of another one."""
+    """Kernels run on the current device and have no gradients: refuse a tensor of
+    another device, and one that a gradient is recorded for."""
     if not t.is_cuda:
         raise RuntimeError(f"{what}: a GPU tensor is needed, got one on {t.device}")
     if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: a tensor on {t.device} while device "
                          f"{torch._C._cuda_getDevice()} is current")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: inference only (no gradient); call under torch.no_grad()")
 
 
 def current_stream():
     """The current stream of the current device as an integer handle."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-
-
-def require_no_grad(what, *tensors):
-    if any(t.requires_grad for t in tensors) and torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: inference only (no gradient); call under torch.no_grad()")
 
 
 def release_workspaces():

@@ -90,28 +90,55 @@ __device__ __forceinline__ void store8(void* p, int64_t at, bool vec, int n, con
   }
 }
 
-// Range of a group: min(x, 0) and max(x, 0), and the largest |x| by its bits,
-// which orders NaN above infinity above every number.
+// Range of a group: the largest |x| by its bits, which orders NaN above infinity
+// above every number; in the asymmetric grid min(x, 0) and max(x, 0) too.
+template <bool SYM>
 struct Range {
   float lo = 0.f, hi = 0.f;
   uint32_t top = 0;
   __device__ __forceinline__ void add(float x) {
-    lo = fminf(lo, x);
-    hi = fmaxf(hi, x);
+    if (!SYM) {
+      lo = fminf(lo, x);
+      hi = fmaxf(hi, x);
+    }
     top = max(top, __float_as_uint(x) & 0x7fffffffu);
   }
   __device__ __forceinline__ void merge(float l, float h, uint32_t t) {
-    lo = fminf(lo, l);
-    hi = fmaxf(hi, h);
+    if (!SYM) {
+      lo = fminf(lo, l);
+      hi = fmaxf(hi, h);
+    }
     top = max(top, t);
   }
 };
 
-template <int L>
-__device__ __forceinline__ void reduce_range(Range& r) {  // over L neighbouring lanes
+// x of another lane of the same 16: neighbours, pairs, halves of 8, halves of 16 (once
+// all lanes below agree, the mirrors bring the other half's value).
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL, bool SYM>
+__device__ __forceinline__ void merge_dpp(Range<SYM>& r) {
+  float l = 0.f, h = 0.f;
+  if (!SYM) {
+    l = __uint_as_float(dpp<CTRL>(__float_as_uint(r.lo)));
+    h = __uint_as_float(dpp<CTRL>(__float_as_uint(r.hi)));
+  }
+  r.merge(l, h, dpp<CTRL>(r.top));
+}
+
+// Over L neighbouring lanes (a power of two); every lane gets the result.
+template <int L, bool SYM>
+__device__ __forceinline__ void reduce_range(Range<SYM>& r) {
+  if (L >= 2) merge_dpp<0xb1>(r);    // quad_perm 1 0 3 2
+  if (L >= 4) merge_dpp<0x4e>(r);    // quad_perm 2 3 0 1
+  if (L >= 8) merge_dpp<0x141>(r);   // row_half_mirror
+  if (L >= 16) merge_dpp<0x140>(r);  // row_mirror
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1)
-    r.merge(__shfl_xor(r.lo, o, L), __shfl_xor(r.hi, o, L), __shfl_xor(r.top, o, L));
+  for (int o = 16; o < L; o *= 2)
+    r.merge(SYM ? 0.f : __shfl_xor(r.lo, o), SYM ? 0.f : __shfl_xor(r.hi, o),
+            __shfl_xor(r.top, o));
 }
 
 struct Grid {
@@ -120,7 +147,7 @@ struct Grid {
 };
 
 template <bool SYM>
-__device__ __forceinline__ Grid make_grid(const Range& r, int bits) {
+__device__ __forceinline__ Grid make_grid(const Range<SYM>& r, int bits) {
   Grid g;
   const float levels = (float)((1 << bits) - 1);
   g.minq = -(float)(1 << (bits - 1));

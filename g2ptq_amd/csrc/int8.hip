@@ -20,24 +20,44 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int64_t kMaxK = 65536;
 
 // ---------------------------------------------------------------------------
-// Token quantiser: one workgroup per token.  Codes are written in rows of ldc
-// bytes, columns from K up to the next multiple of 16 as zeros.
+// Token quantiser: one workgroup per token, its row in registers between the range and
+// the codes where it fits (V pieces of eight values per thread; V = 0: read again).
+// Codes are written in rows of ldc bytes, columns from K up to the next multiple of 16
+// as zeros.
 // ---------------------------------------------------------------------------
-template <int DT, bool SYM>
-__global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __restrict__ x,
-                                                              int64_t K, int64_t ldx, bool vec,
+__device__ __forceinline__ uint2 eight_codes(const Grid& g, const float (&v)[8], int n) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) w[i >> 2] |= ((uint32_t)to_code(g, v[i]) & 0xffu) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
+}
+
+template <int DT, bool SYM, int V>
+__global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __restrict__ x, int K,
+                                                              int64_t ldx, bool vec,
                                                               int8_t* __restrict__ codes,
                                                               int64_t ldc, float* scale,
                                                               float* zero) {
   __shared__ float slo[4], shi[4];
   __shared__ uint32_t stop[4];
   const int64_t t = blockIdx.x, row = t * ldx;
-  Range r;
-  for (int64_t k = threadIdx.x * 8; k < K; k += 256 * 8) {
-    float v[8];
-    load8<DT>(x, row + k, vec, (int)min<int64_t>(8, K - k), v);
+  const int k0 = threadIdx.x * 8;
+  float v[V ? V : 1][8];
+  Range<SYM> r;
+  if constexpr (V > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.add(v[i]);
+    for (int p = 0; p < V; ++p) load8<DT>(x, row + k0 + p * 2048, vec, K - k0 - p * 2048, v[p]);
+#pragma unroll
+    for (int p = 0; p < V; ++p)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.add(v[p][i]);
+  } else {
+    for (int k = k0; k < K; k += 2048) {
+      load8<DT>(x, row + k, vec, K - k, v[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.add(v[0][i]);
+    }
   }
   reduce_range<64>(r);
   const int wave = threadIdx.x >> 6;
@@ -50,16 +70,18 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __rest
     scale[t] = g.s;
     if (!SYM) zero[t] = g.z;
   }
-  const int64_t K16 = (K + 15) / 16 * 16;
-  for (int64_t k = threadIdx.x * 8; k < K16; k += 256 * 8) {
-    float v[8];
-    const int n = (int)min<int64_t>(8, K - k);
-    load8<DT>(x, row + k, vec, n, v);
-    uint32_t w[2] = {0, 0};
+  const int K16 = (K + 15) / 16 * 16;
+  if constexpr (V > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) w[i >> 2] |= ((uint32_t)to_code(g, v[i]) & 0xffu) << (8 * (i & 3));
-    *reinterpret_cast<uint2*>(codes + t * ldc + k) = make_uint2(w[0], w[1]);
+    for (int p = 0; p < V; ++p) {
+      const int k = k0 + p * 2048;
+      if (k < K16) *reinterpret_cast<uint2*>(codes + t * ldc + k) = eight_codes(g, v[p], K - k);
+    }
+  } else {
+    for (int k = k0; k < K16; k += 2048) {
+      load8<DT>(x, row + k, vec, K - k, v[0]);
+      *reinterpret_cast<uint2*>(codes + t * ldc + k) = eight_codes(g, v[0], K - k);
+    }
   }
 }
 
@@ -280,7 +302,7 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
     }
   if constexpr (FUSED) {
     for (int t = 0; t < (int)a.T; ++t) {
-      Range r;
+      Range<SYM> r;
       for (int k = tid * 8; k < a.K; k += 512 * 8) {
         float v[8];
         load8<DT>(x, t * ldx + k, vec, min(8, (int)a.K - k), v);
@@ -296,13 +318,8 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* 
       if (tid == 0) sxL[t] = gr.s, zxL[t] = gr.z;
       for (int k = tid * 8; k < K256; k += 512 * 8) {
         float v[8];
-        const int m = min(8, (int)a.K - k);
-        load8<DT>(x, t * ldx + k, vec, m, v);
-        uint32_t o[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < m) o[i >> 2] |= ((uint32_t)to_code(gr, v[i]) & 0xffu) << (8 * (i & 3));
-        *reinterpret_cast<uint2*>(cL + t * K256 + k) = make_uint2(o[0], o[1]);
+        load8<DT>(x, t * ldx + k, vec, (int)a.K - k, v);
+        *reinterpret_cast<uint2*>(cL + t * K256 + k) = eight_codes(gr, v, (int)a.K - k);
       }
       __syncthreads();
     }
@@ -371,12 +388,20 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 int quantize_tokens(hipStream_t st, const void* x, int dtype, int64_t T, int64_t K, int64_t ldx,
                     int sym, int8_t* codes, int64_t ldc, float* scale, float* zero) {
   const bool vec = aligned16(x) && ldx * (dtype == 2 ? 4 : 2) % 16 == 0;
-#define G2_QT(DT, SYM)                                                                       \
-  hipLaunchKernelGGL((quantize_tokens_kernel<DT, SYM>), dim3((unsigned)T), dim3(256), 0, st, \
-                     x, K, ldx, vec, codes, ldc, scale, zero)
+#define G2_QV(DT, SYM, V)                                                                       \
+  hipLaunchKernelGGL((quantize_tokens_kernel<DT, SYM, V>), dim3((unsigned)T), dim3(256), 0, st, \
+                     x, (int)K, ldx, vec, codes, ldc, scale, zero)
+#define G2_QT(DT, SYM)                     \
+  do {                                     \
+    if (K <= 2048) G2_QV(DT, SYM, 1);      \
+    else if (K <= 4096) G2_QV(DT, SYM, 2); \
+    else if (K <= 8192) G2_QV(DT, SYM, 4); \
+    else G2_QV(DT, SYM, 0);                \
+  } while (0)
   if (dtype == 0) { if (sym) G2_QT(0, true); else G2_QT(0, false); }
   else if (dtype == 1) { if (sym) G2_QT(1, true); else G2_QT(1, false); }
   else { if (sym) G2_QT(2, true); else G2_QT(2, false); }
+#undef G2_QV
 #undef G2_QT
   G2PTQ_LAUNCHED();
   return G2PTQ_OK;

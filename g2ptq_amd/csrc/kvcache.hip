@@ -21,30 +21,31 @@ struct WriteArgs {
   const void* x[2];        // keys, values: T × H × D, channels contiguous
   int64_t st[2], sh[2];    // strides of token and head (elements)
   const int64_t* slots;    // page·(page size) + offset; negative: not written
-  int64_t T;
+  uint32_t items;          // T·H
   KvCache c;
   bool vec[2];
 };
 
-// L lanes hold one token's head, eight channels each (lanes past D idle).
+// L lanes hold one token's head, eight channels each (lanes past D idle), and reduce
+// it among themselves; a workgroup takes 256 / L consecutive heads of the T × H.
 // grid.y: 0 keys, 1 values.
 template <int DT, bool SYM, int L>
 __global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
   const int w = blockIdx.y;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 8;
-  if (item >= a.T * a.c.H) return;
-  const int64_t t = item / a.c.H, h = item - t * a.c.H;
+  if (item >= a.items) return;
+  const uint32_t t = item / (uint32_t)a.c.H, h = item - t * (uint32_t)a.c.H;
   const int64_t slot = a.slots[t];
+  const bool on = d < a.c.D;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (on) load8<DT>(a.x[w], t * a.st[w] + h * a.sh[w] + d, a.vec[w], 8, v);
   if (slot < 0) return;
   if (slot >= a.c.pages << a.c.shift) {
     if (d == 0) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
     return;
   }
-  const bool on = d < a.c.D;
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (on) load8<DT>(a.x[w], t * a.st[w] + h * a.sh[w] + d, a.vec[w], 8, v);
-  Range r;
+  Range<SYM> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.add(v[i]);
   reduce_range<L>(r);
@@ -77,38 +78,63 @@ struct ReadArgs {
   const int32_t* cu;  // B + 1 offsets of the sequences in the output
   int64_t total;
   void* out[2];       // total × H × D
+  int tokens;         // of a workgroup, at most kReadTokens
 };
 
-// One output token's head per L lanes, as in kv_write_kernel.  Output rows
+constexpr int kReadTokens = 64;
+
+// A workgroup takes `tokens` consecutive output rows: their slots first (one thread each),
+// then their pieces of 16 channels, consecutive threads consecutive pieces.  Output rows
 // outside every sequence, and tokens whose page is not in the cache, are zero.
-template <int DT, bool SYM, int L>
+template <int DT, int BITS>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
+  __shared__ int64_t slotL[kReadTokens];
   const int w = blockIdx.y;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const int d = (threadIdx.x % L) * 8;
-  if (item >= a.total * a.c.H || d >= a.c.D) return;
-  const int64_t t = item / a.c.H, h = item - t * a.c.H;
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  const int64_t slot = a.c.find(a.table, a.ldt, a.width, a.cu, a.B, t);
-  if (slot >= 0) {
-    const int64_t at = a.c.row(slot, h);
-    const float s = a.c.scale[w][at];
-    const int z = SYM ? 1 << (a.c.bits - 1) : a.c.zero[w][at];
-    if (a.c.bits == 8) {
-      const uint2 o = *reinterpret_cast<const uint2*>(a.c.codes[w] + at * a.c.D + d);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = s * (float)((int)((i < 4 ? o.x : o.y) >> (8 * (i & 3)) & 0xffu) - z);
-    } else {
-      const uint32_t o =
-          *reinterpret_cast<const uint32_t*>(a.c.codes[w] + at * (a.c.D / 2) + d / 2);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = s * (float)((int)(o >> (4 * i) & 15u) - z);
-    }
-  } else if (slot == -2 && d == 0) {
-    atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int n = (int)min<int64_t>(a.tokens, a.total - t0);
+  if ((int)threadIdx.x < n) {
+    const int64_t slot = a.c.find(a.table, a.ldt, a.width, a.cu, a.B, t0 + threadIdx.x);
+    if (slot == -2) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+    slotL[threadIdx.x] = slot;
   }
-  store8<DT>(a.out[w], item * a.c.D + d, true, 8, v);
+  __syncthreads();
+  // piece = (token t, head h, 16 channels c), counted on by 256 in mixed radix
+  const uint32_t C = (uint32_t)a.c.D / 16, H = (uint32_t)a.c.H, rest = 256 / C;
+  const uint32_t dc = 256 - rest * C, dt = rest / H, dh = rest - dt * H;
+  uint32_t q = threadIdx.x / C, c = threadIdx.x - q * C, t = q / H, h = q - t * H;
+  const int64_t base = t0 * H * C;
+  for (uint32_t piece = threadIdx.x; t < (uint32_t)n; piece += 256) {
+    const int64_t slot = slotL[t];
+    float lo[8] = {0, 0, 0, 0, 0, 0, 0, 0}, hi[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (slot >= 0) {
+      const int64_t at = a.c.row(slot, h);
+      const float s = a.c.scale[w][at];
+      const int z = a.c.zero[w] ? a.c.zero[w][at] : 1 << (BITS - 1);
+      uint32_t u[4];
+      if constexpr (BITS == 8) {
+        const uint4 o = *reinterpret_cast<const uint4*>(a.c.codes[w] + at * a.c.D + c * 16);
+        u[0] = o.x, u[1] = o.y, u[2] = o.z, u[3] = o.w;
+      } else {
+        const uint2 o = *reinterpret_cast<const uint2*>(a.c.codes[w] + at * (a.c.D / 2) + c * 8);
+        u[0] = o.x, u[1] = o.y, u[2] = u[3] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (BITS == 8) {
+          lo[i] = s * (float)((int)(u[i >> 2] >> (8 * (i & 3)) & 0xffu) - z);
+          hi[i] = s * (float)((int)(u[2 + (i >> 2)] >> (8 * (i & 3)) & 0xffu) - z);
+        } else {
+          lo[i] = s * (float)((int)(u[0] >> (4 * i) & 15u) - z);
+          hi[i] = s * (float)((int)(u[1] >> (4 * i) & 15u) - z);
+        }
+      }
+    }
+    store8<DT>(a.out[w], (base + piece) * 16, true, 8, lo);
+    store8<DT>(a.out[w], (base + piece) * 16 + 8, true, 8, hi);
+    c += dc, h += dh, t += dt;
+    if (c >= C) c -= C, ++h;
+    if (h >= H) h -= H, ++t;
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -172,12 +198,12 @@ extern "C" int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const v
   a.vec[0] = aligned16(k) && k_token * e % 16 == 0 && k_head * e % 16 == 0;
   a.vec[1] = aligned16(v) && v_token * e % 16 == 0 && v_head * e % 16 == 0;
   a.slots = slots;
-  a.T = T;
+  a.items = (uint32_t)(T * a.c.H);
   hipStream_t st = as_stream(stream);
   const bool sym = cache->sym != 0;
   return by_lanes(a.c.D, [&](auto lanes) -> int {
     constexpr int L = decltype(lanes)::value;
-    const dim3 grid((unsigned)cdiv(T * a.c.H * L, 256), 2);
+    const dim3 grid((unsigned)cdiv(T * a.c.H, 256 / L), 2);
 #define G2_WR(DT, SYM) \
   hipLaunchKernelGGL((kv_write_kernel<DT, SYM, L>), grid, dim3(256), 0, st, a)
     if (dtype == 0) { if (sym) G2_WR(0, true); else G2_WR(0, false); }
@@ -203,18 +229,24 @@ extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const in
   G2PTQ_CHECK(aligned16(k) && aligned16(v), "kv_read: outputs not 16-byte aligned");
   a.table = table, a.ldt = ldt, a.B = B, a.width = width, a.cu = cu, a.total = total;
   a.out[0] = k, a.out[1] = v;
+  // some eight pieces per thread, fewer where that leaves CUs idle
+  const int64_t pieces = a.c.H * a.c.D / 16;
+  int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(kReadTokens, 2048 / pieces));
+  while (tokens > 1 && cdiv(total, tokens) < 1024) tokens /= 2;
+  a.tokens = (int)tokens;
   hipStream_t st = as_stream(stream);
-  const bool sym = cache->sym != 0;
-  return by_lanes(a.c.D, [&](auto lanes) -> int {
-    constexpr int L = decltype(lanes)::value;
-    const dim3 grid((unsigned)cdiv(total * a.c.H * L, 256), 2);
-#define G2_RD(DT, SYM) \
-  hipLaunchKernelGGL((kv_read_kernel<DT, SYM, L>), grid, dim3(256), 0, st, a)
-    if (dtype == 0) { if (sym) G2_RD(0, true); else G2_RD(0, false); }
-    else if (dtype == 1) { if (sym) G2_RD(1, true); else G2_RD(1, false); }
-    else { if (sym) G2_RD(2, true); else G2_RD(2, false); }
+  const dim3 grid((unsigned)cdiv(total, tokens), 2);
+#define G2_RD(DT)                                                                          \
+  do {                                                                                     \
+    if (a.c.bits == 8)                                                                     \
+      hipLaunchKernelGGL((kv_read_kernel<DT, 8>), grid, dim3(256), 0, st, a);              \
+    else                                                                                   \
+      hipLaunchKernelGGL((kv_read_kernel<DT, 4>), grid, dim3(256), 0, st, a);              \
+  } while (0)
+  if (dtype == 0) G2_RD(0);
+  else if (dtype == 1) G2_RD(1);
+  else G2_RD(2);
 #undef G2_RD
-    G2PTQ_LAUNCHED();
-    return G2PTQ_OK;
-  });
+  G2PTQ_LAUNCHED();
+  return G2PTQ_OK;
 }

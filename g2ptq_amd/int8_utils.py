@@ -25,7 +25,6 @@ def _rows(x, columns, what):
         raise ValueError(f"{what}: tokens of shape {tuple(x.shape)} where the last dimension "
                          f"should be {columns}")
     _lib.require_current(x, what)
-    _lib.require_no_grad(what, x)
     x2 = x if x.dim() == 2 else x.reshape(-1, columns)
     if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < columns):
         x2 = x2.contiguous()

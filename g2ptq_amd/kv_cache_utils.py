@@ -27,10 +27,10 @@ _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _heads(x, heads, dim, what):
     """``x`` (tokens, heads, dim) with contiguous channels on the GPU."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim:
-        raise ValueError(f"{what} of shape {tuple(x.shape)}, expected (tokens, {heads}, {dim})")
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{what} of shape {tuple(shape)}, expected (tokens, {heads}, {dim})")
     _lib.require_current(x, what)
-    _lib.require_no_grad(what, x)
     return x if x.stride(2) == 1 else x.contiguous()
 
 
@@ -40,8 +40,11 @@ def _index(t, dtype, dims, what, device):
                          f"{t.dtype} of shape {tuple(t.shape)}")
     if not t.is_cuda or t.get_device() != device.index:
         raise ValueError(f"{what} on {t.device}, the cache on {device}")
-    rows = dims == 1 or t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
-    return t if rows and (t.stride(-1) == 1 or t.shape[-1] <= 1) else t.contiguous()
+    return t if t.is_contiguous() or _rows_apart(t) else t.contiguous()
+
+
+def _rows_apart(t):
+    return t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]
 
 
 class PagedKVCache:
@@ -95,13 +98,14 @@ class PagedKVCache:
             raise NotImplementedError(f"PagedKVCache.write takes bf16, fp16 or fp32 keys and "
                                       f"values, got {k.dtype} and {v.dtype}")
         slots = _index(slots, torch.int64, 1, "slots", self.device)
-        if k.shape[0] != v.shape[0] or k.shape[0] != slots.shape[0]:
-            raise ValueError(f"{k.shape[0]} keys, {v.shape[0]} values, {slots.shape[0]} slots")
+        n = len(k)
+        if n != len(v) or n != len(slots):
+            raise ValueError(f"{n} keys, {len(v)} values, {len(slots)} slots")
         if k.get_device() != self.device.index:
             raise ValueError(f"keys on {k.device}, the cache on {self.device}")
         (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
         _lib.call_fast("kv_write", _lib.current_stream(), self._address, k.data_ptr(), kt, kh,
-                       v.data_ptr(), vt, vh, _DTYPE_CODE[k.dtype], k.shape[0], slots.data_ptr())
+                       v.data_ptr(), vt, vh, _DTYPE_CODE[k.dtype], n, slots.data_ptr())
 
     def read(self, table, cu_tokens, total, dtype=torch.bfloat16):
         """``(k, v)``, each (total, kv_heads, head_dim) of ``dtype``: rows
