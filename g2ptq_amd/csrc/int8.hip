@@ -118,16 +118,85 @@ __device__ __forceinline__ void store_y(const GemmI8& a, int64_t o, float y) {
 // ahead into registers and written to the other buffer during the products, one
 // barrier a stage.  LDS rows are 128 bytes, the 16-byte chunk c of row r at
 // c ^ f(r), f(r) = (r & 7) ^ ((r >> 3) & 1): fragment reads (16 consecutive rows, one
-// chunk) are free of bank conflicts.
+// chunk) are free of bank conflicts.  S > 1: S groups of waves share K and add their
+// integer sums in LDS (tiles too few for the chip, which then wait for each stage's loads).
 constexpr int KS = 128;
 __device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
 
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm, int tn) {
-  constexpr int NT = 64 * WM * WN;
+// A wave's rows × columns of the tile: scaled, turned in LDS (its own part of it) so that
+// rows are written in 16-byte pieces.  32×32 output: lane holds rows
+// 8(v/4) + 4·(lane/32) + v%4 of column lane%32.
+template <int DT, int MT, int NTL>
+__device__ __forceinline__ void finish_tile(const GemmI8& a, const i32x16 (&acc)[MT][NTL],
+                                            int64_t t0, int64_t n0, const float* sxL,
+                                            const int* zxL, int8_t* mine, int lane) {
+  constexpr int E = DT == 2 ? 4 : 2, BYTES = NTL * 32 * E, PITCH = BYTES + 16;
+  constexpr int LPR = BYTES / 16, RPP = 64 / LPR;  // lanes of a row, rows of a pass
+  const int lr = lane & 31, lh = lane >> 5;
+  float sw[NTL], bias[NTL];
+  int wsum[NTL];
+#pragma unroll
+  for (int n = 0; n < NTL; ++n) {
+    const int64_t j = min<int64_t>(n0 + n * 32 + lr, a.N - 1);
+    sw[n] = a.sw[j];
+    bias[n] = a.bias ? a.bias[j] : 0.f;
+    wsum[n] = a.zx ? a.wsum[j] : 0;
+  }
+  const bool whole = n0 + NTL * 32 <= a.N && a.ldo * E % 16 == 0 &&
+                     (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int r = 8 * (v >> 2) + 4 * lh + (v & 3);
+      const float sx = sxL[m * 32 + r];
+      const int zx = zxL[m * 32 + r];
+#pragma unroll
+      for (int n = 0; n < NTL; ++n) {
+        const float y = scaled(a, sx, zx, acc[m][n][v], sw[n], wsum[n], bias[n]);
+        int8_t* to = mine + r * PITCH + (n * 32 + lr) * E;
+        if constexpr (DT == 0) *reinterpret_cast<__bf16*>(to) = (__bf16)y;
+        else if constexpr (DT == 1) *reinterpret_cast<_Float16*>(to) = (_Float16)y;
+        else *reinterpret_cast<float*>(to) = y;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    int8_t* out = static_cast<int8_t*>(a.out) + ((t0 + m * 32) * a.ldo + n0) * E;
+    const int rows = (int)min<int64_t>(32, a.T - t0 - m * 32);
+    if (whole) {
+#pragma unroll
+      for (int p = 0; p < 32 / RPP; ++p) {
+        const int r = p * RPP + lane / LPR, c = lane % LPR * 16;
+        if (r < rows)
+          *reinterpret_cast<i32x4*>(out + r * a.ldo * E + c) =
+              *reinterpret_cast<const i32x4*>(mine + r * PITCH + c);
+      }
+    } else {
+      const int cols = (int)min<int64_t>(NTL * 32, a.N - n0);
+      for (int i = lane; i < 32 * NTL * 32; i += 64) {
+        const int r = i / (NTL * 32), c = i % (NTL * 32);
+        if (r < rows && c < cols) {
+          if constexpr (E == 2)
+            *reinterpret_cast<uint16_t*>(out + (r * a.ldo + c) * E) =
+                *reinterpret_cast<const uint16_t*>(mine + r * PITCH + c * E);
+          else
+            *reinterpret_cast<uint32_t*>(out + (r * a.ldo + c) * E) =
+                *reinterpret_cast<const uint32_t*>(mine + r * PITCH + c * E);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN * S) void gemm_i8_kernel(GemmI8 a, int tm, int tn) {
+  constexpr int NT = 64 * WM * WN;                      // threads of a group
   constexpr int MT = BM / WM / 32, NTL = BN / WN / 32;  // 32×32 tiles of a wave
   constexpr int AL = BM * 8 / NT, BL = BN * 8 / NT;     // 16-byte loads of a thread per stage
-  __shared__ __attribute__((aligned(16))) int8_t Ls[2][(BM + BN) * KS];
+  __shared__ __attribute__((aligned(16))) int8_t Lall[S][2][(BM + BN) * KS];
+  __shared__ float sxL[BM];
+  __shared__ int zxL[BM];
 
   // Workgroups go round the 8 XCDs: an XCD takes a contiguous range of tiles, in bands of
   // eight token tiles walked channel tile by channel tile.
@@ -140,8 +209,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm,
   const int band = id / (8 * tn), in = id - band * 8 * tn, h = min(8, tm - band * 8);
   const int64_t t0 = (int64_t)(band * 8 + in % h) * BM, n0 = (int64_t)(in / h) * BN;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
-  const int wm = wave / WN, wn = wave % WN;
+  const int group = S == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
+  const int tid = (int)threadIdx.x - group * NT, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, lh = lane >> 5, wm = wave / WN, wn = wave % WN;
+  int8_t(&Ls)[2][(BM + BN) * KS] = Lall[group];
+  if ((int)threadIdx.x < BM) {
+    const int64_t i = min<int64_t>(t0 + threadIdx.x, a.T - 1);
+    sxL[threadIdx.x] = a.sx[i];
+    zxL[threadIdx.x] = a.zx ? (int)a.zx[i] : 0;
+  }
   const int row = tid >> 3, c = tid & 7;  // load i: row + i·NT/8
   const int8_t* Ab = a.A + t0 * a.lda;
   const int8_t* Wb = a.W + n0 * a.ldw;
@@ -154,11 +230,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm,
     boff[i] = (uint32_t)min<int64_t>(row + i * (NT / 8), a.N - 1 - n0) * (uint32_t)a.ldw + c * 16;
   const int lpos = row * KS + ((c ^ swz(row)) << 4);  // (NT/8 is a multiple of 16)
   const uint32_t klast = (uint32_t)((a.K + 15) / 16 * 16 - 16);
-  const int nk = (int)((a.K + 255) / 256 * 2);  // even; weights are zero past K
+  // stages, even in number (weights are zero past K), and the group's share of them
+  const int all = (int)((a.K + 255) / 256 * 2);
+  const int each = S == 1 ? all : (all + 2 * S - 1) / (2 * S) * 2;
+  const int first = group * each, nk = min(first + each, all);
   i32x4 xa[AL], xb[BL], ya[AL], yb[BL];
 #define G2_LOAD(R, st)                                                              \
   do {                                                                              \
-    const uint32_t k_ = (uint32_t)((st) < nk ? (st) : nk - 1) * KS;                 \
+    const uint32_t k_ = (uint32_t)min(st, all - 1) * KS;                            \
     const uint32_t ka_ = min(k_ + c * 16, klast);                                   \
     _Pragma("unroll") for (int i = 0; i < AL; ++i)                                  \
       R##a[i] = *reinterpret_cast<const i32x4*>(Ab + (aoff[i] + ka_));              \
@@ -216,20 +295,20 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm,
     }                                                                                     \
     __builtin_amdgcn_sched_barrier(0);                                                    \
   } while (0)
-  G2_LOAD(x, 0);
+  G2_LOAD(x, first);
   G2_STORE(x, 0);
-  G2_LOAD(x, 1);
-  G2_LOAD(y, 2);
+  G2_LOAD(x, first + 1);
+  G2_LOAD(y, first + 2);
   __syncthreads();
-  for (int kt = 0; kt < nk; kt += 2) {
+  for (int kt = first; kt < first + each; kt += 2) {
     __builtin_amdgcn_sched_barrier(0);
-    G2_MMA(0);      // stage kt
+    if (S == 1 || kt < nk) G2_MMA(0);      // stage kt
     G2_STORE(x, 1);  // stage kt + 1
     G2_LOAD(x, kt + 3);
     G2_PATTERN();
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
-    G2_MMA(1);      // stage kt + 1
+    if (S == 1 || kt < nk) G2_MMA(1);      // stage kt + 1
     G2_STORE(y, 0);  // stage kt + 2
     G2_LOAD(y, kt + 4);
     G2_PATTERN();
@@ -239,31 +318,42 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(GemmI8 a, int tm,
 #undef G2_STORE
 #undef G2_MMA
 #undef G2_PATTERN
-  // 32×32 output: lane holds rows 8(v/4) + 4·(lane/32) + v%4 of column lane%32
-  float sw[NTL], bias[NTL];
-  int wsum[NTL];
+  if constexpr (S > 1) {  // the groups' sums, in the first group's registers
+    int* sums = reinterpret_cast<int*>(&Lall[0][0][0]);
+    constexpr int TILE = MT * NTL * 16 * NT;
+    static_assert((S - 1) * TILE * 4 <= (int)sizeof(Lall), "sums do not fit");
+    if (group > 0)
 #pragma unroll
-  for (int n = 0; n < NTL; ++n) {
-    const int64_t j = min<int64_t>(n0 + wn * (BN / WN) + n * 32 + lr, a.N - 1);
-    sw[n] = a.sw[j];
-    bias[n] = a.bias ? a.bias[j] : 0.f;
-    wsum[n] = a.zx ? a.wsum[j] : 0;
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NTL; ++n)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            sums[(group - 1) * TILE + ((m * NTL + n) * 16 + v) * NT + tid] = acc[m][n][v];
+    __syncthreads();
+    if (group == 0)
+#pragma unroll
+      for (int g = 0; g < S - 1; ++g)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < NTL; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+              acc[m][n][v] += sums[g * TILE + ((m * NTL + n) * 16 + v) * NT + tid];
+    __syncthreads();
+    if (group > 0) return;
   }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int64_t i = t0 + wm * (BM / WM) + m * 32 + 8 * (v >> 2) + 4 * lh + (v & 3);
-      const int64_t ic = min<int64_t>(i, a.T - 1);
-      const float sx = a.sx[ic];
-      const int zx = a.zx ? (int)a.zx[ic] : 0;
-#pragma unroll
-      for (int n = 0; n < NTL; ++n) {
-        const int64_t j = n0 + wn * (BN / WN) + n * 32 + lr;
-        if (i < a.T && j < a.N)
-          store_y(a, i * a.ldo + j, scaled(a, sx, zx, acc[m][n][v], sw[n], wsum[n], bias[n]));
-      }
-    }
+  constexpr int MINE = 32 * (NTL * 32 * 4 + 16);  // a wave's part of LDS
+  static_assert(WM * WN * MINE <= (int)sizeof(Lall), "output does not fit");
+  int8_t* mine = &Lall[0][0][0] + wave * MINE;
+  const int64_t tw = t0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
+  const float* sx = sxL + wm * (BM / WM);
+  const int* zx = zxL + wm * (BM / WM);
+  if (nw >= a.N) return;
+  if (a.dtype == 0) finish_tile<0, MT, NTL>(a, acc, tw, nw, sx, zx, mine, lane);
+  else if (a.dtype == 1) finish_tile<1, MT, NTL>(a, acc, tw, nw, sx, zx, mine, lane);
+  else finish_tile<2, MT, NTL>(a, acc, tw, nw, sx, zx, mine, lane);
 }
 
 // Few tokens (TB blocks of 16): the weights' bytes are what counts.  A workgroup takes
@@ -428,11 +518,11 @@ void launch_few(hipStream_t st, const GemmI8& a) {
 // fewer workgroups that read the codes again.
 int few_rows(int64_t N) { return N >= 16 * 4 * 192 ? 4 : N >= 16 * 2 * 192 ? 2 : 1; }
 
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int S>
 void launch_tiles(hipStream_t st, const GemmI8& a) {
   const int64_t tm = cdiv(a.T, BM), tn = cdiv(a.N, BN);
-  hipLaunchKernelGGL((gemm_i8_kernel<BM, BN, WM, WN>), dim3((unsigned)(tm * tn)),
-                     dim3(64 * WM * WN), 0, st, a, (int)tm, (int)tn);
+  hipLaunchKernelGGL((gemm_i8_kernel<BM, BN, WM, WN, S>), dim3((unsigned)(tm * tn)),
+                     dim3(64 * WM * WN * S), 0, st, a, (int)tm, (int)tn);
 }
 
 int gemm_i8(hipStream_t st, const GemmI8& a) {
@@ -443,9 +533,11 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
     else launch_few<1>(st, a);
   } else {
     G2PTQ_CHECK(cdiv(a.T, 64) * cdiv(a.N, 64) < (1ll << 31), "int8_gemm: output too large");
-    if (cdiv(a.T, 256) * cdiv(a.N, 256) >= 192) launch_tiles<256, 256, 2, 4>(st, a);
-    else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 128) launch_tiles<128, 128, 2, 2>(st, a);
-    else launch_tiles<64, 64, 2, 2>(st, a);
+    if (cdiv(a.T, 256) * cdiv(a.N, 256) >= 192) launch_tiles<256, 256, 2, 4, 1>(st, a);
+    else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 128) launch_tiles<128, 128, 2, 2, 1>(st, a);
+    else if (cdiv(a.T, 64) * cdiv(a.N, 64) > 512) launch_tiles<64, 64, 2, 2, 1>(st, a);
+    else if (cdiv(a.T, 64) * cdiv(a.N, 64) > 256) launch_tiles<64, 64, 2, 2, 2>(st, a);
+    else launch_tiles<64, 64, 2, 2, 4>(st, a);
   }
   G2PTQ_LAUNCHED();
   return G2PTQ_OK;
