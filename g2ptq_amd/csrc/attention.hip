@@ -826,16 +826,50 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
     };
     int stage = 1;
     if (steps > 0) {
-      if (wave < 2) {
-#pragma unroll
-        for (int s = 0; s < 3; ++s) {
-          G2_PAGE(s);
-          G2_META(s);
-          G2_SHOW(s);
-        }
+      if (wave < 2) {  // three steps' pages, then their numbers, under way together
+        int page0, page1, page2, page3, page4;
+        G2_PAGE(0);
+        page0 = page;
+        G2_PAGE(1);
+        page1 = page;
+        G2_PAGE(2);
+        page2 = page;
         G2_PAGE(3);
-        G2_META(3);
+        page3 = page;
         G2_PAGE(4);
+        page4 = page;
+        page = page0;
+        G2_META(0);
+        const uint32_t row0 = srow;
+        const float sc0 = sc;
+        const int sz0 = sz;
+        const bool ok0 = sok;
+        page = page1;
+        G2_META(1);
+        const uint32_t row1 = srow;
+        const float sc1 = sc;
+        const int sz1 = sz;
+        const bool ok1 = sok;
+        page = page2;
+        G2_META(2);
+        const uint32_t row2 = srow;
+        const float sc2 = sc;
+        const int sz2 = sz;
+        const bool ok2 = sok;
+        page = page3;
+        G2_META(3);
+        const uint32_t row3 = srow;
+        const float sc3 = sc;
+        const int sz3 = sz;
+        const bool ok3 = sok;
+        srow = row0, sc = sc0, sz = sz0, sok = ok0;
+        G2_SHOW(0);
+        srow = row1, sc = sc1, sz = sz1, sok = ok1;
+        G2_SHOW(1);
+        srow = row2, sc = sc2, sz = sz2, sok = ok2;
+        G2_SHOW(2);
+        srow = row3, sc = sc3, sz = sz3, sok = ok3;
+        page = page4;
       }
       __syncthreads();
       G2_FETCH_K(0);

@@ -533,8 +533,13 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
     else launch_few<1>(st, a);
   } else {
     G2PTQ_CHECK(cdiv(a.T, 64) * cdiv(a.N, 64) < (1ll << 31), "int8_gemm: output too large");
+    // The largest tile that still fills the chip.  MI355X, product alone: 256 against 128 at
+    // 256 tiles of 256 (4096³) 64 against 86 µs; 128 against 64 at 256 tiles of 128
+    // (1024 × 4096, K 4096) 28 against 34 µs, at 128 of them (512 × 4096, K 14336) 71
+    // against 54 µs; 208 tiles of 64 (777 × 1000, K 2752) 10.4 µs with K shared by four
+    // groups, 12.8 µs without.
     if (cdiv(a.T, 256) * cdiv(a.N, 256) >= 192) launch_tiles<256, 256, 2, 4, 1>(st, a);
-    else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 128) launch_tiles<128, 128, 2, 2, 1>(st, a);
+    else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 224) launch_tiles<128, 128, 2, 2, 1>(st, a);
     else if (cdiv(a.T, 64) * cdiv(a.N, 64) > 512) launch_tiles<64, 64, 2, 2, 1>(st, a);
     else if (cdiv(a.T, 64) * cdiv(a.N, 64) > 256) launch_tiles<64, 64, 2, 2, 2>(st, a);
     else launch_tiles<64, 64, 2, 2, 4>(st, a);

@@ -26,20 +26,26 @@ struct WriteArgs {
   bool vec[2];
 };
 
-// L lanes hold one token's head, eight channels each (lanes past D idle), and reduce
-// it among themselves; a workgroup takes 256 / L consecutive heads of the T × H.
+// L lanes hold one token's head, sixteen channels each (lanes past D idle), and reduce
+// it among themselves; a workgroup takes 256 / L consecutive heads of the T × H.  Bound
+// by vector arithmetic (the grid's divisions and the reduction are per lane).
 // grid.y: 0 keys, 1 values.
-template <int DT, bool SYM, int L>
+template <int DT, bool SYM, int BITS, int L>
 __global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
+  constexpr int OFF = 1 << (BITS - 1);
   const int w = blockIdx.y;
   const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int d = (threadIdx.x % L) * 8;
+  const int d = (threadIdx.x % L) * 16;
   if (item >= a.items) return;
   const uint32_t t = item / (uint32_t)a.c.H, h = item - t * (uint32_t)a.c.H;
   const int64_t slot = a.slots[t];
   const bool on = d < a.c.D;
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (on) load8<DT>(a.x[w], t * a.st[w] + h * a.sh[w] + d, a.vec[w], 8, v);
+  float v[2][8] = {};
+  if (on) {
+    const int64_t at = t * a.st[w] + h * a.sh[w] + d;
+    load8<DT>(a.x[w], at, a.vec[w], 8, v[0]);
+    load8<DT>(a.x[w], at + 8, a.vec[w], 8, v[1]);
+  }
   if (slot < 0) return;
   if (slot >= a.c.pages << a.c.shift) {
     if (d == 0) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
@@ -47,28 +53,26 @@ __global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
   }
   Range<SYM> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.add(v[i]);
+  for (int i = 0; i < 16; ++i) r.add(v[i >> 3][i & 7]);
   reduce_range<L>(r);
-  const Grid g = make_grid<SYM>(r, a.c.bits);
+  const Grid g = make_grid<SYM>(r, BITS);
   const int64_t at = a.c.row(slot, h);
   if (d == 0) {
     a.c.scale[w][at] = g.s;
-    if (!SYM) a.c.zero[w][at] = (uint8_t)((int)g.z + (1 << (a.c.bits - 1)));
+    if (!SYM) a.c.zero[w][at] = (uint8_t)((int)g.z + OFF);
   }
   if (!on) return;
-  uint32_t u[8];
+  uint32_t o[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = (uint32_t)(to_code(g, v[i]) + (1 << (a.c.bits - 1)));
-  if (a.c.bits == 8) {
-    uint2 o = make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24,
-                         u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
-    *reinterpret_cast<uint2*>(a.c.codes[w] + at * a.c.D + d) = o;
-  } else {
-    uint32_t o = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o |= u[i] << (4 * i);
-    *reinterpret_cast<uint32_t*>(a.c.codes[w] + at * (a.c.D / 2) + d / 2) = o;
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t u = (uint32_t)(to_code(g, v[i >> 3][i & 7]) + OFF);
+    if constexpr (BITS == 8) o[i >> 2] |= u << (8 * (i & 3));
+    else o[i >> 3] |= u << (4 * (i & 7));
   }
+  if constexpr (BITS == 8)
+    *reinterpret_cast<uint4*>(a.c.codes[w] + at * a.c.D + d) = make_uint4(o[0], o[1], o[2], o[3]);
+  else
+    *reinterpret_cast<uint2*>(a.c.codes[w] + at * (a.c.D / 2) + d / 2) = make_uint2(o[0], o[1]);
 }
 
 struct ReadArgs {
@@ -141,11 +145,11 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <typename F>
 int by_lanes(int64_t D, F f) {
-  if (D <= 16) return f(std::integral_constant<int, 2>());
-  if (D <= 32) return f(std::integral_constant<int, 4>());
-  if (D <= 64) return f(std::integral_constant<int, 8>());
-  if (D <= 128) return f(std::integral_constant<int, 16>());
-  return f(std::integral_constant<int, 32>());
+  if (D <= 16) return f(std::integral_constant<int, 1>());
+  if (D <= 32) return f(std::integral_constant<int, 2>());
+  if (D <= 64) return f(std::integral_constant<int, 4>());
+  if (D <= 128) return f(std::integral_constant<int, 8>());
+  return f(std::integral_constant<int, 16>());
 }
 
 }  // namespace
@@ -204,8 +208,13 @@ extern "C" int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const v
   return by_lanes(a.c.D, [&](auto lanes) -> int {
     constexpr int L = decltype(lanes)::value;
     const dim3 grid((unsigned)cdiv(T * a.c.H, 256 / L), 2);
-#define G2_WR(DT, SYM) \
-  hipLaunchKernelGGL((kv_write_kernel<DT, SYM, L>), grid, dim3(256), 0, st, a)
+#define G2_WR(DT, SYM)                                                                      \
+  do {                                                                                      \
+    if (a.c.bits == 8)                                                                      \
+      hipLaunchKernelGGL((kv_write_kernel<DT, SYM, 8, L>), grid, dim3(256), 0, st, a);      \
+    else                                                                                    \
+      hipLaunchKernelGGL((kv_write_kernel<DT, SYM, 4, L>), grid, dim3(256), 0, st, a);      \
+  } while (0)
     if (dtype == 0) { if (sym) G2_WR(0, true); else G2_WR(0, false); }
     else if (dtype == 1) { if (sym) G2_WR(1, true); else G2_WR(1, false); }
     else { if (sym) G2_WR(2, true); else G2_WR(2, false); }
