@@ -578,9 +578,10 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 
 template <int BITS, int DP, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && DP <= 128 ? 2 : 1) void
+attend_tiles_kernel(AttnArgs a) {
   constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
-  constexpr int KP = BN * (DP / 16), KC = (KP + NT - 1) / NT;      // 16-channel pieces of keys
+  constexpr int KC = BN * (DP / 16) / NT;                          // 16-channel pieces of keys
   constexpr int VP = BN / 4 * (DP / 8), VQ = (VP + NT - 1) / NT;   // 4-key × 8-channel of values
   constexpr int KW = BITS / 2, VW = BITS / 4;   // words of 16 and of 8 channels
   constexpr int KPITCH = DP * 2 + 16, VPITCH = BN * 2 + 16;  // bytes of an LDS row
@@ -627,7 +628,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   // group's other bits, 3 of the chunk; with fewer pieces than threads the upper half
   // of the workgroup takes them.
   const int tv = VP < NT ? (tid + NT / 2) % NT : tid;
-  const int first = wave * 64, first_v = VP < NT ? (first + NT / 2) % NT : first;  // of the wave
+  const int first_v = VP < NT ? (wave * 64 + NT / 2) % NT : wave * 64;  // of the wave
   constexpr int OH = DP / 64;  // 8-channel groups over 8
 
   // the longest tiles (the last rows) first
@@ -716,7 +717,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
       const int p_ = tid + i * NT, c_ = p_ % (DP / 16);                                      \
-      if (KP % NT && first + i * NT >= KP) break;                                            \
       uint64_t o_ = (uint64_t)rowL[at4][p_ / (DP / 16)] * rowb + c_ * (2 * BITS);            \
       if (!FULL) o_ = c_ * 16 < D ? o_ : 0;                                                  \
       const uint8_t* s_ = a.c.codes[0] + o_;                                                 \
@@ -754,7 +754,6 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
   do {                                                                                       \
     _Pragma("unroll") for (int i = 0; i < KC; ++i) {                                         \
       const int p_ = tid + i * NT, key_ = p_ / (DP / 16), c_ = p_ % (DP / 16);               \
-      if (KP % NT && first + i * NT >= KP) break;                                            \
       const f16x2 zc_ = as_h2(zkL[(step) & 3][key_]);                                        \
       char* at_ = kL + ((step) & 1) * KB + key_ * KPITCH + c_ * 16;                          \
       *reinterpret_cast<f16x8*>(at_) = key_codes<BITS>(&kw[i][0], zc_);                      \
@@ -1043,7 +1042,7 @@ __global__ __launch_bounds__(64 * NW) void attend_tiles_kernel(AttnArgs a) {
 
 // Joins the shares of a query row: one wave per (token, head).
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= (int64_t)a.T * a.Hq) return;
   const int lane = threadIdx.x & 63, t = (int)(row / a.Hq), hq = (int)(row % a.Hq);
   const int b = (int)KvCache::sequence(a.cu, a.B, t);
@@ -1064,6 +1063,13 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
       : a.part + row * a.split * part_size(a);
   const int D = (int)a.c.D;
   const int64_t pitch = part_size(a);
+  // sixteen shares' outputs under way at a time, the first before the weights are known
+  const int d = lane * 4;
+  const float* pd = p + (d < D ? d : 0);
+  float4 o[16];
+#pragma unroll
+  for (int s = 0; s < 16; ++s)
+    o[s] = *reinterpret_cast<const float4*>(pd + min(s, split - 1) * pitch);
   // lane s has share s's maximum and sum (at most 64 shares); a share without keys has a
   // maximum of -inf and adds nothing, unless its sum is NaN
   float m = -INFINITY, L = 0.f;
@@ -1076,16 +1082,15 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o);
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int d = lane * 4;
   float y[4] = {0, 0, 0, 0};
-  const float* pd = p + (d < D ? d : 0);
-  for (int s0 = 0; s0 < split; s0 += 8) {  // eight loads under way
-    float4 o[8];
+  for (int s0 = 0; s0 < split; s0 += 16) {
+    if (s0 > 0) {
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      o[s] = *reinterpret_cast<const float4*>(pd + min(s0 + s, split - 1) * pitch);
+      for (int s = 0; s < 16; ++s)
+        o[s] = *reinterpret_cast<const float4*>(pd + min(s0 + s, split - 1) * pitch);
+    }
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < 16; ++s) {
       const float ws = s0 + s < split ? __shfl(w, s0 + s) : 0.f;
       if (ws != 0.f) {  // (also where ws is NaN)
         y[0] += ws * o[s].x, y[1] += ws * o[s].y, y[2] += ws * o[s].z, y[3] += ws * o[s].w;
@@ -1117,8 +1122,9 @@ struct Plan {
     // per CU (sequences of a batch differ in length), at most 64 shares
     const int64_t want = std::min<int64_t>(64, cdiv(8 * kCUs, pairs));
     few_split = cdiv(keys, cdiv(cdiv(keys, want), 128) * 128);
-    nw = rows > 192 ? 8 : rows > 64 ? 4 : 2;
-    if (D > 128) nw = rows > 64 ? 4 : 2;
+    // 128 rows a workgroup, two workgroups to a CU.  (256 rows, one to a CU: MI355X, 2048
+    // tokens over 16384 keys 714 against 702 µs, six uneven chunks 44 against 35 µs.)
+    nw = rows > 64 ? 4 : 2;
     ntiles = std::max<int64_t>(1, cdiv(rows, 32 * nw));
     split = std::max<int64_t>(1, std::min(2 * kCUs / (pairs * ntiles), keys / 256));
     split = std::min<int64_t>(split, 32);
@@ -1140,14 +1146,8 @@ int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
     const dim3 grid((unsigned)(a.B * a.c.H * a.split * a.tiles + 1));
 #define G2_AT(NW)                                                                            \
   hipLaunchKernelGGL((attend_tiles_kernel<BITS, DP, FULL, NW>), grid, dim3(64 * NW), 0, st, a)
-    if constexpr (DP <= 128) {
-      if (p.nw == 8) G2_AT(8);
-      else if (p.nw == 4) G2_AT(4);
-      else G2_AT(2);
-    } else {
-      if (p.nw == 4) G2_AT(4);
-      else G2_AT(2);
-    }
+    if (p.nw == 4) G2_AT(4);
+    else G2_AT(2);
 #undef G2_AT
     G2PTQ_LAUNCHED();
   }
