@@ -482,11 +482,11 @@ int quantize_tokens(hipStream_t st, const void* x, int dtype, int64_t T, int64_t
   hipLaunchKernelGGL((quantize_tokens_kernel<DT, SYM, V>), dim3((unsigned)T), dim3(256), 0, st, \
                      x, (int)K, ldx, vec, codes, ldc, scale, zero)
 #define G2_QT(DT, SYM)                     \
-  do {                                     \
-    if (K <= 2048) G2_QV(DT, SYM, 1);      \
-    else if (K <= 4096) G2_QV(DT, SYM, 2); \
-    else if (K <= 8192) G2_QV(DT, SYM, 4); \
-    else G2_QV(DT, SYM, 0);                \
+  do {                                      \
+    if (K <= 4096) G2_QV(DT, SYM, 2);       \
+    else if (K <= 8192) G2_QV(DT, SYM, 4);  \
+    else if (K <= 16384) G2_QV(DT, SYM, 8); \
+    else G2_QV(DT, SYM, 0);                 \
   } while (0)
   if (dtype == 0) { if (sym) G2_QT(0, true); else G2_QT(0, false); }
   else if (dtype == 1) { if (sym) G2_QT(1, true); else G2_QT(1, false); }
@@ -497,8 +497,17 @@ int quantize_tokens(hipStream_t st, const void* x, int dtype, int64_t T, int64_t
   return G2PTQ_OK;
 }
 
-constexpr int kFewTokens = 64;    // up to which the weights are streamed
-constexpr int64_t kFusedCodes = 16384;  // bytes of codes up to which they are made in that kernel
+// Channels of a workgroup of few tokens, /16: enough workgroups for every CU first, then
+// fewer workgroups that read the codes again.  MI355X, 16 tokens, K 4096, 1 / 2 / 4:
+// 4096 channels 12.0 / 12.7 / 16.4 µs, 8192 16.5 / 15.2 / 18.1, 14336 24.7 / 22.4 / 20.4.
+int few_rows(int64_t N) { return N >= 16 * 4 * 192 ? 4 : N >= 16 * 2 * 192 ? 2 : 1; }
+
+// Whether the weights are streamed for few tokens or tiled: up to 32 tokens, and up to 64
+// where 64-channel tiles would leave half the CUs idle.  MI355X, streamed against tiles,
+// K 4096: 32 tokens × 8192 17.7 against 19.2 µs, × 14336 22.0 against 21.9; 48 × 8192 19.5
+// against 19.9, × 14336 25.6 against 23.2; 64 × 4096 18.2 against 18.7, × 12288 26.9
+// against 22.9.
+bool few_tokens(int64_t T, int64_t N) { return T <= 32 || (T <= 64 && N <= 64 * 128); }
 
 template <int R, int TB>
 void launch_few(hipStream_t st, const GemmI8& a) {
@@ -510,13 +519,11 @@ template <int R>
 void launch_few(hipStream_t st, const GemmI8& a) {
   if (a.T <= 16) launch_few<R, 1>(st, a);
   else if (a.T <= 32) launch_few<R, 2>(st, a);
-  else if (a.T <= 48) launch_few<R, 3>(st, a);
-  else launch_few<R, 4>(st, a);
+  else if constexpr (R < 4) {  // (more channels are tiled)
+    if (a.T <= 48) launch_few<R, 3>(st, a);
+    else launch_few<R, 4>(st, a);
+  }
 }
-
-// Channels of a workgroup of few tokens: enough workgroups for every CU first, then
-// fewer workgroups that read the codes again.
-int few_rows(int64_t N) { return N >= 16 * 4 * 192 ? 4 : N >= 16 * 2 * 192 ? 2 : 1; }
 
 template <int BM, int BN, int WM, int WN, int S>
 void launch_tiles(hipStream_t st, const GemmI8& a) {
@@ -526,7 +533,7 @@ void launch_tiles(hipStream_t st, const GemmI8& a) {
 }
 
 int gemm_i8(hipStream_t st, const GemmI8& a) {
-  if (a.T <= kFewTokens) {
+  if (few_tokens(a.T, a.N)) {
     const int r = few_rows(a.N);
     if (r == 4) launch_few<4>(st, a);
     else if (r == 2) launch_few<2>(st, a);
@@ -548,17 +555,19 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
   return G2PTQ_OK;
 }
 
-// Tokens quantized and multiplied in one launch.
-bool fused(int64_t T, int64_t K) { return T <= 4 && T * (cdiv(K, 256) * 256) <= kFusedCodes; }
+// Tokens quantized and multiplied in one launch: one token, or two of up to 16384 columns
+// (LDS holds the codes).  MI355X, fused against apart: one token, 4096 × 4096 9.4 against
+// 10.8 µs, K 14336 19.1 against 25.7, 8192 channels of K 28672 53 against 62; two,
+// 4096 × 4096 10.8 against 11.1, K 11008 21.0 against 23.1; four, 13.4 against 11.2.
+bool fused(int64_t T, int64_t K) { return T <= 2 && T * K <= 32768; }
 template <int DT, bool SYM>
 void launch_fused(hipStream_t st, const GemmI8& a, const void* x, int64_t ldx, bool vec) {
   const size_t lds = (size_t)(a.T * (cdiv(a.K, 256) * 256));
-  const int r = few_rows(a.N);
 #define G2_FU(R)                                                                             \
   hipLaunchKernelGGL((gemm_i8_few_kernel<R, 1, true, DT, SYM>), dim3((unsigned)cdiv(a.N, 16 * R)), \
                      dim3(512), lds, st, a, x, ldx, vec)
-  if (r == 4) G2_FU(4);
-  else if (r == 2) G2_FU(2);
+  // (four: one token × 14336 channels 18.1 µs, two 17.0)
+  if (few_rows(a.N) >= 2) G2_FU(2);
   else G2_FU(1);
 #undef G2_FU
 }
