@@ -54,7 +54,8 @@ struct AttnArgs {
   float scale;
   float kscale;    // |scale|·log2 e·2^9: multiplies the keys' scales
   int tiles;       // row tiles a launch provides for a sequence and head (attend_tiles_kernel)
-  int split, few_split;  // shares of the keys (tiles; few rows)
+  int split, few_split;  // most shares of a sequence's keys (tiles; few rows)
+  int share, few_share;  // keys of a share, unless a sequence needs larger ones
   bool by_rows, by_tiles;  // kernels that run; with both, sequences of at most kFewRows rows
                            // go to attend_rows_kernel
   float *part, *few_part;  // partial results of the shares, or null
@@ -79,10 +80,14 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   return s;
 }
 
-// Keys of one of `split` shares of n keys, in multiples of `step`.
-__device__ __forceinline__ int share_of(int n, int split, int step) {
-  const int each = (n + split - 1) / split;
-  return max(step, (each + step - 1) / step * step);
+// The shares of n keys: of `share` keys each (a multiple of `step`; sequences of a batch
+// differ in length, their shares do not), larger ones where `most` would not do.
+struct Shares {
+  int each, count;
+};
+__device__ __forceinline__ Shares shares_of(int n, int most, int share, int step) {
+  const int each = max(share, ((n + most - 1) / most + step - 1) / step * step);
+  return {each, max(1, (n + each - 1) / each)};
 }
 
 __device__ __forceinline__ f16x2 as_h2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
@@ -270,7 +275,9 @@ attend_rows_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) float oL[4][16 * PITCH];
   __shared__ float mL[4][16], lL[4][16];
 
-  const int b = blockIdx.z, h = blockIdx.y, split = blockIdx.x;
+  // Workgroups go round the 8 XCDs: the heads' shares of the same pages mostly meet on one,
+  // and turned by the sequence, the last shares (short sequences have fewer) on all.
+  const int b = blockIdx.z, h = blockIdx.y, split = (blockIdx.x + b) % gridDim.x;
   if (b == a.B) {
     if (h == 0 && split == 0) clear_outside(a);
     return;
@@ -278,9 +285,9 @@ attend_rows_kernel(AttnArgs a) {
   const Span sp = span_of(a, b);
   const int rows = sp.qlen * a.G;
   if (rows == 0 || (a.by_tiles && rows > kFewRows)) return;
-  const int shares = rows > kFewRows ? 1 : a.few_split;
-  if (split >= shares) return;
-  const int share = share_of(sp.n, shares, 128);
+  const Shares sh = rows > kFewRows ? Shares{sp.n, 1}
+                                    : shares_of(sp.n, a.few_split, a.few_share, 128);
+  if (split >= sh.count) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int D = FULL ? DP : (int)a.c.D;
@@ -293,7 +300,7 @@ attend_rows_kernel(AttnArgs a) {
     // the last key that the lane's row sees, and that any of the block's rows sees
     const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
     const int last_all = min(sp.pos0 + (min(r0 + 15, rows - 1)) / a.G, sp.n - 1);
-    const int k0 = split * share + 32 * wave, k1 = min(last_all + 1, (split + 1) * share);
+    const int k0 = split * sh.each + 32 * wave, k1 = min(last_all + 1, (split + 1) * sh.each);
     const int steps = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;  // blocks of 32 keys, every 128
 
     // A step's pages (P), rows and numbers (M, shown to the wave by S), codes (C): loaded
@@ -529,7 +536,7 @@ attend_rows_kernel(AttnArgs a) {
       for (int k = 0; k < 8; ++k)
         y[k] = (oL[0][r * PITCH + d + k] + oL[1][r * PITCH + d + k] + oL[2][r * PITCH + d + k] +
                 oL[3][r * PITCH + d + k]) * inv;
-      if (shares > 1) {
+      if (sh.count > 1) {
         float* o = a.few_part +
                    ((((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split + split) * part_size(a);
         *reinterpret_cast<float4*>(o + d) = make_float4(y[0], y[1], y[2], y[3]);
@@ -595,7 +602,8 @@ attend_tiles_kernel(AttnArgs a) {
   __shared__ uint64_t okL[4];
 
   // Workgroups go round the 8 XCDs; number them so that an XCD takes a contiguous
-  // range: the row tiles of one sequence and head share its keys in one L2.
+  // range: the row tiles of one sequence and head share its keys in one L2.  (Heads last:
+  // the sequences, which differ in length, are spread over the XCDs.)
   const int total = a.B * (int)a.c.H * a.split * a.tiles;
   if ((int)blockIdx.x == total) {
     clear_outside(a);
@@ -610,11 +618,12 @@ attend_tiles_kernel(AttnArgs a) {
   id /= a.tiles;
   const int split = id % a.split;
   id /= a.split;
-  const int h = id % (int)a.c.H, b = id / (int)a.c.H;
+  const int b = id % a.B, h = id / a.B;
   const Span sp = span_of(a, b);
   const int rows = sp.qlen * a.G;
   if (rows == 0 || (a.by_rows && rows <= kFewRows)) return;
-  const int share = share_of(sp.n, a.split, BN);
+  const Shares sh = shares_of(sp.n, a.split, a.share, BN);
+  if (split >= sh.count) return;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = FULL ? DP : (int)a.c.D;
@@ -638,7 +647,7 @@ attend_tiles_kernel(AttnArgs a) {
     const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
     const int first_all = min(sp.pos0 + r0 / a.G, sp.n - 1);  // seen by every row of the tile
     const int last_all = min(sp.pos0 + (min(r0 + BM, rows) - 1) / a.G, sp.n - 1);
-    const int k0 = split * share, k1 = min(last_all + 1, k0 + share);
+    const int k0 = split * sh.each, k1 = min(last_all + 1, k0 + sh.each);
     const int steps = k1 > k0 ? (k1 - k0 + BN - 1) / BN : 0;
 
     // query fragments: chunk c = 2s + lh of keys' LDS rows holds channels 16c .. + 7
@@ -1026,12 +1035,12 @@ attend_tiles_kernel(AttnArgs a) {
           if (!FULL && d >= D) continue;
           const float y[4] = {acc[e][4 * q] * inv, acc[e][4 * q + 1] * inv,
                               acc[e][4 * q + 2] * inv, acc[e][4 * q + 3] * inv};
-          if (a.split > 1)
+          if (sh.count > 1)
             *reinterpret_cast<float4*>(o + d) = make_float4(y[0], y[1], y[2], y[3]);
           else
             store_out(a, row * D + d, y);
         }
-      if (a.split > 1 && lh == 0) {
+      if (sh.count > 1 && lh == 0) {
         o[D] = m == -INFINITY ? -INFINITY : m * C;
         o[D + 1] = __builtin_amdgcn_ldexpf(l, exponent(ref) - 15);
       }
@@ -1055,7 +1064,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   const int rows = sp.qlen * a.G, h = hq / a.G;
   // which kernel had the row, and in how many shares
   const bool by_rows = a.by_rows && (rows <= kFewRows || !a.by_tiles);
-  const int split = by_rows ? (rows <= kFewRows ? a.few_split : 1) : a.split;
+  if (by_rows && rows > kFewRows) return;
+  const int split = by_rows ? shares_of(sp.n, a.few_split, a.few_share, 128).count
+                            : shares_of(sp.n, a.split, a.share, 64).count;
   if (split == 1) return;
   const int r = (t - sp.q0) * a.G + hq - h * a.G;
   const float* p = by_rows
@@ -1110,24 +1121,43 @@ constexpr int64_t kCUs = 256;
 struct Plan {
   bool few, tiles;     // which kernels run
   int nw;              // waves of a tile's workgroup
-  int64_t ntiles, split, few_split;
+  int64_t ntiles, split, few_split, share, few_share;
   int64_t part, few_part;  // bytes of partial results
   Plan(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t max_q, int64_t max_kv) {
     const int64_t G = Hq / H, rows = max_q * G, pairs = std::max<int64_t>(1, B * H);
     tiles = rows > kFewRows;
     // a batch of chunks only has sequences of few rows if some are shorter than the rest
     few = !tiles || B > 1;
-    const int64_t keys = std::max<int64_t>(1, max_kv);
-    // few rows: shares of 128 keys (a step of every wave) or more, some eight workgroups
-    // per CU (sequences of a batch differ in length), at most 64 shares
-    const int64_t want = std::min<int64_t>(64, cdiv(8 * kCUs, pairs));
-    few_split = cdiv(keys, cdiv(cdiv(keys, want), 128) * 128);
+    const int64_t keys = std::min<int64_t>(std::max<int64_t>(1, max_kv), 1 << 30);
+    // Few rows: shares of 1024 keys or more, up to sixteen workgroups per CU (sequences of a
+    // batch differ in length, and the last ones to run should be short); smaller ones, from
+    // 256 keys (two steps of every wave), for six per CU.  MI355X, heads 32 on 8 of 128:
+    //   64 uneven sequences of up to 8192 keys, 4 bits: 79 µs in 8, 88 in 3, 116 unshared
+    //   96 of them: 115 µs in 6 shares, 154 in 2
+    //   16 uneven of up to 8192, 4 bits: 33 µs in 12, 41 in 4, 55 in 32
+    //   one of 8192, 8 bits: 13.4 µs in shares of 256, 15.6 of 128, 14.5 of 512
+    // None where two workgroups per CU are there without and short: 64 uneven sequences of up
+    // to 4096 keys 58 µs, 62 in 4; 160 of up to 2048, 70 µs and 94 in 2.  At most 32: 8
+    // sequences of 16384, two heads, 21 µs in 32 and 27 in 64, whose joining costs more; up
+    // to 64 for a few heads, which are not enough otherwise.
+    int64_t want = std::max(std::min(cdiv(16 * kCUs, pairs), keys / 1024),
+                            std::min(cdiv(6 * kCUs, pairs), cdiv(keys, 256)));
+    if (pairs >= 2 * kCUs && keys < 5120) want = 1;
+    want = std::min<int64_t>(want, pairs > 4 ? 32 : 64);
+    few_share = cdiv(cdiv(keys, want), 128) * 128;
+    few_split = cdiv(keys, few_share);
     // 128 rows a workgroup, two workgroups to a CU.  (256 rows, one to a CU: MI355X, 2048
-    // tokens over 16384 keys 714 against 702 µs, six uneven chunks 44 against 35 µs.)
+    // tokens over 16384 keys 714 against 702 µs, six uneven chunks 44 against 35 µs; 64 rows:
+    // 1197 µs, but 23 against 25 for 32 tokens over 600 keys.)
     nw = rows > 64 ? 4 : 2;
     ntiles = std::max<int64_t>(1, cdiv(rows, 32 * nw));
-    split = std::max<int64_t>(1, std::min(2 * kCUs / (pairs * ntiles), keys / 256));
+    // Shares for two workgroups per CU, three in a batch (its sequences differ in length).
+    // MI355X, heads 32 on 8 of 128, two / three / four: 512 tokens over 2048 keys 51.7 / 60.8
+    // / 62.9 µs; four chunks of 300 over up to 4096 keys 163 / 122 / 131 µs; six of 100, 104 /
+    // 75 / 88 µs.  Of 256 keys or more: 8 chunks of 16 tokens over 2048 keys 33 µs, 40 with 512.
+    split = std::max<int64_t>(1, std::min((B > 1 ? 3 : 2) * kCUs / (pairs * ntiles), keys / 256));
     split = std::min<int64_t>(split, 32);
+    share = cdiv(cdiv(keys, split), 64) * 64;
     part = tiles && split > 1 ? cdiv(T * Hq * split * (D + 4) * 4, 256) * 256 : 0;
     few_part = few && few_split > 1
                    ? cdiv(B * H * kFewRows * few_split * (D + 4) * 4, 256) * 256 : 0;
@@ -1216,6 +1246,7 @@ extern "C" int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, 
   a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_token % 8 == 0 && q_head % 8 == 0;
   a.scale = scale, a.kscale = fabsf(scale) * 1.44269504088896340736f * 512.f;
   a.tiles = (int)p.ntiles, a.split = (int)p.split, a.few_split = (int)p.few_split;
+  a.share = (int)p.share, a.few_share = (int)p.few_share;
   a.by_rows = p.few, a.by_tiles = p.tiles;
   a.part = p.part ? static_cast<float*>(ws) : nullptr;
   a.few_part = p.few_part ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.part) : nullptr;
