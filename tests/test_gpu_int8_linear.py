@@ -100,6 +100,21 @@ def test_linear_matches_the_exact_product(dev, T, N, K, sym, with_bias):
         _check(lin(x.to(dev)), rc, rs, rz, w, wscale, bias, dtype)
 
 
+@pytest.mark.parametrize("T,N,K", [
+    (1, 70, 32768), (1, 70, 32769), (2, 70, 16384), (2, 70, 16400), (1, 6150, 40),
+    (2, 12300, 40), (16, 12300, 100), (32, 12300, 64), (33, 8193, 96), (48, 8192, 64),
+    (64, 6150, 80), (64, 8200, 48), (50, 4000, 48)])
+def test_each_side_of_the_choices_by_size(dev, T, N, K):
+    test_linear_matches_the_exact_product(dev, T, N, K, False, True)
+    test_linear_matches_the_exact_product(dev, T, N, K, True, False)
+
+
+@pytest.mark.parametrize("K", [4097, 8192, 8200, 16384, 16391])
+def test_token_codes_of_long_rows(dev, K):
+    for dtype in DTYPES:
+        test_token_codes_are_the_grids(dev, 3, K, K % 2 == 0, dtype)
+
+
 @pytest.mark.parametrize("T", [1, 16, 40, 200, 600])
 def test_extreme_codes_and_zero_points(dev, T):
     """The sums' range: every code at an end of the grid, K at its limit."""

@@ -98,6 +98,21 @@ def test_long_contexts_with_few_rows(dev, q_lens, kv_lens, bits):
     b.check(b.run(max_q=0, max_kv=0), "no hints")
 
 
+@pytest.mark.parametrize("q_lens,kv_lens,heads,kv_heads,dim", [
+    ([300, 20, 100], [4000, 20, 900], 4, 2, 64),       # chunks in as many shares as they need
+    ([90, 1, 2, 40], [1500, 3000, 20, 41], 4, 2, 48),  # and short ones with them
+    ([1] * 64, [5200] + [(37 * i) % 900 for i in range(1, 64)], 8, 8, 16),
+    ([2] * 20, [1 + (613 * i) % 3000 for i in range(20)], 2, 1, 32)],
+    ids=["chunks", "mixed", "many", "pairs"])
+def test_batches_of_sequences_of_very_different_lengths(dev, q_lens, kv_lens, heads, kv_heads,
+                                                        dim):
+    b = Batch(dev, q_lens, kv_lens, heads, kv_heads, dim, 16, 8, False, torch.bfloat16)
+    b.check(b.run(max_q=max(q_lens), max_kv=max(kv_lens)), "sized")
+    b.check(b.run(max_q=max(q_lens), max_kv=300), "lengths beyond the stated one")
+    b.check(b.run(max_q=1, max_kv=max(kv_lens)), "more rows than stated")
+    b.check(b.run(), "unsized")
+
+
 def test_scale_and_strides(dev):
     b = Batch(dev, [20, 1], [50, 77], 4, 2, 64, 16, 8, False, torch.bfloat16)
     for scale in (0.0, -0.3, 1.0):
