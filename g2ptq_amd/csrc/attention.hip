@@ -1049,17 +1049,26 @@ attend_tiles_kernel(AttnArgs a) {
   }
 }
 
-// Joins the shares of a query row: one wave per (token, head).
+// Joins the shares of a query row (token, head): LW lanes of four channels each, with the
+// shares' weights in LDS; sixteen shares' outputs are under way at a time.
+template <int LW>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= (int64_t)a.T * a.Hq) return;
-  const int lane = threadIdx.x & 63, t = (int)(row / a.Hq), hq = (int)(row % a.Hq);
-  const int b = (int)KvCache::sequence(a.cu, a.B, t);
+  __shared__ float wL[256 / LW][64];  // (at most 64 shares)
+  const int64_t rows_all = (int64_t)a.T * a.Hq;
+  const int sub = threadIdx.x % LW, group = threadIdx.x / LW;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LW) + group;
+  const int64_t row0 = (int64_t)blockIdx.x * (256 / LW) +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (64 / LW);
+  if (row0 >= rows_all) return;
+  const int64_t near = KvCache::sequence_of_wave(a.cu, a.B, row0 / a.Hq);
+  // from here on groups go their own ways
+  if (row >= rows_all) return;
+  const int t = (int)(row / a.Hq), hq = (int)(row % a.Hq);
+  const int b = (int)KvCache::sequence_near(a.cu, a.B, t, near);
   if (b < 0) return;
   Span sp;
   sp.q0 = min(max(a.cu[b], 0), a.T);
   sp.qlen = min(max(a.cu[b + 1], sp.q0), a.T) - sp.q0;
-  sp.pos0 = a.kv[b] - sp.qlen;
   sp.n = a.c.pages == 0 ? 0 : (int)min<int64_t>(max(a.kv[b], 0), (int64_t)a.width << a.c.shift);
   const int rows = sp.qlen * a.G, h = hq / a.G;
   // which kernel had the row, and in how many shares
@@ -1069,42 +1078,59 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
                             : shares_of(sp.n, a.split, a.share, 64).count;
   if (split == 1) return;
   const int r = (t - sp.q0) * a.G + hq - h * a.G;
-  const float* p = by_rows
-      ? a.few_part + (((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split * part_size(a)
-      : a.part + row * a.split * part_size(a);
-  const int D = (int)a.c.D;
   const int64_t pitch = part_size(a);
-  // sixteen shares' outputs under way at a time, the first before the weights are known
-  const int d = lane * 4;
+  const float* p = by_rows
+      ? a.few_part + (((int64_t)b * a.c.H + h) * kFewRows + r) * a.few_split * pitch
+      : a.part + row * a.split * pitch;
+  const int D = (int)a.c.D, d = sub * 4;
   const float* pd = p + (d < D ? d : 0);
-  float4 o[16];
+  float4 o[2][8];
+  // (before the weights are known)
 #pragma unroll
-  for (int s = 0; s < 16; ++s)
-    o[s] = *reinterpret_cast<const float4*>(pd + min(s, split - 1) * pitch);
-  // lane s has share s's maximum and sum (at most 64 shares); a share without keys has a
-  // maximum of -inf and adds nothing, unless its sum is NaN
-  float m = -INFINITY, L = 0.f;
-  if (lane < split) m = p[lane * pitch + D], L = p[lane * pitch + D + 1];
-  float M = m;
+  for (int s = 0; s < 8; ++s)
+    o[0][s] = *reinterpret_cast<const float4*>(pd + min(s, split - 1) * pitch);
+  // a share without keys has a maximum of -inf and adds nothing, unless its sum is NaN
+  constexpr int J = 64 / LW;
+  float m[J], w[J], M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-  if (m != -INFINITY) L *= __builtin_amdgcn_exp2f(m - M);
-  const float w = m == -INFINITY ? 0.f : L;
+  for (int j = 0; j < J; ++j) {
+    const int s = sub + j * LW;
+    m[j] = -INFINITY, w[j] = 0.f;
+    if (s < split) m[j] = p[s * pitch + D], w[j] = p[s * pitch + D + 1];
+    M = fmaxf(M, m[j]);
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o);
+  for (int k = LW / 2; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (m[j] != -INFINITY) w[j] *= __builtin_amdgcn_exp2f(m[j] - M);
+    L += w[j];
+    wL[group][sub + j * LW] = m[j] == -INFINITY ? 0.f : w[j];
+  }
+#pragma unroll
+  for (int k = LW / 2; k > 0; k >>= 1) L += __shfl_xor(L, k);
   const float inv = L == 0.f ? 0.f : 1.f / L;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   float y[4] = {0, 0, 0, 0};
   for (int s0 = 0; s0 < split; s0 += 16) {
-    if (s0 > 0) {
 #pragma unroll
-      for (int s = 0; s < 16; ++s)
-        o[s] = *reinterpret_cast<const float4*>(pd + min(s0 + s, split - 1) * pitch);
-    }
+    for (int half = 0; half < 2; ++half) {
+      const int at = s0 + 8 * half;
+      if (at + 8 < split) {
 #pragma unroll
-    for (int s = 0; s < 16; ++s) {
-      const float ws = s0 + s < split ? __shfl(w, s0 + s) : 0.f;
-      if (ws != 0.f) {  // (also where ws is NaN)
-        y[0] += ws * o[s].x, y[1] += ws * o[s].y, y[2] += ws * o[s].z, y[3] += ws * o[s].w;
+        for (int s = 0; s < 8; ++s)
+          o[half ^ 1][s] =
+              *reinterpret_cast<const float4*>(pd + min(at + 8 + s, split - 1) * pitch);
+      }
+      if (at >= split) break;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float ws = wL[group][at + s];  // (zero past the last share)
+        if (ws != 0.f) {                     // (also where it is NaN)
+          y[0] += ws * o[half][s].x, y[1] += ws * o[half][s].y;
+          y[2] += ws * o[half][s].z, y[3] += ws * o[half][s].w;
+        }
       }
     }
   }
@@ -1182,8 +1208,9 @@ int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
     G2PTQ_LAUNCHED();
   }
   if (a.part || a.few_part) {
-    hipLaunchKernelGGL(attend_join_kernel, dim3((unsigned)cdiv((int64_t)a.T * a.Hq, 4)), dim3(256),
-                       0, st, a);
+    constexpr int LW = DP / 4;
+    hipLaunchKernelGGL((attend_join_kernel<LW>),
+                       dim3((unsigned)cdiv((int64_t)a.T * a.Hq, 256 / LW)), dim3(256), 0, st, a);
     G2PTQ_LAUNCHED();
   }
   return G2PTQ_OK;

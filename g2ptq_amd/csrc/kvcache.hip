@@ -96,10 +96,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
   const int w = blockIdx.y;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n = (int)min<int64_t>(a.tokens, a.total - t0);
-  if ((int)threadIdx.x < n) {
-    const int64_t slot = a.c.find(a.table, a.ldt, a.width, a.cu, a.B, t0 + threadIdx.x);
-    if (slot == -2) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
-    slotL[threadIdx.x] = slot;
+  if (threadIdx.x < 64) {  // (one wave: n <= 64)
+    const int64_t b = KvCache::sequence_of_wave(a.cu, a.B, t0);
+    if ((int)threadIdx.x < n) {
+      const int64_t slot = a.c.find(a.table, a.ldt, a.width, a.cu, a.B, t0 + threadIdx.x, b);
+      if (slot == -2) atomicOr(a.c.flags, G2PTQ_FLAG_BAD_INDEX);
+      slotL[threadIdx.x] = slot;
+    }
   }
   __syncthreads();
   // piece = (token t, head h, 16 channels c), counted on by 256 in mixed radix
@@ -243,7 +246,7 @@ extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const in
   // tokens of 8 × 64 35 against 31.6 µs).
   const int64_t pieces = a.c.H * a.c.D / 16;
   int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(kReadTokens, 1024 / pieces));
-  while (tokens > 1 && cdiv(total, tokens) < 1024) tokens /= 2;
+  while (tokens > 1 && cdiv(total, tokens) < 256) tokens /= 2;
   a.tokens = (int)tokens;
   hipStream_t st = as_stream(stream);
   const dim3 grid((unsigned)cdiv(total, tokens), 2);

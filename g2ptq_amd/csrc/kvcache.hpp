@@ -40,10 +40,34 @@ struct KvCache {
     return lo;
   }
 
+  // The same where a whole wave looks for one t: 64 offsets at a time, so that up to 64
+  // sequences cost one load's latency and 4096 two.
+  static __device__ __forceinline__ int64_t sequence_of_wave(const int32_t* cu, int64_t B,
+                                                             int64_t t) {
+    if (B == 0) return -1;
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, n = B;  // cu[i + 1] <= t for i < lo, and for none from lo + n up
+    while (n > 0) {
+      const int64_t step = (n + 63) >> 6, i = (lane + 1) * step - 1;
+      const uint64_t before = __builtin_amdgcn_ballot_w64(i < n && cu[lo + min(i, n - 1) + 1] <= t);
+      const int64_t next = lo + __builtin_popcountll(before) * step;
+      n = min(step - 1, lo + n - next);
+      lo = next;
+    }
+    return lo < B && cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+  }
+
+  // The same where `near` is likely the one (or -1).
+  static __device__ __forceinline__ int64_t sequence_near(const int32_t* cu, int64_t B, int64_t t,
+                                                          int64_t near) {
+    return near >= 0 && t >= cu[near] && t < cu[near + 1] ? near : sequence(cu, B, t);
+  }
+
   // Slot of row t of a ragged batch; -1 outside every sequence.
   __device__ __forceinline__ int64_t find(const int32_t* table, int64_t ldt, int64_t width,
-                                          const int32_t* cu, int64_t B, int64_t t) const {
-    const int64_t b = sequence(cu, B, t);
+                                          const int32_t* cu, int64_t B, int64_t t,
+                                          int64_t near) const {
+    const int64_t b = sequence_near(cu, B, t, near);
     if (b < 0) return -1;
     return slot(table + b * ldt, width, t - cu[b]);
   }
