@@ -74,18 +74,22 @@ class PagedKVCache:
         if dev.type != "cuda":
             raise RuntimeError("PagedKVCache lives on the GPU")
         shape = (num_pages, kv_heads, page_size)
-        self.k_codes, self.v_codes = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8,
-                                                  device=dev) for _ in range(2))
-        self.k_scale, self.v_scale = (torch.zeros(shape, device=dev) for _ in range(2))
-        self.k_zero, self.v_zero = (None if self.sym else torch.zeros(
-            shape, dtype=torch.uint8, device=dev) for _ in range(2))
-        self.flags = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.device = self.flags.device
+        codes = [torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=dev)
+                 for _ in range(2)]
+        scales = [torch.zeros(shape, device=dev) for _ in range(2)]
+        zeros = [None if self.sym else torch.zeros(shape, dtype=torch.uint8, device=dev)
+                 for _ in range(2)]
+        flags = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.device = flags.device
+        self._held = (*codes, *scales, *zeros, flags)
         self._struct = _lib.KvCacheStruct(
-            *(_lib.ptr(t) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale,
-                                    self.k_zero, self.v_zero, self.flags)),
+            *(_lib.ptr(t) for t in self._held),
             num_pages, kv_heads, page_size, head_dim, bits, int(self.sym))
         self._address = ctypes.addressof(self._struct)
+
+    # (the kernels know these by their addresses: changed in place, never replaced)
+    k_codes, v_codes, k_scale, v_scale, k_zero, v_zero, flags = (
+        property(lambda self, i=i: self._held[i]) for i in range(7))
 
     def write(self, k, v, slots):
         """Quantize tokens' keys and values (tokens, kv_heads, head_dim; bf16, fp16
@@ -120,7 +124,7 @@ class PagedKVCache:
             raise ValueError(f"cu_tokens has {cu.shape[0]} entries for {table.shape[0]} sequences")
         if total < 0:
             raise ValueError(f"total is {total}")
-        _lib.require_current(self.flags, "PagedKVCache.read")
+        _lib.require_current(self._held[6], "PagedKVCache.read")
         k = torch.empty(total, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         B, width = table.shape

@@ -228,3 +228,16 @@ def test_refusals(dev):
         cache.read(table.long(), torch.zeros(2, dtype=torch.int32, device=dev), 1)
     with pytest.raises(NotImplementedError):
         cache.read(table, torch.zeros(2, dtype=torch.int32, device=dev), 1, dtype=torch.float64)
+
+
+def test_a_caches_tensors_are_not_replaced(dev):
+    """The kernels know them by their addresses."""
+    from g2ptq_amd import PagedKVCache
+    c = PagedKVCache(2, 16, 1, 16, device=dev)
+    for name in ("k_codes", "v_codes", "k_scale", "v_scale", "k_zero", "v_zero", "flags"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, torch.zeros(1, device=dev))
+    c.k_scale.fill_(1.0)
+    k, v = c.read(torch.zeros(1, 1, dtype=torch.int32, device=dev),
+                  torch.tensor([0, 3], dtype=torch.int32, device=dev), 3, torch.float32)
+    assert bool((k == -128).all()) and bool((v == 0).all())
