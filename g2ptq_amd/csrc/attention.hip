@@ -258,6 +258,12 @@ __device__ void clear_outside(const AttnArgs& a) {
 // Row statistics are per lane (row = lane % 16).  Four waves interleave blocks of 32
 // keys and join through LDS; `few_split` workgroups share a sequence's keys.
 // DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
+// Bound by the cache's bytes at 8 bits and by the codes' conversion (four instructions of
+// vector arithmetic per two codes) at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
+// 131072 keys 51 µs (5.4 TB/s), 64 over 4096 each 104 µs (5.3 TB/s); 4 bits: 64 over 4096
+// 66 µs (4.3 TB/s); one over 4001 at 8 bits 8.6 µs and 4 to join, latency.  Up to 16 rows, one
+// block of the product's columns: 32 uneven sequences with 2 tokens of 8 heads 49 µs, 100 by
+// attend_tiles_kernel; 4 tokens over 8192 keys 17.6 against 23.4 µs.
 // ---------------------------------------------------------------------------
 template <int BITS, int DP, bool FULL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? (BITS == 4 ? 3 : 2) : 1) void
@@ -567,6 +573,11 @@ attend_rows_kernel(AttnArgs a) {
 // LDS rows are 16 bytes longer than their data, so that fragment reads (16 consecutive
 // rows, one 16-byte chunk) touch all banks; values' rows also hold chunk c at
 // c ^ (channel / 16), which spreads the writes (8 rows 8 channels apart, one chunk).
+// Bound by the products, whose operands come from LDS at about the rate the matrix cores
+// take them, and the softmax between them, which the two workgroups of a CU overlap only in
+// part: MI355X, 2048 tokens over 16384 keys, heads 32 on 8 of 128, 8 bits, 660 µs, 780
+// TFLOP/s (the library's largest bf16 product: 1520).  Slower: waves in two groups that take
+// turns at softmax and products (780 against 688 µs then), steps of 32 keys (915 against 795).
 // ---------------------------------------------------------------------------
 // Largest of 64 lanes' non-negative x (rows of 16 lanes, then across rows, into lane 63).
 __device__ __forceinline__ float wave_max(float x) {
@@ -1050,7 +1061,9 @@ attend_tiles_kernel(AttnArgs a) {
 }
 
 // Joins the shares of a query row (token, head): LW lanes of four channels each, with the
-// shares' weights in LDS; sixteen shares' outputs are under way at a time.
+// shares' weights in LDS; sixteen shares' outputs are under way at a time.  Bound by
+// latency (MI355X, one row of 16 shares 4 µs; 2048 rows of up to 8 of 128 channels 5.2 µs,
+// 8400 of 64 channels 4.6; with a wave per row those took 5.4 and 8.4).
 template <int LW>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   __shared__ float wL[256 / LW][64];  // (at most 64 shares)
