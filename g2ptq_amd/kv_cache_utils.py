@@ -81,6 +81,7 @@ class PagedKVCache:
                  for _ in range(2)]
         flags = torch.zeros(1, dtype=torch.int32, device=dev)
         self.device = flags.device
+        self._device = self.device.index
         self._held = (*codes, *scales, *zeros, flags)
         self._struct = _lib.KvCacheStruct(
             *(_lib.ptr(t) for t in self._held),
@@ -96,6 +97,20 @@ class PagedKVCache:
         or fp32, any strides of token and head) into their slots (int64).
         Negative slots are skipped (padding of a batch); slots must not repeat
         within a call."""
+        here, code = self._device, _DTYPE_CODE.get(k.dtype)
+        # what is usual passes in one go (a call is a few microseconds); the rest is told apart
+        if not (slots.dim() == 1 and slots.dtype is torch.int64 and slots.is_contiguous()
+                and k.shape == v.shape == (slots.shape[0], self.kv_heads, self.head_dim)
+                and k.stride(2) == v.stride(2) == 1 and code is not None and v.dtype is k.dtype
+                and k.get_device() == v.get_device() == slots.get_device() == here
+                and torch._C._cuda_getDevice() == here
+                and not k.requires_grad and not v.requires_grad):
+            return self._write_checked(k, v, slots)
+        (n, _, _), (kt, kh, _), (vt, vh, _) = k.shape, k.stride(), v.stride()
+        _lib.call_fast("kv_write", _lib.current_stream(), self._address, k.data_ptr(), kt, kh,
+                       v.data_ptr(), vt, vh, code, n, slots.data_ptr())
+
+    def _write_checked(self, k, v, slots):
         k = _heads(k, self.kv_heads, self.head_dim, "keys")
         v = _heads(v, self.kv_heads, self.head_dim, "values")
         if k.dtype not in _DTYPE_CODE or v.dtype is not k.dtype:
@@ -105,7 +120,7 @@ class PagedKVCache:
         n = len(k)
         if n != len(v) or n != len(slots):
             raise ValueError(f"{n} keys, {len(v)} values, {len(slots)} slots")
-        if k.get_device() != self.device.index:
+        if k.get_device() != self._device:
             raise ValueError(f"keys on {k.device}, the cache on {self.device}")
         (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
         _lib.call_fast("kv_write", _lib.current_stream(), self._address, k.data_ptr(), kt, kh,
@@ -120,14 +135,14 @@ class PagedKVCache:
             raise NotImplementedError(f"PagedKVCache.read gives bf16, fp16 or fp32, not {dtype}")
         table = _index(table, torch.int32, 2, "table", self.device)
         cu = _index(cu_tokens, torch.int32, 1, "cu_tokens", self.device)
-        if cu.shape[0] != table.shape[0] + 1:
-            raise ValueError(f"cu_tokens has {cu.shape[0]} entries for {table.shape[0]} sequences")
+        B, width = table.shape
+        if cu.shape[0] != B + 1:
+            raise ValueError(f"cu_tokens has {cu.shape[0]} entries for {B} sequences")
         if total < 0:
             raise ValueError(f"total is {total}")
         _lib.require_current(self._held[6], "PagedKVCache.read")
         k = torch.empty(total, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        B, width = table.shape
         _lib.call_fast("kv_read", _lib.current_stream(), self._address, table.data_ptr(),
                        max(table.stride(0), width), B, width, cu.data_ptr(), total, k.data_ptr(),
                        v.data_ptr(), _DTYPE_CODE[dtype])
