@@ -97,6 +97,14 @@ __device__ __forceinline__ f16x2 centred(uint32_t two, f16x2 zc) {
   const f16x2 up = {(_Float16)32768.f, (_Float16)32768.f};
   return __builtin_elementwise_fma(as_h2(two), up, zc);
 }
+// The same of 4-bit codes in the low (H = 0) or high half of the words' low bytes: 16u is as
+// good a subnormal as u, and needs no shift.
+template <int H>
+__device__ __forceinline__ f16x2 centred4(uint32_t two, f16x2 zc) {
+  const _Float16 f = (_Float16)(H ? 2048.f : 32768.f);
+  const f16x2 up = {f, f};
+  return __builtin_elementwise_fma(as_h2(two & (H ? 0x00f000f0u : 0x000f000fu)), up, zc);
+}
 __device__ __forceinline__ f16x2 centre(int z0, int z1) {
   return f16x2{(_Float16)((float)-z0 * 0x1p-9f), (_Float16)((float)-z1 * 0x1p-9f)};
 }
@@ -112,8 +120,8 @@ __device__ __forceinline__ f16x8 key_codes(const uint32_t* w, f16x2 zc) {
       h[2 * i + 1] = centred(__builtin_amdgcn_perm(0, w[i], 0x0c030c02), zc);
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = centred((w[0] >> (4 * i)) & 0x000f000fu, zc);
+    h[0] = centred4<0>(w[0], zc), h[1] = centred4<1>(w[0], zc);
+    h[2] = centred4<0>(w[0] >> 8, zc), h[3] = centred4<1>(w[0] >> 8, zc);
   }
   return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
@@ -133,7 +141,7 @@ __device__ __forceinline__ f16x2 value_codes(const uint32_t* a, const uint32_t* 
   } else {
     const uint32_t k = e >> 1;
     const uint32_t two = __builtin_amdgcn_perm(b[0], a[0], 0x0c000c00u | (4 + k) << 16 | k);
-    return centred((two >> (4 * (e & 1))) & 0x000f000fu, zc);
+    return e & 1 ? centred4<1>(two, zc) : centred4<0>(two, zc);
   }
 }
 
@@ -258,8 +266,8 @@ __device__ void clear_outside(const AttnArgs& a) {
 // Row statistics are per lane (row = lane % 16).  Four waves interleave blocks of 32
 // keys and join through LDS; `few_split` workgroups share a sequence's keys.
 // DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
-// Bound by the cache's bytes at 8 bits and by the codes' conversion (four instructions of
-// vector arithmetic per two codes) at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
+// Bound by the cache's bytes at 8 bits and by the codes' conversion (two to three
+// instructions of vector arithmetic per two codes) at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
 // 131072 keys 51 µs (5.4 TB/s), 64 over 4096 each 104 µs (5.3 TB/s); 4 bits: 64 over 4096
 // 66 µs (4.3 TB/s); one over 4001 at 8 bits 8.6 µs and 4 to join, latency.  Up to 16 rows, one
 // block of the product's columns: 32 uneven sequences with 2 tokens of 8 heads 49 µs, 100 by
