@@ -140,18 +140,25 @@ class Int8Linear(torch.nn.Module):
         return cls(codes.to(torch.int8), scale, bias=linear.bias, sym=sym)
 
     def forward(self, x):
-        x2 = _rows(x, self.in_features, "Int8Linear")
-        rows, columns, out = x2.shape[0], self.in_features, self.out_features
+        columns, out = self.in_features, self.out_features
         held = self._buffers  # (attribute access of a module's buffers is slow)
         weight, total, bias = held["weight"], held["weight_sum"], held["bias"]
-        if weight.get_device() != x.get_device():
-            raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {weight.device}")
+        # what is usual passes in one go (a call is a few microseconds); the rest is told apart
+        if (x.is_cuda and x.dim() == 2 and x.shape[1] == columns and x.is_contiguous()
+                and x.dtype in _DTYPE_CODE and not x.requires_grad
+                and x.get_device() == weight.get_device() == torch._C._cuda_getDevice()):
+            x2, rows, stride = x, x.shape[0], columns
+        else:
+            x2 = _rows(x, columns, "Int8Linear")
+            if weight.get_device() != x.get_device():
+                raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {weight.device}")
+            rows, stride = x2.shape[0], _row_stride(x2)
         y = x.new_empty((rows, out))
         if rows:
             need = _lib.workspace_fast("int8_linear_workspace", rows, out, columns)
             ws = _lib.scratch(need, x.device) if need else None
             _lib.call_fast("int8_linear", _lib.current_stream(), x2.data_ptr(),
-                           _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), self.sym,
+                           _DTYPE_CODE[x.dtype], rows, columns, stride, self.sym,
                            weight.data_ptr(), weight.stride(0), held["weight_scale"].data_ptr(),
                            None if total is None else total.data_ptr(),
                            None if bias is None else bias.data_ptr(), out, y.data_ptr(), out,

@@ -131,16 +131,22 @@ class PagedKVCache:
         ``cu_tokens[b]`` to ``cu_tokens[b + 1]`` hold the first positions of the
         sequence whose pages are ``table[b]`` (both int32).  Rows outside every
         sequence, and positions without a page, are zero."""
+        here, cu = self._device, cu_tokens
+        # (as in write)
+        if not (table.dtype is cu.dtype is torch.int32 and table.dim() == 2 and cu.dim() == 1
+                and table.is_contiguous() and cu.is_contiguous()
+                and table.get_device() == cu.get_device() == here
+                and torch._C._cuda_getDevice() == here):
+            table = _index(table, torch.int32, 2, "table", self.device)
+            cu = _index(cu, torch.int32, 1, "cu_tokens", self.device)
+            _lib.require_current(self._held[6], "PagedKVCache.read")
         if dtype not in _DTYPE_CODE:
             raise NotImplementedError(f"PagedKVCache.read gives bf16, fp16 or fp32, not {dtype}")
-        table = _index(table, torch.int32, 2, "table", self.device)
-        cu = _index(cu_tokens, torch.int32, 1, "cu_tokens", self.device)
         B, width = table.shape
         if cu.shape[0] != B + 1:
             raise ValueError(f"cu_tokens has {cu.shape[0]} entries for {B} sequences")
         if total < 0:
             raise ValueError(f"total is {total}")
-        _lib.require_current(self._held[6], "PagedKVCache.read")
         k = torch.empty(total, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         _lib.call_fast("kv_read", _lib.current_stream(), self._address, table.data_ptr(),
