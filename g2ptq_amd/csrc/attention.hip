@@ -311,8 +311,9 @@ attend_rows_kernel(AttnArgs a) {
 
   for (int r0 = 0; r0 < rows; r0 += 16) {
     const RowAt at = row_at(a, sp, h, min(r0 + n, rows - 1));
-    // the last key that the lane's row sees, and that any of the block's rows sees
+    // the last key that the lane's row sees; that every and that any of the block's rows sees
     const int last = min(sp.pos0 + (at.token - sp.q0), sp.n - 1);
+    const int first_all = min(sp.pos0 + r0 / a.G, sp.n - 1);  // seen by every row of the block
     const int last_all = min(sp.pos0 + (min(r0 + 15, rows - 1)) / a.G, sp.n - 1);
     const int k0 = split * sh.each + 32 * wave, k1 = min(last_all + 1, (split + 1) * sh.each);
     const int steps = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;  // blocks of 32 keys, every 128
@@ -339,7 +340,7 @@ attend_rows_kernel(AttnArgs a) {
 #define G2_S(buf, ok)                                                                        \
   do {                                                                                       \
     if (!sok) sc = 0.f;                                                                      \
-    ok = (uint32_t)__builtin_amdgcn_ballot_w64(sok);                                         \
+    ok = __builtin_amdgcn_ballot_w64(sok && (!kv || sc < __builtin_inff()));                 \
     if (kv) {                                                                                \
       svL[wave][buf][lane - 32] = sc;                                                        \
       zvL[wave][buf][lane - 32] = centre(sz, sz)[0];                                         \
@@ -389,7 +390,8 @@ attend_rows_kernel(AttnArgs a) {
     }                                                                                        \
   } while (0)
     uint32_t ka[2][KW], va[8][VW], kb_[2][KW], vb[8][VW];
-    uint32_t oka = 0, okb = 0;
+    // low half: keys that are there; high half: those whose value's scale is finite
+    uint64_t oka = 0, okb = 0;
     if (steps > 0) {
       G2_P(0);
       G2_M(0);
@@ -424,16 +426,10 @@ attend_rows_kernel(AttnArgs a) {
     for (int e = 0; e < DV; ++e) acc[e] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.f, ref = 0x1p-90f;
 
-    auto arithmetic = [&](int j0, int buf, uint32_t ok, const uint32_t (&kw)[2][KW],
+    auto arithmetic = [&](int j0, int buf, uint64_t ok, const uint32_t (&kw)[2][KW],
                           const uint32_t (&vw)[8][VW]) __attribute__((always_inline)) {
       float p[8], sv[8];
       float mx = m, vx = 0.f;
-      uint32_t see = 0;  // bit i: element i = 4kb + i%4 is key 16kb + 4g + i%4 of the step
-      {
-        const int c = last - j0;  // the last key seen
-        const uint32_t seen = (c < 0 ? 0u : ok) & (~0u >> (31 - min(max(c, 0), 31)));
-        see = (seen >> (4 * g) & 15u) | (seen >> (16 + 4 * g) & 15u) << 4;
-      }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const f16x2 zc = as_h2(zkL[wave][buf][16 * kb + n]);
@@ -445,20 +441,30 @@ attend_rows_kernel(AttnArgs a) {
         const f32x4 sk = *reinterpret_cast<const f32x4*>(&skL[wave][buf][16 * kb + 4 * g]);
         const f32x4 s4 = *reinterpret_cast<const f32x4*>(&svL[wave][buf][16 * kb + 4 * g]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool on = see >> (4 * kb + i) & 1;
-          p[4 * kb + i] = x[i] * sk[i];
-          sv[4 * kb + i] = s4[i];
-          mx = fmaxf(mx, on ? p[4 * kb + i] : -INFINITY);
-          vx = fmaxf(vx, on && s4[i] < __builtin_inff() ? s4[i] : 0.f);
+        for (int i = 0; i < 4; ++i) p[4 * kb + i] = x[i] * sk[i], sv[4 * kb + i] = s4[i];
+      }
+      const bool whole = ok == ~0ull && j0 + 31 <= first_all;  // every row sees every key
+      uint32_t see = 0;  // bit i: element i = 4kb + i%4 is key 16kb + 4g + i%4 of the step
+      if (__builtin_expect(whole, 1)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[i]), vx = fmaxf(vx, sv[i]);
+      } else {
+        const int c = last - j0;  // the last key seen
+        const uint32_t seen = (c < 0 ? 0u : (uint32_t)ok) & (~0u >> (31 - min(max(c, 0), 31)));
+        see = (seen >> (4 * g) & 15u) | (seen >> (16 + 4 * g) & 15u) << 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool on = see >> i & 1;
+          mx = fmaxf(mx, on ? p[i] : -INFINITY);
+          vx = fmaxf(vx, on && sv[i] < __builtin_inff() ? sv[i] : 0.f);
         }
       }
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      vx = fmaxf(vx, __shfl_xor(vx, 16));
-      vx = fmaxf(vx, __shfl_xor(vx, 32));
-      // ---- the row's units ----
+      // ---- the row's units: m and ref are the same in its four lanes, and grow rarely ----
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        vx = fmaxf(vx, __shfl_xor(vx, 16));
+        vx = fmaxf(vx, __shfl_xor(vx, 32));
         const float nref = vx >= ref ? above(vx) : ref;
         float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
         if (m == mx) f = 1.f;
@@ -471,12 +477,22 @@ attend_rows_kernel(AttnArgs a) {
       asm volatile("" : "+v"(m), "+v"(ref));  // (as in attend_tiles_kernel)
       const float e0 = (float)(15 - exponent(ref)), m0 = m == -INFINITY ? 0.f : m;
       f16x8 w;
+      if (__builtin_expect(whole, 1)) {
+        asm volatile("");  // (keeps the branches apart: no selects here)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool on = see >> i & 1;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
-        l += on ? x : 0.f;
-        w[i] = (_Float16)(on ? x * sv[i] : 0.f);
+        for (int i = 0; i < 8; ++i) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
+          l += x;
+          w[i] = (_Float16)(x * sv[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool on = see >> i & 1;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i] - m0, C, e0));
+          l += on ? x : 0.f;
+          w[i] = (_Float16)(on ? x * sv[i] : 0.f);
+        }
       }
       // ---- values ----
       const f16x4 z0 = *reinterpret_cast<const f16x4*>(&zvL[wave][buf][4 * g]);
@@ -947,10 +963,11 @@ attend_tiles_kernel(AttnArgs a) {
               mx = fmaxf(mx, on ? x[kb][v] : -INFINITY);
               vx = fmaxf(vx, on && s1 < __builtin_inff() ? s1 : 0.f);
             }
-          vx = fmaxf(vx, __shfl_xor(vx, 32));
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        // (m and ref are the same in a row's two lanes)
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m || vx >= ref) != 0, 0)) {
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          vx = fmaxf(vx, __shfl_xor(vx, 32));
           const float nref = vx >= ref ? above(vx) : ref;
           float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * C);
           if (m == mx) f = 1.f;
