@@ -39,6 +39,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+constexpr int kTileRows = 128;  // of a workgroup of attend_tiles_kernel
 constexpr int kFewRows = 16;  // rows of a sequence and head up to which attend_rows_kernel runs
 
 struct AttnArgs {
@@ -266,12 +267,12 @@ __device__ void clear_outside(const AttnArgs& a) {
 // Row statistics are per lane (row = lane % 16).  Four waves interleave blocks of 32
 // keys and join through LDS; `few_split` workgroups share a sequence's keys.
 // DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
-// Bound by the cache's bytes at 8 bits and by the codes' conversion (two to three
-// instructions of vector arithmetic per two codes) at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
-// 131072 keys 51 µs (5.4 TB/s), 64 over 4096 each 104 µs (5.3 TB/s); 4 bits: 64 over 4096
-// 66 µs (4.3 TB/s); one over 4001 at 8 bits 8.6 µs and 4 to join, latency.  Up to 16 rows, one
-// block of the product's columns: 32 uneven sequences with 2 tokens of 8 heads 49 µs, 100 by
-// attend_tiles_kernel; 4 tokens over 8192 keys 17.6 against 23.4 µs.
+// Bound by the cache's bytes at 8 bits and by vector arithmetic (two to three
+// instructions per two codes) and the loads a CU keeps under way about alike at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
+// 131072 keys 51 µs (5.4 TB/s), 64 over 4096 each 98–102 µs (5.5 TB/s); 4 bits: 64 over 4096
+// 61 µs (4.7 TB/s); one over 4001 at 8 bits 8.6 µs and 4 to join, latency.  Up to 16 rows, one
+// block of the product's columns: 32 uneven sequences with 2 tokens of 8 heads 38 µs, 74 by
+// attend_tiles_kernel; 4 tokens over 8192 keys 14.4 against 24.6 µs.
 // ---------------------------------------------------------------------------
 template <int BITS, int DP, bool FULL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? (BITS == 4 ? 3 : 2) : 1) void
@@ -582,7 +583,7 @@ attend_rows_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows (chunks of prompts): matrix cores.  A workgroup of NW waves takes 32·NW
+// Many rows (chunks of prompts): matrix cores.  A workgroup of four waves takes 128
 // rows, 32 per wave, through 64 keys at a time.  The keys and values of a step are
 // converted to fp16 once per workgroup and kept in LDS, keys as [key][channel], values
 // transposed as [channel][key] (two buffers each); the codes after them are loaded
@@ -619,10 +620,10 @@ __device__ __forceinline__ float wave_max(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
-template <int BITS, int DP, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 && DP <= 128 ? 2 : 1) void
+template <int BITS, int DP, bool FULL>
+__global__ __launch_bounds__(2 * kTileRows, DP <= 128 ? 2 : 1) void
 attend_tiles_kernel(AttnArgs a) {
-  constexpr int NT = 64 * NW, BM = 32 * NW, BN = 64;
+  constexpr int NT = 2 * kTileRows, BM = kTileRows, BN = 64;
   constexpr int KC = BN * (DP / 16) / NT;                          // 16-channel pieces of keys
   constexpr int VP = BN / 4 * (DP / 8), VQ = (VP + NT - 1) / NT;   // 4-key × 8-channel of values
   constexpr int KW = BITS / 2, VW = BITS / 4;   // words of 16 and of 8 channels
@@ -1184,7 +1185,6 @@ constexpr int64_t kCUs = 256;
 
 struct Plan {
   bool few, tiles;     // which kernels run
-  int nw;              // waves of a tile's workgroup
   int64_t ntiles, split, few_split, share, few_share;
   int64_t part, few_part;  // bytes of partial results
   Plan(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t max_q, int64_t max_kv) {
@@ -1196,13 +1196,13 @@ struct Plan {
     // Few rows: shares of 1024 keys or more, up to sixteen workgroups per CU (sequences of a
     // batch differ in length, and the last ones to run should be short); smaller ones, from
     // 256 keys (two steps of every wave), for six per CU.  MI355X, heads 32 on 8 of 128:
-    //   64 uneven sequences of up to 8192 keys, 4 bits: 79 µs in 8, 88 in 3, 116 unshared
-    //   96 of them: 115 µs in 6 shares, 154 in 2
-    //   16 uneven of up to 8192, 4 bits: 33 µs in 12, 41 in 4, 55 in 32
-    //   one of 8192, 8 bits: 13.4 µs in shares of 256, 15.6 of 128, 14.5 of 512
+    //   64 uneven sequences of up to 8192 keys, 4 bits: 72 µs in 8, 76 in 3, 91 unshared
+    //   96 of them: 111 µs in 6 shares, 131 in 2
+    //   16 uneven of up to 8192, 4 bits: 32 µs in 12, 36 in 4, 53 in 32
+    //   one of 8192, 8 bits: 13.1 µs in shares of 256, 16.1 of 128, 14.1 of 512
     // None where two workgroups per CU are there without and short: 64 uneven sequences of up
-    // to 4096 keys 58 µs, 62 in 4; 160 of up to 2048, 70 µs and 94 in 2.  At most 32: 8
-    // sequences of 16384, two heads, 21 µs in 32 and 27 in 64, whose joining costs more; up
+    // to 4096 keys 55 µs, 57 in 4; 160 of up to 2048, 68 µs and 89 in 2.  At most 32: 8
+    // sequences of 16384, two heads, 21 µs in 32 and 26 in 64, whose joining costs more; up
     // to 64 for a few heads, which are not enough otherwise.
     int64_t want = std::max(std::min(cdiv(16 * kCUs, pairs), keys / 1024),
                             std::min(cdiv(6 * kCUs, pairs), cdiv(keys, 256)));
@@ -1212,13 +1212,13 @@ struct Plan {
     few_split = cdiv(keys, few_share);
     // 128 rows a workgroup, two workgroups to a CU.  (256 rows, one to a CU: MI355X, 2048
     // tokens over 16384 keys 714 against 702 µs, six uneven chunks 44 against 35 µs; 64 rows:
-    // 1197 µs, but 23 against 25 for 32 tokens over 600 keys.)
-    nw = rows > 64 ? 4 : 2;
-    ntiles = std::max<int64_t>(1, cdiv(rows, 32 * nw));
+    // 1211 against 671 µs, and where that is all there are, 8 tokens of four heads over 4096
+    // keys, 23.4 against 20.9.)
+    ntiles = std::max<int64_t>(1, cdiv(rows, kTileRows));
     // Shares for two workgroups per CU, three in a batch (its sequences differ in length).
-    // MI355X, heads 32 on 8 of 128, two / three / four: 512 tokens over 2048 keys 51.7 / 60.8
-    // / 62.9 µs; four chunks of 300 over up to 4096 keys 163 / 122 / 131 µs; six of 100, 104 /
-    // 75 / 88 µs.  Of 256 keys or more: 8 chunks of 16 tokens over 2048 keys 33 µs, 40 with 512.
+    // MI355X, heads 32 on 8 of 128, two / three / four: 512 tokens over 2048 keys 53.7 / 62.9
+    // / 66.6 µs; four chunks of 300 over up to 4096 keys 158 / 116 / 123 µs; six of 100, 100 /
+    // 71 / 84 µs.  Of 256 keys or more: 8 chunks of 16 tokens over 2048 keys 33 µs, 40 with 512.
     split = std::max<int64_t>(1, std::min((B > 1 ? 3 : 2) * kCUs / (pairs * ntiles), keys / 256));
     split = std::min<int64_t>(split, 32);
     share = cdiv(cdiv(keys, split), 64) * 64;
@@ -1237,12 +1237,9 @@ int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
     G2PTQ_LAUNCHED();
   }
   if (p.tiles) {
-    const dim3 grid((unsigned)(a.B * a.c.H * a.split * a.tiles + 1));
-#define G2_AT(NW)                                                                            \
-  hipLaunchKernelGGL((attend_tiles_kernel<BITS, DP, FULL, NW>), grid, dim3(64 * NW), 0, st, a)
-    if (p.nw == 4) G2_AT(4);
-    else G2_AT(2);
-#undef G2_AT
+    hipLaunchKernelGGL((attend_tiles_kernel<BITS, DP, FULL>),
+                       dim3((unsigned)(a.B * a.c.H * a.split * a.tiles + 1)), dim3(2 * kTileRows),
+                       0, st, a);
     G2PTQ_LAUNCHED();
   }
   if (a.part || a.few_part) {
