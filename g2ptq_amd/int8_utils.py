@@ -9,11 +9,14 @@ rounded once.  The token grid is the weight quantizer's (``quant_utils``) at
 8 bits with one group per token.  Inference only: nothing here has a
 gradient.
 """
+import math
+
 import torch
 
 from . import _lib
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 MAX_COLUMNS = 65536  # longer rows could overflow the 32-bit sums
 
 
@@ -89,8 +92,8 @@ class Int8Linear(torch.nn.Module):
             raise RuntimeError("Int8Linear requires GPU tensors")
         self.sym = bool(sym)
         dev = codes.device
-        weight = torch.zeros(self.out_features, _padded(self.in_features, 256), dtype=torch.int8,
-                             device=dev)
+        self._shape = (self.out_features, _padded(self.in_features, 256))
+        weight = torch.zeros(self._shape, dtype=torch.int8, device=dev)
         weight[:, :self.in_features] = codes
         self.register_buffer("weight", weight)
         self.register_buffer("weight_scale", scale.detach().reshape(-1).to(
@@ -99,6 +102,46 @@ class Int8Linear(torch.nn.Module):
                              codes.sum(dim=1, dtype=torch.int32))
         self.register_buffer("bias", None if bias is None else bias.detach().to(
             device=dev, dtype=torch.float32, copy=True))
+
+    def _apply(self, fn, recurse=True):
+        """The module follows its model to another device; a cast of the model leaves it as it
+        is: the kernels read int8 codes and fp32 scales and biases, whatever the tokens' type."""
+        before = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, was in before.items():
+            now = self._buffers[name]
+            if now is not None and now.dtype is not was.dtype:
+                self._buffers[name] = was.to(now.device)
+        return self
+
+    def _operands(self):
+        """The weights, scales, sums and biases (the last two or None) and their device's index.
+        The kernels know them by their addresses, and buffers can be replaced by any tensor
+        (``load_state_dict`` with ``assign``, an attribute set), so every call looks at them."""
+        held, n, shape = self._buffers, self.out_features, self._shape
+        # (attribute access of a module's buffers is slow)
+        weight, scale, total, bias = (held["weight"], held["weight_scale"], held["weight_sum"],
+                                      held["bias"])
+        here = weight.get_device()
+        if not (weight.dtype is _I8 and weight.shape == shape and weight.is_contiguous()
+                and scale.dtype is _F32 and scale.numel() == n and scale.is_contiguous()
+                and scale.get_device() == here
+                and (bias is None or (bias.dtype is _F32 and bias.numel() == n
+                                      and bias.is_contiguous() and bias.get_device() == here))
+                and (total is None or (total.dtype is _I32 and total.numel() == n
+                                       and total.is_contiguous()
+                                       and total.get_device() == here))):
+            for name, dtype, size in (("weight", _I8, shape), ("weight_scale", _F32, (n,)),
+                                      ("weight_sum", _I32, (n,)), ("bias", _F32, (n,))):
+                t = held[name]
+                if t is not None and (t.dtype is not dtype or t.numel() != math.prod(size)
+                                      or (name == "weight" and t.shape != shape)
+                                      or not t.is_contiguous() or t.get_device() != here):
+                    raise ValueError(f"Int8Linear: {name} is {t.dtype} of shape {tuple(t.shape)} "
+                                     f"and strides {t.stride()} on {t.device}; a contiguous "
+                                     f"{dtype} tensor of shape {size} on {weight.device} is "
+                                     "needed")
+        return weight, scale, total, bias, here
 
     @classmethod
     def from_export(cls, qparams, bias=None, sym=True):
@@ -141,16 +184,15 @@ class Int8Linear(torch.nn.Module):
 
     def forward(self, x):
         columns, out = self.in_features, self.out_features
-        held = self._buffers  # (attribute access of a module's buffers is slow)
-        weight, total, bias = held["weight"], held["weight_sum"], held["bias"]
+        weight, scale, total, bias, here = self._operands()
         # what is usual passes in one go (a call is a few microseconds); the rest is told apart
-        if (x.is_cuda and x.dim() == 2 and x.shape[1] == columns and x.is_contiguous()
+        if (x.dim() == 2 and x.shape[1] == columns and x.is_contiguous()
                 and x.dtype in _DTYPE_CODE and not x.requires_grad
-                and x.get_device() == weight.get_device() == torch._C._cuda_getDevice()):
+                and x.get_device() == here == torch._C._cuda_getDevice()):
             x2, rows, stride = x, x.shape[0], columns
         else:
             x2 = _rows(x, columns, "Int8Linear")
-            if weight.get_device() != x.get_device():
+            if here != x.get_device():
                 raise ValueError(f"Int8Linear: tokens on {x.device}, weights on {weight.device}")
             rows, stride = x2.shape[0], _row_stride(x2)
         y = x.new_empty((rows, out))
@@ -159,7 +201,7 @@ class Int8Linear(torch.nn.Module):
             ws = _lib.scratch(need, x.device) if need else None
             _lib.call_fast("int8_linear", _lib.current_stream(), x2.data_ptr(),
                            _DTYPE_CODE[x.dtype], rows, columns, stride, self.sym,
-                           weight.data_ptr(), weight.stride(0), held["weight_scale"].data_ptr(),
+                           weight.data_ptr(), self._shape[1], scale.data_ptr(),
                            None if total is None else total.data_ptr(),
                            None if bias is None else bias.data_ptr(), out, y.data_ptr(), out,
                            None if ws is None else ws.data_ptr(), need)
@@ -201,13 +243,13 @@ def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
         c2 = padded
     y = torch.empty(rows, out, dtype=dtype, device=codes.device)
     if rows:
+        weight, wscale, total, bias, _ = linear._operands()
         scale, zero = scale.contiguous(), None if zero is None else zero.contiguous()
         ws = _lib.scratch(_lib.query_size("g2ptq_int8_gemm_workspace", rows, out, columns),
                           codes.device)
         _lib.call("g2ptq_int8_gemm", _lib.stream_ptr(codes.device), _lib.ptr(c2), c2.stride(0),
-                  _lib.ptr(scale), _lib.ptr(zero), _lib.ptr(linear.weight),
-                  linear.weight.stride(0), _lib.ptr(linear.weight_scale),
-                  _lib.ptr(linear.weight_sum if zero is not None else None),
-                  _lib.ptr(linear.bias), rows, out, columns, _lib.ptr(y), _DTYPE_CODE[dtype], out,
-                  _lib.ptr(ws), ws.numel())
+                  _lib.ptr(scale), _lib.ptr(zero), _lib.ptr(weight), linear._shape[1],
+                  _lib.ptr(wscale), _lib.ptr(None if zero is None else total), _lib.ptr(bias),
+                  rows, out, columns, _lib.ptr(y), _DTYPE_CODE[dtype], out, _lib.ptr(ws),
+                  ws.numel())
     return y.view(*lead, out)

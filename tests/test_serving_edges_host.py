@@ -1,0 +1,71 @@
+"""CPU: what a user's program can do around the operators of a quantized layer without
+a launch: casts of a model, replaced buffers, exports that are not 8-bit codes."""
+import pytest
+import torch
+
+from g2ptq_amd import Int8Linear
+
+
+def on_cpu(rows=5, columns=20, asym=True, bias=True):
+    """An Int8Linear whose buffers are on the CPU (where it cannot be made or called)."""
+    lin = Int8Linear.__new__(Int8Linear)
+    torch.nn.Module.__init__(lin)
+    lin.out_features, lin.in_features, lin._shape = rows, columns, (rows, 256)
+    lin.sym = not asym
+    g = torch.Generator().manual_seed(1)
+    lin.register_buffer("weight", torch.randint(-128, 128, (rows, 256), generator=g,
+                                                dtype=torch.int8))
+    lin.register_buffer("weight_scale", torch.rand(rows, generator=g))
+    lin.register_buffer("weight_sum", lin.weight.sum(1, dtype=torch.int32) if asym else None)
+    lin.register_buffer("bias", torch.randn(rows, generator=g) if bias else None)
+    return lin
+
+
+CASTS = [lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(),
+         lambda m: m.type(torch.float16), lambda m: m.half().float()]
+
+
+@pytest.mark.parametrize("cast", CASTS)
+@pytest.mark.parametrize("asym,bias", [(True, True), (False, False)])
+def test_a_cast_of_the_model_leaves_the_operands_as_they_are(cast, asym, bias):
+    lin = on_cpu(asym=asym, bias=bias)
+    before = {n: None if b is None else b.clone() for n, b in lin._buffers.items()}
+    model = cast(torch.nn.Sequential(torch.nn.Linear(20, 20), lin))
+    assert model[1] is lin
+    for name, was in before.items():
+        now = lin._buffers[name]
+        assert (now is None) == (was is None), name
+        if was is not None:
+            assert now.dtype is was.dtype and torch.equal(now, was), name
+    lin._operands()
+
+
+def test_moves_still_follow_the_model():
+    lin = on_cpu()
+    assert all(b.device.type == "meta" for b in lin.to("meta", torch.float16)._buffers.values())
+    assert lin.weight_scale.dtype is torch.float32
+
+
+@pytest.mark.parametrize("name,make", [
+    ("weight", lambda t: t.half()), ("weight", lambda t: t[:, :128].contiguous()),
+    ("weight", lambda t: t.reshape(-1, 128)), ("weight", lambda t: t.t().contiguous().t()),
+    ("weight", lambda t: t[:-1]), ("weight_scale", lambda t: t.bfloat16()),
+    ("weight_scale", lambda t: t[:-1]), ("weight_scale", lambda t: t[:1].expand(5)),
+    ("bias", lambda t: t.half()),
+    ("bias", lambda t: torch.stack([t, t], 1)[:, 0]), ("weight_sum", lambda t: t.long())])
+def test_replaced_buffers_are_refused_before_a_launch(name, make):
+    lin = on_cpu()
+    setattr(lin, name, make(getattr(lin, name)))
+    with pytest.raises(ValueError, match=name + " is"):
+        lin._operands()
+
+
+def test_a_checkpoint_of_another_type():
+    lin = on_cpu()
+    state = {k: v.half() if v.is_floating_point() else v for k, v in lin.state_dict().items()}
+    other = on_cpu()
+    other.load_state_dict(state)  # copied into the fp32 buffers
+    other._operands()
+    other.load_state_dict(state, assign=True)
+    with pytest.raises(ValueError, match="weight_scale is torch.float16"):
+        other._operands()
