@@ -64,7 +64,8 @@ class G2PTQ:
                 self.gradients[b].copy_(gradient, non_blocking=True)
         self.H = _core.alloc((self.num_layers, self.num_groups, self.columns, self.columns),
                              H_device)
-        self.act_square = torch.zeros((self.num_layers, self.columns), device=self.dev)
+        self.act_square = torch.zeros((self.num_layers, self.columns), dtype=torch.float32,
+                                      device=self.dev)
         self.index = torch.tensor([0] * self.num_layers, device=self.dev)
         self.total_tokens = torch.tensor([0] * self.num_layers, device=self.dev)
         self._k = [0] * self.num_layers
@@ -219,7 +220,7 @@ class G2PTQ:
             if Q_sub is not None and actorder:
                 Q_sub = _core.permute_cols(Q_sub, perm)
         if gradient_step:
-            beta = torch.empty(B * G * Rg, device=self.dev)
+            beta = torch.empty(B * G * Rg, dtype=torch.float32, device=self.dev)
             Z = torch.empty_like(W_sub)
             GH = torch.empty_like(W_sub)
             ws = _lib.workspace(_lib.query_size("g2ptq_trust_region_workspace", B * G, Rg, C),

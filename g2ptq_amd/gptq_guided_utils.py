@@ -30,7 +30,8 @@ class GPTQGuided(GPTQ):
         H_device = "cpu" if offload_hessians else self.dev
         self.H = _core.alloc((self.num_layers, self.num_groups, self.columns, self.columns),
                              H_device)
-        self.act_square = torch.zeros((self.num_layers, self.columns), device=self.dev)
+        self.act_square = torch.zeros((self.num_layers, self.columns), dtype=torch.float32,
+                                      device=self.dev)
         self.index = torch.tensor([0] * self.num_layers, device=self.dev)
         self._k = [0] * self.num_layers
         self._stagers = [None] * self.num_layers

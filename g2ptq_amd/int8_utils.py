@@ -56,8 +56,8 @@ def quantize_tokens(x, sym=True):
     x2 = _rows(x, columns, "quantize_tokens")
     rows, ldc = x2.shape[0], _padded(columns)
     codes = torch.empty(rows, ldc, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, device=x.device)
-    zero = None if sym else torch.empty(rows, device=x.device)
+    scale = torch.empty(rows, dtype=_F32, device=x.device)
+    zero = None if sym else torch.empty(rows, dtype=_F32, device=x.device)
     _lib.call("g2ptq_quantize_tokens", _lib.stream_ptr(x.device), _lib.ptr(x2),
               _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), int(bool(sym)),
               _lib.ptr(codes), ldc, _lib.ptr(scale), _lib.ptr(zero))

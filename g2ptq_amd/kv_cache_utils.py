@@ -76,7 +76,7 @@ class PagedKVCache:
         shape = (num_pages, kv_heads, page_size)
         codes = [torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=dev)
                  for _ in range(2)]
-        scales = [torch.zeros(shape, device=dev) for _ in range(2)]
+        scales = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in range(2)]
         zeros = [None if self.sym else torch.zeros(shape, dtype=torch.uint8, device=dev)
                  for _ in range(2)]
         flags = torch.zeros(1, dtype=torch.int32, device=dev)

@@ -34,3 +34,41 @@ def test_casts_of_a_model_leave_its_int8_linears_right(dev, sym):
     lin.weight_scale = lin.weight_scale.cpu()
     with pytest.raises(ValueError, match="weight_scale is .* on cpu"):
         lin(x.to(dev))
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64], ids=str)
+def test_torchs_default_type_changes_nothing(dev, default):
+    from g2ptq_amd import GPTQGuided, G2PTQ, Int8Linear, PagedKVCache, int8_matmul, quantize_tokens
+    from g2ptq_amd import paged_attention
+    T, K, H, D, page = 40, 130, 2, 64, 16
+    w, wscale, bias = _weights(70, K, 4)
+    x = _tokens(T, K, torch.bfloat16, 5)
+    k = _tokens(T, H * D, torch.float16, 6).view(T, H, D).to(dev)
+    q = _tokens(T, 4 * D, torch.float16, 7).view(T, 4, D).to(dev)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=dev)
+    cu, lens = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([0, T], [T]))
+    slots = serving.slot_map(table.cpu(), page, [0, T], [T]).to(dev)
+
+    def serve():
+        lin = Int8Linear(w.to(dev), wscale.to(dev), bias=bias.to(dev), sym=False)
+        c, s, z = quantize_tokens(x.to(dev), sym=False)
+        cache = PagedKVCache(3, page, H, D, bits=4, sym=False, device=dev)
+        cache.write(k, k, slots)
+        return [c, s, z, lin(x.to(dev)), int8_matmul(c, s, lin, zero=z),
+                *cache.read(table, cu, T), paged_attention(q, cache, table, cu, lens),
+                cache.k_scale, cache.v_scale]
+
+    ref = serve()
+    layers = [torch.nn.Linear(64, 32, bias=False, device=dev)]
+    sal = [torch.ones(1, 4, 1, device=dev)]
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        got = serve()
+        acts = (GPTQGuided(layers, sal, 1).act_square, G2PTQ(layers, [sal], [None], 1).act_square)
+    finally:
+        torch.set_default_dtype(was)
+    for i, (a, b) in enumerate(zip(got, ref)):
+        assert a.dtype is b.dtype
+        assert_bitexact(a, b, f"output {i}")
+    assert all(a.dtype is torch.float32 for a in acts)

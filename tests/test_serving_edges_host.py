@@ -1,8 +1,13 @@
 """CPU: what a user's program can do around the operators of a quantized layer without
 a launch: casts of a model, replaced buffers, exports that are not 8-bit codes."""
+import ast
+import glob
+import os
+
 import pytest
 import torch
 
+import g2ptq_amd
 from g2ptq_amd import Int8Linear
 
 
@@ -69,3 +74,18 @@ def test_a_checkpoint_of_another_type():
     other.load_state_dict(state, assign=True)
     with pytest.raises(ValueError, match="weight_scale is torch.float16"):
         other._operands()
+
+
+def test_memory_that_kernels_read_has_its_type_from_the_code():
+    """The kernels read and write fp32 by address: under torch.set_default_dtype with a
+    16-bit type, memory without a type of its own would be half as large as they take it for."""
+    allocators = ("empty", "zeros", "ones", "full", "rand", "randn")
+    for path in sorted(glob.glob(os.path.join(os.path.dirname(g2ptq_amd.__file__), "*.py"))):
+        with open(path) as f:
+            tree = ast.parse(f.read())
+        for call in ast.walk(tree):
+            if (isinstance(call, ast.Call) and isinstance(call.func, ast.Attribute)
+                    and isinstance(call.func.value, ast.Name) and call.func.value.id == "torch"
+                    and call.func.attr in allocators):
+                given = {k.arg for k in call.keywords}
+                assert "device" not in given or "dtype" in given, (path, call.lineno)
