@@ -44,12 +44,15 @@ def pack_to_int32(value, num_bits):
     return packed
 
 
-def compress(layer, Scale, W_int, bits, groupsize):
+def compress(layer, Scale, W_int, bits, groupsize, sym=None):
     """utils/compressed_tensors_utils.py:22-45: stash the layer's packed codes,
     per-group scales (weight dtype) and shape in ``layer._export_qparams``.
 
     ``Scale`` and ``W_int`` are the compensation's per-element scales and
-    integer codes (fp32, any shape with ``weight.numel()`` elements)."""
+    integer codes (fp32, any shape with ``weight.numel()`` elements).  The
+    tensors tell neither the codes' width nor that codes of an asymmetric grid
+    want a zero point: ``layer._export_grid`` holds ``(bits, sym)``, ``sym``
+    None where the caller does not say."""
     weight = layer.weight
     rows, columns = weight.shape
     dtype, dev = weight.dtype, weight.device
@@ -74,13 +77,14 @@ def compress(layer, Scale, W_int, bits, groupsize):
         "weight_scale": wscale,
         "weight_shape": torch.tensor(weight.shape).to(dev).contiguous(),
     }
+    layer._export_grid = (int(bits), None if sym is None else bool(sym))
 
 
-def compress_layers(layers, Scale, W_int, bits, groupsize, columns):
+def compress_layers(layers, Scale, W_int, bits, groupsize, columns, sym=None):
     """The ``export_compressed_tensors`` step of every ``fasterquant``
     (e.g. gptq_utils.py:336-344): ``compress`` per layer of the batch."""
     for b, layer in enumerate(layers):
-        compress(layer, Scale[b], W_int[b], bits, columns if groupsize == -1 else groupsize)
+        compress(layer, Scale[b], W_int[b], bits, columns if groupsize == -1 else groupsize, sym)
 
 
 def register_qparam_buffers(modules):

@@ -250,7 +250,7 @@ class G2PTQ:
         Q = Q.view(B, R, C)
         if export_compressed_tensors:
             compress_layers(self.layers, Scale.view(B, R, C), W_int.view(B, R, C),
-                            self.quantizer[0].bits, groupsize, C)
+                            self.quantizer[0].bits, groupsize, C, self.quantizer[0].sym)
         _core.write_back(self.layers, Q, flags)
         _core.finish(flags)
 

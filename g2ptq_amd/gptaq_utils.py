@@ -180,7 +180,7 @@ class GPTAQ:
             Scale = _core.permute_cols(Scale, invperm)
         if export_compressed_tensors:
             compress_layers(self.layers, Scale.view(B, R, C), W_int.view(B, R, C),
-                            self.quantizer[0].bits, groupsize, C)
+                            self.quantizer[0].bits, groupsize, C, self.quantizer[0].sym)
         _core.write_back(self.layers, Q, flags)
         _core.finish(flags)
 

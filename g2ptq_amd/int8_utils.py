@@ -144,15 +144,28 @@ class Int8Linear(torch.nn.Module):
         return weight, scale, total, bias, here
 
     @classmethod
-    def from_export(cls, qparams, bias=None, sym=True):
-        """From a layer's exported tensors (``layer._export_qparams`` of an 8-bit
-        ``fasterquant(..., export_compressed_tensors=True)`` with one group per
-        row, or the buffers that ``register_qparam_buffers`` made of them)."""
+    def from_export(cls, qparams, bias=None, sym=True, bits=None):
+        """From a layer's exported tensors (``layer._export_qparams`` of a symmetric 8-bit
+        ``fasterquant(..., export_compressed_tensors=True)`` with one group per row, or the
+        buffers that ``register_qparam_buffers`` made of them): the layer itself, or a dict
+        of them.
+
+        The tensors do not tell the codes' width.  A layer that was exported here knows it;
+        where nothing does, codes without a single bit that narrower ones cannot have are
+        refused unless ``bits=8`` vouches for them."""
+        grid = None
         if isinstance(qparams, torch.nn.Module):
             layer = qparams
+            grid = layer.__dict__.get("_export_grid")
             qparams = layer.__dict__.get("_export_qparams") or {
                 k: b for k, b in layer.named_buffers(recurse=False)}
             bias = getattr(layer, "bias", None) if bias is None else bias
+        if bits not in (None, 8) or (grid and grid[0] != 8):
+            raise ValueError(f"Int8Linear.from_export: codes of "
+                             f"{bits if bits not in (None, 8) else grid[0]} bits are no 8-bit codes")
+        if grid and grid[1] is False:
+            raise ValueError("Int8Linear.from_export: an asymmetric quantization's export holds "
+                             "codes without their zero points; quantize with sym=True")
         try:
             packed, scale = qparams["weight_packed"], qparams["weight_scale"]
             rows, columns = (int(n) for n in qparams["weight_shape"])
@@ -165,6 +178,13 @@ class Int8Linear(torch.nn.Module):
         if scale.numel() != rows:
             raise ValueError(f"Int8Linear.from_export: scales of shape {tuple(scale.shape)}; "
                              "one group per row (groupsize -1) is needed")
+        # 7-bit codes lie four to a word as well, narrower ones too in rows of up to four: none
+        # reaches past bit 7n of a word of n codes
+        if bits is None and grid is None and packed.numel():
+            n = min(columns, 4)
+            if not bool(((packed >> (7 * n)) & ((1 << n) - 1)).any()):
+                raise ValueError("Int8Linear.from_export: the packed words look like codes of 7 "
+                                 "bits or fewer, not like 8-bit codes; bits=8 if they are")
         codes = packed.contiguous().view(torch.uint8)[:, :columns]
         return cls((codes ^ 0x80).view(torch.int8), scale, bias=bias, sym=sym)
 

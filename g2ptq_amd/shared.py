@@ -140,7 +140,7 @@ class SharedInputHessian:
             Qi = Q[0, sl].view(B, R, C)
             if export_compressed_tensors:
                 compress_layers(inst.layers, Scale[0, sl].view(B, R, C),
-                                W_int[0, sl].view(B, R, C), q0.bits, groupsize, C)
+                                W_int[0, sl].view(B, R, C), q0.bits, groupsize, C, q0.sym)
             _core.write_back(inst.layers, Qi, flags)
             off += n
         _core.finish(flags)

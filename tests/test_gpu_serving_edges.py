@@ -72,3 +72,27 @@ def test_torchs_default_type_changes_nothing(dev, default):
         assert a.dtype is b.dtype
         assert_bitexact(a, b, f"output {i}")
     assert all(a.dtype is torch.float32 for a in acts)
+
+
+@pytest.mark.parametrize("bits,sym,match", [(7, True, "codes of 7 bits"), (8, False, "zero points"),
+                                            (8, True, None)])
+def test_a_layer_knows_what_was_exported_from_it(dev, bits, sym, match):
+    from g2ptq_amd import GPTQ, Int8Linear, WeightQuantizer, make_group_quantizers
+    from g2ptq_amd.compressed_tensors_utils import register_qparam_buffers
+    lin = torch.nn.Linear(64, 48, device=dev)
+    gq = GPTQ([lin])
+    q = WeightQuantizer()
+    q.configure(bits, perchannel=True, sym=sym)
+    gq.quantizer = make_group_quantizers(q, 64, -1)
+    gq.add_batch(0, _tokens(256, 64, torch.float32, 1).to(dev).unsqueeze(0), None)
+    gq.fasterquant(blocksize=32, percdamp=0.01, groupsize=-1, backend="hip",
+                   export_compressed_tensors=True)
+    for _ in range(2):
+        if match:
+            with pytest.raises(ValueError, match=match):
+                Int8Linear.from_export(lin)
+        else:
+            run = Int8Linear.from_export(lin)
+            assert_bitexact(run.weight[:, :64].float() * run.weight_scale[:, None], lin.weight,
+                            "export")
+        register_qparam_buffers([lin])

@@ -9,6 +9,7 @@ import torch
 
 import g2ptq_amd
 from g2ptq_amd import Int8Linear
+from oracle import pack
 
 
 def on_cpu(rows=5, columns=20, asym=True, bias=True):
@@ -89,3 +90,33 @@ def test_memory_that_kernels_read_has_its_type_from_the_code():
                     and call.func.attr in allocators):
                 given = {k.arg for k in call.keywords}
                 assert "device" not in given or "dtype" in given, (path, call.lineno)
+
+
+def exported(bits, columns, rows=6):
+    g = torch.Generator().manual_seed(bits)
+    codes = torch.randint(-2 ** (bits - 1), 2 ** (bits - 1), (rows, columns), generator=g).float()
+    return pack.compress((rows, columns), torch.float32, torch.full((rows, columns), 0.01), codes,
+                         bits, columns)
+
+
+@pytest.mark.parametrize("bits,columns", [(7, 64), (7, 130), (7, 4), (6, 4), (5, 3), (4, 2), (7, 1)])
+def test_exports_of_fewer_bits_with_as_many_words_are_refused(bits, columns):
+    wide, narrow = exported(8, columns), exported(bits, columns)
+    assert narrow["weight_packed"].shape == wide["weight_packed"].shape
+    with pytest.raises(ValueError, match="8-bit codes"):
+        Int8Linear.from_export(narrow)
+    with pytest.raises(ValueError, match="no 8-bit codes"):
+        Int8Linear.from_export(wide, bits=bits)
+    for kw in ({}, {"bits": 8}):  # past the checks of the codes
+        with pytest.raises(RuntimeError, match="GPU"):
+            Int8Linear.from_export(wide, **kw)
+    with pytest.raises(RuntimeError, match="GPU"):
+        Int8Linear.from_export(narrow, bits=8)
+
+
+def test_a_layer_knows_what_was_exported_from_it():
+    for grid, match in (((7, True), "codes of 7 bits"), ((8, False), "zero points")):
+        layer = torch.nn.Linear(64, 6)
+        layer._export_qparams, layer._export_grid = exported(8, 64), grid
+        with pytest.raises(ValueError, match=match):
+            Int8Linear.from_export(layer)
