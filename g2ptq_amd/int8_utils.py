@@ -62,7 +62,10 @@ def quantize_tokens(x, sym=True):
               _DTYPE_CODE[x.dtype], rows, columns, _row_stride(x2), int(bool(sym)),
               _lib.ptr(codes), ldc, _lib.ptr(scale), _lib.ptr(zero))
     lead = x.shape[:-1]
-    codes = codes[:, :columns].unflatten(0, lead) if len(lead) != 1 else codes[:, :columns]
+    # (views of the padded rows, also where there is no or more than one leading dimension)
+    codes = codes[:, :columns]
+    if len(lead) != 1:
+        codes = codes.unflatten(0, lead) if lead else codes[0]
     return codes, scale.view(lead), (None if zero is None else zero.view(lead))
 
 

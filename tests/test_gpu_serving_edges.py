@@ -96,3 +96,23 @@ def test_a_layer_knows_what_was_exported_from_it(dev, bits, sym, match):
             assert_bitexact(run.weight[:, :64].float() * run.weight_scale[:, None], lin.weight,
                             "export")
         register_qparam_buffers([lin])
+
+
+@pytest.mark.parametrize("sym", [True, False])
+@pytest.mark.parametrize("shape", [(37,), (1, 37), (2, 3, 37), (0, 37), (0, 4, 37), (4, 0, 37)])
+def test_tokens_of_any_shape(dev, shape, sym):
+    from g2ptq_amd import Int8Linear, int8_matmul, quantize_tokens
+    x = _tokens(max(1, int(torch.tensor(shape[:-1]).prod())), 37, torch.float16, 8)
+    x = x[:0].reshape(shape) if 0 in shape else x.reshape(shape)
+    c, s, z = quantize_tokens(x.to(dev), sym=sym)
+    assert c.shape == shape and s.shape == shape[:-1] and (z is None) == sym
+    if x.numel():
+        rc, rs, rz = serving.quantize(x, 8, sym)
+        assert_bitexact(c.float(), rc, "codes")
+        assert_bitexact(s, rs, "scale")
+        assert sym or torch.equal(z.cpu(), rz)
+    w, wscale, bias = _weights(20, 37, 9)
+    lin = Int8Linear(w.to(dev), wscale.to(dev), bias=bias.to(dev), sym=sym)
+    y = int8_matmul(c, s, lin, zero=z, dtype=torch.float16)
+    assert y.shape == shape[:-1] + (20,)
+    assert_bitexact(y, lin(x.to(dev)), "linear")
