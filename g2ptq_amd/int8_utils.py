@@ -252,7 +252,12 @@ def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
         if t is not None and (t.dtype is not torch.float32 or t.shape != lead):
             raise ValueError(f"int8_matmul: {name} of {t.dtype} and shape {tuple(t.shape)}, "
                              f"expected fp32 {tuple(lead)}")
-    if zero is not None and linear.weight_sum is None:
+        if t is not None and t.get_device() != codes.get_device():
+            raise ValueError(f"int8_matmul: {name} on {t.device}, codes on {codes.device}")
+    weight, wscale, total, bias, here = linear._operands()
+    if here != codes.get_device():
+        raise ValueError(f"int8_matmul: codes on {codes.device}, weights on {weight.device}")
+    if zero is not None and total is None:
         raise ValueError("int8_matmul: tokens with zero points need a linear made with sym=False")
     c2 = codes if codes.dim() == 2 else codes.flatten(0, -2) if codes.dim() > 2 \
         else codes.unsqueeze(0)
@@ -266,7 +271,6 @@ def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
         c2 = padded
     y = torch.empty(rows, out, dtype=dtype, device=codes.device)
     if rows:
-        weight, wscale, total, bias, _ = linear._operands()
         scale, zero = scale.contiguous(), None if zero is None else zero.contiguous()
         ws = _lib.scratch(_lib.query_size("g2ptq_int8_gemm_workspace", rows, out, columns),
                           codes.device)

@@ -116,3 +116,17 @@ def test_tokens_of_any_shape(dev, shape, sym):
     y = int8_matmul(c, s, lin, zero=z, dtype=torch.float16)
     assert y.shape == shape[:-1] + (20,)
     assert_bitexact(y, lin(x.to(dev)), "linear")
+
+
+def test_the_product_takes_tensors_of_one_device(dev):
+    from g2ptq_amd import Int8Linear, int8_matmul, quantize_tokens
+    w, wscale, bias = _weights(20, 37, 9)
+    lin = Int8Linear(w.to(dev), wscale.to(dev), bias=bias.to(dev), sym=False)
+    c, s, z = quantize_tokens(_tokens(3, 37, torch.float16, 8).to(dev), sym=False)
+    for scale, zero, name in ((s.cpu(), z, "scale"), (s, z.cpu(), "zero")):
+        with pytest.raises(ValueError, match=f"{name} on cpu, codes on cuda"):
+            int8_matmul(c, scale, lin, zero=zero)
+    with pytest.raises(ValueError, match="weights on cpu"):
+        int8_matmul(c, s, lin.cpu(), zero=z)
+    with pytest.raises(ValueError, match="weights on cpu"):
+        int8_matmul(c[:0], s[:0], lin, zero=z[:0])
