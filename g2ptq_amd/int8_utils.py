@@ -18,6 +18,7 @@ from . import _lib
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 MAX_COLUMNS = 65536  # longer rows could overflow the 32-bit sums
+_MAX_PITCH = (1 << 20) - 16  # bytes between rows of codes
 
 
 def _rows(x, columns, what):
@@ -262,10 +263,11 @@ def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
     c2 = codes if codes.dim() == 2 else codes.flatten(0, -2) if codes.dim() > 2 \
         else codes.unsqueeze(0)
     rows, need = c2.shape[0], _padded(columns)
-    # rows have to be readable in 16-byte steps to their end
+    # rows have to be readable in 16-byte steps to their end, and at most _MAX_PITCH apart (a
+    # tile's offsets are 32-bit); others are laid out again
     room = c2.untyped_storage().nbytes() - c2.storage_offset()
-    if (c2.stride(1) != 1 or c2.stride(0) % 16 or c2.stride(0) < need or c2.data_ptr() % 16
-            or (rows - 1) * c2.stride(0) + need > room):
+    if (c2.stride(1) != 1 or c2.stride(0) % 16 or not need <= c2.stride(0) <= _MAX_PITCH
+            or c2.data_ptr() % 16 or (rows - 1) * c2.stride(0) + need > room):
         padded = torch.zeros(rows, need, dtype=torch.int8, device=codes.device)
         padded[:, :columns] = c2
         c2 = padded

@@ -130,3 +130,16 @@ def test_the_product_takes_tensors_of_one_device(dev):
         int8_matmul(c, s, lin.cpu(), zero=z)
     with pytest.raises(ValueError, match="weights on cpu"):
         int8_matmul(c[:0], s[:0], lin, zero=z[:0])
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_codes_with_rows_far_apart(dev, T):
+    from g2ptq_amd import Int8Linear, int8_matmul, quantize_tokens
+    w, wscale, _ = _weights(20, 4096, 9)
+    lin = Int8Linear(w.to(dev), wscale.to(dev))
+    c, s, _ = quantize_tokens(_tokens(T, 4096, torch.float16, 8).to(dev))
+    ref = int8_matmul(c, s, lin)
+    for pitch in ((1 << 20) - 16, 1 << 20, (1 << 20) + 4096):
+        wide = torch.zeros(T, pitch, dtype=torch.int8, device=dev)
+        wide[:, :4096] = c
+        assert_bitexact(int8_matmul(wide[:, :4096], s, lin), ref, f"{pitch}")
