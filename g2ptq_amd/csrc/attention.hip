@@ -12,11 +12,11 @@
 //
 // Numbers.  u − z is an integer of at most 255, exact in fp16 (formed as
 // (u − z)·2^-9 from the subnormal fp16 whose bits are u).  A query row is scaled
-// by a power of two so that its largest element is in [1, 2) and rounded to fp16
-// (exact for fp16 and, above 2^-14 of the largest element, for bf16).  Both
-// products run on the fp16 matrix cores with fp32 accumulators; scales, softmax
-// statistics and sums are fp32:
-//   s_j = (Σ q·(u − z)2^-9)·(2^9·scale·log2 e·sk_j),  p_j = exp2(C·(s_j − max) + e),
+// by a power of two so that its largest element is in [2^15, 2^16), the top of fp16's
+// range, and rounded to fp16: exact for fp16, and for bf16 down to 2^-32 of the largest
+// element (smaller ones move by at most 2^-40 of it).  Both products run on the fp16
+// matrix cores with fp32 accumulators; scales, softmax statistics and sums are fp32:
+//   s_j = (Σ q·(u − z)2^-9)·(2^-6·scale·log2 e·sk_j),  p_j = exp2(C·(s_j − max) + e),
 //   l = Σ p_j,  o = 2^9·Σ fp16(p_j·sv_j)·(u − z)2^-9 / l,
 // C the row's power of two (so C·max is exact), e = 15 − log2(ref), ref
 // a power of two above the scales sv of the values that the row has seen: the
@@ -53,7 +53,7 @@ struct AttnArgs {
   int dtype;
   bool vec;        // 16-byte loads of queries
   float scale;
-  float kscale;    // |scale|·log2 e·2^9: multiplies the keys' scales
+  float kscale;    // |scale|·log2 e·2^(9 − 15): multiplies the keys' scales
   int tiles;       // row tiles a launch provides for a sequence and head (attend_tiles_kernel)
   int split, few_split;  // most shares of a sequence's keys (tiles; few rows)
   int share, few_share;  // keys of a share, unless a sequence needs larger ones
@@ -153,8 +153,9 @@ __device__ __forceinline__ float above(float x) {
 }
 __device__ __forceinline__ int exponent(float p) { return (int)(__float_as_uint(p) >> 23) - 127; }
 
-// Power of two that brings a query row into [1, 2) and its inverse, from the row's
-// largest |q| (16 bits of the query's type in the high half of m).
+// Power of two that brings a query row's largest |q| (16 bits of the query's type in the
+// high half of m) into [2^15, 2^16), and 2^15 times its inverse.  Rows below 2^-112 stay
+// below that (the power has to be a number).
 struct RowScale {
   float down, up;
 };
@@ -162,8 +163,8 @@ __device__ __forceinline__ RowScale row_scale(int dtype, uint32_t m) {
   const float x = dtype == 0 ? __uint_as_float(m)
                              : (float)__builtin_bit_cast(_Float16, (uint16_t)(m >> 16));
   uint32_t e = __float_as_uint(x) >> 23;
-  e = e >= 255 ? 127 : min(max(e, 1u), 253u);  // a NaN or infinite row stays one as it is
-  return {__uint_as_float((254 - e) << 23), __uint_as_float(e << 23)};
+  e = e >= 255 ? 127 : max(e, 15u);  // a NaN or infinite row stays one as it is
+  return {__uint_as_float((269 - e) << 23), __uint_as_float(e << 23)};
 }
 
 // Output row of sequence row r, or -1 past the sequence's rows.
@@ -1306,7 +1307,7 @@ extern "C" int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, 
   a.T = (int)T, a.Hq = (int)Hq, a.B = (int)B, a.G = (int)(Hq / a.c.H), a.width = (int)width;
   a.dtype = dtype;
   a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_token % 8 == 0 && q_head % 8 == 0;
-  a.scale = scale, a.kscale = fabsf(scale) * 1.44269504088896340736f * 512.f;
+  a.scale = scale, a.kscale = fabsf(scale) * 1.44269504088896340736f * 0x1p-6f;
   a.tiles = (int)p.ntiles, a.split = (int)p.split, a.few_split = (int)p.few_split;
   a.share = (int)p.share, a.few_share = (int)p.few_share;
   a.by_rows = p.few, a.by_tiles = p.tiles;

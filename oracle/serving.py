@@ -93,9 +93,10 @@ def attention_bound(dtype, out, size, logit, span, count, dim):
     - weights p·scale are rounded to 11 significant bits before the products
       with the values: 2^-11;
     - a logit's fp32 sum of dim products and its scaling: (dim + 4)·2^-24 of
-      Σ|q·k|, and the query's conversion to a scaled fp16 row moves it by at most
-      2^-14 of the largest element's 2^-11: below 2^-24·dim of Σ|q·k| again.
-      A logit's error changes p, and through the sum every other p: twice;
+      Σ|q·k|; the query's conversion to a scaled fp16 row is exact, but for elements
+      below 2^-32 of the largest of a bf16 row, which move by at most 2^-40 of it:
+      another 2^-24·dim of Σ|q·k| is there for them.  A logit's error changes p, and
+      through the sum every other p: twice;
     - exp2, its argument's rounding (2^-24 of the logit, counted above) and the
       joining of partial results: 16 units of 2^-24;
     - fp32 sums over ``count`` keys, numerator and denominator: 2·count·2^-24;

@@ -5,6 +5,7 @@ import torch
 from oracle import serving
 from tests._util import assert_bitexact, gen
 from tests.test_gpu_int8_linear import _check, _tokens, _weights
+from tests.test_gpu_paged_attention import Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +144,18 @@ def test_codes_with_rows_far_apart(dev, T):
         wide = torch.zeros(T, pitch, dtype=torch.int8, device=dev)
         wide[:, :4096] = c
         assert_bitexact(int8_matmul(wide[:, :4096], s, lin), ref, f"{pitch}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bits,sym", [(8, True), (4, False)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [60]), ([3, 1], [90, 300]), ([70], [100])], ids=str)
+def test_small_queries_beside_a_large_one(dev, q_lens, kv_lens, bits, sym, dtype):
+    """One channel of the queries 2^24 above the others, where the keys are zero: the others
+    alone make the logits, and the bound has the sum of |q k|, which has no part of it."""
+    def edit(q, k, v, cu):
+        q *= 2.0 ** -9
+        q[:, :, 5] = 3e4
+        k *= 30
+        k[:, :, 5] = 0
+    b = Batch(dev, q_lens, kv_lens, 4, 2, 64, 16, bits, sym, dtype, edit=edit)
+    b.check(b.run())
