@@ -163,7 +163,10 @@ __device__ __forceinline__ RowScale row_scale(int dtype, uint32_t m) {
   const float x = dtype == 0 ? __uint_as_float(m)
                              : (float)__builtin_bit_cast(_Float16, (uint16_t)(m >> 16));
   uint32_t e = __float_as_uint(x) >> 23;
-  e = e >= 255 ? 127 : max(e, 15u);  // a NaN or infinite row stays one as it is
+  // A NaN or an infinity makes every logit of the row NaN or infinite, and their softmax NaN
+  // (also where all are -inf, which would look like a row without keys): NaN as the unit.
+  if (e >= 255) return {1.f, __builtin_nanf("")};
+  e = max(e, 15u);
   return {__uint_as_float((269 - e) << 23), __uint_as_float(e << 23)};
 }
 

@@ -159,3 +159,28 @@ def test_small_queries_beside_a_large_one(dev, q_lens, kv_lens, bits, sym, dtype
         k[:, :, 5] = 0
     b = Batch(dev, q_lens, kv_lens, 4, 2, 64, 16, bits, sym, dtype, edit=edit)
     b.check(b.run())
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [1]), ([1], [700]), ([5, 2], [3, 400]),
+                                            ([70], [70]), ([30, 200], [20, 900])], ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_queries_without_a_finite_logit_are_nan(dev, bad, q_lens, kv_lens):
+    """An infinite element makes every logit of its row infinite or NaN, and a softmax of
+    those is NaN, also where all are -inf; rows without keys are zero all the same."""
+    def edit(q, k, v, cu):
+        q[::2, 1, 7] = bad
+        k[:, :, 7] = k[:, :, 7].abs() + 0.5
+        if bad < 0:
+            q[::2, 1, 8], k[:, :, 8] = -bad, -k[:, :, 8].abs() - 0.5
+    for kw in ({}, {"max_q": max(q_lens), "max_kv": max(kv_lens)}):
+        b = Batch(dev, q_lens, kv_lens, 4, 2, 64, 16, 8, True, torch.bfloat16, edit=edit)
+        got = b.run(**kw)
+        rows = torch.zeros(got.shape[:2], dtype=torch.bool)
+        rows[::2, 1] = True
+        count = torch.cat([torch.arange(n - m + 1, n + 1) for m, n in zip(q_lens, kv_lens)])
+        assert bool(got.cpu()[rows & (count > 0)[:, None]].isnan().all())
+        assert bool((got.cpu()[count <= 0] == 0).all())
+        good = Batch(dev, q_lens, kv_lens, 4, 2, 64, 16, 8, True, torch.bfloat16,
+                     edit=lambda q, k, v, cu: (edit(q, k, v, cu), q.nan_to_num_(0, 0, 0)))
+        keep = ~rows & (count > 0)[:, None]
+        assert_bitexact(got.cpu()[keep], good.run(**kw).cpu()[keep], "other rows")
