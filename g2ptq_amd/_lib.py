@@ -7,6 +7,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libg2ptq_hip.so")
 
@@ -268,7 +269,7 @@ def scratch(nbytes, device):
 
 def require_current(t, what):
     """Kernels run on the current device and have no gradients: refuse a tensor of
-    another device, and one that a gradient is recorded for."""
+    another device, and one that a gradient is recorded for or that carries a tangent."""
     if not t.is_cuda:
         raise RuntimeError(f"{what}: a GPU tensor is needed, got one on {t.device}")
     if t.get_device() != torch._C._cuda_getDevice():
@@ -276,6 +277,9 @@ def require_current(t, what):
                          f"{torch._C._cuda_getDevice()} is current")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: inference only (no gradient); call under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{what}: inference only (no forward-mode derivative); pass the "
+                           "dual tensor's primal")
 
 
 def current_stream():

@@ -212,6 +212,7 @@ class Int8Linear(torch.nn.Module):
         # what is usual passes in one go (a call is a few microseconds); the rest is told apart
         if (x.dim() == 2 and x.shape[1] == columns and x.is_contiguous()
                 and x.dtype in _DTYPE_CODE and not x.requires_grad
+                and _lib.forward_ad._current_level < 0
                 and x.get_device() == here == torch._C._cuda_getDevice()):
             x2, rows, stride = x, x.shape[0], columns
         else:

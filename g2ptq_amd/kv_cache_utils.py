@@ -104,7 +104,8 @@ class PagedKVCache:
                 and k.stride(2) == v.stride(2) == 1 and code is not None and v.dtype is k.dtype
                 and k.get_device() == v.get_device() == slots.get_device() == here
                 and torch._C._cuda_getDevice() == here
-                and not k.requires_grad and not v.requires_grad):
+                and not k.requires_grad and not v.requires_grad
+                and _lib.forward_ad._current_level < 0):
             return self._write_checked(k, v, slots)
         (n, _, _), (kt, kh, _), (vt, vh, _) = k.shape, k.stride(), v.stride()
         _lib.call_fast("kv_write", _lib.current_stream(), self._address, k.data_ptr(), kt, kh,

@@ -184,3 +184,32 @@ def test_queries_without_a_finite_logit_are_nan(dev, bad, q_lens, kv_lens):
                      edit=lambda q, k, v, cu: (edit(q, k, v, cu), q.nan_to_num_(0, 0, 0)))
         keep = ~rows & (count > 0)[:, None]
         assert_bitexact(got.cpu()[keep], good.run(**kw).cpu()[keep], "other rows")
+
+
+def test_tangents_are_refused_like_gradients(dev):
+    from torch.autograd import forward_ad
+    from g2ptq_amd import Int8Linear, PagedKVCache, paged_attention, quantize_tokens
+    w, wscale, _ = _weights(20, 64, 9)
+    lin = Int8Linear(w.to(dev), wscale.to(dev))
+    cache = PagedKVCache(2, 16, 1, 64, device=dev)
+    x = _tokens(3, 64, torch.float16, 8).to(dev)
+    slots = torch.arange(3, device=dev)
+    table, cu, lens = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([[0]], [0, 3], [3]))
+
+    def calls(t):
+        k = t.view(3, 1, 64)
+        plain = x.view(3, 1, 64)
+        return (lambda: lin(t), lambda: quantize_tokens(t), lambda: cache.write(k, plain, slots),
+                lambda: cache.write(plain, k, slots),
+                lambda: paged_attention(k, cache, table, cu, lens))
+
+    for call in calls(x):
+        call()
+    ref = lin(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls(dual):
+            with pytest.raises(RuntimeError, match="inference only"):
+                call()
+        assert_bitexact(lin(x), ref, "a tensor without a tangent")
+        assert_bitexact(lin(forward_ad.unpack_dual(dual).primal), ref, "primal")
