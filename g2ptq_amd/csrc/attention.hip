@@ -60,6 +60,7 @@ struct AttnArgs {
   bool by_rows, by_tiles;  // kernels that run; with both, sequences of at most kFewRows rows
                            // go to attend_rows_kernel
   float *part, *few_part;  // partial results of the shares, or null
+  int64_t row0;            // first row of a launch of attend_join_kernel
 };
 
 // A sequence's rows of the query and its keys.
@@ -1099,9 +1100,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   __shared__ float wL[256 / LW][64];  // (at most 64 shares)
   const int64_t rows_all = (int64_t)a.T * a.Hq;
   const int sub = threadIdx.x % LW, group = threadIdx.x / LW;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LW) + group;
-  const int64_t row0 = (int64_t)blockIdx.x * (256 / LW) +
-                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (64 / LW);
+  const int64_t first = a.row0 + (int64_t)blockIdx.x * (256 / LW);
+  const int64_t row = first + group;
+  const int64_t row0 = first + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (64 / LW);
   if (row0 >= rows_all) return;
   const int64_t near = KvCache::sequence_of_wave(a.cu, a.B, row0 / a.Hq);
   // from here on groups go their own ways
@@ -1218,7 +1219,9 @@ struct Plan {
     // tokens over 16384 keys 714 against 702 µs, six uneven chunks 44 against 35 µs; 64 rows:
     // 1211 against 671 µs, and where that is all there are, 8 tokens of four heads over 4096
     // keys, 23.4 against 20.9.)
-    ntiles = std::max<int64_t>(1, cdiv(rows, kTileRows));
+    // As many tiles as the largest sequence may have, unless the launch gets too large (many
+    // sequences whose sizes are not given): workgroups then take further tiles in turn.
+    ntiles = std::max<int64_t>(1, std::min(cdiv(rows, kTileRows), kMaxGroups / pairs));
     // Shares for two workgroups per CU, three in a batch (its sequences differ in length).
     // MI355X, heads 32 on 8 of 128, two / three / four: 512 tokens over 2048 keys 53.7 / 62.9
     // / 66.6 µs; four chunks of 300 over up to 4096 keys 158 / 116 / 123 µs; six of 100, 100 /
@@ -1248,9 +1251,14 @@ int launch(hipStream_t st, const AttnArgs& a, const Plan& p) {
   }
   if (a.part || a.few_part) {
     constexpr int LW = DP / 4;
-    hipLaunchKernelGGL((attend_join_kernel<LW>),
-                       dim3((unsigned)cdiv((int64_t)a.T * a.Hq, 256 / LW)), dim3(256), 0, st, a);
-    G2PTQ_LAUNCHED();
+    const int64_t groups = cdiv((int64_t)a.T * a.Hq, 256 / LW);
+    for (int64_t g = 0; g < groups; g += kMaxGroups) {
+      AttnArgs part = a;
+      part.row0 = g * (256 / LW);
+      hipLaunchKernelGGL((attend_join_kernel<LW>), dim3((unsigned)std::min(groups - g, kMaxGroups)),
+                         dim3(256), 0, st, part);
+      G2PTQ_LAUNCHED();
+    }
   }
   return G2PTQ_OK;
 }
@@ -1297,7 +1305,9 @@ extern "C" int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, 
   G2PTQ_CHECK((reinterpret_cast<uintptr_t>(out) & 15) == 0,
               "paged_attention: output not 16-byte aligned");
   const Plan p(T, Hq, a.c.H, a.c.D, B, max_q, max_kv);
-  G2PTQ_CHECK(B * a.c.H * p.split * p.ntiles < (1ll << 31) - 1, "paged_attention: batch too large");
+  G2PTQ_CHECK(!p.tiles || B * a.c.H * p.split * p.ntiles <= kMaxGroups,
+              "paged_attention: %lld sequences of %lld heads (at most %lld in all)", (long long)B,
+              (long long)a.c.H, (long long)kMaxGroups);
   const size_t need = (size_t)(p.part + p.few_part);
   if (need && (!ws || ws_bytes < need)) {
     set_error("paged_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);

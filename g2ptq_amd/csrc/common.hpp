@@ -135,6 +135,10 @@ __device__ __forceinline__ int64_t row_step(int shift) {
   return (int64_t)gridDim.y * (256 >> shift);
 }
 
+// Workgroups of one launch along x, of up to 256 threads: a launch's threads along a dimension
+// are counted in 32 bits, and one with more runs only what is left modulo 2^32, without an error.
+constexpr int64_t kMaxGroups = (int64_t)1 << 23;
+
 // p[0..n) = v with a kernel (graph-capture safe, unlike hipMemsetAsync).
 int fill_f32(hipStream_t stream, float* p, int64_t n, float v);
 

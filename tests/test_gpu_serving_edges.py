@@ -213,3 +213,53 @@ def test_tangents_are_refused_like_gradients(dev):
                 call()
         assert_bitexact(lin(x), ref, "a tensor without a tangent")
         assert_bitexact(lin(forward_ad.unpack_dual(dual).primal), ref, "primal")
+
+
+def test_many_sequences_without_stated_sizes(dev):
+    """Without max_q every sequence is taken to have all tokens: 2^24 row tiles here, more
+    threads than a launch can have."""
+    from g2ptq_amd import PagedKVCache, paged_attention
+    B, n, T = 8192, 32, 1 << 18
+    k = _tokens(2 * n, 16, torch.float16, 1).view(2 * n, 1, 16).to(dev)
+    cache = PagedKVCache(4, 16, 1, 16, device=dev)
+    cache.write(k, k, torch.arange(2 * n, device=dev))
+    q = _tokens(T, 16, torch.float16, 2).view(T, 1, 16).to(dev)
+    # the sequences' keys: two texts, shared by all
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=dev).repeat(B // 2, 1)
+    cu = torch.arange(0, T + 1, n, dtype=torch.int32, device=dev)
+    lens = torch.full((B,), n, dtype=torch.int32, device=dev)
+    out = paged_attention(q, cache, table, cu, lens)
+    ref = paged_attention(q, cache, table, cu, lens, max_q=n, max_kv=n)
+    assert_bitexact(out, ref, "stated sizes")
+    cache.check()
+    for b in (0, 1, B - 1):
+        one = paged_attention(q[b * n:(b + 1) * n], cache, table[b:b + 1], cu[:2], lens[:1])
+        assert_bitexact(out[b * n:(b + 1) * n], one, f"sequence {b}")
+
+
+@pytest.mark.parametrize("bits,heads,kv_heads,dim", [(8, 4, 2, 64), (4, 3, 1, 128), (8, 2, 1, 256)])
+def test_more_row_tiles_than_stated(dev, bits, heads, kv_heads, dim):
+    """Workgroups take further tiles of rows in turn."""
+    b = Batch(dev, [300, 40, 700], [500, 900, 700], heads, kv_heads, dim, 16, bits, False,
+              torch.bfloat16)
+    b.check(b.run(max_q=20), "one tile for six")
+    b.check(b.run(max_q=260, max_kv=300), "some")
+
+
+def test_joining_very_many_rows(dev):
+    """Two sequences, the second's few rows in shares whose joined rows lie past 2^28."""
+    from g2ptq_amd import PagedKVCache, paged_attention
+    T, n, D = (1 << 28) + 4, 3000, 16
+    k = _tokens(n, D, torch.float16, 1).view(n, 1, D).to(dev)
+    cache = PagedKVCache(188, 16, 1, D, device=dev)
+    cache.write(k, k, torch.arange(n, device=dev))
+    q = _tokens(1, D, torch.float16, 2).view(1, 1, D).to(dev)
+    table = torch.arange(188, dtype=torch.int32, device=dev).repeat(2, 1)
+    i32 = dict(dtype=torch.int32, device=dev)
+    out = paged_attention(q.expand(T, 1, D), cache, table, torch.tensor([0, T - 4, T], **i32),
+                          torch.tensor([0, n], **i32))
+    one = paged_attention(q.expand(4, 1, D), cache, table[:1], torch.tensor([0, 4], **i32),
+                          torch.tensor([n], **i32))
+    assert float(one.abs().min()) > 0
+    torch.testing.assert_close(out[-4:], one, rtol=2 ** -9, atol=2 ** -9)
+    assert float(out[:1 << 20].abs().max()) == 0 and float(out[-(1 << 20):-4].abs().max()) == 0
