@@ -21,7 +21,7 @@ struct WriteArgs {
   const void* x[2];        // keys, values: T × H × D, channels contiguous
   int64_t st[2], sh[2];    // strides of token and head (elements)
   const int64_t* slots;    // page·(page size) + offset; negative: not written
-  uint32_t items;          // T·H
+  uint32_t items, first;   // T·H, and the launch's first of them
   KvCache c;
   bool vec[2];
 };
@@ -37,7 +37,7 @@ template <int DT, bool SYM, int BITS, int L>
 __global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
   constexpr int OFF = 1 << (BITS - 1);
   const int w = blockIdx.y;
-  const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L;
+  const uint32_t item = a.first + blockIdx.x * (256 / L) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 16;
   if (item >= a.items) return;
   const uint32_t t = item / (uint32_t)a.c.H, h = item - t * (uint32_t)a.c.H;
@@ -83,7 +83,7 @@ struct ReadArgs {
   const int32_t* table;
   int64_t ldt, B, width;
   const int32_t* cu;  // B + 1 offsets of the sequences in the output
-  int64_t total;
+  int64_t total, first;  // rows, and the launch's first of them
   void* out[2];       // total × H × D
   int tokens;         // of a workgroup, at most kReadTokens
 };
@@ -99,7 +99,7 @@ template <int DT, int BITS>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
   __shared__ int64_t slotL[kReadTokens];
   const int w = blockIdx.y;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int64_t t0 = a.first + (int64_t)blockIdx.x * a.tokens;
   const int n = (int)min<int64_t>(a.tokens, a.total - t0);
   if (threadIdx.x < 64) {  // (one wave: n <= 64)
     const int64_t b = KvCache::sequence_of_wave(a.cu, a.B, t0);
@@ -215,7 +215,6 @@ extern "C" int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const v
   const bool sym = cache->sym != 0;
   return by_lanes(a.c.D, [&](auto lanes) -> int {
     constexpr int L = decltype(lanes)::value;
-    const dim3 grid((unsigned)cdiv(T * a.c.H, 256 / L), 2);
 #define G2_WR(DT, SYM)                                                                      \
   do {                                                                                      \
     if (a.c.bits == 8)                                                                      \
@@ -223,11 +222,15 @@ extern "C" int g2ptq_kv_write(void* stream, const g2ptq_kv_cache* cache, const v
     else                                                                                    \
       hipLaunchKernelGGL((kv_write_kernel<DT, SYM, 4, L>), grid, dim3(256), 0, st, a);      \
   } while (0)
-    if (dtype == 0) { if (sym) G2_WR(0, true); else G2_WR(0, false); }
-    else if (dtype == 1) { if (sym) G2_WR(1, true); else G2_WR(1, false); }
-    else { if (sym) G2_WR(2, true); else G2_WR(2, false); }
+    for (int64_t first = 0; first < a.items; first += kMaxGroups * (256 / L)) {
+      a.first = (uint32_t)first;
+      const dim3 grid((unsigned)std::min(cdiv(a.items - first, 256 / L), kMaxGroups), 2);
+      if (dtype == 0) { if (sym) G2_WR(0, true); else G2_WR(0, false); }
+      else if (dtype == 1) { if (sym) G2_WR(1, true); else G2_WR(1, false); }
+      else { if (sym) G2_WR(2, true); else G2_WR(2, false); }
+      G2PTQ_LAUNCHED();
+    }
 #undef G2_WR
-    G2PTQ_LAUNCHED();
     return G2PTQ_OK;
   });
 }
@@ -254,7 +257,8 @@ extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const in
   while (tokens > 1 && cdiv(total, tokens) < 256) tokens /= 2;
   a.tokens = (int)tokens;
   hipStream_t st = as_stream(stream);
-  const dim3 grid((unsigned)cdiv(total, tokens), 2);
+  for (a.first = 0; a.first < total; a.first += kMaxGroups * tokens) {
+    const dim3 grid((unsigned)std::min(cdiv(total - a.first, tokens), kMaxGroups), 2);
 #define G2_RD(DT)                                                                          \
   do {                                                                                     \
     if (a.c.bits == 8)                                                                     \
@@ -262,10 +266,11 @@ extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const in
     else                                                                                   \
       hipLaunchKernelGGL((kv_read_kernel<DT, 4>), grid, dim3(256), 0, st, a);              \
   } while (0)
-  if (dtype == 0) G2_RD(0);
-  else if (dtype == 1) G2_RD(1);
-  else G2_RD(2);
+    if (dtype == 0) G2_RD(0);
+    else if (dtype == 1) G2_RD(1);
+    else G2_RD(2);
+    G2PTQ_LAUNCHED();
+  }
 #undef G2_RD
-  G2PTQ_LAUNCHED();
   return G2PTQ_OK;
 }

@@ -263,3 +263,41 @@ def test_joining_very_many_rows(dev):
     assert float(one.abs().min()) > 0
     torch.testing.assert_close(out[-4:], one, rtol=2 ** -9, atol=2 ** -9)
     assert float(out[:1 << 20].abs().max()) == 0 and float(out[-(1 << 20):-4].abs().max()) == 0
+
+
+def test_writing_very_many_tokens(dev):
+    """2^30 heads of tokens, four lanes each: more threads than a launch can have.  The last
+    token is written like the first."""
+    from g2ptq_amd import PagedKVCache
+    H, D, T = 65535, 64, (1 << 30) // 65535 + 2
+    cache = PagedKVCache(2, 1, H, D, device=dev)
+    x = torch.linspace(-3, 5, D, device=dev)
+    slots = torch.full((T,), -1, dtype=torch.int64, device=dev)
+    slots[0], slots[-1] = 0, 1
+    cache.write(x.expand(T, H, D), (x * 2).expand(T, H, D), slots)
+    rc, rs, _ = serving.quantize(x.cpu(), 8, True)
+    for codes, scale, f in ((cache.k_codes, cache.k_scale, 1), (cache.v_codes, cache.v_scale, 2)):
+        assert bool((scale == float(rs) * f).all())
+        assert bool((codes.float() - 128 == rc.to(dev)).all())
+
+
+def test_reading_very_many_tokens(dev):
+    """2^30 tokens and some, 64 to a workgroup: the last sequence lies past the first launch."""
+    from g2ptq_amd import PagedKVCache
+    T = (1 << 30) + 40
+    cache = PagedKVCache(2, 64, 1, 16, bits=4, device=dev)
+    x = _tokens(64, 16, torch.float16, 3).view(64, 1, 16).to(dev)
+    cache.write(x, x, torch.arange(64, device=dev))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 50], dtype=torch.int32, device=dev)
+    first = cache.read(table, cu, 50, dtype=torch.float16)
+    for b in range(2):  # the first rows, then the last
+        cu = torch.tensor([0, 50] if b == 0 else [T - 50, T], dtype=torch.int32, device=dev)
+        k, v = cache.read(table, cu, T, dtype=torch.float16)
+        for got, ref in zip((k, v), first):
+            assert_bitexact(got[:50] if b == 0 else got[-50:], ref, "rows")
+            rest = got[50:] if b == 0 else got[:-50]
+            assert all(not bool(rest[i:i + (1 << 24)].any())
+                       for i in range(0, len(rest), 1 << 27)) and not bool(rest[-1000:].any())
+        del k, v, got, rest
+    torch.cuda.empty_cache()
