@@ -548,7 +548,6 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
     else if (r == 2) launch_few<2>(st, a);
     else launch_few<1>(st, a);
   } else {
-    G2PTQ_CHECK(cdiv(a.T, 64) * cdiv(a.N, 64) < (1ll << 31), "int8_gemm: output too large");
     // The largest tile that still fills the chip.  MI355X, product alone: 256 against 128 at
     // 256 tiles of 256 (4096³) 64 against 86 µs; 128 against 64 at 256 tiles of 128
     // (1024 × 4096, K 4096) 28 against 34 µs, at 128 of them (512 × 4096, K 14336) 71
@@ -593,9 +592,10 @@ int check_tokens(const char* who, const void* x, int dtype, int64_t T, int64_t K
 
 int check_product(const char* who, const GemmI8& a) {
   G2PTQ_CHECK(a.dtype >= 0 && a.dtype <= 2, "%s: dtype code %d", who, a.dtype);
+  // (a launch has 512 threads for 32 channels of few tokens, or for 256 × 256 outputs)
   G2PTQ_CHECK(a.T >= 0 && a.T < (1ll << 22) && a.K >= 1 && a.K <= kMaxK && a.N >= 0 &&
-                  a.N < (1ll << 31),
-              "%s: %lld tokens × %lld columns × %lld channels", who, (long long)a.T,
+                  cdiv(a.N, 32) < kMaxGroups && cdiv(a.T, 256) * cdiv(a.N, 256) < kMaxGroups,
+              "%s: %lld tokens × %lld columns × %lld channels are too many", who, (long long)a.T,
               (long long)a.K, (long long)a.N);
   if (a.T == 0 || a.N == 0) return G2PTQ_OK;
   G2PTQ_CHECK(a.W && a.sw && a.out && a.ldo >= a.N, "%s: null pointer or output stride", who);

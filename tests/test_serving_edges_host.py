@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import g2ptq_amd
-from g2ptq_amd import Int8Linear
+from g2ptq_amd import Int8Linear, _lib
 from oracle import pack
 
 
@@ -120,3 +120,15 @@ def test_a_layer_knows_what_was_exported_from_it():
         layer._export_qparams, layer._export_grid = exported(8, 64), grid
         with pytest.raises(ValueError, match=match):
             Int8Linear.from_export(layer)
+
+
+def test_products_that_no_launch_can_hold_are_refused():
+    """More than 2^32 threads: the runtime would run what is left modulo 2^32."""
+    lib, fake = _lib.load(), 4096
+    for T, N in ((1, 1 << 28), (20, 1 << 29), (1 << 20, 1 << 20), ((1 << 22) - 1, 1 << 18)):
+        assert lib.g2ptq_int8_linear(None, fake, 0, T, 64, 64, 1, fake, 256, fake, None, None, N,
+                                     fake, N, None, 0) == -1
+        assert b"too many" in lib.g2ptq_last_error()
+        assert lib.g2ptq_int8_gemm(None, fake, 64, fake, None, fake, 256, fake, None, None, T, N,
+                                   64, fake, 0, N, None, 0) == -1
+        assert b"too many" in lib.g2ptq_last_error()
