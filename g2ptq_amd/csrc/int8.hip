@@ -9,6 +9,7 @@
 // the order of summation.  A sum is rounded to fp32 once (2^-24 of it), then by the
 // scales' products and to the output's type.
 #include <algorithm>
+#include <type_traits>
 
 #include "grid8.hpp"
 
@@ -136,7 +137,9 @@ template <int DT, int MT, int NTL>
 __device__ __forceinline__ void finish_tile(const GemmI8& a, const i32x16 (&acc)[MT][NTL],
                                             int64_t t0, int64_t n0, const float* sxL,
                                             const int* zxL, int8_t* mine, int lane) {
-  constexpr int E = DT == 2 ? 4 : 2, BYTES = NTL * 32 * E, PITCH = BYTES + 16;
+  // (also read back as what was written: another scalar type could be read before the writes)
+  using Out = std::conditional_t<DT == 0, __bf16, std::conditional_t<DT == 1, _Float16, float>>;
+  constexpr int E = sizeof(Out), BYTES = NTL * 32 * E, PITCH = BYTES + 16;
   constexpr int LPR = BYTES / 16, RPP = 64 / LPR;  // lanes of a row, rows of a pass
   const int lr = lane & 31, lh = lane >> 5;
   float sw[NTL], bias[NTL];
@@ -160,10 +163,7 @@ __device__ __forceinline__ void finish_tile(const GemmI8& a, const i32x16 (&acc)
 #pragma unroll
       for (int n = 0; n < NTL; ++n) {
         const float y = scaled(a, sx, zx, acc[m][n][v], sw[n], wsum[n], bias[n]);
-        int8_t* to = mine + r * PITCH + (n * 32 + lr) * E;
-        if constexpr (DT == 0) *reinterpret_cast<__bf16*>(to) = (__bf16)y;
-        else if constexpr (DT == 1) *reinterpret_cast<_Float16*>(to) = (_Float16)y;
-        else *reinterpret_cast<float*>(to) = y;
+        *reinterpret_cast<Out*>(mine + r * PITCH + (n * 32 + lr) * E) = (Out)y;
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -181,14 +181,9 @@ __device__ __forceinline__ void finish_tile(const GemmI8& a, const i32x16 (&acc)
       const int cols = (int)min<int64_t>(NTL * 32, a.N - n0);
       for (int i = lane; i < 32 * NTL * 32; i += 64) {
         const int r = i / (NTL * 32), c = i % (NTL * 32);
-        if (r < rows && c < cols) {
-          if constexpr (E == 2)
-            *reinterpret_cast<uint16_t*>(out + (r * a.ldo + c) * E) =
-                *reinterpret_cast<const uint16_t*>(mine + r * PITCH + c * E);
-          else
-            *reinterpret_cast<uint32_t*>(out + (r * a.ldo + c) * E) =
-                *reinterpret_cast<const uint32_t*>(mine + r * PITCH + c * E);
-        }
+        if (r < rows && c < cols)
+          *reinterpret_cast<Out*>(out + (r * a.ldo + c) * E) =
+              *reinterpret_cast<const Out*>(mine + r * PITCH + c * E);
       }
     }
     __builtin_amdgcn_wave_barrier();
