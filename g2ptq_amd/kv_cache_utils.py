@@ -68,6 +68,9 @@ class PagedKVCache:
                              "256 is needed)")
         if num_pages < 0 or not 1 <= kv_heads <= 65535:
             raise ValueError(f"PagedKVCache: {num_pages} pages of {kv_heads} heads")
+        if num_pages * kv_heads * page_size >= 1 << 31:
+            raise ValueError(f"PagedKVCache: {num_pages} pages of {kv_heads} heads of {page_size} "
+                             "slots (fewer than 2^31 in all)")
         self.num_pages, self.page_size = num_pages, page_size
         self.kv_heads, self.head_dim, self.bits, self.sym = kv_heads, head_dim, bits, bool(sym)
         dev = torch.device(device)
@@ -156,8 +159,8 @@ class PagedKVCache:
         return k, v
 
     def check(self):
-        """Raise if a slot or page outside the cache was met since the last check
-        (waits for the GPU)."""
+        """Raise if a slot or page outside the cache was met since the last check, by the
+        work that the current stream has or waits for (waits for that stream)."""
         v = int(self.flags.item())
         self.flags.zero_()
         if v & _lib.FLAG_BAD_INDEX:

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import g2ptq_amd
-from g2ptq_amd import Int8Linear, _lib
+from g2ptq_amd import Int8Linear, PagedKVCache, _lib
 from oracle import pack
 
 
@@ -132,3 +132,11 @@ def test_products_that_no_launch_can_hold_are_refused():
         assert lib.g2ptq_int8_gemm(None, fake, 64, fake, None, fake, 256, fake, None, None, T, N,
                                    64, fake, 0, N, None, 0) == -1
         assert b"too many" in lib.g2ptq_last_error()
+
+
+def test_a_cache_that_no_call_takes_is_not_made():
+    for pages, page, heads in ((1 << 20, 64, 32), (1 << 31, 1, 1), (1 << 12, 4096, 128)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            PagedKVCache(pages, page, heads, 64, device="cpu")
+    with pytest.raises(RuntimeError, match="GPU"):
+        PagedKVCache((1 << 19) - 1, 64, 64, 64, device="cpu")
