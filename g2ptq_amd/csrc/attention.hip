@@ -843,35 +843,35 @@ attend_tiles_kernel(AttnArgs a) {
     // Products of a step's keys and the query; element v of block kb: key
     // 32kb + 8(v/4) + 4lh + v%4.  Fragments are read one group of products ahead.
     auto logits = [&](int step) __attribute__((always_inline)) {
-      #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-      #pragma unroll
-                  for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
-                const char* kp = kL + (step & 1) * KB + lr * KPITCH + lh * 16;
-                f16x8 kf[2][2][2];
-      #pragma unroll
-                for (int s = 0; s < 2; ++s)
-      #pragma unroll
-                  for (int kb = 0; kb < 2; ++kb)
-                    kf[0][s][kb] = *reinterpret_cast<const f16x8*>(kp + kb * (32 * KPITCH) + s * 32);
-      #pragma unroll
-                for (int g = 0; g < DP / 32; ++g) {
-                  if (g + 1 < DP / 32) {
-      #pragma unroll
-                    for (int s = 0; s < 2; ++s)
-      #pragma unroll
-                      for (int kb = 0; kb < 2; ++kb)
-                        kf[(g + 1) & 1][s][kb] = *reinterpret_cast<const f16x8*>(
-                            kp + kb * (32 * KPITCH) + (2 * g + 2 + s) * 32);
-                  }
-                  __builtin_amdgcn_sched_barrier(0);
-      #pragma unroll
-                  for (int s = 0; s < 2; ++s)
-      #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-                      x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g & 1][s][kb], qf[2 * g + s],
-                                                                     x[kb], 0, 0, 0);
-                }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[kb][v] = 0.f;
+      const char* kp = kL + (step & 1) * KB + lr * KPITCH + lh * 16;
+      f16x8 kf[2][2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          kf[0][s][kb] = *reinterpret_cast<const f16x8*>(kp + kb * (32 * KPITCH) + s * 32);
+#pragma unroll
+      for (int g = 0; g < DP / 32; ++g) {
+        if (g + 1 < DP / 32) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+              kf[(g + 1) & 1][s][kb] = *reinterpret_cast<const f16x8*>(
+                  kp + kb * (32 * KPITCH) + (2 * g + 2 + s) * 32);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+            x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g & 1][s][kb], qf[2 * g + s],
+                                                           x[kb], 0, 0, 0);
+      }
     };
     int stage = 1;
     if (steps > 0) {
@@ -1027,27 +1027,27 @@ attend_tiles_kernel(AttnArgs a) {
         __syncthreads();
         // ---- products of this step's values and the next one's keys ----
         __builtin_amdgcn_sched_barrier(0);
-                  const char* vp = vL + (step & 1) * VB + lr * VPITCH;
-                  // chunk 2t + lh of row 32e + lr: vc ^ 32(t ^ e % 4)
-                  const int vc = (lh ^ (lr >> 4)) << 4;
-                  f16x8 vf[2][DP / 32];
-        #pragma unroll
-                  for (int e = 0; e < DP / 32; ++e)
-                    vf[0][e] =
-                        *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (32 * (e & 3))));
-        #pragma unroll
-                  for (int t = 0; t < 4; ++t) {
-                    if (t < 3) {
-        #pragma unroll
-                      for (int e = 0; e < DP / 32; ++e)
-                        vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
-                            vp + e * (32 * VPITCH) + (vc ^ (32 * ((t + 1) ^ (e & 3)))));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-        #pragma unroll
-                    for (int e = 0; e < DP / 32; ++e)
-                      acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
-                  }
+        const char* vp = vL + (step & 1) * VB + lr * VPITCH;
+        // chunk 2t + lh of row 32e + lr: vc ^ 32(t ^ e % 4)
+        const int vc = (lh ^ (lr >> 4)) << 4;
+        f16x8 vf[2][DP / 32];
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+          vf[0][e] =
+              *reinterpret_cast<const f16x8*>(vp + e * (32 * VPITCH) + (vc ^ (32 * (e & 3))));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (t < 3) {
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e)
+              vf[(t + 1) & 1][e] = *reinterpret_cast<const f16x8*>(
+                  vp + e * (32 * VPITCH) + (vc ^ (32 * ((t + 1) ^ (e & 3)))));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < DP / 32; ++e)
+            acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][e], w[t], acc[e], 0, 0, 0);
+        }
         logits(step + 1);
         __builtin_amdgcn_sched_barrier(0);
       }

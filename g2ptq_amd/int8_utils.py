@@ -275,11 +275,8 @@ def int8_matmul(codes, scale, linear, zero=None, dtype=torch.bfloat16):
     y = torch.empty(rows, out, dtype=dtype, device=codes.device)
     if rows:
         scale, zero = scale.contiguous(), None if zero is None else zero.contiguous()
-        ws = _lib.scratch(_lib.query_size("g2ptq_int8_gemm_workspace", rows, out, columns),
-                          codes.device)
         _lib.call("g2ptq_int8_gemm", _lib.stream_ptr(codes.device), _lib.ptr(c2), c2.stride(0),
                   _lib.ptr(scale), _lib.ptr(zero), _lib.ptr(weight), linear._shape[1],
                   _lib.ptr(wscale), _lib.ptr(None if zero is None else total), _lib.ptr(bias),
-                  rows, out, columns, _lib.ptr(y), _DTYPE_CODE[dtype], out, _lib.ptr(ws),
-                  ws.numel())
+                  rows, out, columns, _lib.ptr(y), _DTYPE_CODE[dtype], out, None, 0)
     return y.view(*lead, out)

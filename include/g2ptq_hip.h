@@ -420,7 +420,8 @@ int g2ptq_quantize_tokens(void* stream, const void* x, int dtype, int64_t T, int
  * (dtype as above, ld ldo).  codes as written by g2ptq_quantize_tokens; W: N
  * rows of ldw bytes, 16-byte aligned, ldw a multiple of 16, zero in the columns
  * from K to the next multiple of 256; wsum[n] = Σ_k W[n][k].  zero (with wsum)
- * and bias are nullable.  Sums are exact integers. */
+ * and bias are nullable.  Sums are exact integers.  No form of the product needs a
+ * workspace at present: the size is 0 and ws is not used. */
 int g2ptq_int8_gemm_workspace(int64_t T, int64_t N, int64_t K, size_t* bytes);
 int g2ptq_int8_gemm(void* stream, const int8_t* codes, int64_t ldc, const float* scale,
                     const float* zero, const int8_t* W, int64_t ldw, const float* wscale,
