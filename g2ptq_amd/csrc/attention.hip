@@ -20,7 +20,10 @@
 //   l = Σ p_j,  o = 2^9·Σ fp16(p_j·sv_j)·(u − z)2^-9 / l,
 // C the row's power of two (so C·max is exact), e = 15 − log2(ref), ref
 // a power of two above the scales sv of the values that the row has seen: the
-// weights p·sv reach up to 2^15 and keep their 11 bits down to 2^-29 of that.
+// weights p·sv reach up to 2^15 and keep their 11 bits down to 2^-29 of that.  Rounding
+// the weights to fp16 is what lets the matrix cores take them at speed (their fp32 rate is a
+// sixteenth).  It moves a weight by at most 2^-11, which the last rounding of bf16 outputs
+// covers; fp16 outputs end 3e-4 (relative) from the exact ones where 32-bit weights leave 2e-4.
 // One pass over the keys: when the maximum or ref grows, the row's sums are
 // scaled back.  Scales are the only numbers of the cache that can be NaN or
 // infinite, and a key that a row does not see enters neither its maximum, its
@@ -273,11 +276,14 @@ __device__ void clear_outside(const AttnArgs& a) {
 // keys and join through LDS; `few_split` workgroups share a sequence's keys.
 // DP: channels rounded up to 64, 128 or 256 (FULL: D == DP).
 // Bound by the cache's bytes at 8 bits and by vector arithmetic (two to three
-// instructions per two codes) and the loads a CU keeps under way about alike at 4: MI355X, heads 32 on 8 of 128, 8 bits: one query over
-// 131072 keys 51 µs (5.4 TB/s), 64 over 4096 each 98–102 µs (5.5 TB/s); 4 bits: 64 over 4096
-// 61 µs (4.7 TB/s); one over 4001 at 8 bits 8.6 µs and 4 to join, latency.  Up to 16 rows, one
+// instructions per two codes) and the loads a CU keeps under way about alike at 4, where heads
+// of 128 also spill 13 of a lane's registers under the bound of three waves.  MI355X, back to
+// back and with the join, heads 32 on 8 of 128, 8 bits: one query over 131072 keys 51 µs
+// (5.4 TB/s), 64 over 4096 each 99 µs (5.6 TB/s); 4 bits: 64 over 4096 60 µs (4.8 TB/s); one
+// over 4001 at 8 bits 12 µs, of which 8.3 here and 4 in the join, latency.  Up to 16 rows, one
 // block of the product's columns: 32 uneven sequences with 2 tokens of 8 heads 38 µs, 74 by
-// attend_tiles_kernel; 4 tokens over 8192 keys 14.4 against 24.6 µs.
+// attend_tiles_kernel; 4 tokens over 8192 keys 14.4 against 24.6 µs.  More rows of one token
+// (over 16 query heads on a head of the cache) go to attend_tiles_kernel unmeasured.
 // ---------------------------------------------------------------------------
 template <int BITS, int DP, bool FULL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? (BITS == 4 ? 3 : 2) : 1) void
@@ -604,10 +610,13 @@ attend_rows_kernel(AttnArgs a) {
 // rows, one 16-byte chunk) touch all banks; values' rows also hold chunk c at
 // c ^ (channel / 16), which spreads the writes (8 rows 8 channels apart, one chunk).
 // Bound by the products, whose operands come from LDS at about the rate the matrix cores
-// take them, and the softmax between them, which the two workgroups of a CU overlap only in
-// part: MI355X, 2048 tokens over 16384 keys, heads 32 on 8 of 128, 8 bits, 660 µs, 780
-// TFLOP/s (the library's largest bf16 product: 1520).  Slower: waves in two groups that take
-// turns at softmax and products (780 against 688 µs then), steps of 32 keys (915 against 795).
+// take them (a wave's 32 rows read all of a step's keys and values), and the softmax between
+// them, which the two workgroups of a CU overlap only in part: MI355X, 2048 tokens over 16384
+// keys, heads 32 on 8 of 128, 8 bits, back to back 654–668 µs, 770–790 TFLOP/s (the library's
+// largest bf16 product: 1520; under the profiler, with the clocks of single launches, 689 at
+// best and 746 on average).  Slower: waves in two groups that take turns at softmax and
+// products (780 against 688 µs then), steps of 32 keys (915 against 795); both read as much
+// from LDS for a product.  Heads of 129 to 256 channels put 20 bytes a lane into scratch.
 // ---------------------------------------------------------------------------
 // Largest of 64 lanes' non-negative x (rows of 16 lanes, then across rows, into lane 63).
 __device__ __forceinline__ float wave_max(float x) {

@@ -124,9 +124,10 @@ __device__ __forceinline__ void store_y(const GemmI8& a, int64_t o, float y) {
 // chunk) are free of bank conflicts.  S > 1: S groups of waves share K and add their
 // integer sums in LDS (tiles too few for the chip, which then wait for each stage's loads).
 // Tiles of 256 × 256 are bound by the matrix cores, with clocks as the power allows (MI355X,
-// 8192 × 14336 × 4096: 427–490 µs, 2.0–2.25 POP/s; a large library product reaches 2.35);
-// small ones by the latency of their stages and of the launch (777 × 1000 × 2752: 12 µs;
-// 48 × 14336 × 4096: 13.6 µs, 4.3 TB/s of weights).
+// the product alone under the profiler, fastest and average: 8192 × 14336 × 4096 424 and 485
+// µs, 2.0–2.27 POP/s; a large library product reaches 2.35); small ones by the latency of
+// their stages and of the launch (777 × 1000 × 2752 11.4 and 12.4 µs; 48 × 14336 × 4096 12.8
+// and 14.1 µs, 4.2–4.6 TB/s of weights).
 constexpr int KS = 128;
 __device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
 
@@ -365,8 +366,9 @@ __global__ __launch_bounds__(64 * WM * WN * S) void gemm_i8_kernel(GemmI8 a, int
 // FUSED: the tokens themselves are quantized here, by every workgroup, into LDS (one or
 // two tokens: cheaper than another launch before this one).
 // Bound by the weights' bytes and, where those are few, by the launch and the latency of
-// the first loads: MI355X, one token fused, 4096 × 4096 7.0 µs (2.4 TB/s), 14336 × 4096 17 µs
-// (3.5 TB/s), 8192 × 28672 53 µs (4.4 TB/s); 16 tokens and their quantiser, 14336 × 4096 20.4 µs.
+// the first loads: MI355X, back to back over weights that no cache holds, one token fused,
+// 4096 × 4096 9.4 µs (1.8 TB/s; 6.7 where the last cache holds them), 14336 × 4096 17 µs
+// (3.5 TB/s), 8192 × 28672 55 µs (4.3 TB/s); 16 tokens and their quantiser, 14336 × 4096 21 µs.
 template <int R, int TB, bool FUSED, int DT, bool SYM>
 __global__ __launch_bounds__(512) void gemm_i8_few_kernel(GemmI8 a, const void* __restrict__ x,
                                                           int64_t ldx, bool vec) {
@@ -547,7 +549,7 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
     // 256 tiles of 256 (4096³) 64 against 86 µs; 128 against 64 at 256 tiles of 128
     // (1024 × 4096, K 4096) 28 against 34 µs, at 128 of them (512 × 4096, K 14336) 71
     // against 54 µs; 208 tiles of 64 (777 × 1000, K 2752) 10.4 µs with K shared by four
-    // groups, 12.8 µs without.
+    // groups, 12.8 µs without (back to back over the same operands, as the others here).
     if (cdiv(a.T, 256) * cdiv(a.N, 256) >= 192) launch_tiles<256, 256, 2, 4, 1>(st, a);
     else if (cdiv(a.T, 128) * cdiv(a.N, 128) >= 224) launch_tiles<128, 128, 2, 2, 1>(st, a);
     else if (cdiv(a.T, 64) * cdiv(a.N, 64) > 512) launch_tiles<64, 64, 2, 2, 1>(st, a);
@@ -559,9 +561,10 @@ int gemm_i8(hipStream_t st, const GemmI8& a) {
 }
 
 // Tokens quantized and multiplied in one launch: one token, or two of up to 16384 columns
-// (LDS holds the codes).  MI355X, fused against apart: one token, 4096 × 4096 9.4 against
-// 10.8 µs, K 14336 19.1 against 25.7, 8192 channels of K 28672 53 against 62; two,
-// 4096 × 4096 10.8 against 11.1, K 11008 21.0 against 23.1; four, 13.4 against 11.2.
+// (LDS holds the codes).  MI355X, over weights that no cache holds, fused against apart: one
+// token, 4096 × 4096 9.4 against 10.8 µs, K 14336 19.1 against 25.7, 8192 channels of K 28672
+// 53 against 62; two, 4096 × 4096 10.8 against 11.1, K 11008 21.0 against 23.1; four, 13.4
+// against 11.2.
 bool fused(int64_t T, int64_t K) { return T <= 2 && T * K <= 32768; }
 template <int DT, bool SYM>
 void launch_fused(hipStream_t st, const GemmI8& a, const void* x, int64_t ldx, bool vec) {

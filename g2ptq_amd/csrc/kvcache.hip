@@ -29,9 +29,11 @@ struct WriteArgs {
 // L lanes hold one token's head, sixteen channels each (lanes past D idle), and reduce
 // it among themselves; a workgroup takes 256 / L consecutive heads of the T × H.  Sixteen
 // channels are the largest store of a lane at 8 bits and leave few lanes to reduce over.
-// Bound by memory and the arithmetic of the codes (a division each) about alike: MI355X,
-// 8192 tokens of 8 × 128 bf16, 8 bits 15–22 µs, 4 bits asymmetric 11.4–13 µs (3.5 TB/s); 32
-// tokens 3.4 µs, a launch's latency.
+// A wave loads, then computes, then stores, once.  At 8 bits its waves wait for memory seven
+// tenths of the time; at 4 bits asymmetric they execute 22 vector instructions a value (18 at
+// 8 bits; range, corrected product, code, packing), 9 µs of the whole by themselves.  MI355X,
+// 8192 tokens of 8 × 128 bf16, 8 bits 15–22 µs (bytes 10), 4 bits asymmetric 11–13 µs (bytes
+// 8.3); 32 tokens 3.4 µs, a launch's latency.
 // grid.y: 0 keys, 1 values.
 template <int DT, bool SYM, int BITS, int L>
 __global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
@@ -94,7 +96,7 @@ constexpr int kReadTokens = 64;
 // then their pieces of 16 channels, consecutive threads consecutive pieces.  Output rows
 // outside every sequence, and tokens whose page is not in the cache, are zero.  Bound by
 // the bytes: MI355X, 131072 tokens of 8 × 128, 8 bits to bf16, 177 µs (4.6 TB/s); 8192 at 4
-// bits 11 µs (3.8 TB/s); 512 tokens 4.2 µs, the latency of offset, page, scale and code.
+// bits 10.5–12 µs (3.5–4 TB/s); 512 tokens 4 µs, the latency of offset, page, scale and code.
 template <int DT, int BITS>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
   __shared__ int64_t slotL[kReadTokens];
@@ -249,9 +251,9 @@ extern "C" int g2ptq_kv_read(void* stream, const g2ptq_kv_cache* cache, const in
   G2PTQ_CHECK(aligned16(k) && aligned16(v), "kv_read: outputs not 16-byte aligned");
   a.table = table, a.ldt = ldt, a.B = B, a.width = width, a.cu = cu, a.total = total;
   a.out[0] = k, a.out[1] = v;
-  // Some four pieces per thread, fewer where that leaves CUs idle.  MI355X, 8 bits, 131072
-  // tokens of 8 × 128: 179 µs, 191 with eight (158 with two, which lose at 4 bits: 65536
-  // tokens of 8 × 64 35 against 31.6 µs).
+  // Some four pieces per thread, fewer where that leaves CUs idle: one number for both widths.
+  // MI355X, 8 bits, 131072 tokens of 8 × 128: 177 µs, 191 with eight.  Two take 158 there, but
+  // lose at 4 bits (65536 tokens of 8 × 64 35 against 31.6 µs).
   const int64_t pieces = a.c.H * a.c.D / 16;
   int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(kReadTokens, 1024 / pieces));
   while (tokens > 1 && cdiv(total, tokens) < 256) tokens /= 2;

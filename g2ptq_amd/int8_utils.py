@@ -4,8 +4,8 @@ quantized on the fly, one scale (and zero point) per token.
 
     Y[t, n] = s_t · w_n · (Σ_k c[t, k]·W[n, k] − z_t·Σ_k W[n, k]) + b_n
 
-The integer sums are exact; scales are applied in fp32 and the result is
-rounded once.  The token grid is the weight quantizer's (``quant_utils``) at
+The integer sums are exact.  Their conversion, the two scales and the bias
+round in fp32, then the result to its type.  The token grid is the weight quantizer's (``quant_utils``) at
 8 bits with one group per token.  Inference only: nothing here has a
 gradient.
 """
