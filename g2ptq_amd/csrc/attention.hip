@@ -1237,6 +1237,10 @@ struct Plan {
     // 71 / 84 µs.  Of 256 keys or more: 8 chunks of 16 tokens over 2048 keys 33 µs, 40 with 512.
     split = std::max<int64_t>(1, std::min((B > 1 ? 3 : 2) * kCUs / (pairs * ntiles), keys / 256));
     split = std::min<int64_t>(split, 32);
+    // Every token has its partial results, also where more tokens than stated came: at most a
+    // GiB of them (sizes stated right need a sixth of that at most).
+    const int64_t one = T * Hq * (D + 4) * 4;
+    split = std::min(split, std::max<int64_t>(1, (1 << 30) / std::max<int64_t>(1, one)));
     share = cdiv(cdiv(keys, split), 64) * 64;
     part = tiles && split > 1 ? cdiv(T * Hq * split * (D + 4) * 4, 256) * 256 : 0;
     few_part = few && few_split > 1

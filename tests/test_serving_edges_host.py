@@ -140,3 +140,14 @@ def test_a_cache_that_no_call_takes_is_not_made():
             PagedKVCache(pages, page, heads, 64, device="cpu")
     with pytest.raises(RuntimeError, match="GPU"):
         PagedKVCache((1 << 19) - 1, 64, 64, 64, device="cpu")
+
+
+def test_sizes_stated_too_small_do_not_ask_for_all_memory():
+    """A million tokens where max_q says eight: partial results of every share of every token
+    would be half a TiB.  Sizes stated right are as before."""
+    def size(*a):
+        return _lib.query_size("g2ptq_paged_attention_workspace", *a)
+    assert size(1 << 20, 32, 8, 128, 1, 8, 131072) <= 1 << 30
+    assert size(8192, 32, 8, 128, 1, 5, 131072) <= 1 << 30
+    assert size(512, 32, 8, 128, 1, 512, 2048) == 512 * 32 * 4 * 132 * 4
+    assert size(1, 32, 8, 128, 1, 1, 4096) == 8 * 16 * 16 * 132 * 4
