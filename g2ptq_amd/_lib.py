@@ -15,6 +15,7 @@ FLAG_BAD_SCALE = 1
 FLAG_NAN_OUTPUT = 2
 FLAG_GROUP_SCALE = 4
 FLAG_BAD_INDEX = 8
+FLAG_NO_ROOM = 16
 VARIANT_GPTQ, VARIANT_GPTAQ, VARIANT_G2PTQ = 0, 1, 2
 
 _p = ctypes.c_void_p
@@ -30,6 +31,19 @@ class KvCacheStruct(ctypes.Structure):
     _fields_ = [("k_codes", _p), ("v_codes", _p), ("k_scale", _p), ("v_scale", _p),
                 ("k_zero", _p), ("v_zero", _p), ("flags", _p), ("pages", _i64), ("heads", _i64),
                 ("page", _i64), ("dim", _i64), ("bits", _i32), ("sym", _i32)]
+
+
+class PageTablesStruct(ctypes.Structure):
+    """``g2ptq_page_tables`` of include/g2ptq_hip.h."""
+    _fields_ = [("table", _p), ("lengths", _p), ("free_pages", _p), ("free_count", _p),
+                ("mark", _p), ("flags", _p), ("seqs", _i64), ("width", _i64), ("pages", _i64),
+                ("page", _i64)]
+
+
+class AdapterSetStruct(ctypes.Structure):
+    """``g2ptq_adapter_set`` of include/g2ptq_hip.h."""
+    _fields_ = [("down", _p), ("up", _p), ("rank", _p), ("scale", _p), ("flags", _p), ("n", _i64),
+                ("R", _i64), ("K", _i64), ("N", _i64), ("dtype", _i32)]
 
 
 # name -> argtypes (all functions return int status except the two string ones)
@@ -102,6 +116,18 @@ SIGNATURES = {
     "g2ptq_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _szp],
     "g2ptq_paged_attention": [_p, ctypes.POINTER(KvCacheStruct), _p, _i64, _i64, _i32, _i64, _i64,
                               _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _f32, _p, _p, _sz],
+    "g2ptq_rms_norm": [_p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i32, _i64, _i64, _i64, _f32,
+                       _p, _p, _i32, _p, _i64, _p, _p],
+    "g2ptq_dequantize_tokens": [_p, _p, _i64, _p, _p, _i64, _i64, _p, _i32],
+    "g2ptq_rotary": [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _i32,
+                     _p, _p, _f32, _p, _p],
+    "g2ptq_pages_workspace": [_i64, _szp],
+    "g2ptq_pages_extend": [_p, ctypes.POINTER(PageTablesStruct), _p, _p, _i64, _i64, _p, _p, _p,
+                           _p, _p, _p, _sz],
+    "g2ptq_pages_release": [_p, ctypes.POINTER(PageTablesStruct), _p, _p, _i64, _p, _sz],
+    "g2ptq_adapters_workspace": [_i64, _i64, _i64, _i64, _szp],
+    "g2ptq_adapters": [_p, ctypes.POINTER(AdapterSetStruct), _p, _i64, _p, _i64, _p, _i64, _p,
+                       _i64, _p, _sz],
 }
 STRING_FUNCS = ("g2ptq_status_string", "g2ptq_last_error")
 
@@ -182,8 +208,10 @@ def call_fast(name, *args):
         if status != 0:
             raise_status("g2ptq_" + name, status)
         return status
-    args = [ctypes.byref(KvCacheStruct.from_address(a)) if i == 1 and name != "int8_linear" else a
-            for i, a in enumerate(args)]
+    # (an entry point that takes a host struct takes it after the stream)
+    struct = getattr(SIGNATURES["g2ptq_" + name][1], "_type_", None)
+    if isinstance(struct, type) and issubclass(struct, ctypes.Structure):
+        args = (args[0], ctypes.byref(struct.from_address(args[1])), *args[2:])
     return call("g2ptq_" + name, *args)
 
 

@@ -29,7 +29,8 @@ FLAGS = [
 # Per-file extra flags.  The quantize / sweep kernels must round every product
 # and sum separately (the reference's torch ops never fuse); the flag also
 # covers the HIP header's __f*_rn helpers, which a source-level pragma cannot.
-EXTRA = {f: ["-ffp-contract=off"] for f in ("quant.hip", "calib.hip", "int8.hip", "kvcache.hip")}
+EXTRA = {f: ["-ffp-contract=off"] for f in ("quant.hip", "calib.hip", "int8.hip", "kvcache.hip",
+                                            "norm.hip")}
 
 
 def sources():

@@ -70,6 +70,39 @@ def quantize_tokens(x, sym=True):
     return codes, scale.view(lead), (None if zero is None else zero.view(lead))
 
 
+def dequantize_tokens(codes, scale, zero=None, dtype=torch.bfloat16):
+    """What codes stand for, ``scale · (code − zero)`` in ``dtype``: the inverse of
+    ``quantize_tokens``.  ``codes`` (..., K) int8; ``scale`` and ``zero`` (fp32; ``zero`` may be
+    None) have their shape without the last dimension."""
+    if codes.dtype is not torch.int8 or codes.dim() == 0 \
+            or not 1 <= codes.shape[-1] <= MAX_COLUMNS:
+        raise ValueError(f"dequantize_tokens: codes of {codes.dtype} and shape "
+                         f"{tuple(codes.shape)} (int8, rows of 1 to {MAX_COLUMNS})")
+    if dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"dequantize_tokens gives bf16, fp16 or fp32, not {dtype}")
+    _lib.require_current(codes, "dequantize_tokens")
+    lead, columns = codes.shape[:-1], codes.shape[-1]
+    for name, t in (("scale", scale), ("zero", zero)):
+        if t is not None and (t.dtype is not _F32 or t.shape != lead
+                              or t.get_device() != codes.get_device()):
+            raise ValueError(f"dequantize_tokens: {name} of {t.dtype} and shape {tuple(t.shape)} "
+                             f"on {t.device}, expected fp32 {tuple(lead)} on {codes.device}")
+        if t is not None:
+            _lib.require_current(t, "dequantize_tokens")
+    c2 = codes if codes.dim() == 2 else codes.flatten(0, -2) if codes.dim() > 2 \
+        else codes.unsqueeze(0)
+    if columns > 1 and c2.stride(1) != 1:
+        c2 = c2.contiguous()
+    rows = c2.shape[0]
+    out = torch.empty(rows, columns, dtype=dtype, device=codes.device)
+    if rows:
+        scale, zero = scale.contiguous(), None if zero is None else zero.contiguous()
+        _lib.call_fast("dequantize_tokens", _lib.current_stream(), c2.data_ptr(), c2.stride(0),
+                       scale.data_ptr(), None if zero is None else zero.data_ptr(), rows, columns,
+                       out.data_ptr(), _DTYPE_CODE[dtype])
+    return out if codes.dim() == 2 else out.view(codes.shape)
+
+
 class Int8Linear(torch.nn.Module):
     """``y = x̂ · Ŵᵀ + b`` with x̂ the tokens quantized to 8 bits and Ŵ = scale · codes.
 

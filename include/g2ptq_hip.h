@@ -36,7 +36,9 @@ extern "C" {
 #define G2PTQ_FLAG_BAD_SCALE 1   /* a scale was <= 0 or NaN (quant_utils.py:432 assert) */
 #define G2PTQ_FLAG_NAN_OUTPUT 2  /* NaN in quantized weights (gptq_utils.py:346-350) */
 #define G2PTQ_FLAG_GROUP_SCALE 4 /* scales differ within a group (compressed_tensors_utils.py:35 assert) */
-#define G2PTQ_FLAG_BAD_INDEX 8   /* a cache slot or page outside the cache */
+#define G2PTQ_FLAG_BAD_INDEX 8   /* a cache slot or page outside the cache; a row, count or index of
+                                  * page tables or adapters that is none */
+#define G2PTQ_FLAG_NO_ROOM 16    /* page tables: no free page, or a request longer than its row */
 
 /* Compensation variants. */
 #define G2PTQ_VARIANT_GPTQ 0
@@ -486,6 +488,92 @@ int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, const void*
                           const int32_t* table, int64_t ldt, int64_t B, int64_t width,
                           const int32_t* cu_q, const int32_t* kv_lens, int64_t max_q,
                           int64_t max_kv, float scale, void* out, void* ws, size_t ws_bytes);
+
+/* What stands between a quantized layer's products. */
+
+/* Root-mean-square norm of `rows` rows of C columns (1 to 65536): s = x + r (r nullable),
+ * y_c = s_c·w_c / sqrt(Σ s²/C + eps), in fp32.  Row i of x is at (i / inner)·x_outer +
+ * (i % inner)·x_inner (elements, columns contiguous), r's likewise; dtype of x and r, wtype of
+ * w (0 bf16, 1 fp16, 2 fp32).  y and sum (s), rows × C of dtype, are nullable; with codes they
+ * and scale (and, with sym == 0, zero) are y's row on the 8-bit grid, as
+ * g2ptq_quantize_tokens writes them, but of y before its rounding to dtype. */
+int g2ptq_rms_norm(void* stream, const void* x, int64_t x_outer, int64_t x_inner, const void* r,
+                   int64_t r_outer, int64_t r_inner, int dtype, const void* w, int wtype,
+                   int64_t rows, int64_t inner, int64_t C, float eps, void* y, void* sum, int sym,
+                   int8_t* codes, int64_t ldc, float* scale, float* zero);
+
+/* What codes stand for: out[t][k] = scale[t]·(codes[t][k] − zero[t]) (T × K of dtype; zero
+ * nullable; rows of ldc bytes). */
+int g2ptq_dequantize_tokens(void* stream, const int8_t* codes, int64_t ldc, const float* scale,
+                            const float* zero, int64_t T, int64_t K, void* out, int dtype);
+
+/* Rotary positions of queries and keys (T tokens of q_heads and k_heads heads of dim channels,
+ * strides of token and head in elements, channels contiguous; either may have no heads): pair i
+ * of a head's first n channels is turned by φ = 2π·positions[t]·freq[i] (freq: n / 2 turns a
+ * position, fp64) and scaled, (a, b) → factor·(a·cos φ − b·sin φ, a·sin φ + b·cos φ).  Pairs are
+ * channels (i, i + n/2), or (2i, 2i + 1) with interleaved != 0.  Outputs are contiguous.
+ * dim at most 1024, n even. */
+int g2ptq_rotary(void* stream, const void* q, int64_t q_token, int64_t q_head, int64_t q_heads,
+                 const void* k, int64_t k_token, int64_t k_head, int64_t k_heads, int dtype,
+                 int64_t T, int64_t dim, int64_t n, int interleaved, const int64_t* positions,
+                 const double* freq, float factor, void* q_out, void* k_out);
+
+/* Page tables of a paged cache (the struct is host memory, its pointers device memory): a row
+ * of `width` page numbers (−1 where there is none) and a length for each of `seqs` requests,
+ * and a stack of free pages, the first free_count[0] of free_pages, the last on top.  mark: one
+ * int32 per row, 0x7fffffff between calls.  page: slots of a page, a power of two up to 4096;
+ * width·page < 2^31.  flags: one int32. */
+typedef struct g2ptq_page_tables {
+  int32_t* table;
+  int32_t* lengths;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int32_t* mark;
+  int* flags;
+  int64_t seqs, width, pages, page;
+} g2ptq_page_tables;
+
+/* Request i of a batch of B (at most 2^20) gets counts[i] new tokens in row rows[i], with pages
+ * from the top of the stack, request by request.  Writes the batch's tables (B × width), the
+ * offsets cu (B + 1) of its tokens, its lengths, and each token's slot and position (total;
+ * −1 and 0 for tokens that are not placed).  A request is left as it was, and its tokens are
+ * not placed, where the pages or its row do not suffice (G2PTQ_FLAG_NO_ROOM), where rows[i] is
+ * no row, or named by an earlier request, or its tokens end past total (G2PTQ_FLAG_BAD_INDEX).
+ * Negative rows are padding: not placed, not flagged.  Negative counts are flagged and count as
+ * 0.  ws: g2ptq_pages_workspace(B), 8-byte aligned. */
+int g2ptq_pages_workspace(int64_t B, size_t* bytes);
+int g2ptq_pages_extend(void* stream, const g2ptq_page_tables* tables, const int32_t* rows,
+                       const int32_t* counts, int64_t B, int64_t total, int32_t* table, int32_t* cu,
+                       int32_t* kv_lens, int64_t* slots, int64_t* positions, void* ws,
+                       size_t ws_bytes);
+
+/* Request i is cut to keep[i] tokens (null: none); its other pages go back to the stack so that
+ * the first request's first page ends on top: a release of what one extend took restores the
+ * stack.  Rows as above; keep outside 0 .. length is flagged and changes nothing. */
+int g2ptq_pages_release(void* stream, const g2ptq_page_tables* tables, const int32_t* rows,
+                        const int32_t* keep, int64_t B, void* ws, size_t ws_bytes);
+
+/* Low-rank adapters (the struct is host memory, its pointers device memory): n of up to R ranks
+ * (a multiple of 16, at most 512).  down: n × R × K', up: n × N' × R of dtype (0 bf16, 1 fp16),
+ * K' and N' the next multiples of 64, zero where padded, 16-byte aligned.  rank (n, 1 to R) and
+ * scale (n).  flags: one int32. */
+typedef struct g2ptq_adapter_set {
+  const void* down;
+  const void* up;
+  const int32_t* rank;
+  const float* scale;
+  int* flags;
+  int64_t n, R, K, N;
+  int dtype;
+} g2ptq_adapter_set;
+
+/* out[t] = base[t] + scale[a]·up[a]·(down[a]·x[t]), a = index[t]; out[t] = base[t] where the index
+ * is negative, and where it is not below n, which is flagged.  x: T × K (ld ldx), base (nullable: zeros)
+ * and out: T × N, of the adapters' dtype; out may be base.  ws is 16-byte aligned. */
+int g2ptq_adapters_workspace(int64_t T, int64_t K, int64_t n, int64_t R, size_t* bytes);
+int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const void* x, int64_t ldx,
+                   const int32_t* index, int64_t T, const void* base, int64_t ldb, void* out,
+                   int64_t ldo, void* ws, size_t ws_bytes);
 
 #ifdef __cplusplus
 }
