@@ -24,7 +24,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWindow = 64;  // tokens
-constexpr int kRankGroup = 64;
 
 struct AdapterArgs {
   const uint16_t* x;
@@ -74,15 +73,16 @@ __device__ __forceinline__ u32x4 piece(const uint16_t* p, bool vec, int64_t n) {
   return v;
 }
 
-// f(adapter, list of its tokens in the window, their number) for every adapter whose first
-// token of the window is at a lane that this slot takes.  The list is the wave's own.
+// f(adapter, number of its tokens) for every adapter whose first token of the window is at a
+// lane that this slot takes, with `list` (the wave's own) their lanes.  none: tokens without
+// an adapter too, as −1.
 template <typename F>
-__device__ __forceinline__ void each_adapter(const AdapterArgs& a, int64_t t0, int slot,
-                                             int32_t idx, uint8_t* list, F f) {
+__device__ __forceinline__ void each_adapter(const AdapterArgs& a, int slot, int32_t idx,
+                                             bool none, uint8_t* list, F f) {
   const int lane = threadIdx.x & 63;
   for (int first = slot; first < kWindow; first += a.slots) {
     const int32_t which = __builtin_amdgcn_readlane(idx, first);
-    if (which < 0) continue;
+    if (which < (none ? -1 : 0)) continue;
     const uint64_t same = __ballot(idx == which);
     if (__builtin_ctzll(same) != first) continue;
     __builtin_amdgcn_wave_barrier();
@@ -92,58 +92,91 @@ __device__ __forceinline__ void each_adapter(const AdapterArgs& a, int64_t t0, i
   }
 }
 
+// The adapter of the lane's token: −1 none, −2 no token.
 __device__ __forceinline__ int32_t index_of_lane(const AdapterArgs& a, int64_t t0) {
   const int64_t t = t0 + (threadIdx.x & 63);
-  int32_t idx = t < a.T ? a.index[t] : -1;
-  if (idx >= a.n) {
-    if (threadIdx.x < 64 && blockIdx.y == 0) atomicOr(a.flags, G2PTQ_FLAG_BAD_INDEX);
-    idx = -1;
-  }
-  return idx;
+  if (t >= a.T) return -2;
+  const int32_t idx = a.index[t];
+  if (idx >= a.n && threadIdx.x < 64 && blockIdx.y == 0) atomicOr(a.flags, G2PTQ_FLAG_BAD_INDEX);
+  return idx >= a.n ? -1 : max(idx, -1);
 }
 
-// h of 16·TB tokens for 16·RB ranks from r0 on: ranks × tokens, 64 columns of K a step (lane
-// (n, g) holds 16 of row n from 16·g on).  The workgroup's waves and the launch's parts take
-// turns at the steps.
+// h of 16·TB tokens for up to 16·RB ranks from r0 on: ranks × tokens, 64 columns of K a step
+// (lane (n, g) holds 16 of row n from 16·g on).  The workgroup's waves and the launch's parts
+// take turns at rounds of U steps, whose loads are all under way together.
 template <bool F16, int RB, int TB>
 __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int which, int64_t r0,
-                                       const uint8_t* list, int count, f32x4 (*sums)[16][64]) {
+                                       int blocks, const uint8_t* list, int count,
+                                       f32x4 (*sums)[RB * 4][64]) {
+  constexpr int U = TB == 1 ? 2 : 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const uint16_t* xrow[TB];
   const uint16_t* drow[RB];
 #pragma unroll
   for (int b = 0; b < TB; ++b)
-    xrow[b] = a.x + (t0 + list[min(16 * b + n, count - 1)]) * a.ldx;
+    xrow[b] = a.x + (t0 + list[min(16 * b + n, count - 1)]) * a.ldx + g * 16;
 #pragma unroll
-  for (int r = 0; r < RB; ++r) drow[r] = a.down + ((int64_t)which * a.R + r0 + 16 * r + n) * a.Kp;
+  for (int r = 0; r < RB; ++r)  // (blocks that the adapter lacks: the first again, not stored)
+    drow[r] = a.down + ((int64_t)which * a.R + r0 + (r < blocks ? 16 * r : 0) + n) * a.Kp + g * 16;
   f32x4 acc[RB][TB];
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int b = 0; b < TB; ++b) acc[r][b] = f32x4{0, 0, 0, 0};
-  for (int64_t k = (int64_t)(blockIdx.y * 4 + wave) * 64 + g * 16; k - g * 16 < a.Kp;
-       k += a.parts * 256) {
+  struct Step {
     u32x4 d[RB][2], x[TB][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int r = 0; r < RB; ++r) d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k + 8 * i);
-#pragma unroll
-      for (int b = 0; b < TB; ++b) x[b][i] = piece(xrow[b] + k + 8 * i, a.vx, a.K - k - 8 * i);
-    }
+  };
+  auto products = [&](const Step& s) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < RB; ++r)
 #pragma unroll
-        for (int b = 0; b < TB; ++b) acc[r][b] = mfma<F16>(d[r][i], x[b][i], acc[r][b]);
+        for (int b = 0; b < TB; ++b) acc[r][b] = mfma<F16>(s.d[r][i], s.x[b][i], acc[r][b]);
+  };
+  auto fetch = [&](Step& s, int64_t k) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k + 8 * i);
+#pragma unroll
+      for (int b = 0; b < TB; ++b) s.x[b][i] = *reinterpret_cast<const u32x4*>(xrow[b] + k + 8 * i);
+    }
+  };
+  const int each = a.parts * 4 * U;
+  int step = (blockIdx.y * 4 + wave) * U;
+  const int whole = a.vx ? (int)(a.K / 64) - (U - 1) : 0;
+  for (; step < whole; step += each) {
+    Step s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(s[u], (int64_t)(step + u) * 64);
+#pragma unroll
+    for (int u = 0; u < U; ++u) products(s[u]);
   }
+  // the last columns, and all where rows are not aligned
+  for (; step * 64 < a.Kp; step += each)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = (int64_t)(step + u) * 64;
+      if (k >= a.Kp) break;
+      Step s;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+          s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k + 8 * i);
+#pragma unroll
+        for (int b = 0; b < TB; ++b)
+          s.x[b][i] = piece(xrow[b] + k + 8 * i, a.vx, a.K - k - g * 16 - 8 * i);
+      }
+      products(s);
+    }
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int b = 0; b < TB; ++b) sums[wave][r * TB + b][lane] = acc[r][b];
   __syncthreads();
-  for (int i = threadIdx.x; i < RB * TB * 64; i += 256) {
+  for (int i = threadIdx.x; i < blocks * TB * 64; i += 256) {
     const int at = i >> 6, l = i & 63, t = at % TB * 16 + (l & 15);
     if (t < count) {
       f32x4 s = sums[0][at][l];
@@ -157,27 +190,18 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
   __syncthreads();
 }
 
-template <bool F16>
-__global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterArgs a) {
-  __shared__ f32x4 sums[4][16][64];
+template <bool F16, int RB>
+__global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
+  __shared__ f32x4 sums[4][RB * 4][64];
   __shared__ uint8_t lists[4][kWindow];
   const int64_t t0 = (a.window + blockIdx.x / a.slots) * kWindow;
   uint8_t* list = lists[threadIdx.x >> 6];
-  each_adapter(a, t0, blockIdx.x % a.slots, index_of_lane(a, t0), list, [&](int which, int count) {
-    const int rank = a.rank[which];
-    for (int64_t r0 = 0; r0 < rank; r0 += kRankGroup) {
-      const int blocks = (int)min<int64_t>(kRankGroup, rank - r0 + 15) / 16;
-      if (count <= 16) {
-        if (blocks <= 1) shrink<F16, 1, 1>(a, t0, which, r0, list, count, sums);
-        else if (blocks <= 2) shrink<F16, 2, 1>(a, t0, which, r0, list, count, sums);
-        else if (blocks <= 3) shrink<F16, 3, 1>(a, t0, which, r0, list, count, sums);
-        else shrink<F16, 4, 1>(a, t0, which, r0, list, count, sums);
-      } else {
-        if (blocks <= 1) shrink<F16, 1, 4>(a, t0, which, r0, list, count, sums);
-        else if (blocks <= 2) shrink<F16, 2, 4>(a, t0, which, r0, list, count, sums);
-        else if (blocks <= 3) shrink<F16, 3, 4>(a, t0, which, r0, list, count, sums);
-        else shrink<F16, 4, 4>(a, t0, which, r0, list, count, sums);
-      }
+  each_adapter(a, blockIdx.x % a.slots, index_of_lane(a, t0), false, list,
+               [&](int which, int count) {
+    const int blocks = (a.rank[which] + 15) / 16;
+    for (int r = 0; r < blocks; r += RB) {
+      if (count <= 16) shrink<F16, RB, 1>(a, t0, which, r * 16, min(RB, blocks - r), list, count, sums);
+      else shrink<F16, RB, 4>(a, t0, which, r * 16, min(RB, blocks - r), list, count, sums);
     }
   });
 }
@@ -197,126 +221,182 @@ __device__ __forceinline__ void load_h(const AdapterArgs& a, int64_t t, int64_t 
   for (int i = 0; i < 8; ++i) v[i] = i < left ? s[i >> 2][i & 3] * scale : 0.f;
 }
 
-// Sixteen channels from c on of a token's row: out = base + add.
+// Eight channels from c on of a token's row of the base, as they lie in memory.
+__device__ __forceinline__ u32x4 base_piece(const AdapterArgs& a, int64_t t, int64_t c) {
+  if (!a.base) return u32x4{0, 0, 0, 0};
+  return piece(a.base + t * a.ldb + c, a.vo, a.N - c);
+}
 template <bool F16>
-__device__ __forceinline__ void add_row(const AdapterArgs& a, int64_t t, int64_t c,
-                                        const float (&add)[16]) {
+__device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int64_t c, u32x4 base,
+                                            f32x4 lo, f32x4 hi) {
+  const int64_t n = a.N - c;
+  uint16_t* o = a.out + t * a.ldo + c;
+  uint16_t h[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t n = a.N - c - 8 * i;
-    if (n <= 0) return;
-    u32x4 v = {0, 0, 0, 0};
-    if (a.base) v = piece(a.base + t * a.ldb + c + 8 * i, a.vo, n);
-    uint16_t h[8];
+  for (int j = 0; j < 8; ++j) {
+    const float add = j < 4 ? lo[j & 3] : hi[j & 3];
+    // (−0 is the number that changes nothing: a base of −0 stays, and no base is +0)
+    h[j] = narrow<F16>(widen<F16>((uint16_t)(base[j >> 1] >> (16 * (j & 1)))) + add);
+  }
+  if (a.vo && n >= 8) {
+    u32x4 v;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t b = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
-      h[j] = narrow<F16>(a.base ? widen<F16>(b) + add[8 * i + j] : add[8 * i + j]);
-    }
-    uint16_t* o = a.out + t * a.ldo + c + 8 * i;
-    if (a.vo && n >= 8) {
+    for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+    *reinterpret_cast<u32x4*>(o) = v;
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-      *reinterpret_cast<u32x4*>(o) = v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n) o[j] = h[j];
-    }
+    for (int j = 0; j < 8; ++j)
+      if (j < n) o[j] = h[j];
   }
 }
 
-// 16·TB tokens × the wave's 64 channels from c0 on: channels × tokens; row m of block j is
-// channel 16·(m / 4) + 4·j + m % 4, so that a lane ends with 16 channels in a row.  A step
-// of 32 is 16 ranks twice: with h rounded, and with what that left out.
-template <bool F16, int TB>
-__device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which, int64_t c0,
-                                       const uint8_t* list, int count, int from) {
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+// An adapter's tokens' h into LDS as it enters the product: per token and 16 ranks four pieces
+// of 16 bytes, both halves of the ranks rounded, then what the rounding left out.  Eight lanes
+// take a token.  back: what a token's products are multiplied with, fp16's rows being brought
+// to the top of its range by a power of two.
+template <bool F16>
+__device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int which,
+                                        const uint8_t* list, int count, u32x4* hL, int pitch,
+                                        float* back) {
   const float scale = a.scale[which];
-  const int64_t rank = a.rank[which];
-  const uint16_t* urow = a.up + ((int64_t)which * a.Np + c0 + (n >> 2) * 16 + (n & 3)) * a.R;
-  const bool low = g >= 2;
-  const int part = (g & 1) * 8;
-  int64_t token[TB];
-  float fit[TB];       // the row's power of two
-  bool infinite[TB];
-  f32x4 acc[TB][4];
-#pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    token[b] = t0 + list[min(from + 16 * b + n, count - 1)];
-    fit[b] = 1.f, infinite[b] = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[b][j] = f32x4{0, 0, 0, 0};
+  const int rank = a.rank[which], pieces = (rank + 15) / 16 * 2;
+  for (int i = threadIdx.x; i < (count + 31) / 32 * 256; i += 256) {
+    const int t = i >> 3, l = i & 7;
+    const int64_t token = t0 + list[min(t, count - 1)];
+    float fit = 1.f;
+    bool infinite = false;
     if constexpr (F16) {
       uint32_t top = 0;
-      for (int64_t r = part; r - part < rank; r += 16) {
+      for (int p = l; p < pieces; p += 8) {
         float v[8];
-        load_h(a, token[b], r, rank - r, scale, v);
+        load_h(a, token, p * 8, rank - p * 8, scale, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       }
-      top = max(top, (uint32_t)__shfl_xor((int)top, 16));  // (lanes n, n + 16: all ranks)
-      infinite[b] = top >= 0x7f800000u;
-      if (!infinite[b] && top) fit[b] = __uint_as_float((uint32_t)min(254, max(1, 127 + 14 + 127 - (int)(top >> 23))) << 23);
+#pragma unroll
+      for (int o = 1; o < 8; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+      infinite = top >= 0x7f800000u;
+      if (!infinite && top)
+        fit = __uint_as_float((uint32_t)min(254, max(1, 268 - (int)(top >> 23))) << 23);
+      if (l == 0 && t < count) back[t] = __fdiv_rn(1.f, fit);
     }
-  }
-  for (int64_t r = 0; r < rank; r += 16) {
-    u32x4 u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      u[j] = *reinterpret_cast<const u32x4*>(urow + 4 * j * a.R + r + part);
-#pragma unroll
-    for (int b = 0; b < TB; ++b) {
+    for (int p = l; p < pieces; p += 8) {
       float v[8];
-      load_h(a, token[b], r + part, rank - r - part, scale, v);
-      u32x4 w;
+      load_h(a, token, p * 8, rank - p * 8, scale, v);
+      u32x4 hi, lo;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f = v[i] * fit[b];
+      for (int j = 0; j < 8; ++j) {
+        float f = v[j] * fit;
         // (beside an infinity or a NaN finite terms do not count, and fp16 has no room for them)
-        if (F16 && infinite[b] && fabsf(f) < __builtin_inff()) f = 0.f;
-        uint16_t q = narrow<F16>(f);
-        if (low) {
-          const float left = f - widen<F16>(q);
-          q = narrow<F16>(fabsf(left) < __builtin_inff() ? left : 0.f);
-        }
-        if (i & 1) w[i >> 1] |= (uint32_t)q << 16;
-        else w[i >> 1] = q;
+        if (F16 && infinite && fabsf(f) < __builtin_inff()) f = 0.f;
+        const uint16_t q = narrow<F16>(f);
+        const float left = f - widen<F16>(q);
+        const uint16_t u = narrow<F16>(fabsf(left) < __builtin_inff() ? left : 0.f);
+        if (j & 1) hi[j >> 1] |= (uint32_t)q << 16, lo[j >> 1] |= (uint32_t)u << 16;
+        else hi[j >> 1] = q, lo[j >> 1] = u;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[b][j] = mfma<F16>(u[j], w, acc[b][j]);
+      if (t < count) {
+        u32x4* o = hL + t * pitch + (p >> 1) * 4 + (p & 1);
+        o[0] = hi, o[2] = lo;
+      }
     }
-  }
-#pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    if (from + 16 * b + n >= count) continue;
-    const float back = F16 ? __fdiv_rn(1.f, fit[b]) : 1.f;
-    float add[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) add[i] = acc[b][i >> 2][i & 3] * back;
-    add_row<F16>(a, token[b], c0 + g * 16, add);
   }
 }
 
-template <bool F16>
-__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterArgs a) {
-  __shared__ uint8_t lists[4][kWindow];
-  const int64_t t0 = (a.window + blockIdx.x / a.slots) * kWindow;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, slot = blockIdx.x % a.slots;
-  const int64_t c0 = (int64_t)blockIdx.y * 256 + wave * 64;
-  if (c0 >= a.N) return;
-  const int32_t idx = index_of_lane(a, t0);
-  uint8_t* list = lists[wave];
-  each_adapter(a, t0, slot, idx, list, [&](int which, int count) {
-    if (count <= 16) expand<F16, 1>(a, t0, which, c0, list, count, 0);
-    else expand<F16, 4>(a, t0, which, c0, list, count, 0);
-  });
-  if (a.out != a.base) {  // rows without an adapter
-    const float none[16] = {};
-    for (int t = slot; t < kWindow && t0 + t < a.T; t += a.slots)
-      if (__builtin_amdgcn_readlane(idx, t) < 0 && lane < 4) add_row<F16>(a, t0 + t, c0 + lane * 16, none);
+// 16·TB tokens × 64 channels at a time, channels × tokens: row m of block j is channel
+// 32·(j / 2) + 8·(m / 4) + 4·(j % 2) + m % 4, so that a lane ends with two pieces of eight
+// channels.  A step of 32 is 16 ranks twice: with h rounded, and with what that left out.
+// RB: blocks of 16 ranks whose weights are loaded together.
+template <bool F16, int RB, int TB>
+__device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which,
+                                       const uint8_t* list, int count, const u32x4* hL, int pitch,
+                                       const float* back) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int blocks = (a.rank[which] + 15) / 16, chunks = (int)(a.Np / 64);
+  const uint16_t* urow =
+      a.up + ((int64_t)which * a.Np + (n >> 2) * 8 + (n & 3)) * a.R + (g & 1) * 8;
+  int64_t token[TB];
+  const u32x4* h[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    const int t = min(16 * b + n, count - 1);
+    token[b] = t0 + list[t];
+    h[b] = hL + t * pitch + g;
   }
+  for (int chunk = blockIdx.y * 4 + wave; chunk < chunks; chunk += gridDim.y * 4) {
+    const int64_t c = (int64_t)chunk * 64;
+    u32x4 base[TB][2];
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) base[b][i] = base_piece(a, token[b], c + 32 * i + g * 8);
+    f32x4 acc[TB][4];
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[b][j] = f32x4{0, 0, 0, 0};
+    const uint16_t* u = urow + c * a.R;
+    for (int r0 = 0; r0 < blocks; r0 += RB) {
+      u32x4 w[RB][4];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+        if (r0 + r < blocks)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[r][j] = *reinterpret_cast<const u32x4*>(u + (32 * (j >> 1) + 4 * (j & 1)) * a.R +
+                                                      (r0 + r) * 16);
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+        if (r0 + r < blocks)
+#pragma unroll
+          for (int b = 0; b < TB; ++b) {
+            const u32x4 v = h[b][(r0 + r) * 4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[b][j] = mfma<F16>(w[r][j], v, acc[b][j]);
+          }
+    }
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      if (16 * b + n >= count) continue;
+      if (F16) {
+        const float f = back[16 * b + n];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[b][j] *= f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (c + 32 * i + g * 8 < a.N)
+          store_piece<F16>(a, token[b], c + 32 * i + g * 8, base[b][i], acc[b][2 * i],
+                           acc[b][2 * i + 1]);
+    }
+  }
+}
+
+// grid.y: shares of the channels.
+template <bool F16, int RB>
+__global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch) {
+  extern __shared__ u32x4 hL[];
+  __shared__ uint8_t lists[4][kWindow];
+  __shared__ float back[kWindow];
+  const int64_t t0 = (a.window + blockIdx.x / a.slots) * kWindow;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  uint8_t* list = lists[wave];
+  each_adapter(a, blockIdx.x % a.slots, index_of_lane(a, t0), a.out != a.base, list,
+               [&](int which, int count) {
+    if (which < 0) {  // rows without an adapter
+      const f32x4 none = {-0.f, -0.f, -0.f, -0.f};
+      for (int64_t c = ((int64_t)blockIdx.y * 4 + wave) * 64 + (lane & 7) * 8; c < a.N;
+           c += gridDim.y * 256)
+        for (int t = lane >> 3; t < count; t += 8)
+          store_piece<F16>(a, t0 + list[t], c, base_piece(a, t0 + list[t], c), none, none);
+      return;
+    }
+    stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
+    __syncthreads();
+    if (count <= 16) expand<F16, RB, 1>(a, t0, which, list, count, hL, pitch, back);
+    else expand<F16, RB, 4>(a, t0, which, list, count, hL, pitch, back);
+    __syncthreads();
+  });
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -325,17 +405,52 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // its own), fewer where windows fill the chip.
 int slots_of(int64_t T, int64_t n) {
   const int64_t windows = cdiv(T, kWindow);
-  int64_t s = std::min<int64_t>(std::min<int64_t>(kWindow, n), T);
-  while (s > 2 && windows * s > 1024) s /= 2;
-  return (int)std::max<int64_t>(1, s);
+  int64_t s = std::min<int64_t>(std::min<int64_t>(kWindow, n + 1), T);
+  while (s > 2 && windows * s > 512) s /= 2;
+  return (int)s;
+}
+// Workgroups that have an adapter's tokens, at least: a window's tokens are one request's
+// where there are many, and every token may have its own where there are few.
+int64_t busy_of(int64_t T, int64_t n) {
+  return std::max<int64_t>(cdiv(T, kWindow), T <= kWindow ? std::min(T, n) : 0);
 }
 
 // Shares of K: enough workgroups for the chip where there are few.
 int parts_of(int64_t T, int64_t K, int64_t n) {
-  const int64_t groups = cdiv(T, kWindow) * slots_of(T, n);
   int p = 1;
-  while (p < 8 && groups * p < 512 && K >= (int64_t)p * 2 * 512) p *= 2;
+  while (p < 8 && busy_of(T, n) * p < 512 && K >= (int64_t)p * 2 * 512) p *= 2;
   return p;
+}
+// Shares of the channels, of equally many rounds of 256.
+int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
+  const int64_t rounds = cdiv(N, 256);
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 2048 / busy_of(T, n)));
+  return cdiv(rounds, cdiv(rounds, shares));
+}
+
+template <bool F16, int RB>
+int launch_adapters(hipStream_t st, AdapterArgs& a) {
+  const int64_t windows = cdiv(a.T, kWindow), most = (1 << 20) / a.slots;
+  // a token's pieces in LDS, and one more against bank conflicts
+  const int pitch = (int)(a.R / 4) + 1;
+  const size_t lds = (size_t)kWindow * pitch * 16;
+  for (a.window = 0; a.window < windows; a.window += most) {
+    const unsigned groups = (unsigned)(std::min(windows - a.window, most) * a.slots);
+    hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st, a);
+    G2PTQ_LAUNCHED();
+    hipLaunchKernelGGL((adapter_expand_kernel<F16, RB>),
+                       dim3(groups, (unsigned)channel_shares(a.T, a.N, a.n)), dim3(256), lds, st,
+                       a, pitch);
+    G2PTQ_LAUNCHED();
+  }
+  return G2PTQ_OK;
+}
+
+template <bool F16>
+int adapters_by_rank(hipStream_t st, AdapterArgs& a) {
+  if (a.R <= 16) return launch_adapters<F16, 1>(st, a);
+  if (a.R <= 32) return launch_adapters<F16, 2>(st, a);
+  return launch_adapters<F16, 4>(st, a);
 }
 
 }  // namespace
@@ -388,18 +503,5 @@ extern "C" int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const 
   a.vx = aligned16(x) && ldx % 8 == 0;
   a.vo = aligned16(base) && aligned16(out) && ldb % 8 == 0 && ldo % 8 == 0;
   hipStream_t st = as_stream(stream);
-  const int64_t windows = cdiv(T, kWindow), most = (1 << 20) / a.slots;
-  for (a.window = 0; a.window < windows; a.window += most) {
-    const unsigned groups = (unsigned)(std::min(windows - a.window, most) * a.slots);
-    const dim3 shrink(groups, a.parts), expand(groups, (unsigned)cdiv(set->N, 256));
-    if (set->dtype == 0) {
-      hipLaunchKernelGGL((adapter_shrink_kernel<false>), shrink, dim3(256), 0, st, a);
-      hipLaunchKernelGGL((adapter_expand_kernel<false>), expand, dim3(256), 0, st, a);
-    } else {
-      hipLaunchKernelGGL((adapter_shrink_kernel<true>), shrink, dim3(256), 0, st, a);
-      hipLaunchKernelGGL((adapter_expand_kernel<true>), expand, dim3(256), 0, st, a);
-    }
-    G2PTQ_LAUNCHED();
-  }
-  return G2PTQ_OK;
+  return set->dtype == 0 ? adapters_by_rank<false>(st, a) : adapters_by_rank<true>(st, a);
 }
