@@ -68,6 +68,11 @@ class LowRankAdapters:
             for i, r in enumerate(self.ranks):
                 d[i, :r, :self.in_features] = down[i]
                 u[i, :self.out_features, :r] = up[i]
+            # the order in which the kernels' lanes take 16 bytes each: down by 16 ranks and 64
+            # columns (2 × 4 × 16 pieces: half of 16 columns, 16 columns, rank), up by 64 channels
+            # and 16 ranks (4 × 2 × 16: 16 channels, half of the ranks, channel)
+            d = d.view(n, R // 16, 16, -1, 4, 2, 8).permute(0, 1, 3, 5, 4, 2, 6).contiguous()
+            u = u.view(n, -1, 4, 16, R // 16, 2, 8).permute(0, 1, 4, 2, 5, 3, 6).contiguous()
         self._held = (d, u, torch.tensor(self.ranks, dtype=_I32, device=dev),
                       scales.expand(n).to(torch.float32).contiguous().to(dev),
                       torch.zeros(1, dtype=_I32, device=dev))

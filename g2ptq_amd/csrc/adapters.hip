@@ -30,7 +30,7 @@ struct AdapterArgs {
   int64_t ldx;
   const int32_t* index;
   int64_t T, K, N, n;
-  const uint16_t *down, *up;  // n × R × Kp and n × Np × R, zero where padded
+  const uint16_t *down, *up;  // n × R × Kp and n × Np × R in the products' order
   int64_t R, Kp, Np;
   const int32_t* rank;
   const float* scale;
@@ -41,7 +41,8 @@ struct AdapterArgs {
   uint16_t* out;
   int64_t ldo;
   int* flags;
-  bool vx, vo;                // rows of x, of base and out are 16-byte aligned
+  bool vx;                    // rows of x are 16-byte aligned
+  bool vo;                    // rows of base and out too, and whole pieces of eight
   int64_t window;             // the launch's first
 };
 
@@ -117,7 +118,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
     xrow[b] = a.x + (t0 + list[min(16 * b + n, count - 1)]) * a.ldx + g * 16;
 #pragma unroll
   for (int r = 0; r < RB; ++r)  // (blocks that the adapter lacks: the first again, not stored)
-    drow[r] = a.down + ((int64_t)which * a.R + r0 + (r < blocks ? 16 * r : 0) + n) * a.Kp + g * 16;
+    drow[r] = a.down + ((int64_t)which * a.R + r0 + (r < blocks ? 16 * r : 0)) * a.Kp + lane * 8;
   f32x4 acc[RB][TB];
 #pragma unroll
   for (int r = 0; r < RB; ++r)
@@ -138,7 +139,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int r = 0; r < RB; ++r) s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k + 8 * i);
+      for (int r = 0; r < RB; ++r) s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
       for (int b = 0; b < TB; ++b) s.x[b][i] = *reinterpret_cast<const u32x4*>(xrow[b] + k + 8 * i);
     }
@@ -164,7 +165,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int r = 0; r < RB; ++r)
-          s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k + 8 * i);
+          s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
         for (int b = 0; b < TB; ++b)
           s.x[b][i] = piece(xrow[b] + k + 8 * i, a.vx, a.K - k - g * 16 - 8 * i);
@@ -194,9 +195,10 @@ template <bool F16, int RB>
 __global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[4][RB * 4][64];
   __shared__ uint8_t lists[4][kWindow];
-  const int64_t t0 = (a.window + blockIdx.x / a.slots) * kWindow;
+  const uint32_t windows = gridDim.x / (uint32_t)a.slots, slot = blockIdx.x / windows;
+  const int64_t t0 = (a.window + blockIdx.x - slot * windows) * kWindow;
   uint8_t* list = lists[threadIdx.x >> 6];
-  each_adapter(a, blockIdx.x % a.slots, index_of_lane(a, t0), false, list,
+  each_adapter(a, slot, index_of_lane(a, t0), false, list,
                [&](int which, int count) {
     const int blocks = (a.rank[which] + 15) / 16;
     for (int r = 0; r < blocks; r += RB) {
@@ -206,27 +208,45 @@ __global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
   });
 }
 
+// The shares of eight ranks' sums, all loads under way together.
+template <int P>
+__device__ __forceinline__ void sum_parts(const float* p, int64_t next, f32x4 (&s)[2]) {
+  f32x4 v[P][2];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    v[i][0] = *reinterpret_cast<const f32x4*>(p + i * next);
+    v[i][1] = *reinterpret_cast<const f32x4*>(p + i * next + 4);
+  }
+  s[0] = v[0][0], s[1] = v[0][1];
+#pragma unroll
+  for (int i = 1; i < P; ++i) s[0] += v[i][0], s[1] += v[i][1];
+}
+
 // Eight ranks of a token's h from r on, scaled; zero behind the adapter's own (`left` of them:
 // a padded row's zeros times an infinity are no zeros).
 __device__ __forceinline__ void load_h(const AdapterArgs& a, int64_t t, int64_t r, int64_t left,
                                        float scale, float (&v)[8]) {
   const float* p = a.h + t * a.R + r;
-  f32x4 s[2] = {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
-  for (int i = 1; i < a.parts; ++i) {
-    p += a.T * a.R;
-    s[0] += *reinterpret_cast<const f32x4*>(p);
-    s[1] += *reinterpret_cast<const f32x4*>(p + 4);
-  }
+  const int64_t next = a.T * a.R;
+  f32x4 s[2];
+  if (a.parts == 8) sum_parts<8>(p, next, s);
+  else if (a.parts == 4) sum_parts<4>(p, next, s);
+  else if (a.parts == 2) sum_parts<2>(p, next, s);
+  else sum_parts<1>(p, next, s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < left ? s[i >> 2][i & 3] * scale : 0.f;
 }
 
-// Eight channels from c on of a token's row of the base, as they lie in memory.
+// Eight channels from c on of a token's row: out = base + add.  VEC: rows are 16-byte aligned
+// and whole pieces.
+template <bool VEC>
 __device__ __forceinline__ u32x4 base_piece(const AdapterArgs& a, int64_t t, int64_t c) {
   if (!a.base) return u32x4{0, 0, 0, 0};
-  return piece(a.base + t * a.ldb + c, a.vo, a.N - c);
+  // (channels behind the last: the first again, not stored)
+  if (VEC) return *reinterpret_cast<const u32x4*>(a.base + t * a.ldb + (c < a.N ? c : 0));
+  return piece(a.base + t * a.ldb + c, false, a.N - c);
 }
-template <bool F16>
+template <bool F16, bool VEC>
 __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int64_t c, u32x4 base,
                                             f32x4 lo, f32x4 hi) {
   const int64_t n = a.N - c;
@@ -235,14 +255,13 @@ __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float add = j < 4 ? lo[j & 3] : hi[j & 3];
-    // (−0 is the number that changes nothing: a base of −0 stays, and no base is +0)
     h[j] = narrow<F16>(widen<F16>((uint16_t)(base[j >> 1] >> (16 * (j & 1)))) + add);
   }
-  if (a.vo && n >= 8) {
+  if (VEC) {
     u32x4 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-    *reinterpret_cast<u32x4*>(o) = v;
+    if (n > 0) *reinterpret_cast<u32x4*>(o) = v;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -265,11 +284,12 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
     const int64_t token = t0 + list[min(t, count - 1)];
     float fit = 1.f;
     bool infinite = false;
+    float v[8];
+    if (l < pieces) load_h(a, token, l * 8, rank - l * 8, scale, v);
     if constexpr (F16) {
       uint32_t top = 0;
       for (int p = l; p < pieces; p += 8) {
-        float v[8];
-        load_h(a, token, p * 8, rank - p * 8, scale, v);
+        if (p != l) load_h(a, token, p * 8, rank - p * 8, scale, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       }
@@ -281,8 +301,8 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
       if (l == 0 && t < count) back[t] = __fdiv_rn(1.f, fit);
     }
     for (int p = l; p < pieces; p += 8) {
-      float v[8];
-      load_h(a, token, p * 8, rank - p * 8, scale, v);
+      // (ranks from 64 on, and then all of fp16's, are read again)
+      if (p != l || (F16 && pieces > 8)) load_h(a, token, p * 8, rank - p * 8, scale, v);
       u32x4 hi, lo;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -303,99 +323,132 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
   }
 }
 
-// 16·TB tokens × 64 channels at a time, channels × tokens: row m of block j is channel
-// 32·(j / 2) + 8·(m / 4) + 4·(j % 2) + m % 4, so that a lane ends with two pieces of eight
-// channels.  A step of 32 is 16 ranks twice: with h rounded, and with what that left out.
-// RB: blocks of 16 ranks whose weights are loaded together.
-template <bool F16, int RB, int TB>
+constexpr int kTurn = 17;  // 16-byte pieces of a token's 64 sums in LDS, one against bank conflicts
+
+// 16·TB tokens × 64 channels at a time, channels × tokens.  A step of 32 is 16 ranks twice:
+// with h rounded, and with what that left out.  The sums are turned in LDS so that eight lanes
+// read and write 128 consecutive bytes of a token's row.  A wave walks its channels, and for
+// each 64 the window's tokens; what comes next is loaded before what was computed is stored.
+// RB: blocks of 16 ranks whose weights are held together.
+template <bool F16, bool VEC, int RB, int TB>
 __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which,
-                                       const uint8_t* list, int count, const u32x4* hL, int pitch,
-                                       const float* back) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int blocks = (a.rank[which] + 15) / 16, chunks = (int)(a.Np / 64);
-  const uint16_t* urow =
-      a.up + ((int64_t)which * a.Np + (n >> 2) * 8 + (n & 3)) * a.R + (g & 1) * 8;
-  int64_t token[TB];
-  const u32x4* h[TB];
+                                       const uint8_t* list, int count, int chunk, int chunks,
+                                       u32x4* hL, int pitch, float* back, f32x4* turn) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, row = lane >> 3, col = lane & 7;
+  const int blocks = (a.rank[which] + 15) / 16;
+  // (the weights as they enter the product: per 64 channels and 16 ranks four pieces of 16
+  // channels × 2 halves of the ranks)
+  const uint16_t* up = a.up + (int64_t)which * a.Np * a.R + (lane & 31) * 8;
+  u32x4 w[RB][4], base[TB][2];
+  auto weights = [&](int chunk, int r0) {
+    const uint16_t* u = up + ((int64_t)chunk * (a.R / 16) + r0) * 1024;
 #pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    const int t = min(16 * b + n, count - 1);
-    token[b] = t0 + list[t];
-    h[b] = hL + t * pitch + g;
-  }
-  for (int chunk = blockIdx.y * 4 + wave; chunk < chunks; chunk += gridDim.y * 4) {
-    const int64_t c = (int64_t)chunk * 64;
-    u32x4 base[TB][2];
+    for (int r = 0; r < RB; ++r)
+      if (r0 + r < blocks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[r][j] = *reinterpret_cast<const u32x4*>(u + (r * 4 + j) * 256);
+  };
+  auto token = [&](int t) { return t0 + list[min(t, count - 1)]; };
+  auto bases = [&](int chunk, int from) {
 #pragma unroll
     for (int b = 0; b < TB; ++b)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) base[b][i] = base_piece(a, token[b], c + 32 * i + g * 8);
+      for (int i = 0; i < 2; ++i)
+        base[b][i] = base_piece<VEC>(a, token(from + 16 * b + 8 * i + row),
+                                     (int64_t)chunk * 64 + col * 8);
+  };
+  int from = 0;
+  const bool ahead = TB == 1;  // (few tokens) on their way while h is prepared
+  if (ahead && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
+  stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
+  __syncthreads();
+  if (!ahead && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
+  while (chunk < chunks) {
     f32x4 acc[TB][4];
 #pragma unroll
     for (int b = 0; b < TB; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[b][j] = f32x4{0, 0, 0, 0};
-    const uint16_t* u = urow + c * a.R;
     for (int r0 = 0; r0 < blocks; r0 += RB) {
-      u32x4 w[RB][4];
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        if (r0 + r < blocks)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[r][j] = *reinterpret_cast<const u32x4*>(u + (32 * (j >> 1) + 4 * (j & 1)) * a.R +
-                                                      (r0 + r) * 16);
+      if (blocks > RB) weights(chunk, r0);
 #pragma unroll
       for (int r = 0; r < RB; ++r)
         if (r0 + r < blocks)
 #pragma unroll
           for (int b = 0; b < TB; ++b) {
-            const u32x4 v = h[b][(r0 + r) * 4];
+            const u32x4 v = hL[min(from + 16 * b + n, count - 1) * pitch + (r0 + r) * 4 + g];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[b][j] = mfma<F16>(w[r][j], v, acc[b][j]);
           }
     }
+    u32x4 old[TB][2];
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) old[b][i] = base[b][i];
+    const int64_t c = (int64_t)chunk * 64 + col * 8;
+    const int those = from;
+    from += 16 * TB;
+    if (from >= count) {
+      from = 0, chunk += 4;
+      if (chunk < chunks && blocks <= RB) weights(chunk, 0);
+    }
+    if (chunk < chunks) bases(chunk, from);
 #pragma unroll
     for (int b = 0; b < TB; ++b) {
-      if (16 * b + n >= count) continue;
-      if (F16) {
-        const float f = back[16 * b + n];
+      if (those + 16 * b >= count) break;
+      const float f = F16 ? back[min(those + 16 * b + n, count - 1)] : 1.f;
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[b][j] *= f;
+      for (int j = 0; j < 4; ++j)  // lane (token n, channels 16j + 4g .. + 3)
+        turn[n * kTurn + j * 4 + g] = F16 ? acc[b][j] * f : acc[b][j];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = those + 16 * b + 8 * i + row;
+        const f32x4* p = turn + (8 * i + row) * kTurn + col * 2;
+        if (t < count) store_piece<F16, VEC>(a, t0 + list[t], c, old[b][i], p[0], p[1]);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (c + 32 * i + g * 8 < a.N)
-          store_piece<F16>(a, token[b], c + 32 * i + g * 8, base[b][i], acc[b][2 * i],
-                           acc[b][2 * i + 1]);
     }
   }
+  __syncthreads();
 }
 
-// grid.y: shares of the channels.
-template <bool F16, int RB>
-__global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch) {
+// A window's channels are shared by `shares` workgroups, each walking its own range.  Workgroups
+// that follow each other take the same range of neighbouring windows, so that its weights are
+// read from memory once, and the same slot: the first slots have the work where a window's
+// tokens share an adapter, and these are spread over the XCDs.
+template <bool F16, bool VEC, int RB>
+__global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch,
+                                                                int shares) {
   extern __shared__ u32x4 hL[];
   __shared__ uint8_t lists[4][kWindow];
   __shared__ float back[kWindow];
-  const int64_t t0 = (a.window + blockIdx.x / a.slots) * kWindow;
+  __shared__ f32x4 turns[4][16 * kTurn];
+  const uint32_t groups = gridDim.x / (uint32_t)shares;
+  const uint32_t share = blockIdx.x / groups, group = blockIdx.x - share * groups;
+  const uint32_t windows = groups / (uint32_t)a.slots, slot = group / windows;
+  const uint32_t window = group - slot * windows;
+  const int64_t t0 = (a.window + window) * kWindow;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int all = (int)(a.Np / 64), each = (all + 4 * shares - 1) / (4 * shares) * 4;
+  const int first = share * each + wave, last = min((int)(share + 1) * each, all);
   uint8_t* list = lists[wave];
-  each_adapter(a, blockIdx.x % a.slots, index_of_lane(a, t0), a.out != a.base, list,
-               [&](int which, int count) {
+  each_adapter(a, slot, index_of_lane(a, t0), a.out != a.base, list, [&](int which, int count) {
     if (which < 0) {  // rows without an adapter
+      // (−0 is the number that changes nothing: a base of −0 stays, and no base is +0)
       const f32x4 none = {-0.f, -0.f, -0.f, -0.f};
-      for (int64_t c = ((int64_t)blockIdx.y * 4 + wave) * 64 + (lane & 7) * 8; c < a.N;
-           c += gridDim.y * 256)
+      for (int64_t c = (int64_t)first * 64 + (lane & 7) * 8; c < min<int64_t>(a.N, last * 64);
+           c += 256)
         for (int t = lane >> 3; t < count; t += 8)
-          store_piece<F16>(a, t0 + list[t], c, base_piece(a, t0 + list[t], c), none, none);
+          store_piece<F16, VEC>(a, t0 + list[t], c, base_piece<VEC>(a, t0 + list[t], c), none, none);
       return;
     }
-    stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
-    __syncthreads();
-    if (count <= 16) expand<F16, RB, 1>(a, t0, which, list, count, hL, pitch, back);
-    else expand<F16, RB, 4>(a, t0, which, list, count, hL, pitch, back);
-    __syncthreads();
+    if (count <= 16) expand<F16, VEC, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back,
+                                            turns[wave]);
+    else expand<F16, VEC, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back,
+                                            turns[wave]);
   });
 }
 
@@ -418,19 +471,20 @@ int64_t busy_of(int64_t T, int64_t n) {
 // Shares of K: enough workgroups for the chip where there are few.
 int parts_of(int64_t T, int64_t K, int64_t n) {
   int p = 1;
-  while (p < 8 && busy_of(T, n) * p < 512 && K >= (int64_t)p * 2 * 512) p *= 2;
+  while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 2 * 512) p *= 2;
   return p;
 }
 // Shares of the channels, of equally many rounds of 256.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   const int64_t rounds = cdiv(N, 256);
-  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 2048 / busy_of(T, n)));
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / busy_of(T, n)));
   return cdiv(rounds, cdiv(rounds, shares));
 }
 
 template <bool F16, int RB>
 int launch_adapters(hipStream_t st, AdapterArgs& a) {
-  const int64_t windows = cdiv(a.T, kWindow), most = (1 << 20) / a.slots;
+  const int64_t shares = channel_shares(a.T, a.N, a.n);
+  const int64_t windows = cdiv(a.T, kWindow), most = (1 << 22) / (a.slots * shares);
   // a token's pieces in LDS, and one more against bank conflicts
   const int pitch = (int)(a.R / 4) + 1;
   const size_t lds = (size_t)kWindow * pitch * 16;
@@ -438,9 +492,13 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
     const unsigned groups = (unsigned)(std::min(windows - a.window, most) * a.slots);
     hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st, a);
     G2PTQ_LAUNCHED();
-    hipLaunchKernelGGL((adapter_expand_kernel<F16, RB>),
-                       dim3(groups, (unsigned)channel_shares(a.T, a.N, a.n)), dim3(256), lds, st,
-                       a, pitch);
+    const dim3 grid((unsigned)(groups * shares));
+    if (a.vo)
+      hipLaunchKernelGGL((adapter_expand_kernel<F16, true, RB>), grid, dim3(256), lds, st, a, pitch,
+                         (int)shares);
+    else
+      hipLaunchKernelGGL((adapter_expand_kernel<F16, false, RB>), grid, dim3(256), lds, st, a,
+                         pitch, (int)shares);
     G2PTQ_LAUNCHED();
   }
   return G2PTQ_OK;
@@ -501,7 +559,7 @@ extern "C" int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const 
   a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
   a.flags = set->flags;
   a.vx = aligned16(x) && ldx % 8 == 0;
-  a.vo = aligned16(base) && aligned16(out) && ldb % 8 == 0 && ldo % 8 == 0;
+  a.vo = aligned16(base) && aligned16(out) && ldb % 8 == 0 && ldo % 8 == 0 && a.N % 8 == 0;
   hipStream_t st = as_stream(stream);
   return set->dtype == 0 ? adapters_by_rank<false>(st, a) : adapters_by_rank<true>(st, a);
 }

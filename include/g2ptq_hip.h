@@ -554,9 +554,11 @@ int g2ptq_pages_release(void* stream, const g2ptq_page_tables* tables, const int
                         const int32_t* keep, int64_t B, void* ws, size_t ws_bytes);
 
 /* Low-rank adapters (the struct is host memory, its pointers device memory): n of up to R ranks
- * (a multiple of 16, at most 512).  down: n × R × K', up: n × N' × R of dtype (0 bf16, 1 fp16),
- * K' and N' the next multiples of 64, zero where padded, 16-byte aligned.  rank (n, 1 to R) and
- * scale (n).  flags: one int32. */
+ * (a multiple of 16, at most 512), of dtype 0 bf16 or 1 fp16, zero where padded, 16-byte aligned,
+ * in pieces of 8 values as the products take them, K' and N' the next multiples of 64:
+ *   down [n][R/16][K'/64][2][4][16][8]: rank 16b + m, column 64s + 16g + 8i + e at [b][s][i][g][m][e]
+ *   up   [n][N'/64][R/16][4][2][16][8]: channel 64c + 16j + m, rank 16b + 8p + e at [c][b][j][p][m][e]
+ * rank (n, 1 to R) and scale (n).  flags: one int32. */
 typedef struct g2ptq_adapter_set {
   const void* down;
   const void* up;
