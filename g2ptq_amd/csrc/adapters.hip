@@ -439,10 +439,17 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
     if (which < 0) {  // rows without an adapter
       // (−0 is the number that changes nothing: a base of −0 stays, and no base is +0)
       const f32x4 none = {-0.f, -0.f, -0.f, -0.f};
+      const int row = lane >> 3;
       for (int64_t c = (int64_t)first * 64 + (lane & 7) * 8; c < min<int64_t>(a.N, last * 64);
-           c += 256)
-        for (int t = lane >> 3; t < count; t += 8)
-          store_piece<F16, VEC>(a, t0 + list[t], c, base_piece<VEC>(a, t0 + list[t], c), none, none);
+           c += 256) {
+        u32x4 v[kWindow / 8];  // all loads under way together
+#pragma unroll
+        for (int i = 0; i < kWindow / 8; ++i)
+          if (8 * i < count) v[i] = base_piece<VEC>(a, t0 + list[min(8 * i + row, count - 1)], c);
+#pragma unroll
+        for (int i = 0; i < kWindow / 8; ++i)
+          if (8 * i + row < count) store_piece<F16, VEC>(a, t0 + list[8 * i + row], c, v[i], none, none);
+      }
       return;
     }
     if (count <= 16) expand<F16, VEC, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back,
