@@ -19,8 +19,9 @@
 namespace g2ptq {
 namespace {
 
-constexpr int kPlan = 1024;  // threads of the planning workgroup
-// Entries (tables' and tokens') that the planning workgroup fills by itself.
+constexpr int kPlan = 1024;   // threads of the planning workgroup, and requests of a round
+constexpr int kHash = 4096;   // places of a round's rows in LDS
+// Tables' entries and tokens that the planning workgroup fills by itself.
 constexpr int64_t kSmall = 16384;
 
 struct Tables {
@@ -33,9 +34,7 @@ struct Tables {
 // What a plan says of a request: its row (−1: none), its length before (−1: its tokens are
 // not placed), its pages before and after, the stack's place of its first page to move.
 struct Plan {
-  int32_t row, before;
-  int64_t place;
-  int32_t had, need;
+  int32_t row, before, had, need, place;
 };
 
 struct StepArgs {
@@ -46,48 +45,85 @@ struct StepArgs {
   int32_t* table;                // B × width
   int32_t *cu, *kv_lens;         // B + 1, B
   int64_t *slots, *positions;    // total
-  bool fill;                     // the planning workgroup fills too
+  int token_blocks;              // of the filling launch
 };
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int64_t u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
+// Sums that stay at 2^32 − 1 once they reach it: beyond every count and total, which are below 2^31.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  return __builtin_elementwise_add_sat(a, b);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+  return add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
+}
+// Inclusive sums over the wave: within 16 lanes, then the rows before.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = scan_step<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+  return scan_step<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
 }
 
-// Inclusive sums over the planning workgroup of two numbers each; all: their totals.
-__device__ __forceinline__ void group_scan(int64_t (&v)[2], int64_t (&all)[2],
-                                           int64_t (*lds)[kPlan / 64]) {
-  const int wave = threadIdx.x >> 6;
+struct Sums {
+  uint32_t v[2];
+};
+// Inclusive sums over the planning workgroup of two numbers each, on top of `before`; returns
+// the totals.
+__device__ __forceinline__ Sums group_scan(Sums& s, const Sums& before,
+                                           uint32_t (*lds)[kPlan / 64]) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  Sums all;
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    v[i] = wave_scan(v[i]);
-    if ((threadIdx.x & 63) == 63) lds[i][wave] = v[i];
+    s.v[i] = wave_scan(s.v[i]);
+    if (lane == 63) lds[i][wave] = s.v[i];
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int64_t sum = 0;
-    for (int w = 0; w < kPlan / 64; ++w) {
-      if (w == wave) v[i] += sum;
-      sum += lds[i][w];
-    }
-    all[i] = sum;
+    // (every wave sums the waves' totals: lane w has those up to wave w)
+    const uint32_t sums = wave_scan(lane < kPlan / 64 ? lds[i][lane] : 0u);
+    all.v[i] = add_sat(before.v[i],
+                       (uint32_t)__builtin_amdgcn_readlane((int)sums, kPlan / 64 - 1));
+    const uint32_t ahead =
+        wave ? (uint32_t)__builtin_amdgcn_readlane((int)sums, max(wave - 1, 0)) : 0u;
+    s.v[i] = add_sat(add_sat(s.v[i], ahead), before.v[i]);
   }
-  __syncthreads();
+  return all;
 }
 
-// Marks rows with the lowest request that names them, so that a row named twice counts once.
-// Marks are INT_MAX between calls.
+// A row named twice counts once, for the first request of the batch.  Up to kPlan requests meet
+// in LDS; more leave the lowest request that names a row in its mark (0x7fffffff between
+// calls).
+struct Rows {
+  int32_t key[kHash], first[kHash];
+};
+__device__ __forceinline__ uint32_t hash_of(int32_t row) {
+  return ((uint32_t)row * 2654435761u) >> 20;
+}
+__device__ __forceinline__ void clear_rows(Rows& r) {
+  for (int i = threadIdx.x; i < kHash; i += kPlan) r.key[i] = -1, r.first[i] = 0x7fffffff;
+}
+// The row's place.  (Ends: there are more places than rows.)
+__device__ __forceinline__ int enter_row(Rows& r, int32_t row, int32_t i) {
+  uint32_t h = hash_of(row);
+  for (;;) {
+    const int32_t was = atomicCAS(&r.key[h], -1, row);
+    if (was == -1 || was == row) break;
+    h = (h + 1) & (kHash - 1);
+  }
+  atomicMin(&r.first[h], i);
+  return (int)h;
+}
+__device__ __forceinline__ bool is_row(const StepArgs& a, int32_t row) {
+  return row >= 0 && row < a.s.seqs;
+}
 __device__ __forceinline__ void mark_rows(const StepArgs& a) {
-  for (int64_t i = threadIdx.x; i < a.B; i += kPlan) {
-    const int32_t row = a.rows[i];
-    if (row >= 0 && row < a.s.seqs) atomicMin(a.s.mark + row, (int32_t)i);
-  }
+  for (int64_t i = threadIdx.x; i < a.B; i += kPlan)
+    if (is_row(a, a.rows[i])) atomicMin(a.s.mark + a.rows[i], (int32_t)i);
   __threadfence();
   __syncthreads();
 }
@@ -97,189 +133,238 @@ __device__ __forceinline__ bool first_of_row(const StepArgs& a, int32_t row, int
 }
 __device__ __forceinline__ void unmark_rows(const StepArgs& a) {
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < a.B; i += kPlan) {
-    const int32_t row = a.rows[i];
-    if (row >= 0 && row < a.s.seqs)
-      __hip_atomic_store(a.s.mark + row, 0x7fffffff, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+  for (int64_t i = threadIdx.x; i < a.B; i += kPlan)
+    if (is_row(a, a.rows[i]))
+      __hip_atomic_store(a.s.mark + a.rows[i], 0x7fffffff, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
 }
 
 __device__ __forceinline__ int64_t pages_of(const Tables& s, int64_t n) {
   return (n + (1 << s.shift) - 1) >> s.shift;
 }
 
-// Entry `at` of the batch's tables.
-__device__ __forceinline__ void extend_entry(const StepArgs& a, int64_t at) {
-  const int64_t b = at / a.s.width, c = at - b * a.s.width;
-  const Plan p = a.plan[b];
-  int32_t page = -1;
-  if (p.row >= 0) {
-    if (c < p.had) page = a.s.table[p.row * a.s.width + c];
-    else if (c < p.need) {
-      page = a.s.free_pages[p.place - (c - p.had)];
-      a.s.table[p.row * a.s.width + c] = page;
-    }
-  }
-  a.table[at] = page;
+// The request's page of column c.
+__device__ __forceinline__ int32_t page_of(const StepArgs& a, const Plan& p, int64_t c) {
+  return c < p.had ? a.s.table[p.row * a.s.width + c] : a.s.free_pages[p.place - (c - p.had)];
 }
 
-// Token t's slot and position.
-__device__ __forceinline__ void extend_token(const StepArgs& a, int64_t t) {
+// A wave's part of request b's row of the batch's tables, and its new pages into its own row.
+__device__ __forceinline__ void extend_row(const StepArgs& a, int64_t b, const Plan& p, int lane) {
+  int32_t* out = a.table + b * a.s.width;
+  const int64_t end = p.row < 0 ? 0 : p.need;
+#pragma unroll 4
+  for (int64_t c = lane; c < a.s.width; c += 64) {
+    const int32_t page = c < end ? page_of(a, p, c) : -1;
+    if (c >= p.had && c < end) a.s.table[p.row * a.s.width + c] = page;
+    out[c] = page;
+  }
+}
+
+// Token t's slot and position.  cu: the requests' offsets.
+__device__ __forceinline__ void extend_token(const StepArgs& a, int64_t t, const int32_t* cu,
+                                             const Plan* plan) {
   int64_t slot = -1, position = 0;
-  if (t < a.cu[a.B]) {
-    int64_t lo = 0, hi = a.B - 1;  // the request with cu[b] <= t < cu[b + 1]
+  if (t < cu[a.B]) {
+    int lo = 0, hi = (int)a.B - 1;  // the request with cu[b] <= t < cu[b + 1]
     while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.cu[mid + 1] > t) hi = mid;
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid + 1] > t) hi = mid;
       else lo = mid + 1;
     }
-    const Plan p = a.plan[lo];
+    const Plan p = plan[lo];
     if (p.row >= 0 && p.before >= 0) {
-      position = p.before + (t - a.cu[lo]);
-      const int64_t c = position >> a.s.shift;
-      const int32_t page = c < p.had ? a.s.table[p.row * a.s.width + c]
-                                     : a.s.free_pages[p.place - (c - p.had)];
-      slot = ((int64_t)page << a.s.shift) + (position & ((1 << a.s.shift) - 1));
+      position = p.before + (t - cu[lo]);
+      slot = ((int64_t)page_of(a, p, position >> a.s.shift) << a.s.shift) +
+             (position & ((1 << a.s.shift) - 1));
     }
   }
   a.slots[t] = slot;
   a.positions[t] = position;
 }
 
+// One workgroup: rows and counts to plans.  ONE: up to kPlan requests, whose plans stay in LDS
+// where the workgroup fills too (FILL).  A step of few requests is a chain of four memory
+// latencies and a launch.
+template <bool ONE, bool FILL>
 __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
-  __shared__ int64_t lds[2][kPlan / 64];
-  mark_rows(a);
-  const int64_t count = *a.s.free_count;
-  int64_t tokens = 0, pages = 0, taken = 0;  // of the requests before this round's
+  static_assert(ONE || !FILL, "plans in LDS are of one round");
+  __shared__ uint32_t lds[2][kPlan / 64];
+  __shared__ Rows hashed;
+  __shared__ Plan planL[FILL ? kPlan : 1];
+  __shared__ int32_t cuL[FILL ? kPlan + 1 : 1];
+  __shared__ int taken;
+  if (threadIdx.x == 0) taken = 0;
+  const int32_t count = *a.s.free_count;
+  if (ONE) clear_rows(hashed);
+  else mark_rows(a);
+  Sums before_all = {{0, 0}};  // tokens and pages of the rounds before
   for (int64_t b0 = 0; b0 < a.B; b0 += kPlan) {
     const int64_t b = b0 + threadIdx.x;
-    int32_t row = -1, before = 0;
-    int64_t n = 0;
-    bool known = false, bad = false, full = false;
-    if (b < a.B) {
-      row = a.rows[b];
-      n = a.counts[b];
-      if (n < 0) n = 0, bad = true;
-      if (row >= a.s.seqs) bad = true;
-      else if (row >= 0) {
-        known = first_of_row(a, row, b);
-        bad |= !known;
-      }
-      if (known) before = a.s.lengths[row];
+    const bool on = b < a.B;
+    const int32_t row = on ? a.rows[b] : -1;
+    int64_t n = on ? a.counts[b] : 0;
+    const bool inside = is_row(a, row);
+    const int32_t held = inside ? a.s.lengths[row] : 0;
+    bool known = inside, bad = n < 0 || row >= a.s.seqs;
+    if (ONE) {
+      __syncthreads();
+      int place = 0;
+      if (inside) place = enter_row(hashed, row, (int32_t)b);
+      __syncthreads();
+      if (inside) known = hashed.first[place] == (int32_t)b;
+    } else if (inside) {
+      known = first_of_row(a, row, b);
     }
+    bad |= inside && !known;
+    n = n < 0 ? 0 : n;
+    const int64_t before = known ? held : 0;
     const int64_t had = pages_of(a.s, before), need = pages_of(a.s, before + n);
-    int64_t v[2] = {n, 0}, all[2];
-    group_scan(v, all, lds);
-    const int64_t start = tokens + v[0] - n;
-    // what the step's tokens or its own row have no room for is refused before pages are counted
-    const bool past = start + n > a.total && n > 0;
-    full = known && n > 0 && !past && need > a.s.width;
-    bool ok = known && n > 0 && !full && !past;
-    const int64_t last = tokens + all[0];
-    v[0] = 0, v[1] = ok ? need - had : 0;
-    group_scan(v, all, lds);
-    const int64_t before_pages = pages + v[1] - (ok ? need - had : 0);
-    if (ok && need > had && pages + v[1] > count) ok = false, full = true;
-    if (b < a.B) {
-      a.cu[b] = (int32_t)min(start, a.total);
+    const bool wide = known && n > 0 && need > a.s.width;
+    // A request whose tokens end past total is refused, and so are all later ones that have
+    // any: that their pages are counted changes nothing for those before.
+    Sums s = {{(uint32_t)n, known && n > 0 && !wide ? (uint32_t)(need - had) : 0u}};
+    const uint32_t mine = s.v[1];
+    const Sums all = group_scan(s, before_all, lds);
+    const bool past = n > 0 && s.v[0] > (uint32_t)a.total;
+    bool ok = known && n > 0 && !wide && !past;
+    const bool short_of = ok && mine > 0 && s.v[1] > (uint32_t)count;
+    ok = ok && !short_of;
+    if (on) {
+      const int32_t start = (int32_t)min(s.v[0] - (uint32_t)n, (uint32_t)a.total);
+      a.cu[b] = start;
       a.kv_lens[b] = known ? (int32_t)(before + (ok ? n : 0)) : 0;
       Plan p;
       p.row = known ? row : -1;
-      p.before = before;
-      p.place = count - 1 - before_pages;
+      p.before = known && n > 0 && !ok ? -1 : (int32_t)before;
       p.had = (int32_t)had, p.need = (int32_t)(ok ? need : had);
-      if (known && n > 0 && !ok) p.before = -1;
-      a.plan[b] = p;
+      p.place = (int32_t)(count - 1 - (int64_t)(s.v[1] - mine));
+      if (FILL) planL[threadIdx.x] = p, cuL[threadIdx.x] = start;
+      else a.plan[b] = p;
       if (ok) a.s.lengths[row] = (int32_t)(before + n);
-      if (bad || past) atomicOr(a.s.flags, G2PTQ_FLAG_BAD_INDEX);
-      if (full) atomicOr(a.s.flags, G2PTQ_FLAG_NO_ROOM);
+      // (those that get pages are the first that need any)
+      if (ok && mine) atomicMax(&taken, (int)s.v[1]);
+      const int flag = (bad || past ? G2PTQ_FLAG_BAD_INDEX : 0) |
+                       (short_of || (wide && !past) ? G2PTQ_FLAG_NO_ROOM : 0);
+      if (flag) atomicOr(a.s.flags, flag);
     }
-    tokens = last;
-    pages += all[1];
-    v[0] = 0, v[1] = ok ? need - had : 0;
-    group_scan(v, all, lds);
-    taken += all[1];
+    before_all = all;
   }
+  __syncthreads();
+  const int32_t tokens = (int32_t)min(before_all.v[0], (uint32_t)a.total);
   if (threadIdx.x == 0) {
-    a.cu[a.B] = (int32_t)min(tokens, a.total);
-    *a.s.free_count = (int32_t)(count - taken);
+    a.cu[a.B] = tokens;
+    *a.s.free_count = count - taken;
   }
-  unmark_rows(a);
-  if (a.fill) {
+  if (!ONE) unmark_rows(a);
+  if constexpr (FILL) {
+    if (threadIdx.x == 0) cuL[a.B] = tokens;
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < a.B * a.s.width; i += kPlan) extend_entry(a, i);
-    for (int64_t t = threadIdx.x; t < a.total; t += kPlan) extend_token(a, t);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int64_t t = threadIdx.x; t < a.total; t += kPlan) extend_token(a, t, cuL, planL);
+    for (int64_t b = wave; b < a.B; b += kPlan / 64) extend_row(a, b, planL[b], lane);
   }
 }
 
-__global__ __launch_bounds__(256) void extend_fill_kernel(StepArgs a, int64_t first) {
-  const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x, entries = a.B * a.s.width;
-  if (i < entries) extend_entry(a, i);
-  else if (i < entries + a.total) extend_token(a, i - entries);
+constexpr int kFillTokens = 1024;  // of a filling workgroup
+
+// The first token_blocks workgroups take tokens, the others four rows each.
+__global__ __launch_bounds__(256) void extend_fill_kernel(StepArgs a) {
+  __shared__ int32_t cuL[kPlan + 1];
+  const int64_t block = blockIdx.x;
+  if (block < a.token_blocks) {
+    const int32_t* cu = a.cu;
+    if (a.B <= kPlan) {
+      for (int i = threadIdx.x; i <= a.B; i += 256) cuL[i] = a.cu[i];
+      __syncthreads();
+      cu = cuL;
+    }
+#pragma unroll
+    for (int i = 0; i < kFillTokens / 256; ++i) {
+      const int64_t t = block * kFillTokens + i * 256 + threadIdx.x;
+      if (t < a.total) extend_token(a, t, cu, a.plan);
+    }
+    return;
+  }
+  const int64_t b = (block - a.token_blocks) * 4 + (threadIdx.x >> 6);
+  if (b < a.B) extend_row(a, b, a.plan[b], threadIdx.x & 63);
 }
 
-// Column c of request b's row, where its page goes back.
-__device__ __forceinline__ void release_entry(const StepArgs& a, int64_t at) {
-  const int64_t b = at / a.s.width, c = at - b * a.s.width;
-  const Plan p = a.plan[b];
-  if (p.row < 0 || c < p.need || c >= p.had) return;
-  int32_t* entry = a.s.table + p.row * a.s.width + c;
-  const int64_t place = p.place - (c - p.need);
-  if (place >= 0 && place < a.s.pages) a.s.free_pages[place] = *entry;
-  *entry = -1;
+// A wave's part of what request b gives back.
+__device__ __forceinline__ void release_row(const StepArgs& a, const Plan& p, int lane) {
+  if (p.row < 0) return;
+#pragma unroll 4
+  for (int64_t c = p.need + lane; c < p.had; c += 64) {
+    int32_t* entry = a.s.table + p.row * a.s.width + c;
+    const int64_t place = p.place - (c - p.need);
+    if (place >= 0 && place < a.s.pages) a.s.free_pages[place] = *entry;
+    *entry = -1;
+  }
 }
 
+template <bool ONE, bool FILL>
 __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
-  __shared__ int64_t lds[2][kPlan / 64];
-  mark_rows(a);
-  const int64_t count = *a.s.free_count;
-  int64_t pages = 0;  // of the requests before this round's
-  for (int round = 0; round < 2; ++round) {  // the number of all, then their places
-    const int64_t whole = pages;
-    pages = 0;
+  static_assert(ONE || !FILL, "plans in LDS are of one round");
+  __shared__ uint32_t lds[2][kPlan / 64];
+  __shared__ Rows hashed;
+  __shared__ Plan planL[FILL ? kPlan : 1];
+  const int32_t count = *a.s.free_count;
+  if (ONE) clear_rows(hashed);
+  else mark_rows(a);
+  Sums whole = {{0, 0}};
+  // the number of all pages first, then the requests' places (both known at once in one round)
+  for (int pass = ONE ? 1 : 0; pass < 2; ++pass) {
+    Sums before_all = {{0, 0}};
     for (int64_t b0 = 0; b0 < a.B; b0 += kPlan) {
       const int64_t b = b0 + threadIdx.x;
-      int32_t row = -1, before = 0;
-      int64_t keep = 0;
-      bool known = false, bad = false;
-      if (b < a.B) {
-        row = a.rows[b];
-        keep = a.counts ? a.counts[b] : 0;
-        if (row >= a.s.seqs) bad = true;
-        else if (row >= 0) {
-          known = first_of_row(a, row, b);
-          bad |= !known;
-        }
-        if (known) before = a.s.lengths[row];
-        if (known && (keep < 0 || keep > before)) known = false, bad = true;
+      const bool on = b < a.B;
+      const int32_t row = on ? a.rows[b] : -1;
+      const int32_t keep = on && a.counts ? a.counts[b] : 0;
+      const bool inside = is_row(a, row);
+      const int32_t held = inside ? a.s.lengths[row] : 0;
+      bool known = inside;
+      if (ONE) {
+        __syncthreads();
+        int place = 0;
+        if (inside) place = enter_row(hashed, row, (int32_t)b);
+        __syncthreads();
+        if (inside) known = hashed.first[place] == (int32_t)b;
+      } else if (inside) {
+        known = first_of_row(a, row, b);
       }
-      const int64_t had = known ? pages_of(a.s, before) : 0, kept = known ? pages_of(a.s, keep) : 0;
-      int64_t v[2] = {had - kept, 0}, all[2];
-      group_scan(v, all, lds);
-      if (round == 1 && b < a.B) {
+      const bool bad = row >= a.s.seqs || (inside && !known) ||
+                       (known && (keep < 0 || keep > held));
+      known = known && !bad;
+      const int32_t had = known ? (int32_t)pages_of(a.s, held) : 0;
+      const int32_t kept = known ? (int32_t)pages_of(a.s, keep) : 0;
+      Sums s = {{(uint32_t)(had - kept), 0}};
+      const Sums all = group_scan(s, before_all, lds);
+      if (ONE) whole = all;
+      if (pass == 1 && on) {
         Plan p;
         p.row = known ? row : -1;
-        p.before = before;
-        p.had = (int32_t)had, p.need = (int32_t)kept;
-        p.place = count + whole - 1 - (pages + v[0] - (had - kept));
-        a.plan[b] = p;
+        p.before = held, p.had = had, p.need = kept;
+        p.place = (int32_t)((int64_t)count + whole.v[0] - 1 - (s.v[0] - (had - kept)));
+        if (FILL) planL[threadIdx.x] = p;
+        else a.plan[b] = p;
         if (bad) atomicOr(a.s.flags, G2PTQ_FLAG_BAD_INDEX);
-        if (known) a.s.lengths[row] = (int32_t)keep;
+        if (known) a.s.lengths[row] = keep;
       }
-      pages += all[0];
+      before_all = all;
     }
+    if (pass == 0) whole = before_all;
   }
-  if (threadIdx.x == 0) *a.s.free_count = (int32_t)(count + pages);
-  unmark_rows(a);
-  if (a.fill) {
+  if (threadIdx.x == 0) *a.s.free_count = (int32_t)(count + whole.v[0]);
+  if (!ONE) unmark_rows(a);
+  if constexpr (FILL) {
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < a.B * a.s.width; i += kPlan) release_entry(a, i);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int64_t b = wave; b < a.B; b += kPlan / 64) release_row(a, planL[b], lane);
   }
 }
 
-__global__ __launch_bounds__(256) void release_fill_kernel(StepArgs a, int64_t first) {
-  const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < a.B * a.s.width) release_entry(a, i);
+__global__ __launch_bounds__(256) void release_fill_kernel(StepArgs a) {
+  const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b < a.B) release_row(a, a.plan[b], threadIdx.x & 63);
 }
 
 int check_tables(const char* who, const g2ptq_page_tables* t, int64_t B, const void* rows,
@@ -301,7 +386,7 @@ int check_tables(const char* who, const g2ptq_page_tables* t, int64_t B, const v
     set_error("%s: workspace of %zu bytes, %zu needed", who, ws_bytes, sizeof(Plan) * (size_t)B);
     return G2PTQ_ERR_WORKSPACE;
   }
-  G2PTQ_CHECK((reinterpret_cast<uintptr_t>(ws) & 7) == 0, "%s: workspace not 8-byte aligned", who);
+  G2PTQ_CHECK((reinterpret_cast<uintptr_t>(ws) & 3) == 0, "%s: workspace not 4-byte aligned", who);
   a.s = {t->table, t->lengths, t->free_pages, t->free_count, t->mark, t->flags,
          t->seqs, t->width, t->pages, __builtin_ctzll((unsigned long long)t->page)};
   a.B = B;
@@ -331,17 +416,21 @@ extern "C" int g2ptq_pages_extend(void* stream, const g2ptq_page_tables* tables,
               "pages_extend: null pointer");
   a.rows = rows, a.counts = counts, a.total = total;
   a.table = table, a.cu = cu, a.kv_lens = kv_lens, a.slots = slots, a.positions = positions;
-  const int64_t all = B * a.s.width + total;
-  a.fill = all <= kSmall;
   hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(extend_plan_kernel, dim3(1), dim3(kPlan), 0, st, a);
-  G2PTQ_LAUNCHED();
-  for (int64_t first = 0; !a.fill && first < all; first += kMaxGroups * 256) {
-    hipLaunchKernelGGL(extend_fill_kernel,
-                       dim3((unsigned)std::min(cdiv(all - first, 256), kMaxGroups)), dim3(256), 0,
-                       st, a, first);
+  if (B <= kPlan && B * a.s.width + total <= kSmall) {
+    hipLaunchKernelGGL((extend_plan_kernel<true, true>), dim3(1), dim3(kPlan), 0, st, a);
     G2PTQ_LAUNCHED();
+    return G2PTQ_OK;
   }
+  if (B <= kPlan)
+    hipLaunchKernelGGL((extend_plan_kernel<true, false>), dim3(1), dim3(kPlan), 0, st, a);
+  else
+    hipLaunchKernelGGL((extend_plan_kernel<false, false>), dim3(1), dim3(kPlan), 0, st, a);
+  G2PTQ_LAUNCHED();
+  a.token_blocks = (int)cdiv(total, kFillTokens);
+  hipLaunchKernelGGL(extend_fill_kernel, dim3((unsigned)(a.token_blocks + cdiv(B, 4))), dim3(256),
+                     0, st, a);
+  G2PTQ_LAUNCHED();
   return G2PTQ_OK;
 }
 
@@ -352,16 +441,18 @@ extern "C" int g2ptq_pages_release(void* stream, const g2ptq_page_tables* tables
   G2PTQ_TRY(check_tables("pages_release", tables, B, rows, ws, ws_bytes, a));
   if (B == 0) return G2PTQ_OK;
   a.rows = rows, a.counts = keep;
-  const int64_t all = B * a.s.width;
-  a.fill = all <= kSmall;
   hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(release_plan_kernel, dim3(1), dim3(kPlan), 0, st, a);
-  G2PTQ_LAUNCHED();
-  for (int64_t first = 0; !a.fill && first < all; first += kMaxGroups * 256) {
-    hipLaunchKernelGGL(release_fill_kernel,
-                       dim3((unsigned)std::min(cdiv(all - first, 256), kMaxGroups)), dim3(256), 0,
-                       st, a, first);
+  if (B <= kPlan && B * a.s.width <= kSmall) {
+    hipLaunchKernelGGL((release_plan_kernel<true, true>), dim3(1), dim3(kPlan), 0, st, a);
     G2PTQ_LAUNCHED();
+    return G2PTQ_OK;
   }
+  if (B <= kPlan)
+    hipLaunchKernelGGL((release_plan_kernel<true, false>), dim3(1), dim3(kPlan), 0, st, a);
+  else
+    hipLaunchKernelGGL((release_plan_kernel<false, false>), dim3(1), dim3(kPlan), 0, st, a);
+  G2PTQ_LAUNCHED();
+  hipLaunchKernelGGL(release_fill_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, a);
+  G2PTQ_LAUNCHED();
   return G2PTQ_OK;
 }

@@ -74,6 +74,22 @@ def dequantize_tokens(codes, scale, zero=None, dtype=torch.bfloat16):
     """What codes stand for, ``scale · (code − zero)`` in ``dtype``: the inverse of
     ``quantize_tokens``.  ``codes`` (..., K) int8; ``scale`` and ``zero`` (fp32; ``zero`` may be
     None) have their shape without the last dimension."""
+    here = codes.get_device()
+    # what is usual passes in one go (a call is a few microseconds); the rest is told apart
+    if (codes.dim() == 2 and codes.dtype is _I8 and codes.numel() and codes.stride(1) == 1
+            and dtype in _DTYPE_CODE and scale.dtype is _F32 and scale.shape == codes.shape[:1]
+            and scale.is_contiguous()
+            and here == scale.get_device() == torch._C._cuda_getDevice()
+            and not scale.requires_grad and _lib.forward_ad._current_level < 0
+            and (zero is None or (zero.dtype is _F32 and zero.shape == scale.shape
+                                  and zero.is_contiguous() and zero.get_device() == here
+                                  and not zero.requires_grad))):
+        rows, columns = codes.shape
+        out = torch.empty(rows, columns, dtype=dtype, device=codes.device)
+        _lib.call_fast("dequantize_tokens", _lib.current_stream(), codes.data_ptr(),
+                       codes.stride(0), scale.data_ptr(), None if zero is None else zero.data_ptr(),
+                       rows, columns, out.data_ptr(), _DTYPE_CODE[dtype])
+        return out
     if codes.dtype is not torch.int8 or codes.dim() == 0 \
             or not 1 <= codes.shape[-1] <= MAX_COLUMNS:
         raise ValueError(f"dequantize_tokens: codes of {codes.dtype} and shape "

@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from .int8_utils import _DTYPE_CODE, MAX_COLUMNS, _padded
 
+_F32, _CONTIGUOUS = torch.float32, torch.contiguous_format
 NormedTokens = namedtuple("NormedTokens", "codes scale zero values sum")
 
 
@@ -88,6 +89,23 @@ def _norm(x, weight, eps, residual, y, total, sym, codes, ldc, scale, zero, what
                        None if zero is None else zero.data_ptr())
 
 
+def _usual(x, weight, residual):
+    """Whether the arguments pass all checks in one go and lie as the kernel takes them (a call
+    is a few microseconds); what is not is looked at one by one."""
+    here = x.get_device()
+    return (x.numel() and x.is_contiguous() and x.dtype in _DTYPE_CODE
+            and weight.dtype in _DTYPE_CODE and weight.shape == x.shape[-1:]
+            and weight.is_contiguous()
+            and here == weight.get_device() == torch._C._cuda_getDevice()
+            and _lib.forward_ad._current_level < 0
+            and (residual is None or (residual.dtype is x.dtype and residual.shape == x.shape
+                                      and residual.is_contiguous()
+                                      and residual.get_device() == here))
+            and not (torch.is_grad_enabled()
+                     and (x.requires_grad or weight.requires_grad
+                          or (residual is not None and residual.requires_grad))))
+
+
 def rms_norm(x, weight, eps=1e-6, residual=None):
     """``y`` of every row of ``x`` (..., C; bf16, fp16 or fp32), in its type; with a
     ``residual`` (``x``'s shape and type) the pair ``(y, s)``.
@@ -95,9 +113,19 @@ def rms_norm(x, weight, eps=1e-6, residual=None):
     ``weight`` (C,) is bf16, fp16 or fp32.  Rows may be strided (a projection's heads).  ``y``
     is the norm of the sum before ``s`` is rounded.  A row of zeros is NaN with ``eps=0``; a
     NaN makes its row NaN."""
+    if x.is_cuda and _usual(x, weight, residual):
+        columns, code = x.shape[-1], _DTYPE_CODE[x.dtype]
+        y = torch.empty_like(x)
+        total = None if residual is None else torch.empty_like(x)
+        _lib.call_fast("rms_norm", _lib.current_stream(), x.data_ptr(), columns, 0,
+                       None if residual is None else residual.data_ptr(), columns, 0, code,
+                       weight.data_ptr(), _DTYPE_CODE[weight.dtype], x.numel() // columns, 1,
+                       columns, eps, y.data_ptr(), None if total is None else total.data_ptr(),
+                       True, None, 0, None, None)
+        return y if total is None else (y, total)
     _check(x, weight, eps, residual, "rms_norm")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=_CONTIGUOUS)
+    total = None if residual is None else torch.empty_like(x, memory_format=_CONTIGUOUS)
     _norm(x, weight, eps, residual, y, total, True, None, 0, None, None, "rms_norm")
     return y if residual is None else (y, total)
 
@@ -108,19 +136,30 @@ def rms_norm_quantize(x, weight, eps=1e-6, residual=None, sym=True, values=False
     ``codes``, ``scale`` and ``zero`` are what ``quantize_tokens`` would make of ``y`` before it
     is rounded to ``x``'s type (``zero`` is None with ``sym``); ``values`` is ``y`` in that type
     if it is asked for, ``sum`` is ``x + residual`` where there is one, else None."""
-    _check(x, weight, eps, residual, "rms_norm_quantize")
+    usual = x.is_cuda and _usual(x, weight, residual)
+    if not usual:
+        _check(x, weight, eps, residual, "rms_norm_quantize")
     lead, columns, dev = x.shape[:-1], x.shape[-1], x.device
     rows, ldc = x.numel() // columns, _padded(columns)
     codes = torch.empty(rows, ldc, dtype=torch.int8, device=dev)
-    scale = torch.empty(lead, dtype=torch.float32, device=dev)
-    zero = None if sym else torch.empty(lead, dtype=torch.float32, device=dev)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if values else None
-    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    _norm(x, weight, eps, residual, y, total, bool(sym), codes, ldc, scale, zero,
-          "rms_norm_quantize")
+    scale = torch.empty(rows, dtype=_F32, device=dev)
+    zero = None if sym else torch.empty(rows, dtype=_F32, device=dev)
+    y = torch.empty_like(x, memory_format=_CONTIGUOUS) if values else None
+    total = None if residual is None else torch.empty_like(x, memory_format=_CONTIGUOUS)
+    if usual:
+        _lib.call_fast("rms_norm", _lib.current_stream(), x.data_ptr(), columns, 0,
+                       None if residual is None else residual.data_ptr(), columns, 0,
+                       _DTYPE_CODE[x.dtype], weight.data_ptr(), _DTYPE_CODE[weight.dtype], rows, 1,
+                       columns, eps, None if y is None else y.data_ptr(),
+                       None if total is None else total.data_ptr(), bool(sym), codes.data_ptr(),
+                       ldc, scale.data_ptr(), None if zero is None else zero.data_ptr())
+    else:
+        _norm(x, weight, eps, residual, y, total, bool(sym), codes, ldc, scale, zero,
+              "rms_norm_quantize")
     # (views of the padded rows, as quantize_tokens gives them)
     if ldc != columns:
         codes = codes[:, :columns]
     if len(lead) != 1:
         codes = codes.unflatten(0, lead) if lead else codes[0]
+        scale, zero = scale.view(lead), None if zero is None else zero.view(lead)
     return NormedTokens(codes, scale, zero, y, total)

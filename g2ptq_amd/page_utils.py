@@ -91,24 +91,26 @@ class PageTables:
         (they keep their places in ``cu``) where the free pages or its row do not suffice, in
         the order of the batch, and where its row is none, came before in the batch, or its
         tokens end past ``total``."""
-        rows = self._index(rows, "rows")
-        new = self._index(new, "counts", rows)
-        B, total = rows.shape[0], int(total)
+        # what is usual passes in one go (a call is a few microseconds); the rest is told apart
+        if not (rows.dtype is new.dtype is _I32 and rows.dim() == 1 and rows.shape == new.shape
+                and rows.is_contiguous() and new.is_contiguous() and rows.shape[0] <= 1 << 20
+                and rows.get_device() == new.get_device() == self._device
+                and torch._C._cuda_getDevice() == self._device):
+            rows = self._index(rows, "rows")
+            new = self._index(new, "counts", rows)
+        B, total, width, dev = rows.shape[0], int(total), self.max_pages, self.device
         if not 0 <= total < 1 << 31:
             raise ValueError(f"PageTables: a step of {total} tokens")
-        width = self.max_pages
-        # one allocation each for the 32-bit and the 64-bit outputs, then views of them
-        i32 = torch.empty(B * width + 2 * B + 1, dtype=_I32, device=self.device)
-        i64 = torch.empty(2, total, dtype=_I64, device=self.device)
-        table, cu, kv_lens = i32.split((B * width, B + 1, B))
-        table = table.view(B, width)
-        slots, positions = i64.unbind()
+        # the workspace lies behind the offsets and lengths
         need = _lib.workspace_fast("pages_workspace", B)
-        ws = _lib.scratch(need, self.device) if need else None
+        table = torch.empty(B, width, dtype=_I32, device=dev)
+        small = torch.empty(2 * B + 1 + need // 4, dtype=_I32, device=dev)
+        slots, positions = torch.empty(2, total, dtype=_I64, device=dev).unbind()
+        cu, kv_lens, _ = small.split_with_sizes((B + 1, B, need // 4))
+        at = small.data_ptr()
         _lib.call_fast("pages_extend", _lib.current_stream(), self._address, rows.data_ptr(),
-                       new.data_ptr(), B, total, table.data_ptr(), cu.data_ptr(),
-                       kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                       None if ws is None else ws.data_ptr(), need)
+                       new.data_ptr(), B, total, table.data_ptr(), at, at + 4 * (B + 1),
+                       slots.data_ptr(), positions.data_ptr(), at + 4 * (2 * B + 1), need)
         return PageStep(table, cu, kv_lens, slots, positions)
 
     def release(self, rows, keep=None):
@@ -117,9 +119,14 @@ class PageTables:
         rows, leaves the stack as it was.  ``keep`` outside 0 to the request's length changes
         nothing and is flagged, as are rows that are none or come twice; negative rows are
         padding."""
-        rows = self._index(rows, "rows")
-        if keep is not None:
-            keep = self._index(keep, "counts", rows)
+        if not (rows.dtype is _I32 and rows.dim() == 1 and rows.is_contiguous()
+                and rows.shape[0] <= 1 << 20
+                and (keep is None or (keep.dtype is _I32 and keep.shape == rows.shape
+                                      and keep.is_contiguous()
+                                      and keep.get_device() == self._device))
+                and rows.get_device() == torch._C._cuda_getDevice() == self._device):
+            rows = self._index(rows, "rows")
+            keep = None if keep is None else self._index(keep, "counts", rows)
         B = rows.shape[0]
         if B:
             need = _lib.workspace_fast("pages_workspace", B)

@@ -23,6 +23,7 @@ import torch
 from . import _lib
 from .int8_utils import _DTYPE_CODE
 
+_CONTIGUOUS = torch.contiguous_format
 _FIELDS = {"linear": {"factor"}, "ntk": {"factor"},
            "yarn": {"factor", "original_positions", "beta_fast", "beta_slow", "attention_factor"},
            "bands": {"factor", "original_positions", "low_freq_factor", "high_freq_factor"}}
@@ -127,8 +128,8 @@ class Rotary:
                 and _lib.forward_ad._current_level < 0):
             q, k, positions = self._checked(q, k, positions)
         T = q.shape[0]
-        q_out = q.new_empty(q.shape)
-        k_out = None if k is None else k.new_empty(k.shape)
+        q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+        k_out = None if k is None else torch.empty_like(k, memory_format=_CONTIGUOUS)
         if T:
             (qt, qh, _), (kt, kh, _) = q.stride(), (0, 0, 0) if k is None else k.stride()
             _lib.call_fast("rotary", _lib.current_stream(), q.data_ptr(), qt, qh, q.shape[1],

@@ -540,7 +540,7 @@ typedef struct g2ptq_page_tables {
  * not placed, where the pages or its row do not suffice (G2PTQ_FLAG_NO_ROOM), where rows[i] is
  * no row, or named by an earlier request, or its tokens end past total (G2PTQ_FLAG_BAD_INDEX).
  * Negative rows are padding: not placed, not flagged.  Negative counts are flagged and count as
- * 0.  ws: g2ptq_pages_workspace(B), 8-byte aligned. */
+ * 0.  ws: g2ptq_pages_workspace(B), 4-byte aligned. */
 int g2ptq_pages_workspace(int64_t B, size_t* bytes);
 int g2ptq_pages_extend(void* stream, const g2ptq_page_tables* tables, const int32_t* rows,
                        const int32_t* counts, int64_t B, int64_t total, int32_t* table, int32_t* cu,
