@@ -160,13 +160,13 @@ __device__ __forceinline__ void extend_row(const StepArgs& a, int64_t b, const P
   }
 }
 
-// Token t's slot and position.  cu: the requests' offsets.
+// Token t's slot and position.  cu: the requests' offsets, the batch's tokens end at `end`; its
+// request is one of lo .. hi.
 __device__ __forceinline__ void extend_token(const StepArgs& a, int64_t t, const int32_t* cu,
-                                             const Plan* plan) {
+                                             const Plan* plan, int32_t end, int lo, int hi) {
   int64_t slot = -1, position = 0;
-  if (t < cu[a.B]) {
-    int lo = 0, hi = (int)a.B - 1;  // the request with cu[b] <= t < cu[b + 1]
-    while (lo < hi) {
+  if (t < end) {
+    while (lo < hi) {  // cu[lo] <= t < cu[lo + 1]
       const int mid = (lo + hi) >> 1;
       if (cu[mid + 1] > t) hi = mid;
       else lo = mid + 1;
@@ -260,33 +260,59 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
     if (threadIdx.x == 0) cuL[a.B] = tokens;
     __syncthreads();
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int64_t t = threadIdx.x; t < a.total; t += kPlan) extend_token(a, t, cuL, planL);
+    for (int64_t t = threadIdx.x; t < a.total; t += kPlan) extend_token(a, t, cuL, planL, tokens, 0, (int)a.B - 1);
     for (int64_t b = wave; b < a.B; b += kPlan / 64) extend_row(a, b, planL[b], lane);
   }
 }
 
 constexpr int kFillTokens = 1024;  // of a filling workgroup
+constexpr int kSpan = 256;         // of one of its waves
 
-// The first token_blocks workgroups take tokens, the others four rows each.
+// The first request b of B with cu[b + 1] > t, by the whole wave: 64 ranges a step.
+__device__ __forceinline__ int request_of(const int32_t* cu, int B, int64_t t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = B;
+  while (n > 1) {
+    const int stride = (n + 63) / 64;
+    const uint64_t past = __ballot(cu[lo + min((lane + 1) * stride, n)] > t);
+    const int k = past ? __builtin_ctzll(past) : (n - 1) / stride;
+    lo += k * stride, n = min(stride, n - k * stride);
+  }
+  return lo;
+}
+
+// The first token_blocks workgroups take tokens, the others four rows each.  A wave looks up
+// the requests of its first and last token; where several lie between, their offsets come into
+// LDS if they are few.
 __global__ __launch_bounds__(256) void extend_fill_kernel(StepArgs a) {
-  __shared__ int32_t cuL[kPlan + 1];
+  __shared__ int32_t cuL[4][kSpan + 2];
   const int64_t block = blockIdx.x;
-  if (block < a.token_blocks) {
-    const int32_t* cu = a.cu;
-    if (a.B <= kPlan) {
-      for (int i = threadIdx.x; i <= a.B; i += 256) cuL[i] = a.cu[i];
-      __syncthreads();
-      cu = cuL;
-    }
-#pragma unroll
-    for (int i = 0; i < kFillTokens / 256; ++i) {
-      const int64_t t = block * kFillTokens + i * 256 + threadIdx.x;
-      if (t < a.total) extend_token(a, t, cu, a.plan);
-    }
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (block >= a.token_blocks) {
+    const int64_t b = (block - a.token_blocks) * 4 + wave;
+    if (b < a.B) extend_row(a, b, a.plan[b], lane);
     return;
   }
-  const int64_t b = (block - a.token_blocks) * 4 + (threadIdx.x >> 6);
-  if (b < a.B) extend_row(a, b, a.plan[b], threadIdx.x & 63);
+  const int64_t t0 = block * kFillTokens + wave * kSpan;
+  const int32_t end = a.cu[a.B];
+  int lo = 0, more = 0;  // the first token's request, and how many further ones there are
+  if (t0 < end) {
+    lo = request_of(a.cu, (int)a.B, t0);
+    more = request_of(a.cu + lo, (int)a.B - lo, min<int64_t>(t0 + kSpan, end) - 1);
+  }
+  const int32_t* cu = a.cu + lo;  // (indices below are from this request on)
+  const bool few = more > 0 && more <= kSpan;
+  if (few) {
+    for (int i = lane; i <= more + 1; i += 64) cuL[wave][i] = cu[i];
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int i = 0; i < kSpan / 64; ++i) {
+    const int64_t t = t0 + i * 64 + lane;
+    if (t >= a.total) break;
+    if (few) extend_token(a, t, cuL[wave], a.plan + lo, end, 0, more);
+    else extend_token(a, t, cu, a.plan + lo, end, 0, more);
+  }
 }
 
 // A wave's part of what request b gives back.
