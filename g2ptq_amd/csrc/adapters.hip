@@ -237,16 +237,19 @@ __device__ __forceinline__ void load_h(const AdapterArgs& a, int64_t t, int64_t 
   for (int i = 0; i < 8; ++i) v[i] = i < left ? s[i >> 2][i & 3] * scale : 0.f;
 }
 
-// Eight channels from c on of a token's row: out = base + add.  VEC: rows are 16-byte aligned
-// and whole pieces.
-template <bool VEC>
+// Eight channels from c on of a token's row: out = base + add.  IO: kPieces where rows are
+// 16-byte aligned and whole pieces, kStream where the caches are to keep other data besides.
+enum : int { kElements, kPieces, kStream };
+template <int IO>
 __device__ __forceinline__ u32x4 base_piece(const AdapterArgs& a, int64_t t, int64_t c) {
   if (!a.base) return u32x4{0, 0, 0, 0};
   // (channels behind the last: the first again, not stored)
-  if (VEC) return *reinterpret_cast<const u32x4*>(a.base + t * a.ldb + (c < a.N ? c : 0));
+  const u32x4* p = reinterpret_cast<const u32x4*>(a.base + t * a.ldb + (c < a.N ? c : 0));
+  if (IO == kStream) return __builtin_nontemporal_load(p);
+  if (IO == kPieces) return *p;
   return piece(a.base + t * a.ldb + c, false, a.N - c);
 }
-template <bool F16, bool VEC>
+template <bool F16, int IO>
 __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int64_t c, u32x4 base,
                                             f32x4 lo, f32x4 hi) {
   const int64_t n = a.N - c;
@@ -257,11 +260,13 @@ __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int
     const float add = j < 4 ? lo[j & 3] : hi[j & 3];
     h[j] = narrow<F16>(widen<F16>((uint16_t)(base[j >> 1] >> (16 * (j & 1)))) + add);
   }
-  if (VEC) {
+  if (IO != kElements) {
     u32x4 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-    if (n > 0) *reinterpret_cast<u32x4*>(o) = v;
+    if (n <= 0) return;
+    if (IO == kStream) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(o));
+    else *reinterpret_cast<u32x4*>(o) = v;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -330,7 +335,7 @@ constexpr int kTurn = 17;  // 16-byte pieces of a token's 64 sums in LDS, one ag
 // read and write 128 consecutive bytes of a token's row.  A wave walks its channels, and for
 // each 64 the window's tokens; what comes next is loaded before what was computed is stored.
 // RB: blocks of 16 ranks whose weights are held together.
-template <bool F16, bool VEC, int RB, int TB>
+template <bool F16, int IO, int RB, int TB, bool AHEAD>
 __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which,
                                        const uint8_t* list, int count, int chunk, int chunks,
                                        u32x4* hL, int pitch, float* back, f32x4* turn) {
@@ -355,15 +360,15 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
     for (int b = 0; b < TB; ++b)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        base[b][i] = base_piece<VEC>(a, token(from + 16 * b + 8 * i + row),
+        base[b][i] = base_piece<IO>(a, token(from + 16 * b + 8 * i + row),
                                      (int64_t)chunk * 64 + col * 8);
   };
   int from = 0;
-  const bool ahead = TB == 1;  // (few tokens) on their way while h is prepared
-  if (ahead && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
+  // (AHEAD, for few tokens: on their way while h is prepared)
+  if (AHEAD && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
   stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
   __syncthreads();
-  if (!ahead && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
+  if (!AHEAD && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
   while (chunk < chunks) {
     f32x4 acc[TB][4];
 #pragma unroll
@@ -408,7 +413,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
       for (int i = 0; i < 2; ++i) {
         const int t = those + 16 * b + 8 * i + row;
         const f32x4* p = turn + (8 * i + row) * kTurn + col * 2;
-        if (t < count) store_piece<F16, VEC>(a, t0 + list[t], c, old[b][i], p[0], p[1]);
+        if (t < count) store_piece<F16, IO>(a, t0 + list[t], c, old[b][i], p[0], p[1]);
       }
     }
   }
@@ -419,7 +424,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
 // that follow each other take the same range of neighbouring windows, so that its weights are
 // read from memory once, and the same slot: the first slots have the work where a window's
 // tokens share an adapter, and these are spread over the XCDs.
-template <bool F16, bool VEC, int RB>
+template <bool F16, int IO, int RB, bool FEW>
 __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch,
                                                                 int shares) {
   extern __shared__ u32x4 hL[];
@@ -445,16 +450,16 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
         u32x4 v[kWindow / 8];  // all loads under way together
 #pragma unroll
         for (int i = 0; i < kWindow / 8; ++i)
-          if (8 * i < count) v[i] = base_piece<VEC>(a, t0 + list[min(8 * i + row, count - 1)], c);
+          if (8 * i < count) v[i] = base_piece<IO>(a, t0 + list[min(8 * i + row, count - 1)], c);
 #pragma unroll
         for (int i = 0; i < kWindow / 8; ++i)
-          if (8 * i + row < count) store_piece<F16, VEC>(a, t0 + list[8 * i + row], c, v[i], none, none);
+          if (8 * i + row < count) store_piece<F16, IO>(a, t0 + list[8 * i + row], c, v[i], none, none);
       }
       return;
     }
-    if (count <= 16) expand<F16, VEC, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back,
+    if (count <= 16) expand<F16, IO, RB, 1, FEW>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
-    else expand<F16, VEC, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back,
+    else expand<F16, IO, RB, 2, false>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
   });
 }
@@ -488,6 +493,10 @@ int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   return cdiv(rounds, cdiv(rounds, shares));
 }
 
+// Rows that no cache will hold are kept out of the caches.  MI355X, 5100 tokens × 14336 channels
+// (292 MB in and out), rank 64: 96 µs, and 92 so (x stays cached too: D·x 24 and 21 µs).
+bool streamed(const AdapterArgs& a) { return a.T * a.N >= 1 << 26; }
+
 template <bool F16, int RB>
 int launch_adapters(hipStream_t st, AdapterArgs& a) {
   const int64_t shares = channel_shares(a.T, a.N, a.n);
@@ -500,12 +509,14 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
     hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st, a);
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
-    if (a.vo)
-      hipLaunchKernelGGL((adapter_expand_kernel<F16, true, RB>), grid, dim3(256), lds, st, a, pitch,
-                         (int)shares);
-    else
-      hipLaunchKernelGGL((adapter_expand_kernel<F16, false, RB>), grid, dim3(256), lds, st, a,
-                         pitch, (int)shares);
+#define G2_EXPAND(IO, FEW)                                                                        \
+  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB, FEW>), grid, dim3(256), lds, st, a, pitch, \
+                     (int)shares)
+    if (windows == 1) { if (a.vo) G2_EXPAND(kPieces, true); else G2_EXPAND(kElements, true); }
+    else if (!a.vo) G2_EXPAND(kElements, false);
+    else if (streamed(a)) G2_EXPAND(kStream, false);
+    else G2_EXPAND(kPieces, false);
+#undef G2_EXPAND
     G2PTQ_LAUNCHED();
   }
   return G2PTQ_OK;
