@@ -459,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
     }
     if (count <= 16) expand<F16, IO, RB, 1, FEW>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
-    else expand<F16, IO, RB, 2, false>(a, t0, which, list, count, first, last, hL, pitch, back,
+    else expand<F16, IO, RB, 2, FEW>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
   });
 }
@@ -512,7 +512,7 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
 #define G2_EXPAND(IO, FEW)                                                                        \
   hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB, FEW>), grid, dim3(256), lds, st, a, pitch, \
                      (int)shares)
-    if (windows == 1) { if (a.vo) G2_EXPAND(kPieces, true); else G2_EXPAND(kElements, true); }
+    if (windows <= 32) { if (a.vo) G2_EXPAND(kPieces, true); else G2_EXPAND(kElements, true); }
     else if (!a.vo) G2_EXPAND(kElements, false);
     else if (streamed(a)) G2_EXPAND(kStream, false);
     else G2_EXPAND(kPieces, false);
