@@ -483,7 +483,7 @@ int64_t busy_of(int64_t T, int64_t n) {
 // Shares of K: enough workgroups for the chip where there are few.
 int parts_of(int64_t T, int64_t K, int64_t n) {
   int p = 1;
-  while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 2 * 512) p *= 2;
+  while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 512) p *= 2;
   return p;
 }
 // Shares of the channels, of equally many rounds of 256.
