@@ -281,11 +281,28 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int B, int64_t t) {
   return lo;
 }
 
-// The first token_blocks workgroups take tokens, the others four rows each.  A wave looks up
-// the requests of its first and last token; where several lie between, their offsets come into
-// LDS if they are few.
+// A wave's tokens from t0 on: the requests of the first and the last are looked up by the wave,
+// then each token's between them.  cu: the offsets of the batch.
+__device__ __forceinline__ void extend_span(const StepArgs& a, int64_t t0, int32_t end,
+                                            const int32_t* cu) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, more = 0;  // the first token's request, and how many further ones there are
+  if (t0 < end) {
+    lo = request_of(cu, (int)a.B, t0);
+    more = request_of(cu + lo, (int)a.B - lo, min<int64_t>(t0 + kSpan, end) - 1);
+  }
+#pragma unroll
+  for (int i = 0; i < kSpan / 64; ++i) {
+    const int64_t t = t0 + i * 64 + lane;
+    if (t < a.total) extend_token(a, t, cu + lo, a.plan + lo, end, 0, more);
+  }
+}
+
+// The first token_blocks workgroups take tokens, the others four rows each.  Offsets of up to
+// kPlan requests come into LDS, where they are looked through in a fraction of a memory's
+// latency.
 __global__ __launch_bounds__(256) void extend_fill_kernel(StepArgs a) {
-  __shared__ int32_t cuL[4][kSpan + 2];
+  __shared__ int32_t cuL[kPlan + 1];
   const int64_t block = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (block >= a.token_blocks) {
@@ -294,24 +311,15 @@ __global__ __launch_bounds__(256) void extend_fill_kernel(StepArgs a) {
     return;
   }
   const int64_t t0 = block * kFillTokens + wave * kSpan;
-  const int32_t end = a.cu[a.B];
-  int lo = 0, more = 0;  // the first token's request, and how many further ones there are
-  if (t0 < end) {
-    lo = request_of(a.cu, (int)a.B, t0);
-    more = request_of(a.cu + lo, (int)a.B - lo, min<int64_t>(t0 + kSpan, end) - 1);
-  }
-  const int32_t* cu = a.cu + lo;  // (indices below are from this request on)
-  const bool few = more > 0 && more <= kSpan;
-  if (few) {
-    for (int i = lane; i <= more + 1; i += 64) cuL[wave][i] = cu[i];
-    __builtin_amdgcn_wave_barrier();
-  }
+  if (a.B <= kPlan) {
 #pragma unroll
-  for (int i = 0; i < kSpan / 64; ++i) {
-    const int64_t t = t0 + i * 64 + lane;
-    if (t >= a.total) break;
-    if (few) extend_token(a, t, cuL[wave], a.plan + lo, end, 0, more);
-    else extend_token(a, t, cu, a.plan + lo, end, 0, more);
+    for (int i = 0; i < kPlan; i += 256)
+      if (i + (int)threadIdx.x <= a.B) cuL[i + threadIdx.x] = a.cu[i + threadIdx.x];
+    if (a.B == kPlan && threadIdx.x == 0) cuL[kPlan] = a.cu[kPlan];
+    __syncthreads();
+    extend_span(a, t0, cuL[a.B], cuL);
+  } else {
+    extend_span(a, t0, a.cu[a.B], a.cu);
   }
 }
 
