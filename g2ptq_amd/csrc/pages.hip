@@ -121,6 +121,13 @@ __device__ __forceinline__ int enter_row(Rows& r, int32_t row, int32_t i) {
 __device__ __forceinline__ bool is_row(const StepArgs& a, int32_t row) {
   return row >= 0 && row < a.s.seqs;
 }
+// (the state is the caller's memory: within its bounds whatever was written there)
+__device__ __forceinline__ int32_t free_pages(const StepArgs& a) {
+  return (int32_t)min<int64_t>(max(*a.s.free_count, 0), a.s.pages);
+}
+__device__ __forceinline__ int32_t length_of(const StepArgs& a, int32_t row) {
+  return (int32_t)min<int64_t>(max(a.s.lengths[row], 0), a.s.width << a.s.shift);
+}
 __device__ __forceinline__ void mark_rows(const StepArgs& a) {
   for (int64_t i = threadIdx.x; i < a.B; i += kPlan)
     if (is_row(a, a.rows[i])) atomicMin(a.s.mark + a.rows[i], (int32_t)i);
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
   __shared__ int32_t cuL[FILL ? kPlan + 1 : 1];
   __shared__ int taken;
   if (threadIdx.x == 0) taken = 0;
-  const int32_t count = *a.s.free_count;
+  const int32_t count = free_pages(a);
   if (ONE) clear_rows(hashed);
   else mark_rows(a);
   Sums before_all = {{0, 0}};  // tokens and pages of the rounds before
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
     const int32_t row = on ? a.rows[b] : -1;
     int64_t n = on ? a.counts[b] : 0;
     const bool inside = is_row(a, row);
-    const int32_t held = inside ? a.s.lengths[row] : 0;
+    const int32_t held = inside ? length_of(a, row) : 0;
     bool known = inside, bad = n < 0 || row >= a.s.seqs;
     if (ONE) {
       __syncthreads();
@@ -341,7 +348,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
   __shared__ uint32_t lds[2][kPlan / 64];
   __shared__ Rows hashed;
   __shared__ Plan planL[FILL ? kPlan : 1];
-  const int32_t count = *a.s.free_count;
+  const int32_t count = free_pages(a);
   if (ONE) clear_rows(hashed);
   else mark_rows(a);
   Sums whole = {{0, 0}};
@@ -354,7 +361,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
       const int32_t row = on ? a.rows[b] : -1;
       const int32_t keep = on && a.counts ? a.counts[b] : 0;
       const bool inside = is_row(a, row);
-      const int32_t held = inside ? a.s.lengths[row] : 0;
+      const int32_t held = inside ? length_of(a, row) : 0;
       bool known = inside;
       if (ONE) {
         __syncthreads();

@@ -94,7 +94,7 @@ def _usual(x, weight, residual):
     is a few microseconds); what is not is looked at one by one."""
     here = x.get_device()
     return (x.numel() and x.is_contiguous() and x.dtype in _DTYPE_CODE
-            and weight.dtype in _DTYPE_CODE and weight.shape == x.shape[-1:]
+            and weight.dtype in _DTYPE_CODE and x.dim() and weight.shape == x.shape[-1:]
             and weight.is_contiguous()
             and here == weight.get_device() == torch._C._cuda_getDevice()
             and _lib.forward_ad._current_level < 0

@@ -84,8 +84,9 @@ class Rotary:
     ``layout`` "half": channel i is paired with i + rotary_dim/2; "interleaved": 2i with 2i + 1.
     Channels from ``rotary_dim`` (default: all) on stay as they are.  ``frequencies`` (rotary_dim
     / 2 radians a position, any float type) and ``attention_factor`` take the place of ``base``
-    and ``scaling``.  Angles are computed from fp64 products, so any int64 position below 2^53
-    may come; nothing is tabulated."""
+    and ``scaling``.  Nothing is tabulated: angles are fp64 products less their whole turns, off by
+    some 2^-52 of position · θ, so that positions are not limited (up to 2^28 the fp32 sine and
+    cosine round more), and negative ones turn back."""
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout="half", scaling=None,
                  frequencies=None, attention_factor=None, device="cuda"):

@@ -87,6 +87,39 @@ def test_many_tokens(dev, T):
     s.run(T, "random")
 
 
+def test_rows_that_no_cache_holds(dev):
+    """From 2^26 outputs on rows are streamed past the caches: the same bits as in parts."""
+    T, N = 70000, 1000
+    s = Set(dev, [16, 40, 64, 9], N, 72, torch.bfloat16)
+    g = torch.Generator(dev).manual_seed(1)
+    x = torch.randn(T, 72, generator=g, device=dev).bfloat16()
+    base = torch.randn(T, N, generator=g, device=dev).bfloat16()
+    index = torch.arange(-1, 4, device=dev).repeat_interleave(T // 5).int()
+    index[:3000] = torch.randint(-1, 4, (3000,), generator=g, device=dev)
+    y = s.own(x, index, base=base)
+    z = base.clone()
+    s.own.add_(z, x, index)
+    assert_bitexact(z, y, "in place")
+    for at in range(0, T, 10000):
+        part = slice(at, at + 10000)
+        assert_bitexact(s.own(x[part], index[part], base=base[part]), y[part], f"rows from {at}")
+    s.check(y[-500:], x[-500:].cpu(), index[-500:].cpu(), base[-500:].cpu())
+
+
+def test_more_windows_than_a_launch_takes(dev):
+    """2^27 tokens and some: the last windows lie past the first launch."""
+    T = (1 << 27) + 100
+    s = Set(dev, [4], 8, 8, torch.float16)
+    x = torch.zeros(T, 8, dtype=torch.float16, device=dev)
+    index = torch.full((T,), -1, dtype=torch.int32, device=dev)
+    x[-70:], index[-70:] = s.x(70).to(dev), 0
+    y = s.own(x, index)
+    s.check(y[-70:], x[-70:].cpu(), index[-70:].cpu(), None)
+    assert not bool(y[:1 << 20].any()) and not bool(y[-(1 << 20):-70].any())
+    del x, y
+    torch.cuda.empty_cache()
+
+
 def test_tokens_do_not_depend_on_their_neighbours(dev):
     """A token's row has the same bits with other tokens around it, in any order."""
     s = Set(dev, [16, 24, 64], 200, 300, torch.bfloat16)

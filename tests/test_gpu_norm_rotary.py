@@ -188,6 +188,7 @@ def test_norm_refusals(dev):
                 (NotImplementedError, lambda: f(x.double(), w)), (ValueError, lambda: f(x, w[:7])),
                 (ValueError, lambda: f(x, w.double())), (ValueError, lambda: f(x, w, -1.0)),
                 (ValueError, lambda: f(x, w, float("nan"))), (RuntimeError, lambda: f(x.cpu(), w)),
+                (ValueError, lambda: f(x[0, 0], w[0])),
                 (RuntimeError, lambda: f(x, w.cpu())), (ValueError, lambda: f(x[:, :0], w[:0])),
                 (ValueError, lambda: f(x, w, residual=x[:2])),
                 (ValueError, lambda: f(x, w, residual=x.half())),

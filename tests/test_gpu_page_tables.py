@@ -238,3 +238,21 @@ def test_page_table_refusals(dev):
             call()
     with pytest.raises(AttributeError):
         t.table = i
+
+
+def test_overwritten_state_stays_within_its_memory(dev):
+    """Lengths and counts are the caller's to see; what no call can have left there is clamped."""
+    from g2ptq_amd import PageTables
+    t = PageTables(6, 8, 3, 4, device=dev)
+    rows = torch.arange(3, dtype=torch.int32, device=dev)
+    around = [x.clone() for x in t._held]
+    t.lengths.copy_(torch.tensor([2 ** 31 - 1, -5, 40], dtype=torch.int32))
+    t.free_count.fill_(1000)
+    s = t.extend(rows, torch.ones(3, dtype=torch.int32, device=dev), 3)
+    assert s.kv_lens.tolist() == [32, 1, 32] and s.slots.tolist()[::2] == [-1, -1]
+    assert int(s.slots[1]) == 0 and t.free_count.tolist() == [5]
+    t.release(rows)
+    assert t.lengths.tolist() == [0, 0, 0] and bool((t.table == -1).all())
+    assert 0 <= int(t.free_count) and [len(x) for x in t._held] == [len(x) for x in around]
+    with pytest.raises(RuntimeError):
+        t.check()

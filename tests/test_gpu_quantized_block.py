@@ -98,3 +98,34 @@ def test_a_request_does_not_depend_on_its_batch(dev, example):
         assert_bitexact(beside[1:], alone, f"token {i}")
     a.check()
     b.check()
+
+
+@torch.no_grad()
+def test_two_streams_at_once(dev, example):
+    """Two blocks served on a stream each: no workspace is shared."""
+    i32 = dict(dtype=torch.int32, device=dev)
+    rows, index = torch.tensor([5, 1], **i32), torch.tensor([0, 1], **i32)
+    g = gen(4)
+    steps = [[torch.randn(n, example.HIDDEN, generator=g).bfloat16().to(dev) for n in (130, 2, 2, 2)]
+             for _ in range(2)]
+    counts = [torch.tensor(n, **i32) for n in ([100, 30], [1, 1], [1, 1], [1, 1])]
+
+    def serve(block, xs):
+        return [block(x, rows, n, index.repeat_interleave(n.long(), output_size=len(x)))
+                for x, n in zip(xs, counts)]
+
+    want = [serve(_block(example, dev), xs) for xs in steps]
+    blocks = [_block(example, dev) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for i in range(4):
+        for b in range(2):
+            with torch.cuda.stream(streams[b]):
+                n = counts[i]
+                got[b].append(blocks[b](steps[b][i], rows, n, index.repeat_interleave(
+                    n.long(), output_size=len(steps[b][i]))))
+    torch.cuda.synchronize()
+    for b in range(2):
+        for i, (y, ref) in enumerate(zip(got[b], want[b])):
+            assert_bitexact(y, ref, f"stream {b} step {i}")
