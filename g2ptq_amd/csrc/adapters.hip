@@ -10,6 +10,12 @@
 //
 // Tokens are taken in windows of 64.  A window's adapters are found by comparing the index of
 // every lane (no sort, no launch of its own); each is multiplied with its own tokens only.
+//
+// Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight requests
+// with four adapters of ranks 32 and 64, 4096 to 14336: D·x 21 µs (its 42 MB of tokens at a copy's rate 8), U·h 90
+// (292 MB of rows in and out: 57; a launch that only copies them through the same mapping takes
+// some 70).  By latency where they are few: 48 tokens with 32 adapters of rank 16, 4096 × 4096,
+// 4.9 and 7.4 µs: index, adapter, operands and sums follow each other through memory.
 #include <algorithm>
 #include <type_traits>
 
@@ -335,7 +341,7 @@ constexpr int kTurn = 17;  // 16-byte pieces of a token's 64 sums in LDS, one ag
 // read and write 128 consecutive bytes of a token's row.  A wave walks its channels, and for
 // each 64 the window's tokens; what comes next is loaded before what was computed is stored.
 // RB: blocks of 16 ranks whose weights are held together.
-template <bool F16, int IO, int RB, int TB, bool AHEAD>
+template <bool F16, int IO, int RB, int TB>
 __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which,
                                        const uint8_t* list, int count, int chunk, int chunks,
                                        u32x4* hL, int pitch, float* back, f32x4* turn) {
@@ -364,11 +370,9 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
                                      (int64_t)chunk * 64 + col * 8);
   };
   int from = 0;
-  // (AHEAD, for few tokens: on their way while h is prepared)
-  if (AHEAD && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
   stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
   __syncthreads();
-  if (!AHEAD && chunk < chunks) weights(chunk, 0), bases(chunk, 0);
+  if (chunk < chunks) weights(chunk, 0), bases(chunk, 0);
   while (chunk < chunks) {
     f32x4 acc[TB][4];
 #pragma unroll
@@ -424,7 +428,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
 // that follow each other take the same range of neighbouring windows, so that its weights are
 // read from memory once, and the same slot: the first slots have the work where a window's
 // tokens share an adapter, and these are spread over the XCDs.
-template <bool F16, int IO, int RB, bool FEW>
+template <bool F16, int IO, int RB>
 __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch,
                                                                 int shares) {
   extern __shared__ u32x4 hL[];
@@ -457,21 +461,24 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
       }
       return;
     }
-    if (count <= 16) expand<F16, IO, RB, 1, FEW>(a, t0, which, list, count, first, last, hL, pitch, back,
+    if (count <= 16) expand<F16, IO, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
-    else expand<F16, IO, RB, 2, FEW>(a, t0, which, list, count, first, last, hL, pitch, back,
+    else expand<F16, IO, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back,
                                             turns[wave]);
   });
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Workgroups of a window: one adapter each where there are few windows (every token may have
-// its own), fewer where windows fill the chip.
+// Workgroups of a window: one for every adapter that it can hold where there are few windows
+// (every token may have its own), fewer where windows fill the chip and mostly hold one.
+// MI355X, 4096 × 4096, windows · slots up to 1024 against 512: 8192 tokens of four requests of
+// rank 16 54 and 60 µs, of rank 64 73 and 69, 2048 tokens of 40 adapters in any order 69 and 73;
+// one slot: 48 of 32 adapters 56 against 11, one request's 1024 18 and 20.
 int slots_of(int64_t T, int64_t n) {
   const int64_t windows = cdiv(T, kWindow);
   int64_t s = std::min<int64_t>(std::min<int64_t>(kWindow, n + 1), T);
-  while (s > 2 && windows * s > 512) s /= 2;
+  while (s > 2 && windows * s > 1024) s /= 2;
   return (int)s;
 }
 // Workgroups that have an adapter's tokens, at least: a window's tokens are one request's
@@ -480,21 +487,28 @@ int64_t busy_of(int64_t T, int64_t n) {
   return std::max<int64_t>(cdiv(T, kWindow), T <= kWindow ? std::min(T, n) : 0);
 }
 
-// Shares of K: enough workgroups for the chip where there are few.
+// Shares of K: enough workgroups for the chip where there are few, 128 columns a wave at least.
+// MI355X, 4096 × 4096, with and without: 64 tokens of 32 adapters 11 and 15 µs, 256 tokens 11 and
+// 19, 2048 of rank 64 37 and 55.  Up to 1024 workgroups instead of 256: 8192 of rank 64 73
+// against 69 (the second product reads every share).
 int parts_of(int64_t T, int64_t K, int64_t n) {
   int p = 1;
   while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 512) p *= 2;
   return p;
 }
-// Shares of the channels, of equally many rounds of 256.
+// Shares of the channels, of equally many rounds of 256.  Each prepares h again, so that they
+// are fewer where the windows may hold an adapter for every slot.  MI355X, 4096 channels, 2048
+// tokens of 40 adapters in any order 73 µs, 105 with a share for every 512 / windows; 8192 of
+// four requests 60 with 512 workgroups, 80 with 128 and 68 with 2048.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
-  const int64_t rounds = cdiv(N, 256);
-  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / busy_of(T, n)));
+  const int64_t rounds = cdiv(N, 256), windows = cdiv(T, kWindow);
+  const int64_t groups = std::max(busy_of(T, n), std::min<int64_t>(windows * std::min<int64_t>(n, kWindow), 128));
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / groups));
   return cdiv(rounds, cdiv(rounds, shares));
 }
 
 // Rows that no cache will hold are kept out of the caches.  MI355X, 5100 tokens × 14336 channels
-// (292 MB in and out), rank 64: 96 µs, and 92 so (x stays cached too: D·x 24 and 21 µs).
+// (292 MB in and out), rank 64: 92 µs, 96 without (x stays cached too: D·x 21 and 24 µs).
 bool streamed(const AdapterArgs& a) { return a.T * a.N >= 1 << 26; }
 
 template <bool F16, int RB>
@@ -509,13 +523,12 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
     hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st, a);
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
-#define G2_EXPAND(IO, FEW)                                                                        \
-  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB, FEW>), grid, dim3(256), lds, st, a, pitch, \
+#define G2_EXPAND(IO)                                                                           \
+  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB>), grid, dim3(256), lds, st, a, pitch, \
                      (int)shares)
-    if (windows <= 32) { if (a.vo) G2_EXPAND(kPieces, true); else G2_EXPAND(kElements, true); }
-    else if (!a.vo) G2_EXPAND(kElements, false);
-    else if (streamed(a)) G2_EXPAND(kStream, false);
-    else G2_EXPAND(kPieces, false);
+    if (!a.vo) G2_EXPAND(kElements);
+    else if (streamed(a)) G2_EXPAND(kStream);
+    else G2_EXPAND(kPieces);
 #undef G2_EXPAND
     G2PTQ_LAUNCHED();
   }

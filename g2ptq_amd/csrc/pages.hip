@@ -10,8 +10,14 @@
 //            first request's first page ends on top: releasing what an extend took, in the same
 //            order, restores the stack
 //
-// Everything is whole numbers; sums are 64 bits.  A request whose demand does not fit is left
-// as it was, and flagged.
+// Everything is whole numbers.  A request whose demand does not fit is left as it was, and
+// flagged.
+//
+// One workgroup plans (duplicates, sums over the requests, state), many fill the tables and the
+// tokens' slots.  Bound by latency: MI355X, under the profiler, 32 requests of one token each in
+// one launch 5.4–5.7 µs and 3.2–3.4 for its release; 700 requests of 717000 tokens in all 4.6–5.5 µs to
+// plan and 7.3–8.3 to fill (11.5 MB of slots and positions: 2.3 µs at a copy's rate), their release 2.6
+// and 3.2.
 #include <algorithm>
 
 #include "common.hpp"
@@ -19,9 +25,11 @@
 namespace g2ptq {
 namespace {
 
-constexpr int kPlan = 1024;   // threads of the planning workgroup, and requests of a round
-constexpr int kHash = 4096;   // places of a round's rows in LDS
-// Tables' entries and tokens that the planning workgroup fills by itself.
+constexpr int kPlan = 1024;  // threads of the planning workgroup, and requests of a round
+// Places in LDS of the rows of up to kPlan and of up to kMany requests.
+constexpr int kMany = 4096, kHash = 4 * kPlan, kLargeHash = 2 * kMany;
+// Requests, and tables' entries and tokens, that the planning workgroup fills by itself.
+constexpr int kFew = 64;
 constexpr int64_t kSmall = 16384;
 
 struct Tables {
@@ -95,25 +103,26 @@ __device__ __forceinline__ Sums group_scan(Sums& s, const Sums& before,
   return all;
 }
 
-// A row named twice counts once, for the first request of the batch.  Up to kPlan requests meet
-// in LDS; more leave the lowest request that names a row in its mark (0x7fffffff between
-// calls).
+// A row named twice counts once, for the first request of the batch.  Up to kMany requests meet
+// in LDS (HASH places); more leave the lowest request that names a row in its mark
+// (0x7fffffff between calls; HASH = 0).
+template <int HASH>
 struct Rows {
-  int32_t key[kHash], first[kHash];
+  int32_t key[HASH ? HASH : 1], first[HASH ? HASH : 1];
 };
-__device__ __forceinline__ uint32_t hash_of(int32_t row) {
-  return ((uint32_t)row * 2654435761u) >> 20;
-}
-__device__ __forceinline__ void clear_rows(Rows& r) {
-  for (int i = threadIdx.x; i < kHash; i += kPlan) r.key[i] = -1, r.first[i] = 0x7fffffff;
+template <int HASH>
+__device__ __forceinline__ void clear_rows(Rows<HASH>& r) {
+  for (int i = threadIdx.x; i < HASH; i += kPlan) r.key[i] = -1, r.first[i] = 0x7fffffff;
 }
 // The row's place.  (Ends: there are more places than rows.)
-__device__ __forceinline__ int enter_row(Rows& r, int32_t row, int32_t i) {
-  uint32_t h = hash_of(row);
+template <int HASH>
+__device__ __forceinline__ int enter_row(Rows<HASH>& r, int32_t row, int32_t i) {
+  static_assert((HASH & (HASH - 1)) == 0, "a power of two");
+  uint32_t h = ((uint32_t)row * 2654435761u >> 8) & (HASH - 1);
   for (;;) {
     const int32_t was = atomicCAS(&r.key[h], -1, row);
     if (was == -1 || was == row) break;
-    h = (h + 1) & (kHash - 1);
+    h = (h + 1) & (HASH - 1);
   }
   atomicMin(&r.first[h], i);
   return (int)h;
@@ -189,20 +198,20 @@ __device__ __forceinline__ void extend_token(const StepArgs& a, int64_t t, const
   a.positions[t] = position;
 }
 
-// One workgroup: rows and counts to plans.  ONE: up to kPlan requests, whose plans stay in LDS
-// where the workgroup fills too (FILL).  A step of few requests is a chain of four memory
+// One workgroup: rows and counts to plans.  FILL: up to kFew requests, whose plans stay in LDS and
+// whose entries the workgroup fills too.  A step of few requests is a chain of four memory
 // latencies and a launch.
-template <bool ONE, bool FILL>
+template <int HASH, bool FILL>
 __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
-  static_assert(ONE || !FILL, "plans in LDS are of one round");
+  static_assert(HASH || !FILL, "plans in LDS are of one round");
   __shared__ uint32_t lds[2][kPlan / 64];
-  __shared__ Rows hashed;
-  __shared__ Plan planL[FILL ? kPlan : 1];
-  __shared__ int32_t cuL[FILL ? kPlan + 1 : 1];
+  __shared__ Rows<HASH> hashed;
+  __shared__ Plan planL[FILL ? kFew : 1];
+  __shared__ int32_t cuL[FILL ? kFew + 1 : 1];
   __shared__ int taken;
   if (threadIdx.x == 0) taken = 0;
   const int32_t count = free_pages(a);
-  if (ONE) clear_rows(hashed);
+  if (HASH) clear_rows(hashed);
   else mark_rows(a);
   Sums before_all = {{0, 0}};  // tokens and pages of the rounds before
   for (int64_t b0 = 0; b0 < a.B; b0 += kPlan) {
@@ -213,7 +222,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
     const bool inside = is_row(a, row);
     const int32_t held = inside ? length_of(a, row) : 0;
     bool known = inside, bad = n < 0 || row >= a.s.seqs;
-    if (ONE) {
+    if constexpr (HASH > 0) {
       __syncthreads();
       int place = 0;
       if (inside) place = enter_row(hashed, row, (int32_t)b);
@@ -262,7 +271,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
     a.cu[a.B] = tokens;
     *a.s.free_count = count - taken;
   }
-  if (!ONE) unmark_rows(a);
+  if (!HASH) unmark_rows(a);
   if constexpr (FILL) {
     if (threadIdx.x == 0) cuL[a.B] = tokens;
     __syncthreads();
@@ -342,18 +351,19 @@ __device__ __forceinline__ void release_row(const StepArgs& a, const Plan& p, in
   }
 }
 
-template <bool ONE, bool FILL>
+template <int HASH, bool FILL>
 __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
-  static_assert(ONE || !FILL, "plans in LDS are of one round");
+  static_assert(HASH || !FILL, "plans in LDS are of one round");
   __shared__ uint32_t lds[2][kPlan / 64];
-  __shared__ Rows hashed;
-  __shared__ Plan planL[FILL ? kPlan : 1];
+  __shared__ Rows<HASH> hashed;
+  __shared__ Plan planL[FILL ? kFew : 1];
   const int32_t count = free_pages(a);
-  if (ONE) clear_rows(hashed);
+  if (HASH) clear_rows(hashed);
   else mark_rows(a);
   Sums whole = {{0, 0}};
   // the number of all pages first, then the requests' places (both known at once in one round)
-  for (int pass = ONE ? 1 : 0; pass < 2; ++pass) {
+  const bool one = a.B <= kPlan;
+  for (int pass = one ? 1 : 0; pass < 2; ++pass) {
     Sums before_all = {{0, 0}};
     for (int64_t b0 = 0; b0 < a.B; b0 += kPlan) {
       const int64_t b = b0 + threadIdx.x;
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
       const bool inside = is_row(a, row);
       const int32_t held = inside ? length_of(a, row) : 0;
       bool known = inside;
-      if (ONE) {
+      if constexpr (HASH > 0) {
         __syncthreads();
         int place = 0;
         if (inside) place = enter_row(hashed, row, (int32_t)b);
@@ -379,7 +389,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
       const int32_t kept = known ? (int32_t)pages_of(a.s, keep) : 0;
       Sums s = {{(uint32_t)(had - kept), 0}};
       const Sums all = group_scan(s, before_all, lds);
-      if (ONE) whole = all;
+      if (one) whole = all;
       if (pass == 1 && on) {
         Plan p;
         p.row = known ? row : -1;
@@ -395,7 +405,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(StepArgs a) {
     if (pass == 0) whole = before_all;
   }
   if (threadIdx.x == 0) *a.s.free_count = (int32_t)(count + whole.v[0]);
-  if (!ONE) unmark_rows(a);
+  if (!HASH) unmark_rows(a);
   if constexpr (FILL) {
     __syncthreads();
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -407,6 +417,12 @@ __global__ __launch_bounds__(256) void release_fill_kernel(StepArgs a) {
   const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (b < a.B) release_row(a, a.plan[b], threadIdx.x & 63);
 }
+
+// Whether the planning workgroup fills the entries too, which saves a launch.  MI355X, a step and
+// its release, one launch each against two: 32 requests of 129 pages 9.1 and 10.7 µs, 8 with
+// 2000 tokens each 8.5 and 9.8, 64 of 256 pages 12.8 and 12.1, 200 of 20 pages with 60 tokens
+// each 28.9 and 14.7.
+bool few(int64_t B, int64_t entries) { return B <= kFew && entries <= kSmall; }
 
 int check_tables(const char* who, const g2ptq_page_tables* t, int64_t B, const void* rows,
                  const void* ws, size_t ws_bytes, StepArgs& a) {
@@ -458,15 +474,17 @@ extern "C" int g2ptq_pages_extend(void* stream, const g2ptq_page_tables* tables,
   a.rows = rows, a.counts = counts, a.total = total;
   a.table = table, a.cu = cu, a.kv_lens = kv_lens, a.slots = slots, a.positions = positions;
   hipStream_t st = as_stream(stream);
-  if (B <= kPlan && B * a.s.width + total <= kSmall) {
-    hipLaunchKernelGGL((extend_plan_kernel<true, true>), dim3(1), dim3(kPlan), 0, st, a);
+  if (few(B, B * a.s.width + total)) {
+    hipLaunchKernelGGL((extend_plan_kernel<kHash, true>), dim3(1), dim3(kPlan), 0, st, a);
     G2PTQ_LAUNCHED();
     return G2PTQ_OK;
   }
   if (B <= kPlan)
-    hipLaunchKernelGGL((extend_plan_kernel<true, false>), dim3(1), dim3(kPlan), 0, st, a);
+    hipLaunchKernelGGL((extend_plan_kernel<kHash, false>), dim3(1), dim3(kPlan), 0, st, a);
+  else if (B <= kMany)
+    hipLaunchKernelGGL((extend_plan_kernel<kLargeHash, false>), dim3(1), dim3(kPlan), 0, st, a);
   else
-    hipLaunchKernelGGL((extend_plan_kernel<false, false>), dim3(1), dim3(kPlan), 0, st, a);
+    hipLaunchKernelGGL((extend_plan_kernel<0, false>), dim3(1), dim3(kPlan), 0, st, a);
   G2PTQ_LAUNCHED();
   a.token_blocks = (int)cdiv(total, kFillTokens);
   hipLaunchKernelGGL(extend_fill_kernel, dim3((unsigned)(a.token_blocks + cdiv(B, 4))), dim3(256),
@@ -483,15 +501,17 @@ extern "C" int g2ptq_pages_release(void* stream, const g2ptq_page_tables* tables
   if (B == 0) return G2PTQ_OK;
   a.rows = rows, a.counts = keep;
   hipStream_t st = as_stream(stream);
-  if (B <= kPlan && B * a.s.width <= kSmall) {
-    hipLaunchKernelGGL((release_plan_kernel<true, true>), dim3(1), dim3(kPlan), 0, st, a);
+  if (few(B, B * a.s.width)) {
+    hipLaunchKernelGGL((release_plan_kernel<kHash, true>), dim3(1), dim3(kPlan), 0, st, a);
     G2PTQ_LAUNCHED();
     return G2PTQ_OK;
   }
   if (B <= kPlan)
-    hipLaunchKernelGGL((release_plan_kernel<true, false>), dim3(1), dim3(kPlan), 0, st, a);
+    hipLaunchKernelGGL((release_plan_kernel<kHash, false>), dim3(1), dim3(kPlan), 0, st, a);
+  else if (B <= kMany)
+    hipLaunchKernelGGL((release_plan_kernel<kLargeHash, false>), dim3(1), dim3(kPlan), 0, st, a);
   else
-    hipLaunchKernelGGL((release_plan_kernel<false, false>), dim3(1), dim3(kPlan), 0, st, a);
+    hipLaunchKernelGGL((release_plan_kernel<0, false>), dim3(1), dim3(kPlan), 0, st, a);
   G2PTQ_LAUNCHED();
   hipLaunchKernelGGL(release_fill_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, a);
   G2PTQ_LAUNCHED();

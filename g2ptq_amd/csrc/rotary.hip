@@ -5,7 +5,7 @@
 //   pairs are channels (i, i + n/2) or (2i, 2i + 1) of the first n; the others stay
 //
 // p·f_i is a product of 64 bits, of which whole turns are dropped exactly: a position of 2^31
-// keeps 22 bits behind the point of a turn and more, where fp32 has none.  The angle's sine and cosine and the
+// keeps 24 bits of a turn and more, where fp32 has none.  The angle's sine and cosine and the
 // products are fp32, a result is rounded once to its type.
 #include <algorithm>
 
@@ -32,7 +32,9 @@ struct RotaryArgs {
 };
 
 // A workgroup takes `tokens` tokens: the sines and cosines of their pairs first, once for all
-// heads, then pieces of eight pairs (half layout: sixteen channels) or eight channels.
+// heads, then pieces of eight pairs (half layout: sixteen channels) or eight channels.  Bound by
+// the bytes: MI355X, 16384 tokens of 32 + 8 heads of 128, bf16, 66.6 µs (336 MB, 5.0 TB/s); one
+// token 3.1–3.4 µs, a launch and the latencies of position, angle and channels.
 template <int DT, bool HALF>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   __shared__ float cosL[kAngles], sinL[kAngles];
@@ -133,8 +135,13 @@ extern "C" int g2ptq_rotary(void* stream, const void* q, int64_t q_token, int64_
                a.sh[w] * e % 16 == 0;
   a.T = T, a.dim = (int)dim, a.n = (int)n;
   a.positions = positions, a.freq = freq, a.factor = factor;
-  int64_t tokens = std::min<int64_t>(kMaxTokens, kAngles / (n / 2));
-  while (tokens > 1 && cdiv(T, tokens) < 1024) tokens /= 2;
+  // As many tokens as a workgroup has threads for, mostly one.  MI355X, one token of 40 heads
+  // against eight: 16384 × 128 channels 66.7 and 67.7 µs, 2048 × 64 channels of which 32 turn 7.4
+  // and 8.4; sixteen 82.8 at the first.
+  const int64_t pieces = (interleaved ? cdiv(n, 8) : cdiv(n, 16)) + cdiv(dim - n, 8);
+  const int64_t tokens = std::max<int64_t>(
+      1, std::min<int64_t>(std::min<int64_t>(kMaxTokens, kAngles / (n / 2)),
+                           256 / (pieces * (q_heads + k_heads))));
   a.tokens = (int)tokens;
   hipStream_t st = as_stream(stream);
   for (a.first = 0; a.first < T; a.first += kMaxGroups * tokens) {

@@ -93,7 +93,7 @@ def test_random_steps(dev, seed):
         b.check()
 
 
-@pytest.mark.parametrize("B", [1, 63, 64, 65, 1023, 1024, 1025, 3000])
+@pytest.mark.parametrize("B", [1, 63, 64, 65, 1023, 1024, 1025, 3000, 4090, 4096, 4097, 5000])
 def test_batches_of_any_length(dev, B):
     r = random.Random(B)
     b = Both(dev, 4 * B + 10, 4, B + 7, 6)
