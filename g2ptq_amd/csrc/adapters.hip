@@ -502,7 +502,8 @@ int parts_of(int64_t T, int64_t K, int64_t n) {
 // four requests 60 with 512 workgroups, 80 with 128 and 68 with 2048.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   const int64_t rounds = cdiv(N, 256), windows = cdiv(T, kWindow);
-  const int64_t groups = std::max(busy_of(T, n), std::min<int64_t>(windows * std::min<int64_t>(n, kWindow), 128));
+  const int64_t most = std::min<int64_t>(windows * std::min<int64_t>(n, kWindow), 85);
+  const int64_t groups = std::max(busy_of(T, n), most);
   const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / groups));
   return cdiv(rounds, cdiv(rounds, shares));
 }
