@@ -87,11 +87,13 @@ template <typename F>
 __device__ __forceinline__ void each_adapter(const AdapterArgs& a, int slot, int32_t idx,
                                              bool none, uint8_t* list, F f) {
   const int lane = threadIdx.x & 63;
-  for (int first = slot; first < kWindow; first += a.slots) {
+  uint64_t lanes = __ballot(idx >= (none ? -1 : 0) && lane % a.slots == slot);
+  while (lanes) {
+    const int first = __builtin_ctzll(lanes);
     const int32_t which = __builtin_amdgcn_readlane(idx, first);
-    if (which < (none ? -1 : 0)) continue;
     const uint64_t same = __ballot(idx == which);
-    if (__builtin_ctzll(same) != first) continue;
+    lanes &= ~same;
+    if (__builtin_ctzll(same) != first) continue;  // another slot's
     __builtin_amdgcn_wave_barrier();
     if (idx == which) list[__popcll(same & ((1ull << lane) - 1))] = (uint8_t)lane;
     __builtin_amdgcn_wave_barrier();
@@ -470,14 +472,15 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Workgroups of a window: one for every adapter that it can hold where there are few windows
-// (every token may have its own), fewer where windows fill the chip and mostly hold one.
+// Workgroups of a window: one for every token of a single window (each may have its own adapter),
+// one for every adapter of a few, fewer where windows fill the chip and mostly hold one.
 // MI355X, 4096 × 4096, windows · slots up to 1024 against 512: 8192 tokens of four requests of
 // rank 16 54 and 60 µs, of rank 64 73 and 69, 2048 tokens of 40 adapters in any order 69 and 73;
 // one slot: 48 of 32 adapters 56 against 11, one request's 1024 18 and 20.
 int slots_of(int64_t T, int64_t n) {
   const int64_t windows = cdiv(T, kWindow);
-  int64_t s = std::min<int64_t>(std::min<int64_t>(kWindow, n + 1), T);
+  if (windows == 1) return (int)T;
+  int64_t s = std::min<int64_t>(kWindow, n + 1);
   while (s > 2 && windows * s > 1024) s /= 2;
   return (int)s;
 }
