@@ -11,11 +11,12 @@
 // Tokens are taken in windows of 64.  A window's adapters are found by comparing the index of
 // every lane (no sort, no launch of its own); each is multiplied with its own tokens only.
 //
-// Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight requests
-// with four adapters of ranks 32 and 64, 4096 to 14336: D·x 21 µs (its 42 MB of tokens at a copy's rate 8), U·h 90
-// (292 MB of rows in and out: 57; a launch that only copies them through the same mapping takes
-// some 70).  By latency where they are few: 48 tokens with 32 adapters of rank 16, 4096 × 4096,
-// 4.9 and 7.4 µs: index, adapter, operands and sums follow each other through memory.
+// Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight
+// requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 17–21 µs (its 42 MB of
+// tokens at a copy's rate 8), U·h 80–91 (292 MB of rows in and out: 57; a launch that only copies
+// them through the same mapping takes some 70).  By latency where they are few: 48 tokens with
+// 32 adapters of rank 16, 4096 × 4096, 4.0–4.3 and 6.1–6.5 µs: index, adapter, operands and sums
+// follow each other through memory.
 #include <algorithm>
 #include <type_traits>
 
@@ -147,7 +148,8 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int r = 0; r < RB; ++r) s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
+      for (int r = 0; r < RB; ++r)
+        s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
       for (int b = 0; b < TB; ++b) s.x[b][i] = *reinterpret_cast<const u32x4*>(xrow[b] + k + 8 * i);
     }
@@ -206,12 +208,12 @@ __global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
   const uint32_t windows = gridDim.x / (uint32_t)a.slots, slot = blockIdx.x / windows;
   const int64_t t0 = (a.window + blockIdx.x - slot * windows) * kWindow;
   uint8_t* list = lists[threadIdx.x >> 6];
-  each_adapter(a, slot, index_of_lane(a, t0), false, list,
-               [&](int which, int count) {
+  each_adapter(a, slot, index_of_lane(a, t0), false, list, [&](int which, int count) {
     const int blocks = (a.rank[which] + 15) / 16;
     for (int r = 0; r < blocks; r += RB) {
-      if (count <= 16) shrink<F16, RB, 1>(a, t0, which, r * 16, min(RB, blocks - r), list, count, sums);
-      else shrink<F16, RB, 4>(a, t0, which, r * 16, min(RB, blocks - r), list, count, sums);
+      const int here = min(RB, blocks - r);
+      if (count <= 16) shrink<F16, RB, 1>(a, t0, which, r * 16, here, list, count, sums);
+      else shrink<F16, RB, 4>(a, t0, which, r * 16, here, list, count, sums);
     }
   });
 }
@@ -336,7 +338,8 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
   }
 }
 
-constexpr int kTurn = 17;  // 16-byte pieces of a token's 64 sums in LDS, one against bank conflicts
+// 16-byte pieces of a token's 64 sums in LDS, one of them against bank conflicts.
+constexpr int kTurn = 17;
 
 // 16·TB tokens × 64 channels at a time, channels × tokens.  A step of 32 is 16 ranks twice:
 // with h rounded, and with what that left out.  The sums are turned in LDS so that eight lanes
@@ -459,14 +462,16 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, i
           if (8 * i < count) v[i] = base_piece<IO>(a, t0 + list[min(8 * i + row, count - 1)], c);
 #pragma unroll
         for (int i = 0; i < kWindow / 8; ++i)
-          if (8 * i + row < count) store_piece<F16, IO>(a, t0 + list[8 * i + row], c, v[i], none, none);
+          if (8 * i + row < count)
+            store_piece<F16, IO>(a, t0 + list[8 * i + row], c, v[i], none, none);
       }
       return;
     }
-    if (count <= 16) expand<F16, IO, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back,
-                                            turns[wave]);
-    else expand<F16, IO, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back,
-                                            turns[wave]);
+    f32x4* turn = turns[wave];
+    if (count <= 16)
+      expand<F16, IO, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
+    else
+      expand<F16, IO, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
   });
 }
 
@@ -476,7 +481,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // one for every adapter of a few, fewer where windows fill the chip and mostly hold one.
 // MI355X, 4096 × 4096, windows · slots up to 1024 against 512: 8192 tokens of four requests of
 // rank 16 54 and 60 µs, of rank 64 73 and 69, 2048 tokens of 40 adapters in any order 69 and 73;
-// one slot: 48 of 32 adapters 56 against 11, one request's 1024 18 and 20.
+// one slot: 64 tokens of 32 adapters 56 against 11, 1024 of four requests 18 and 20.
 int slots_of(int64_t T, int64_t n) {
   const int64_t windows = cdiv(T, kWindow);
   if (windows == 1) return (int)T;
@@ -524,7 +529,8 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
   const size_t lds = (size_t)kWindow * pitch * 16;
   for (a.window = 0; a.window < windows; a.window += most) {
     const unsigned groups = (unsigned)(std::min(windows - a.window, most) * a.slots);
-    hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st,
+                       a);
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
 #define G2_EXPAND(IO)                                                                           \

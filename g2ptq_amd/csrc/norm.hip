@@ -311,9 +311,12 @@ extern "C" int g2ptq_dequantize_tokens(void* stream, const int8_t* codes, int64_
   a.vo = aligned16(out) && K * (dtype == 2 ? 4 : 2) % 16 == 0;
   a.shift = l.shift;
   hipStream_t st = as_stream(stream);
-  if (dtype == 0) hipLaunchKernelGGL((dequantize_tokens_kernel<0>), l.grid, dim3(256), 0, st, a);
-  else if (dtype == 1) hipLaunchKernelGGL((dequantize_tokens_kernel<1>), l.grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((dequantize_tokens_kernel<2>), l.grid, dim3(256), 0, st, a);
+#define G2_DQ(DT) \
+  hipLaunchKernelGGL((dequantize_tokens_kernel<DT>), l.grid, dim3(256), 0, st, a)
+  if (dtype == 0) G2_DQ(0);
+  else if (dtype == 1) G2_DQ(1);
+  else G2_DQ(2);
+#undef G2_DQ
   G2PTQ_LAUNCHED();
   return G2PTQ_OK;
 }

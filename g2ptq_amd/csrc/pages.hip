@@ -15,9 +15,9 @@
 //
 // One workgroup plans (duplicates, sums over the requests, state), many fill the tables and the
 // tokens' slots.  Bound by latency: MI355X, under the profiler, 32 requests of one token each in
-// one launch 5.4–5.7 µs and 3.2–3.4 for its release; 700 requests of 717000 tokens in all 4.6–5.5 µs to
-// plan and 7.3–8.3 to fill (11.5 MB of slots and positions: 2.3 µs at a copy's rate), their release 2.6
-// and 3.2.
+// one launch 5.7–5.9 µs and 3.4–3.6 for its release; 700 requests of 717000 tokens in all 4.6–5.3
+// to plan and 6.9–8.5 to fill (11.5 MB of slots and positions: 2.3 µs at a copy's rate), their
+// release 2.8–2.9 and 3.1–3.4.
 #include <algorithm>
 
 #include "common.hpp"
@@ -56,7 +56,8 @@ struct StepArgs {
   int token_blocks;              // of the filling launch
 };
 
-// Sums that stay at 2^32 − 1 once they reach it: beyond every count and total, which are below 2^31.
+// Sums that stay at 2^32 − 1 once they reach it: beyond every count and total, which are below
+// 2^31.
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
   return __builtin_elementwise_add_sat(a, b);
 }
@@ -176,7 +177,7 @@ __device__ __forceinline__ void extend_row(const StepArgs& a, int64_t b, const P
   }
 }
 
-// Token t's slot and position.  cu: the requests' offsets, the batch's tokens end at `end`; its
+// Token t's slot and position.  cu: the requests' offsets; the batch's tokens end at `end`; its
 // request is one of lo .. hi.
 __device__ __forceinline__ void extend_token(const StepArgs& a, int64_t t, const int32_t* cu,
                                              const Plan* plan, int32_t end, int lo, int hi) {
@@ -276,7 +277,8 @@ __global__ __launch_bounds__(kPlan) void extend_plan_kernel(StepArgs a) {
     if (threadIdx.x == 0) cuL[a.B] = tokens;
     __syncthreads();
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int64_t t = threadIdx.x; t < a.total; t += kPlan) extend_token(a, t, cuL, planL, tokens, 0, (int)a.B - 1);
+    for (int64_t t = threadIdx.x; t < a.total; t += kPlan)
+      extend_token(a, t, cuL, planL, tokens, 0, (int)a.B - 1);
     for (int64_t b = wave; b < a.B; b += kPlan / 64) extend_row(a, b, planL[b], lane);
   }
 }
@@ -469,8 +471,8 @@ extern "C" int g2ptq_pages_extend(void* stream, const g2ptq_page_tables* tables,
   StepArgs a{};
   G2PTQ_TRY(check_tables("pages_extend", tables, B, rows, ws, ws_bytes, a));
   G2PTQ_CHECK(total >= 0 && total < (1ll << 31), "pages_extend: %lld tokens", (long long)total);
-  G2PTQ_CHECK(cu && (B == 0 || (counts && table && kv_lens)) && (total == 0 || (slots && positions)),
-              "pages_extend: null pointer");
+  G2PTQ_CHECK(cu && (B == 0 || (counts && table && kv_lens)) &&
+                  (total == 0 || (slots && positions)), "pages_extend: null pointer");
   a.rows = rows, a.counts = counts, a.total = total;
   a.table = table, a.cu = cu, a.kv_lens = kv_lens, a.slots = slots, a.positions = positions;
   hipStream_t st = as_stream(stream);
