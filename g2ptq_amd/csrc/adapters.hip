@@ -285,8 +285,8 @@ __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int
 }
 
 // An adapter's tokens' h into LDS as it enters the product: per token and 16 ranks four pieces
-// of 16 bytes, both halves of the ranks rounded, then what the rounding left out.  Eight lanes
-// take a token.  back: what a token's products are multiplied with, fp16's rows being brought
+// of 16 bytes, both halves of the ranks rounded, then what the rounding left out.  Two, four or
+// eight lanes take a token.  back: what a token's products are multiplied with, fp16's rows being brought
 // to the top of its range by a power of two.
 template <bool F16>
 __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int which,
@@ -294,8 +294,9 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
                                         float* back) {
   const float scale = a.scale[which];
   const int rank = a.rank[which], pieces = (rank + 15) / 16 * 2;
-  for (int i = threadIdx.x; i < (count + 31) / 32 * 256; i += 256) {
-    const int t = i >> 3, l = i & 7;
+  const int shift = pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3, lanes = 1 << shift;
+  for (int i = threadIdx.x; (i & ~255) < count << shift; i += 256) {
+    const int t = i >> shift, l = i & (lanes - 1);
     const int64_t token = t0 + list[min(t, count - 1)];
     float fit = 1.f;
     bool infinite = false;
@@ -303,21 +304,20 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
     if (l < pieces) load_h(a, token, l * 8, rank - l * 8, scale, v);
     if constexpr (F16) {
       uint32_t top = 0;
-      for (int p = l; p < pieces; p += 8) {
+      for (int p = l; p < pieces; p += lanes) {
         if (p != l) load_h(a, token, p * 8, rank - p * 8, scale, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       }
-#pragma unroll
-      for (int o = 1; o < 8; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+      for (int o = 1; o < lanes; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
       infinite = top >= 0x7f800000u;
       if (!infinite && top)
         fit = __uint_as_float((uint32_t)min(254, max(1, 268 - (int)(top >> 23))) << 23);
       if (l == 0 && t < count) back[t] = __fdiv_rn(1.f, fit);
     }
-    for (int p = l; p < pieces; p += 8) {
+    for (int p = l; p < pieces; p += lanes) {
       // (ranks from 64 on, and then all of fp16's, are read again)
-      if (p != l || (F16 && pieces > 8)) load_h(a, token, p * 8, rank - p * 8, scale, v);
+      if (p != l || (F16 && pieces > lanes)) load_h(a, token, p * 8, rank - p * 8, scale, v);
       u32x4 hi, lo;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

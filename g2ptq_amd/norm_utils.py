@@ -92,18 +92,18 @@ def _norm(x, weight, eps, residual, y, total, sym, codes, ldc, scale, zero, what
 def _usual(x, weight, residual):
     """Whether the arguments pass all checks in one go and lie as the kernel takes them (a call
     is a few microseconds); what is not is looked at one by one."""
-    here = x.get_device()
-    return (x.numel() and x.is_contiguous() and x.dtype in _DTYPE_CODE
-            and weight.dtype in _DTYPE_CODE and x.dim() and weight.shape == x.shape[-1:]
-            and weight.is_contiguous()
+    here, dtype = x.get_device(), x.dtype
+    return (x.numel() and x.dim() and weight.dim() == 1 and weight.shape[0] == x.shape[-1]
+            and dtype in _DTYPE_CODE and weight.dtype in _DTYPE_CODE
+            and x.is_contiguous() and weight.is_contiguous()
             and here == weight.get_device() == torch._C._cuda_getDevice()
             and _lib.forward_ad._current_level < 0
-            and (residual is None or (residual.dtype is x.dtype and residual.shape == x.shape
+            and (residual is None or (residual.dtype is dtype and residual.shape == x.shape
                                       and residual.is_contiguous()
-                                      and residual.get_device() == here))
-            and not (torch.is_grad_enabled()
-                     and (x.requires_grad or weight.requires_grad
-                          or (residual is not None and residual.requires_grad))))
+                                      and residual.get_device() == here
+                                      and not (residual.requires_grad
+                                               and torch.is_grad_enabled())))
+            and not ((x.requires_grad or weight.requires_grad) and torch.is_grad_enabled()))
 
 
 def rms_norm(x, weight, eps=1e-6, residual=None):

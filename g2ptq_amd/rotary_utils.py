@@ -51,7 +51,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None):
     d = rotary_dim
     if kind == "ntk" and d > 2:
         base = base * s ** (d / (d - 2))
-    pair = torch.arange(d // 2, dtype=torch.float64)
+    pair = torch.arange(d // 2, dtype=torch.float64, device="cpu")
     theta = float(base) ** (-2 * pair / d)
     if kind == "linear":
         return theta / s, 1.0
@@ -83,7 +83,7 @@ class Rotary:
 
     ``layout`` "half": channel i is paired with i + rotary_dim/2; "interleaved": 2i with 2i + 1.
     Channels from ``rotary_dim`` (default: all) on stay as they are.  ``frequencies`` (rotary_dim
-    / 2 radians a position, any float type) and ``attention_factor`` take the place of ``base``
+    / 2 radians a position, numbers or a tensor of any type) and ``attention_factor`` take the place of ``base``
     and ``scaling``.  Nothing is tabulated: angles are fp64 products less their whole turns, off by
     some 2^-52 of position · θ, so that positions are not limited (up to 2^28 the fp32 sine and
     cosine round more), and negative ones turn back."""
@@ -99,7 +99,8 @@ class Rotary:
         if frequencies is None:
             theta, factor = rotary_frequencies(rotary_dim, base, scaling)
         else:
-            theta, factor = torch.as_tensor(frequencies).detach().to("cpu", torch.float64), 1.0
+            theta = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu()
+            factor = 1.0
             if scaling is not None or tuple(theta.shape) != (rotary_dim // 2,):
                 raise ValueError(f"Rotary: frequencies of shape {tuple(theta.shape)}, expected "
                                  f"({rotary_dim // 2},) and no scaling")

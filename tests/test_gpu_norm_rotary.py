@@ -311,6 +311,8 @@ def test_rotary_frequencies_are_the_formulas(dev, scaling):
     _check_rotary(rotary, out, q, p)
     given = Rotary(d, frequencies=theta, attention_factor=m)
     assert_bitexact(given(q.to(dev), None, p.to(dev))[0], out, "given frequencies")
+    given = Rotary(d, frequencies=theta.tolist(), attention_factor=m)
+    assert_bitexact(given(q.to(dev), None, p.to(dev))[0], out, "given numbers")
 
 
 def test_rotary_strides(dev):

@@ -218,6 +218,12 @@ def test_frequencies():
     ratio = rotary_frequencies(128, 500000.0, bands)[0] / rotary_frequencies(128, 500000.0)[0]
     assert ratio[0] == 1 and abs(float(ratio[-1]) - 0.25) < 1e-12
     assert bool((ratio.diff() <= 1e-15).all())
+    before = torch.get_default_dtype()
+    try:  # numbers stay numbers of 64 bits under any default type
+        torch.set_default_dtype(torch.float16)
+        torch.testing.assert_close(rotary_frequencies(64)[0], theta, rtol=0, atol=0)
+    finally:
+        torch.set_default_dtype(before)
     for bad in ({"type": "linear"}, {"factor": 2.0}, {"type": "linear", "factor": -1.0},
                 {"type": "ntk", "factor": math.inf}, {"type": "bands", "factor": 2.0},
                 {"type": "yarn", "factor": 2.0, "original_positions": 10, "beta_fast": 1,
