@@ -13,7 +13,7 @@
 //
 // Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight
 // requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 17–21 µs (its 42 MB of
-// tokens at a copy's rate 8), U·h 80–91 (292 MB of rows in and out: 57; a launch that only copies
+// tokens at a copy's rate 8), U·h 78–85 (292 MB of rows in and out: 57; a launch that only copies
 // them through the same mapping takes some 70).  By latency where they are few: 48 tokens with
 // 32 adapters of rank 16, 4096 × 4096, 4.0–4.3 and 6.1–6.5 µs: index, adapter, operands and sums
 // follow each other through memory.
@@ -429,19 +429,17 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
   __syncthreads();
 }
 
-// A window's channels are shared by `shares` workgroups, each walking its own range.  Workgroups
-// that follow each other take the same range of neighbouring windows, so that its weights are
-// read from memory once, and the same slot: the first slots have the work where a window's
-// tokens share an adapter, and these are spread over the XCDs.
+// A window's channels are shared by `shares` workgroups, each walking its own range.  First come
+// the first slots: they have the work where a window's tokens share an adapter.
 template <bool F16, int IO, int RB>
-__global__ __launch_bounds__(256, 2) void adapter_expand_kernel(AdapterArgs a, int pitch,
+__global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterArgs a, int pitch,
                                                                 int shares) {
   extern __shared__ u32x4 hL[];
   __shared__ uint8_t lists[4][kWindow];
   __shared__ float back[kWindow];
   __shared__ f32x4 turns[4][16 * kTurn];
   const uint32_t groups = gridDim.x / (uint32_t)shares;
-  const uint32_t share = blockIdx.x / groups, group = blockIdx.x - share * groups;
+  const uint32_t group = blockIdx.x / (uint32_t)shares, share = blockIdx.x - group * shares;
   const uint32_t windows = groups / (uint32_t)a.slots, slot = group / windows;
   const uint32_t window = group - slot * windows;
   const int64_t t0 = (a.window + window) * kWindow;
@@ -504,16 +502,19 @@ int parts_of(int64_t T, int64_t K, int64_t n) {
   while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 512) p *= 2;
   return p;
 }
-// Shares of the channels, of equally many rounds of 256.  Each prepares h again, so that they
-// are fewer where the windows may hold an adapter for every slot.  MI355X, 4096 channels, 2048
-// tokens of 40 adapters in any order 73 µs, 105 with a share for every 512 / windows; 8192 of
-// four requests 60 with 512 workgroups, 80 with 128 and 68 with 2048.
+// Shares of the channels: a power of two, so that an XCD, which takes every eighth workgroup, has
+// the same shares of all windows and keeps their weights in its L2.  Each prepares h again, so
+// that they are fewer where windows may hold many adapters.  MI355X, 4096 × 4096, against six
+// shares in the order of windows: 8192 tokens of four requests of rank 16 46.4 and 50.7 µs, of rank
+// 64 66 and 71, 2048 of rank 64 31 and 35; eight shares against four: 2048 of 40 adapters in any
+// order 82 and 70, 1024 of four requests 16.6 and 21.8.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   const int64_t rounds = cdiv(N, 256), windows = cdiv(T, kWindow);
-  const int64_t most = std::min<int64_t>(windows * std::min<int64_t>(n, kWindow), 85);
-  const int64_t groups = std::max(busy_of(T, n), most);
-  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / groups));
-  return cdiv(rounds, cdiv(rounds, shares));
+  const int64_t mixed = std::min<int64_t>(windows * std::min<int64_t>(n, kWindow) / 4, 128);
+  const int64_t groups = std::max(busy_of(T, n), mixed);
+  int64_t shares = 1;
+  while (shares * 2 <= rounds && shares * 2 * groups <= 768) shares *= 2;
+  return shares;
 }
 
 // Rows that no cache will hold are kept out of the caches.  MI355X, 5100 tokens × 14336 channels
@@ -533,9 +534,11 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
                        a);
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
-#define G2_EXPAND(IO)                                                                           \
-  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB>), grid, dim3(256), lds, st, a, pitch, \
-                     (int)shares)
+    // (weights of 32 ranks at a time: 64 leave a SIMD two waves, 91 against 85 µs where U·h takes
+    // 5100 tokens of ranks 32 and 64 to 14336 channels)
+#define G2_EXPAND(IO)                                                                             \
+  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB < 2 ? 1 : 2>), grid, dim3(256), lds, st, \
+                     a, pitch, (int)shares)
     if (!a.vo) G2_EXPAND(kElements);
     else if (streamed(a)) G2_EXPAND(kStream);
     else G2_EXPAND(kPieces);
