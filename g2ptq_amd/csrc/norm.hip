@@ -24,13 +24,12 @@ struct NormArgs {
   int8_t* codes;           // rows of ldc bytes
   int64_t ldc;
   float *scale, *zero;
-  bool vx, vr, vw, vo;     // rows of x, r, w and the outputs are 16-byte aligned
 };
 
 __device__ __forceinline__ void load_weight(const NormArgs& a, int c, int n, float (&v)[8]) {
-  if (a.wtype == 0) load8<0>(a.w, c, a.vw, n, v);
-  else if (a.wtype == 1) load8<1>(a.w, c, a.vw, n, v);
-  else load8<2>(a.w, c, a.vw, n, v);
+  if (a.wtype == 0) load8_any<0>(a.w, c, n, v);
+  else if (a.wtype == 1) load8_any<1>(a.w, c, n, v);
+  else load8_any<2>(a.w, c, n, v);
 }
 
 // Over the L lanes of a row (L = 256: the workgroup, by its waves' results in LDS).
@@ -79,10 +78,10 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
   float s[N][8], w[N][8];
 
   auto fetch = [&](int c, float (&v)[8]) {
-    load8<DT>(a.x, xat + c, a.vx, a.C - c, v);
+    load8_any<DT>(a.x, xat + c, a.C - c, v);
     if (a.r) {
       float u[8];
-      load8<DT>(a.r, rat + c, a.vr, a.C - c, u);
+      load8_any<DT>(a.r, rat + c, a.C - c, u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += u[j];
     }
@@ -106,7 +105,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
     if constexpr (V == 0) fetch(c, s[0]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = __fmaf_rn(s[p][j], s[p][j], ss);
-    if (a.sum && c < a.C) store8<DT>(a.sum, row * a.C + c, a.vo, a.C - c, s[p]);
+    if (a.sum && c < a.C) store8_any<DT>(a.sum, row * a.C + c, a.C - c, s[p]);
   });
   ss = row_sum<L>(ss, sums[0]);
   // k: a power of two that s is scaled by
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
   if constexpr (Q == 0) {
     each([&](int p, int c) {
       value(p, c);
-      if (c < a.C) store8<DT>(a.y, row * a.C + c, a.vo, a.C - c, s[p]);
+      if (c < a.C) store8_any<DT>(a.y, row * a.C + c, a.C - c, s[p]);
     });
   } else {
     Range<SYM> r;
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
       for (int j = 0; j < 8; ++j)
         if (c + j < a.C) u[j >> 2] |= ((uint32_t)to_code(g, s[p][j]) & 0xffu) << (8 * (j & 3));
       *reinterpret_cast<uint2*>(a.codes + row * a.ldc + c) = make_uint2(u[0], u[1]);
-      if (a.y && c < a.C) store8<DT>(a.y, row * a.C + c, a.vo, a.C - c, s[p]);
+      if (a.y && c < a.C) store8_any<DT>(a.y, row * a.C + c, a.C - c, s[p]);
     };
     if constexpr (V > 0) {
       each([&](int p, int c) { if (c < C16) codes(p, c); });
@@ -190,7 +189,6 @@ struct CodesArgs {
   int64_t ldc, T, K;
   const float *scale, *zero;
   void* out;
-  bool vc, vo;
   int shift;
 };
 
@@ -205,9 +203,8 @@ __global__ __launch_bounds__(256) void dequantize_tokens_kernel(CodesArgs a) {
     const int8_t* p = a.codes + t * a.ldc + c;
     const float s = a.scale[t], z = a.zero ? a.zero[t] : 0.f;
     uint32_t u[4] = {0, 0, 0, 0};
-    if (a.vc && n == 16) {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
+    if (n == 16) {
+      __builtin_memcpy(u, p, 16);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
@@ -217,8 +214,8 @@ __global__ __launch_bounds__(256) void dequantize_tokens_kernel(CodesArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       v[j >> 3][j & 7] = s * ((float)(int8_t)(u[j >> 2] >> (8 * (j & 3))) - z);
-    store8<DT>(a.out, t * a.K + c, a.vo, n, v[0]);
-    if (n > 8) store8<DT>(a.out, t * a.K + c + 8, a.vo, n - 8, v[1]);
+    store8_any<DT>(a.out, t * a.K + c, n, v[0]);
+    if (n > 8) store8_any<DT>(a.out, t * a.K + c + 8, n - 8, v[1]);
   }
 }
 
@@ -284,13 +281,8 @@ extern "C" int g2ptq_rms_norm(void* stream, const void* x, int64_t x_outer, int6
                 "rms_norm: codes need 16-byte aligned rows of at least %lld bytes",
                 (long long)(cdiv(C, 16) * 16));
   }
-  const int e = dtype == 2 ? 4 : 2;
   NormArgs a{x, r, w, x_outer, x_inner, r_outer, r_inner, rows, 0, (uint32_t)inner, (int)C,
              wtype, eps, y, sum, codes, ldc, scale, zero};
-  a.vx = aligned16(x) && x_outer * e % 16 == 0 && (inner == 1 || x_inner * e % 16 == 0);
-  a.vr = aligned16(r) && r_outer * e % 16 == 0 && (inner == 1 || r_inner * e % 16 == 0);
-  a.vw = aligned16(w);
-  a.vo = aligned16(y) && aligned16(sum) && C * e % 16 == 0;
   hipStream_t st = as_stream(stream);
   if (dtype == 0) return norm_by_codes<0>(st, a, sym);
   if (dtype == 1) return norm_by_codes<1>(st, a, sym);
@@ -307,8 +299,6 @@ extern "C" int g2ptq_dequantize_tokens(void* stream, const int8_t* codes, int64_
   G2PTQ_CHECK(codes && scale && out, "dequantize_tokens: null pointer");
   const RowLaunch l = row_launch(cdiv(K, 16), T);
   CodesArgs a{codes, ldc, T, K, scale, zero, out};
-  a.vc = aligned16(codes) && ldc % 16 == 0;
-  a.vo = aligned16(out) && K * (dtype == 2 ? 4 : 2) % 16 == 0;
   a.shift = l.shift;
   hipStream_t st = as_stream(stream);
 #define G2_DQ(DT) \

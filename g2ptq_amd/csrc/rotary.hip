@@ -28,7 +28,6 @@ struct RotaryArgs {
   const double* freq;     // n / 2, turns a position
   float factor;
   int tokens;             // of a workgroup
-  bool vec[2];            // eight channels of a pair's first and second half are 16-byte aligned
 };
 
 // A workgroup takes `tokens` tokens: the sines and cosines of their pairs first, once for all
@@ -61,48 +60,45 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     const uint32_t hw = w ? h - a.heads[0] : h;
     const int64_t in = (t0 + t) * a.st[w] + hw * a.sh[w];
     const int64_t out = ((t0 + t) * a.heads[w] + hw) * a.dim;
-    const bool vec = a.vec[w];
     if (p < turned) {
       const float* cs = cosL + t * pairs;
       const float* sn = sinL + t * pairs;
       if constexpr (HALF) {
         const int j = p * 8, n = pairs - j;
         float u[8], v[8], x[8], y[8];
-        load8<DT>(a.x[w], in + j, vec, n, u);
-        load8<DT>(a.x[w], in + j + pairs, vec, n, v);
+        load8_any<DT>(a.x[w], in + j, n, u);
+        load8_any<DT>(a.x[w], in + j + pairs, n, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int k = i < n ? j + i : 0;
           x[i] = u[i] * cs[k] - v[i] * sn[k];
           y[i] = u[i] * sn[k] + v[i] * cs[k];
         }
-        store8<DT>(a.out[w], out + j, vec, n, x);
-        store8<DT>(a.out[w], out + j + pairs, vec, n, y);
+        store8_any<DT>(a.out[w], out + j, n, x);
+        store8_any<DT>(a.out[w], out + j + pairs, n, y);
       } else {
         const int j = p * 8, n = a.n - j;
         float u[8], x[8];
-        load8<DT>(a.x[w], in + j, vec, n, u);
+        load8_any<DT>(a.x[w], in + j, n, u);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const int k = i < n ? (j + i) / 2 : 0;
           x[i] = u[i] * cs[k] - u[i + 1] * sn[k];
           x[i + 1] = u[i] * sn[k] + u[i + 1] * cs[k];
         }
-        store8<DT>(a.out[w], out + j, vec, n, x);
+        store8_any<DT>(a.out[w], out + j, n, x);
       }
     } else {
       const int j = a.n + (p - turned) * 8, n = a.dim - j;
       float u[8];
-      load8<DT>(a.x[w], in + j, vec, n, u);
-      store8<DT>(a.out[w], out + j, vec, n, u);
+      load8_any<DT>(a.x[w], in + j, n, u);
+      store8_any<DT>(a.out[w], out + j, n, u);
     }
     p += dp, h += dh, t += dt;
     if (p >= P) p -= P, ++h;
     if (h >= H) h -= H, ++t;
   }
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 }  // namespace g2ptq
@@ -124,15 +120,9 @@ extern "C" int g2ptq_rotary(void* stream, const void* q, int64_t q_token, int64_
   if (T == 0 || q_heads + k_heads == 0) return G2PTQ_OK;
   G2PTQ_CHECK(positions && freq && (q_heads == 0 || (q && q_out)) &&
                   (k_heads == 0 || (k && k_out)), "rotary: null pointer");
-  const int e = dtype == 2 ? 4 : 2;
-  // halves start at a multiple of eight pairs, channels behind the turned ones at one of eight
-  const bool whole = dim % 8 == 0 && n % (interleaved ? 8 : 16) == 0;
   RotaryArgs a;
   a.x[0] = q, a.st[0] = q_token, a.sh[0] = q_head, a.heads[0] = (int)q_heads, a.out[0] = q_out;
   a.x[1] = k, a.st[1] = k_token, a.sh[1] = k_head, a.heads[1] = (int)k_heads, a.out[1] = k_out;
-  for (int w = 0; w < 2; ++w)
-    a.vec[w] = whole && aligned16(a.x[w]) && aligned16(a.out[w]) && a.st[w] * e % 16 == 0 &&
-               a.sh[w] * e % 16 == 0;
   a.T = T, a.dim = (int)dim, a.n = (int)n;
   a.positions = positions, a.freq = freq, a.factor = factor;
   // As many tokens as a workgroup has threads for, mostly one.  MI355X, one token of 40 heads
