@@ -77,13 +77,24 @@ __device__ __forceinline__ u32x4 piece(const uint16_t* p) {
   __builtin_memcpy(&v, p, 16);
   return v;
 }
-// Those from n on zero.
-__device__ __forceinline__ u32x4 piece(const uint16_t* p, int64_t n) {
-  if (n >= 8) return piece(p);
+// Eight values of a row of `size` from c ≥ 0 on, those behind its end zero: the last eight moved
+// down, so that no value waits for another's branch.
+__device__ __forceinline__ u32x4 piece(const uint16_t* row, int64_t c, int64_t size) {
+  if (c + 8 <= size) return piece(row + c);
+  if (size >= 8) {
+    const int64_t past = c + 8 - size;
+    const u32x4 v = piece(row + c - past);
+    const uint64_t low = v[0] | (uint64_t)v[1] << 32, high = v[2] | (uint64_t)v[3] << 32;
+    const int s = 16 * (int)(past & 3);
+    const uint64_t a = past >= 8 ? 0 : past >= 4 ? high : low, b = past >= 4 ? 0 : high;
+    const uint64_t l = a >> s | b << 1 << (63 - s), h = b >> s;
+    return u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+  }
   u32x4 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    v[i] = (2 * i < n ? p[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+    v[i] = (c + 2 * i < size ? row[c + 2 * i] : 0u) |
+           (c + 2 * i + 1 < size ? (uint32_t)row[c + 2 * i + 1] << 16 : 0u);
   return v;
 }
 
@@ -184,7 +195,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
           s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
         for (int b = 0; b < TB; ++b)
-          s.x[b][i] = piece(xrow[b] + k + 8 * i, a.K - k - g * 16 - 8 * i);
+          s.x[b][i] = piece(xrow[b] - g * 16, k + g * 16 + 8 * i, a.K);
       }
       products(s);
     }
@@ -261,10 +272,10 @@ template <int IO>
 __device__ __forceinline__ u32x4 base_piece(const AdapterArgs& a, int64_t t, int64_t c) {
   if (!a.base) return u32x4{0, 0, 0, 0};
   // (channels behind the last: the first again, not stored)
+  if (IO == kRagged) return piece(a.base + t * a.ldb, c, a.N);
   const uint16_t* p = a.base + t * a.ldb + (c < a.N ? c : 0);
   if (IO == kStream) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-  if (IO == kPieces) return piece(p);
-  return piece(p, a.N - c);
+  return piece(p);
 }
 template <bool F16, int IO>
 __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int64_t c, u32x4 base,

@@ -100,8 +100,15 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t at, int n, floa
       __builtin_memcpy(v, x, 16);
       __builtin_memcpy(v + 4, x + 4, 16);
     } else {
+      // (no branch a value: their loads are under way together)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < n ? x[i] : 0.f;
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[i < n ? i : 0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.f;
+      }
     }
   } else {
     const uint16_t* x = static_cast<const uint16_t*>(p) + at;
@@ -110,8 +117,16 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t at, int n, floa
       __builtin_memcpy(w, x, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = (2 * i < n ? x[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)x[2 * i + 1] << 16 : 0u);
+      for (int i = 0; i < 4; ++i) w[i] = 0;
+      if (n > 0) {
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = x[i < n ? i : 0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = i < n ? h[i] : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | h[2 * i + 1] << 16;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
