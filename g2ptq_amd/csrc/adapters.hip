@@ -48,6 +48,7 @@ struct AdapterArgs {
   uint16_t* out;
   int64_t ldo;
   int* flags;
+  bool odd;                   // rows of x may start between 32-bit words
   bool aligned;               // rows of base and out are 16-byte aligned
   int64_t window;             // the launch's first
 };
@@ -131,7 +132,11 @@ __device__ __forceinline__ int32_t index_of_lane(const AdapterArgs& a, int64_t t
 // h of 16·TB tokens for up to 16·RB ranks from r0 on: ranks × tokens, 64 columns of K a step
 // (lane (n, g) holds 16 of row n from 16·g on).  The workgroup's waves and the launch's parts
 // take turns at rounds of U steps, whose loads are all under way together.
-template <bool F16, int RB, int TB>
+// ODD: rows may start between two 32-bit words.  There the memory takes a load of sixteen bytes
+// apart, so the words are loaded that hold the values (two bytes before the first and behind the
+// last share theirs and are shifted out).  MI355X, 777 tokens of rank 20 from 2047 columns: 11 µs,
+// 17 without; 2048 tokens of rank 64 from 4097: 14 and 21.
+template <bool F16, int RB, int TB, bool ODD>
 __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int which, int64_t r0,
                                        int blocks, const uint8_t* list, int count,
                                        f32x4 (*sums)[RB * 4][64]) {
@@ -139,9 +144,12 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const uint16_t* xrow[TB];
   const uint16_t* drow[RB];
+  uint32_t odd[TB];
 #pragma unroll
-  for (int b = 0; b < TB; ++b)
+  for (int b = 0; b < TB; ++b) {
     xrow[b] = a.x + (t0 + list[min(16 * b + n, count - 1)]) * a.ldx + g * 16;
+    odd[b] = ODD ? (uint32_t)(reinterpret_cast<uintptr_t>(xrow[b]) >> 1) & 1 : 0;
+  }
 #pragma unroll
   for (int r = 0; r < RB; ++r)  // (blocks that the adapter lacks: the first again, not stored)
     drow[r] = a.down + ((int64_t)which * a.R + r0 + (r < blocks ? 16 * r : 0)) * a.Kp + lane * 8;
@@ -152,6 +160,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
     for (int b = 0; b < TB; ++b) acc[r][b] = f32x4{0, 0, 0, 0};
   struct Step {
     u32x4 d[RB][2], x[TB][2];
+    uint32_t end[TB];
   };
   auto products = [&](const Step& s) {
 #pragma unroll
@@ -168,8 +177,22 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
       for (int r = 0; r < RB; ++r)
         s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
-      for (int b = 0; b < TB; ++b) s.x[b][i] = piece(xrow[b] + k + 8 * i);
+      for (int b = 0; b < TB; ++b) s.x[b][i] = piece(xrow[b] + k + 8 * i - odd[b]);
     }
+    if (ODD)  // (the last value's word; rows on words have no use for a ninth)
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+        s.end[b] = *reinterpret_cast<const uint32_t*>(xrow[b] + k + 14 + odd[b]);
+  };
+  auto shift = [&](Step& s) {
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t next = i < 7 ? s.x[b][(i + 1) >> 2][(i + 1) & 3] : s.end[b];
+        s.x[b][i >> 2][i & 3] =
+            __builtin_amdgcn_alignbit(next, s.x[b][i >> 2][i & 3], 16 * odd[b]);
+      }
   };
   const int each = a.parts * 4 * U;
   int step = (blockIdx.y * 4 + wave) * U;
@@ -179,7 +202,10 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
 #pragma unroll
     for (int u = 0; u < U; ++u) fetch(s[u], (int64_t)(step + u) * 64);
 #pragma unroll
-    for (int u = 0; u < U; ++u) products(s[u]);
+    for (int u = 0; u < U; ++u) {
+      if (ODD) shift(s[u]);
+      products(s[u]);
+    }
   }
   // the last columns
   for (; step * 64 < a.Kp; step += each)
@@ -218,7 +244,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
   __syncthreads();
 }
 
-template <bool F16, int RB>
+template <bool F16, int RB, bool ODD>
 __global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[4][RB * 4][64];
   __shared__ uint8_t lists[4][kWindow];
@@ -229,8 +255,8 @@ __global__ __launch_bounds__(256, 2) void adapter_shrink_kernel(AdapterArgs a) {
     const int blocks = (a.rank[which] + 15) / 16;
     for (int r = 0; r < blocks; r += RB) {
       const int here = min(RB, blocks - r);
-      if (count <= 16) shrink<F16, RB, 1>(a, t0, which, r * 16, here, list, count, sums);
-      else shrink<F16, RB, 4>(a, t0, which, r * 16, here, list, count, sums);
+      if (count <= 16) shrink<F16, RB, 1, ODD>(a, t0, which, r * 16, here, list, count, sums);
+      else shrink<F16, RB, 4, ODD>(a, t0, which, r * 16, here, list, count, sums);
     }
   });
 }
@@ -548,8 +574,11 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
   const size_t lds = (size_t)kWindow * pitch * 16;
   for (a.window = 0; a.window < windows; a.window += most) {
     const unsigned groups = (unsigned)(std::min(windows - a.window, most) * a.slots);
-    hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB>), dim3(groups, a.parts), dim3(256), 0, st,
-                       a);
+#define G2_SHRINK(ODD) \
+  hipLaunchKernelGGL((adapter_shrink_kernel<F16, RB, ODD>), dim3(groups, a.parts), dim3(256), 0, st, a)
+    if (a.odd) G2_SHRINK(true);
+    else G2_SHRINK(false);
+#undef G2_SHRINK
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
     // (weights of 32 ranks at a time: 64 leave a SIMD two waves, 91 against 85 µs where U·h takes
@@ -620,6 +649,7 @@ extern "C" int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const 
   a.base = static_cast<const uint16_t*>(base), a.ldb = ldb;
   a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
   a.flags = set->flags;
+  a.odd = reinterpret_cast<uintptr_t>(x) % 4 || (ldx % 2 && T > 1);
   a.aligned = aligned16(base) && aligned16(out) && ldb % 8 == 0 && ldo % 8 == 0;
   hipStream_t st = as_stream(stream);
   return set->dtype == 0 ? adapters_by_rank<false>(st, a) : adapters_by_rank<true>(st, a);

@@ -132,6 +132,34 @@ def test_tokens_do_not_depend_on_their_neighbours(dev):
         assert_bitexact(s.own(x, index, base=base), y, "again")
 
 
+@pytest.mark.parametrize("K,N", [(1, 1), (3, 7), (7, 9), (63, 65), (65, 127), (129, 190), (191, 64),
+                                 (1023, 129), (2049, 33)])
+@pytest.mark.parametrize("T,ranks", [(5, [16]), (70, [16, 40]), (130, [33, 64, 3])])
+def test_rows_at_any_address(dev, K, N, T, ranks):
+    """Rows that start between words or inside a piece of eight values, NaN on every side."""
+    for dtype in DTYPES:
+        s = Set(dev, ranks, N, K, dtype)
+        x, base, index = s.x(T).to(dev), s.base(T).to(dev), s.index(T, "random").to(dev)
+
+        def inside(v, before, behind):
+            wide = torch.full((T, before + v.shape[1] + behind), float("nan"), dtype=dtype, device=dev)
+            wide[:, before:before + v.shape[1]] = v
+            return wide, wide[:, before:before + v.shape[1]]
+
+        # (rows of whole pieces at aligned addresses)
+        ref = s.own(inside(x, 8, 16 - K % 8)[1], index, base=inside(base, 8, 16 - N % 8)[1])
+        assert not ref.isnan().any()
+        for before, behind in ((1, 0), (0, 1), (1, 1), (2, 0), (3, 2), (8, 7)):
+            xw, xv = inside(x, before, behind)
+            bw, bv = inside(base, before, behind)
+            assert_bitexact(s.own(xv, index, base=bv), ref, f"{before} {behind}")
+            kept = bw.clone()
+            s.own.add_(bv, xv, index)
+            assert_bitexact(bv, ref, f"{before} {behind} in place")
+            kept[:, before:before + N] = ref
+            assert torch.equal(bw.view(torch.int16), kept.view(torch.int16))
+
+
 def test_strides_and_shapes(dev):
     for dtype in DTYPES:
         s = Set(dev, [16, 24], 70, 90, dtype)

@@ -104,6 +104,32 @@ def test_strided_rows(dev):
             assert_bitexact(t.scale, t2.scale, "scale")
 
 
+@pytest.mark.parametrize("C", [1, 7, 9, 15, 63, 333, 2051, 4097, 9001])
+def test_rows_beside_nan(dev, C):
+    """Rows at any address of their type with NaN on every side, which no row takes in."""
+    from g2ptq_amd import rms_norm, rms_norm_quantize
+    for dtype in DTYPES:
+        x, r = _x(6, C, dtype=dtype, seed=C).to(dev), _x(6, C, dtype=dtype, seed=C + 1).to(dev)
+        w = (1 + 0.1 * torch.randn(C, generator=gen(2))).to(dev, dtype)
+        y, s = rms_norm(x, w, residual=r)
+        q = rms_norm_quantize(x, w, residual=r)
+        assert not y.isnan().any()
+        for before, behind in ((1, 0), (2, 1), (5, 3), (8, 8)):
+            def inside(v):
+                wide = torch.full((*v.shape[:-1], before + C + behind), float("nan"), dtype=dtype,
+                                  device=dev)
+                wide[..., before:before + C] = v
+                return wide[..., before:before + C]
+
+            got = rms_norm(inside(x), inside(w), residual=inside(r))
+            assert_bitexact(got[0], y, f"{before} {behind}")
+            assert_bitexact(got[1], s, f"{before} {behind} sum")
+            got = rms_norm_quantize(inside(x), inside(w), residual=inside(r))
+            assert_bitexact(got.codes, q.codes, f"{before} {behind} codes")
+            assert_bitexact(got.scale, q.scale, f"{before} {behind} scale")
+            assert_bitexact(got.sum, q.sum, f"{before} {behind} sum")
+
+
 @pytest.mark.parametrize("C", [40, 500, 2000, 5000, 20000])
 def test_rows_of_extreme_values(dev, C):
     """Squares that overflow or vanish in fp32, rows of zeros, NaN and infinities; their rows
@@ -337,6 +363,29 @@ def test_rotary_strides(dev):
             wide = torch.stack([p, p], 1)[:, 0]
             assert_bitexact(rotary(qkv, qkv, wide)[1], rotary(qkv, qkv, p)[0], "positions")
             assert rotary(qkv[:0], qkv[:0, :2], p[:0])[1].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dim,part", [(2, 2), (10, 6), (18, 18), (36, 14), (70, 70), (134, 66)])
+def test_rotary_heads_beside_nan(dev, dim, part):
+    """Heads at any address of their type with NaN on every side."""
+    from g2ptq_amd import Rotary
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for layout in ("half", "interleaved"):
+            rotary = Rotary(dim, rotary_dim=part, layout=layout)
+            q, k = (_x(9, h, dim, dtype=dtype, seed=h).to(dev) for h in (5, 2))
+            p = _positions(9, 3).to(dev)
+            a, b = rotary(q, k, p)
+            assert not a.isnan().any() and not b.isnan().any()
+            for before, behind in ((1, 0), (3, 2), (8, 8)):
+                def inside(v):
+                    wide = torch.full((*v.shape[:-1], before + dim + behind), float("nan"),
+                                      dtype=dtype, device=dev)
+                    wide[..., before:before + dim] = v
+                    return wide[..., before:before + dim]
+
+                got = rotary(inside(q), inside(k), p)
+                assert_bitexact(got[0], a, f"{before} {behind} q")
+                assert_bitexact(got[1], b, f"{before} {behind} k")
 
 
 def test_rotary_turns_back(dev):
