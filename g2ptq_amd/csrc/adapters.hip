@@ -543,19 +543,23 @@ int64_t busy_of(int64_t T, int64_t n) {
 // against 69 (the second product reads every share).
 int parts_of(int64_t T, int64_t K, int64_t n) {
   int p = 1;
-  while (p < 8 && busy_of(T, n) * p < 256 && K >= (int64_t)p * 512) p *= 2;
+  while (p < 8 && busy_of(T, n) * p < 256 && cdiv(K, 64) >= p * 8) p *= 2;
   return p;
 }
-// Shares of the channels: a power of two, so that an XCD, which takes every eighth workgroup, has
-// the same shares of all windows and keeps their weights in its L2.  Each prepares h again, so
-// that they are fewer where windows may hold many adapters.  MI355X, 4096 × 4096, against six
-// shares in the order of windows: 8192 tokens of four requests of rank 16 46.4 and 50.7 µs, of rank
-// 64 66 and 71, 2048 of rank 64 31 and 35; eight shares against four: 2048 of 40 adapters in any
-// order 82 and 70, 1024 of four requests 16.6 and 21.8.
+// Shares of the channels: 256 each where windows are few.  MI355X, against the power of two below:
+// 1800 tokens of five adapters of rank 64 to 2560 channels 27.7 and 33.4 µs, 200 of eight of rank
+// 16 to 11008 14.7 and 16.4; with more workgroups, busy or not, 1000 tokens to 11008 22.3 and
+// 21.0, 64 of eight adapters 11.0 and 10.1.  Otherwise a power of two, so that an XCD, which takes
+// every eighth workgroup, has the same shares of all windows and keeps their weights in its L2.
+// Each prepares h again, so that they are fewer where windows may hold many adapters.  MI355X,
+// 4096 × 4096, against six shares in the order of windows: 8192 tokens of four requests of rank 16
+// 46.4 and 50.7 µs, of rank 64 66 and 71, 2048 of rank 64 31 and 35; eight shares against four:
+// 2048 of 40 adapters in any order 82 and 70, 1024 of four requests 16.6 and 21.8.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   const int64_t rounds = cdiv(N, 256), windows = cdiv(T, kWindow);
   const int64_t mixed = std::min<int64_t>(windows * std::min<int64_t>(n, kWindow) / 4, 128);
   const int64_t groups = std::max(busy_of(T, n), mixed);
+  if (rounds * groups <= 512 && rounds * windows * slots_of(T, n) <= 2048) return rounds;
   int64_t shares = 1;
   while (shares * 2 <= rounds && shares * 2 * groups <= 768) shares *= 2;
   return shares;
