@@ -236,8 +236,9 @@ int launch_norm(hipStream_t st, NormArgs& a) {
 // those that four waves hold need barriers.  MI355X, bf16 with residual, against a workgroup a
 // row: 16384 × 512 13.3 and 21.1 µs, 8192 × 1000 11.9 and 16.2 (64 × 1000 4.5 and 3.4); against a
 // wave a row: 8192 × 2048 23.1 and 26.0, 8192 × 4096 57 and 97.  Rows of 8193 values and more are
-// read again for each use: 2048 × 16384 60 µs, 74 with eight pieces in registers (16 rows 11.8
-// and 9.9); 2048 × 8192 24.9 with four in registers and 30.3 read again.
+// read again for each use where there are many: 2048 × 16384 60 µs, 74 with eight pieces in
+// registers, 1024 × 9000 18.9 and 21.6, but 512 × 16384 20.9 and 16.2, 64 rows 11.9 and 9.4, of
+// codes 17.0 and 10.8; 2048 × 8192 24.9 with four in registers and 30.3 read again.
 template <int DT, int Q>
 int norm_by_size(hipStream_t st, NormArgs& a) {
   if (a.C <= 64) return launch_norm<DT, Q, 8, 1>(st, a);
@@ -248,6 +249,7 @@ int norm_by_size(hipStream_t st, NormArgs& a) {
   if (a.C <= 2048) return launch_norm<DT, Q, 256, 1>(st, a);
   if (a.C <= 4096) return launch_norm<DT, Q, 256, 2>(st, a);
   if (a.C <= 8192) return launch_norm<DT, Q, 256, 4>(st, a);
+  if (a.C <= 16384 && a.rows <= 512) return launch_norm<DT, Q, 256, 8>(st, a);
   return launch_norm<DT, Q, 256, 0>(st, a);
 }
 

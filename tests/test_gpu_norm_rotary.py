@@ -79,6 +79,23 @@ def test_codes_are_the_grids(dev, T, C, sym):
                 assert_bitexact(got.sum, wide.sum.to(dtype), "sum")
 
 
+@pytest.mark.parametrize("C", [8193, 16384])
+def test_many_long_rows(dev, C):
+    from g2ptq_amd import rms_norm, rms_norm_quantize
+    w = (1 + 0.5 * torch.randn(C, generator=gen(C))).to(dev)
+    for dtype in (torch.bfloat16, torch.float32):
+        for T in (512, 513):
+            x = _x(T, C, dtype=dtype, seed=T).to(dev)
+            r = _x(T, C, dtype=dtype, seed=T + 1).to(dev)
+            y, s = rms_norm(x, w, 1e-5, residual=r)
+            _check_norm(y, x.cpu(), w.cpu(), 1e-5, dtype, r.cpu(), s)
+            q = rms_norm_quantize(x, w, 1e-5, residual=r)
+            for part in (slice(0, 3), slice(T - 3, T)):
+                p = rms_norm_quantize(x[part], w, 1e-5, residual=r[part])
+                assert_bitexact(q.codes[part], p.codes, "codes")
+                assert_bitexact(q.scale[part], p.scale, "scale")
+
+
 def test_strided_rows(dev):
     """Heads of a projection, columns of a wider matrix, transposed and expanded leading
     dimensions, single rows, rows off 16 bytes; residuals laid out otherwise than their rows."""
