@@ -99,14 +99,20 @@ __device__ __forceinline__ u32x4 piece(const uint16_t* row, int64_t c, int64_t s
   return v;
 }
 
-// f(adapter, number of its tokens) for every adapter whose first token of the window is at a
-// lane that this slot takes, with `list` (the wave's own) their lanes.  none: tokens without
-// an adapter too, as −1.
+// f(adapter, number of its tokens) for every adapter that this slot takes, with `list` (the wave's
+// own) their lanes.  none: tokens without an adapter too, as −1.  A slot takes every slots-th run
+// of equal neighbours, and of these the ones that open with the window's first token of theirs.
+// MI355X, 421 tokens of 20 adapters of rank 16, 3500 × 2651: 15 µs, 36 where a slot took every
+// slots-th token (prompts of as many tokens as there are slots all met in one).
 template <typename F>
 __device__ __forceinline__ void each_adapter(const AdapterArgs& a, int slot, int32_t idx,
                                              bool none, uint8_t* list, F f) {
   const int lane = threadIdx.x & 63;
-  uint64_t lanes = __ballot(idx >= (none ? -1 : 0) && lane % a.slots == slot);
+  // (the lane below's; −3 below the first)
+  const int32_t before = __builtin_amdgcn_update_dpp(-3, idx, 0x138, 0xf, 0xf, false);
+  const bool head = idx >= (none ? -1 : 0) && before != idx;
+  const int runs = __popcll(__ballot(head) & ((1ull << lane) - 1));
+  uint64_t lanes = __ballot(head && runs % a.slots == slot);
   while (lanes) {
     const int first = __builtin_ctzll(lanes);
     const int32_t which = __builtin_amdgcn_readlane(idx, first);

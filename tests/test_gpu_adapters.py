@@ -72,6 +72,21 @@ def test_adapters_are_the_formula(dev, ranks, N, K, dtype):
     s.run(70, "none")
 
 
+@pytest.mark.parametrize("n", [2, 7, 20, 40])
+def test_requests_of_any_length(dev, n):
+    """Prompts of as many tokens as there are adapters and about, adapters that come again, and
+    tokens without one between them."""
+    s = Set(dev, [16, 24] * (n // 2) + [8] * (n % 2), 96, 130, torch.bfloat16)
+    for length in (1, n - 1, n, n + 1, 2 * (n + 1), 32):
+        of = torch.arange(1 + 200 // length) % n
+        mixed = torch.randint(-1, n, (len(of),), generator=s.g)
+        for order in (of, of.flip(0), mixed, mixed * (torch.arange(len(of)) % 2) - 1 * (mixed < 0)):
+            index = order.repeat_interleave(length)[:200].int()
+            T = len(index)
+            x, base = s.x(T), s.base(T)
+            s.check(s.own(x.to(dev), index.to(dev), base=base.to(dev)), x, index, base)
+
+
 @pytest.mark.parametrize("T", [1, 48, 64, 2000])
 def test_more_columns_than_one_workgroup_takes(dev, T):
     for dtype in DTYPES:
