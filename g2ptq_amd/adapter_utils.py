@@ -25,7 +25,8 @@ MAX_RANK, MAX_FEATURES = 512, 1 << 20
 class LowRankAdapters:
     """``down``: n tensors (rank_i, in_features), ``up``: n tensors (out_features, rank_i), all
     bf16 or all fp16 on one GPU, ranks of 1 to 512; ``scale``: a number, or one per adapter.
-    They are copied once into the layout of the kernels."""
+    They are copied once into the layout of the kernels.  Equal calls give equal bits; the order in
+    which a token's products are summed in fp32 goes by the call's number of tokens."""
 
     def __init__(self, down, up, scale=1.0):
         down, up = list(down), list(up)

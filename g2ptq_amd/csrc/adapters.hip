@@ -12,10 +12,10 @@
 // every lane (no sort, no launch of its own); each is multiplied with its own tokens only.
 //
 // Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight
-// requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 17–21 µs (its 42 MB of
+// requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 16–20 µs (its 42 MB of
 // tokens at a copy's rate 8), U·h 78–85 (292 MB of rows in and out: 57; a launch that only copies
 // them through the same mapping takes some 70).  By latency where they are few: 48 tokens with
-// 32 adapters of rank 16, 4096 × 4096, 4.0–4.3 and 6.1–6.5 µs: index, adapter, operands and sums
+// 32 adapters of rank 16, 4096 × 4096, 3.8–4.1 and 6.0–6.5 µs: index, adapter, operands and sums
 // follow each other through memory.
 #include <algorithm>
 #include <type_traits>

@@ -62,8 +62,8 @@ __device__ __forceinline__ void row_range(Range<SYM>& r, float (*lds)[3]) {
 
 // L lanes walk a row, eight values at a time: V pieces kept in registers, or read again
 // for each use (V = 0).  Q: 0 y alone, 1 symmetric codes, 2 asymmetric ones.  Bound by the bytes:
-// MI355X, under the profiler, 8192 × 4096 bf16 with residual to codes and sum 55–57 µs (235 MB,
-// 4.2 TB/s), 262144 heads of 128 26.5–28.5 µs (134 MB, 4.9 TB/s); one row of 4096 4.4–4.9 µs, the
+// MI355X, under the profiler, 8192 × 4096 bf16 with residual to codes and sum 53–55 µs (235 MB,
+// 4.3 TB/s), 262144 heads of 128 26.5–28.5 µs (134 MB, 4.9 TB/s); one row of 4096 4.2–4.5 µs, the
 // latencies of a launch, the loads and two reductions.
 template <int DT, int Q, int L, int V>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
