@@ -145,9 +145,10 @@ class LowRankAdapters:
             y = torch.empty_like(base)
             need = _lib.workspace_fast("adapters_workspace", rows, self.in_features, self._n,
                                        self._rank)
+            ws = _lib.scratch(need, self.device)  # (held until the launch)
             _lib.call_fast("adapters", _lib.current_stream(), self._address, x.data_ptr(),
                            self.in_features, index.data_ptr(), rows, base.data_ptr(), out,
-                           y.data_ptr(), out, _lib.scratch(need, self.device).data_ptr(), need)
+                           y.data_ptr(), out, ws.data_ptr(), need)
             return y
         lead = x.shape[:-1]
         x2 = self._rows(x, self.in_features, "tokens")

@@ -3,6 +3,7 @@ errors of the C entry points (each returns before it touches a device), size que
 fast-call bindings, refusals of the Python layer, frequencies, and the oracles."""
 import ctypes
 import math
+import weakref
 
 import pytest
 import torch
@@ -250,3 +251,38 @@ def test_the_oracle_of_pages_keeps_every_page_once():
         held = [x for row in p.rows for x in row]
         assert sorted(held + p.free) == list(range(30))
         assert all(len(x) == -(-n // 4) for x, n in zip(p.rows, p.lengths))
+
+
+def test_calls_hold_their_workspace_until_they_return(monkeypatch):
+    """The buffer of a call on the current stream is in the caller's hand at its launch: another
+    thread's call may replace the cached one by a larger, and what is freed becomes somebody's
+    output.  The Python layer's paths, on host tensors with the launch taken out."""
+    held, launched = [], []
+
+    def scratch(nbytes, device):
+        buf = torch.empty(nbytes + 16, dtype=torch.uint8)
+        held[:] = [weakref.ref(buf), buf.data_ptr()]
+        return buf
+
+    def launch(name, *args):
+        launched.append(name)
+        assert held[0]() is not None, f"{name}: the workspace was dropped before the launch"
+        assert held[1] in args
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1)  # (host tensors' device)
+    monkeypatch.setattr(_lib, "current_stream", lambda: 0)
+    monkeypatch.setattr(_lib, "require_current", lambda t, what: None)
+    monkeypatch.setattr(_lib, "scratch", scratch)
+    monkeypatch.setattr(_lib, "call_fast", launch)
+    a = LowRankAdapters.__new__(LowRankAdapters)
+    a.in_features, a.out_features, a.dtype = 64, 32, torch.bfloat16
+    a.device, a._device, a._n, a._rank, a._address = torch.device("cpu"), -1, 2, 16, FAKE
+    x, y = torch.ones(3, 64).bfloat16(), torch.ones(3, 32).bfloat16()
+    index = torch.zeros(3, dtype=torch.int32)
+    a(x, index, base=y)
+    a(x, index)
+    a.add_(y, x, index)
+    t = PageTables.__new__(PageTables)
+    t.device, t._device, t._address = torch.device("cpu"), -1, FAKE
+    t.release(index)
+    assert launched == ["adapters"] * 3 + ["pages_release"]
