@@ -136,11 +136,14 @@ class PageTables:
 
     def check(self):
         """Raise if a request could not be placed, or a row or count was none, since the last
-        check (waits for the current stream)."""
+        check (waits for the current stream): IndexError for the latter, also where both were met
+        (its message then names both), else RuntimeError."""
         v = int(self.flags.item())
         self.flags.zero_()
+        room = "no free page, or a request longer than its row"
         if v & _lib.FLAG_BAD_INDEX:
             raise IndexError("PageTables: a row outside the tables or given twice, a count out of "
-                             "range, or more tokens than the step's total")
+                             "range, or more tokens than the step's total"
+                             + (f"; and {room}" if v & _lib.FLAG_NO_ROOM else ""))
         if v & _lib.FLAG_NO_ROOM:
-            raise RuntimeError("PageTables: no free page, or a request longer than its row")
+            raise RuntimeError(f"PageTables: {room}")

@@ -286,3 +286,21 @@ def test_calls_hold_their_workspace_until_they_return(monkeypatch):
     t.device, t._device, t._address = torch.device("cpu"), -1, FAKE
     t.release(index)
     assert launched == ["adapters"] * 3 + ["pages_release"]
+
+
+def test_a_check_of_page_tables_names_all_that_was_met():
+    """Both kinds of flags at once: the error names both, since it clears both."""
+    t = PageTables.__new__(PageTables)
+    t._held = (None,) * 5 + (torch.zeros(1, dtype=torch.int32),)
+    t.check()
+    for flags, error, kinds in (
+            (_lib.FLAG_BAD_INDEX, IndexError, ("a row outside",)),
+            (_lib.FLAG_NO_ROOM, RuntimeError, ("no free page",)),
+            (_lib.FLAG_BAD_INDEX | _lib.FLAG_NO_ROOM, IndexError, ("a row outside", "no free page"))):
+        t.flags.fill_(flags)
+        with pytest.raises(error) as raised:
+            t.check()
+        said = str(raised.value)
+        for kind in ("a row outside", "no free page"):
+            assert (kind in said) == (kind in kinds), said
+        t.check()
