@@ -137,7 +137,8 @@ __device__ __forceinline__ int32_t index_of_lane(const AdapterArgs& a, int64_t t
 
 // h of 16·TB tokens for up to 16·RB ranks from r0 on: ranks × tokens, 64 columns of K a step
 // (lane (n, g) holds 16 of row n from 16·g on).  The workgroup's waves and the launch's parts
-// take turns at rounds of U steps, whose loads are all under way together.
+// take turns at steps, whatever TB is: a token's sums are added in an order that its neighbours
+// have no part in.  U steps' loads are under way together.
 // ODD: rows may start between two 32-bit words.  There the memory takes a load of sixteen bytes
 // apart, so the words are loaded that hold the values (two bytes before the first and behind the
 // last share theirs and are shifted out).  MI355X, 777 tokens of rank 20 from 2047 columns: 11 µs,
@@ -200,13 +201,13 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
             __builtin_amdgcn_alignbit(next, s.x[b][i >> 2][i & 3], 16 * odd[b]);
       }
   };
-  const int each = a.parts * 4 * U;
-  int step = (blockIdx.y * 4 + wave) * U;
-  const int whole = (int)(a.K / 64) - (U - 1);
-  for (; step < whole; step += each) {
+  const int each = a.parts * 4;
+  int step = blockIdx.y * 4 + wave;
+  const int whole = (int)(a.K / 64);
+  for (; step + (U - 1) * each < whole; step += U * each) {
     Step s[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) fetch(s[u], (int64_t)(step + u) * 64);
+    for (int u = 0; u < U; ++u) fetch(s[u], (int64_t)(step + u * each) * 64);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (ODD) shift(s[u]);
@@ -214,23 +215,20 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
     }
   }
   // the last columns
-  for (; step * 64 < a.Kp; step += each)
+  for (; step * 64 < a.Kp; step += each) {
+    const int64_t k = (int64_t)step * 64;
+    Step s;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t k = (int64_t)(step + u) * 64;
-      if (k >= a.Kp) break;
-      Step s;
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int r = 0; r < RB; ++r)
+        s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
 #pragma unroll
-        for (int r = 0; r < RB; ++r)
-          s.d[r][i] = *reinterpret_cast<const u32x4*>(drow[r] + k * 16 + 512 * i);
-#pragma unroll
-        for (int b = 0; b < TB; ++b)
-          s.x[b][i] = piece(xrow[b] - g * 16, k + g * 16 + 8 * i, a.K);
-      }
-      products(s);
+      for (int b = 0; b < TB; ++b)
+        s.x[b][i] = piece(xrow[b] - g * 16, k + g * 16 + 8 * i, a.K);
     }
+    products(s);
+  }
 #pragma unroll
   for (int r = 0; r < RB; ++r)
 #pragma unroll

@@ -147,6 +147,32 @@ def test_tokens_do_not_depend_on_their_neighbours(dev):
         assert_bitexact(s.own(x, index, base=base), y, "again")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rank,K,N", [(16, 4096, 3000), (40, 4095, 1030), (64, 2752, 520),
+                                      (200, 1500, 300), (16, 14336, 64)])
+def test_bits_go_by_the_number_of_tokens_alone(dev, dtype, rank, K, N):
+    """At the same number of tokens a token's row has the same bits wherever it stands and however
+    many of the tokens around it share its adapter."""
+    T = 150
+    s = Set(dev, [rank, 16, rank], N, K, dtype)
+    probes = torch.tensor([0, 2, 0])
+    px, pbase, x, base = (v.to(dev) for v in (s.x(3), s.base(3), s.x(T), s.base(T)))
+    want = None
+    for at in (0, 14, 62, 70, 128, 147):
+        for sharers in (0, 1, 13, 14, 20, 61, T):
+            index = torch.ones(T, dtype=torch.int32)
+            index[:min(T, at // 64 * 64 + sharers)] = 0
+            index[at:at + 3] = probes.int()
+            xs, bases = x.clone(), base.clone()
+            xs[at:at + 3], bases[at:at + 3] = px, pbase
+            y = s.own(xs, index.to(dev), base=bases)
+            want = y[at:at + 3].clone() if want is None else want
+            assert_bitexact(y[at:at + 3], want, f"from {at} with {sharers} sharers")
+            s.own.add_(bases, xs, index.to(dev))
+            assert_bitexact(bases, y, "in place")
+    s.check(want, px.cpu(), probes, pbase.cpu())
+
+
 @pytest.mark.parametrize("K,N", [(1, 1), (3, 7), (7, 9), (63, 65), (65, 127), (129, 190), (191, 64),
                                  (1023, 129), (2049, 33)])
 @pytest.mark.parametrize("T,ranks", [(5, [16]), (70, [16, 40]), (130, [33, 64, 3])])
