@@ -105,7 +105,9 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
     if constexpr (V == 0) fetch(c, s[0]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = __fmaf_rn(s[p][j], s[p][j], ss);
-    if (a.sum && c < a.C) store8_any<DT>(a.sum, row * a.C + c, a.C - c, s[p]);
+    // (sum and y may be x or r: a piece is stored after its last fetch)
+    if constexpr (V > 0)
+      if (a.sum && c < a.C) store8_any<DT>(a.sum, row * a.C + c, a.C - c, s[p]);
   });
   ss = row_sum<L>(ss, sums[0]);
   // k: a power of two that s is scaled by
@@ -138,22 +140,23 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
     for (int j = 0; j < 8; ++j) s[p][j] = s[p][j] * k * inv * w[p][j];
   };
   if constexpr (V > 0) each([&](int p, int c) { norm(p); });
-  auto value = [&](int p, int c) {
+  auto value = [&](int p, int c, bool last) {
     if constexpr (V == 0) {
       fetch(c, s[0]);
+      if (last && a.sum && c < a.C) store8_any<DT>(a.sum, row * a.C + c, a.C - c, s[0]);
       load_weight(a, c, a.C - c, w[0]);
       norm(0);
     }
   };
   if constexpr (Q == 0) {
     each([&](int p, int c) {
-      value(p, c);
+      value(p, c, true);
       if (c < a.C) store8_any<DT>(a.y, row * a.C + c, a.C - c, s[p]);
     });
   } else {
     Range<SYM> r;
     each([&](int p, int c) {
-      value(p, c);
+      value(p, c, false);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (c + j < a.C) r.add(s[p][j]);
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
       each([&](int p, int c) { if (c < C16) codes(p, c); });
     } else {
       for (int c = c0; c < C16; c += STEP) {
-        value(0, c);
+        value(0, c, true);
         codes(0, c);
       }
     }

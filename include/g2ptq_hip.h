@@ -494,8 +494,9 @@ int g2ptq_paged_attention(void* stream, const g2ptq_kv_cache* cache, const void*
 /* Root-mean-square norm of `rows` rows of C columns (1 to 65536): s = x + r (r nullable),
  * y_c = s_c·w_c / sqrt(Σ s²/C + eps), in fp32.  Row i of x is at (i / inner)·x_outer +
  * (i % inner)·x_inner (elements, columns contiguous), r's likewise; dtype of x and r, wtype of
- * w (0 bf16, 1 fp16, 2 fp32).  y and sum (s), rows × C of dtype, are nullable; with codes they
- * and scale (and, with sym == 0, zero) are y's row on the 8-bit grid, as
+ * w (0 bf16, 1 fp16, 2 fp32).  y and sum (s), rows × C of dtype, are nullable; one may be x and
+ * the other r, where those rows are contiguous too (otherwise they overlap nothing); with codes
+ * they and scale (and, with sym == 0, zero) are y's row on the 8-bit grid, as
  * g2ptq_quantize_tokens writes them, but of y before its rounding to dtype. */
 int g2ptq_rms_norm(void* stream, const void* x, int64_t x_outer, int64_t x_inner, const void* r,
                    int64_t r_outer, int64_t r_inner, int dtype, const void* w, int wtype,

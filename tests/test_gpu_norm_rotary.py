@@ -186,6 +186,37 @@ def test_rows_of_extreme_values(dev, C):
             assert_bitexact(s.values[i], y[i], "values")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("T,C", [(3, 100), (5, 1000), (3, 4096), (3, 8192), (512, 8200), (513, 8200),
+                                 (2, 16384), (3, 16390), (513, 16384)])
+def test_sum_and_values_in_place(dev, T, C, dtype):
+    """A caller of the C entry updates its residual's stream in place: the sum over either
+    addend, the values over the other, on both sides of the rule for long rows."""
+    from g2ptq_amd import _lib
+    from g2ptq_amd.norm_utils import _DTYPE_CODE
+    code, ldc = _DTYPE_CODE[dtype], -(-C // 64) * 64
+    w = (1 + 0.5 * torch.randn(C, generator=gen(C))).to(dev)
+    x0 = torch.randn(T, C, generator=gen(T), dtype=torch.float32).to(dtype).to(dev)
+    r0 = torch.randn(T, C, generator=gen(C), dtype=torch.float32).to(dtype).to(dev)
+
+    def run(x, r, y, total, quantize, sym):
+        codes = torch.zeros(T, ldc, dtype=torch.int8, device=dev)
+        scale, zero = torch.zeros(2, T, device=dev).unbind()
+        _lib.call("g2ptq_rms_norm", _lib.current_stream(), x.data_ptr(), C, 0, r.data_ptr(), C, 0,
+                  code, w.data_ptr(), 2, T, 1, C, 1e-6, y.data_ptr(), total.data_ptr(), sym,
+                  codes.data_ptr() if quantize else None, ldc, scale.data_ptr(), zero.data_ptr())
+        return y, total, codes, scale, zero
+
+    for quantize, sym in ((False, 1), (True, 1), (True, 0)):
+        want = run(x0, r0, torch.empty_like(x0), torch.empty_like(x0), quantize, sym)
+        for sum_at, y_at in ((0, None), (1, None), (None, 0), (None, 1), (0, 1), (1, 0)):
+            pair = [x0.clone(), r0.clone()]
+            y, total = (torch.empty_like(x0) if at is None else pair[at] for at in (y_at, sum_at))
+            got = run(*pair, y, total, quantize, sym)
+            for name, a, b in zip(("values", "sum", "codes", "scale", "zero"), got, want):
+                assert_bitexact(a, b, f"{name}, sum over {sum_at}, values over {y_at}")
+
+
 def test_dequantized_tokens_are_what_codes_stand_for(dev):
     from g2ptq_amd import dequantize_tokens, quantize_tokens
     for T, K in ((1, 1), (3, 7), (40, 130), (5, 16), (2, 4096), (700, 2752), (1, 65536)):
