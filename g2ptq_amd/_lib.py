@@ -16,6 +16,7 @@ FLAG_NAN_OUTPUT = 2
 FLAG_GROUP_SCALE = 4
 FLAG_BAD_INDEX = 8
 FLAG_NO_ROOM = 16
+ADAPTERS_INFINITE = 4  # beside the dtype of g2ptq_adapter_set
 VARIANT_GPTQ, VARIANT_GPTAQ, VARIANT_G2PTQ = 0, 1, 2
 
 _p = ctypes.c_void_p

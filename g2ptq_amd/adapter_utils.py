@@ -69,6 +69,8 @@ class LowRankAdapters:
             for i, r in enumerate(self.ranks):
                 d[i, :r, :self.in_features] = down[i]
                 u[i, :self.out_features, :r] = up[i]
+            # (a rare set: kernels of its own look after these weights)
+            infinite = bool(torch.stack([t.isinf().any() for t in up]).any())
             # the order in which the kernels' lanes take 16 bytes each: down by 16 ranks and 64
             # columns (2 × 4 × 16 pieces: half of 16 columns, 16 columns, rank), up by 64 channels
             # and 16 ranks (4 × 2 × 16: 16 channels, half of the ranks, channel)
@@ -79,7 +81,8 @@ class LowRankAdapters:
                       torch.zeros(1, dtype=_I32, device=dev))
         self._struct = _lib.AdapterSetStruct(*(_lib.ptr(t) for t in self._held), n, R,
                                              self.in_features, self.out_features,
-                                             _DTYPE_CODE[self.dtype])
+                                             _DTYPE_CODE[self.dtype]
+                                             | (_lib.ADAPTERS_INFINITE if infinite else 0))
         self._address = ctypes.addressof(self._struct)
         self._n, self._rank = n, R
 

@@ -48,6 +48,7 @@ struct AdapterArgs {
   uint16_t* out;
   int64_t ldo;
   int* flags;
+  bool infinite;              // some weights of up are infinite
   bool odd;                   // rows of x may start between 32-bit words
   bool aligned;               // rows of base and out are 16-byte aligned
   int64_t window;             // the launch's first
@@ -335,8 +336,9 @@ __device__ __forceinline__ void store_piece(const AdapterArgs& a, int64_t t, int
 // An adapter's tokens' h into LDS as it enters the product: per token and 16 ranks four pieces
 // of 16 bytes, both halves of the ranks rounded, then what the rounding left out.  Two, four or
 // eight lanes take a token.  back: what a token's products are multiplied with, fp16's rows being brought
-// to the top of its range by a power of two.
-template <bool F16>
+// to the top of its range by a power of two.  INF: some weights are infinite, and take the sign of
+// finite terms beside an infinity.
+template <bool F16, bool INF>
 __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int which,
                                         const uint8_t* list, int count, u32x4* hL, int pitch,
                                         float* back) {
@@ -371,7 +373,8 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
       for (int j = 0; j < 8; ++j) {
         float f = v[j] * fit;
         // (beside an infinity or a NaN finite terms do not count, and fp16 has no room for them)
-        if (F16 && infinite && fabsf(f) < __builtin_inff()) f = 0.f;
+        if (F16 && infinite && fabsf(f) < __builtin_inff())
+          f = INF && f != 0.f ? copysignf(1.f, f) : 0.f;
         const uint16_t q = narrow<F16>(f);
         const float left = f - widen<F16>(q);
         const uint16_t u = narrow<F16>(fabsf(left) < __builtin_inff() ? left : 0.f);
@@ -386,6 +389,14 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
   }
 }
 
+// Two weights as what h's rounding left out takes them: zero for infinities and NaN, which h's
+// rounding has taken (times a remainder of zero or of the other sign they would make a NaN of it).
+template <bool F16>
+__device__ __forceinline__ uint32_t finite16(uint32_t w) {
+  constexpr uint32_t top = F16 ? 0x7c00 : 0x7f80;
+  return ((w & top) == top ? 0 : w & 0xffff) | ((w >> 16 & top) == top ? 0 : w & 0xffff0000);
+}
+
 // 16-byte pieces of a token's 64 sums in LDS, one of them against bank conflicts.
 constexpr int kTurn = 17;
 
@@ -393,8 +404,8 @@ constexpr int kTurn = 17;
 // with h rounded, and with what that left out.  The sums are turned in LDS so that eight lanes
 // read and write 128 consecutive bytes of a token's row.  A wave walks its channels, and for
 // each 64 the window's tokens; what comes next is loaded before what was computed is stored.
-// RB: blocks of 16 ranks whose weights are held together.
-template <bool F16, int IO, int RB, int TB>
+// RB: blocks of 16 ranks whose weights are held together.  INF: some weights are infinite.
+template <bool F16, int IO, int RB, int TB, bool INF>
 __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int which,
                                        const uint8_t* list, int count, int chunk, int chunks,
                                        u32x4* hL, int pitch, float* back, f32x4* turn) {
@@ -412,6 +423,14 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           w[r][j] = *reinterpret_cast<const u32x4*>(u + (r * 4 + j) * 256);
+    if (INF && lane >= 32)  // (these lanes' weights are for what h's rounding left out)
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+        if (r0 + r < blocks)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[r][j][i] = finite16<F16>(w[r][j][i]);
   };
   auto token = [&](int t) { return t0 + list[min(t, count - 1)]; };
   auto bases = [&](int chunk, int from) {
@@ -423,7 +442,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
                                      (int64_t)chunk * 64 + col * 8);
   };
   int from = 0;
-  stage_h<F16>(a, t0, which, list, count, hL, pitch, back);
+  stage_h<F16, INF>(a, t0, which, list, count, hL, pitch, back);
   __syncthreads();
   if (chunk < chunks) weights(chunk, 0), bases(chunk, 0);
   while (chunk < chunks) {
@@ -479,7 +498,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, int64_t t0, int whi
 
 // A window's channels are shared by `shares` workgroups, each walking its own range.  First come
 // the first slots: they have the work where a window's tokens share an adapter.
-template <bool F16, int IO, int RB>
+template <bool F16, int IO, int RB, bool INF>
 __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterArgs a, int pitch,
                                                                 int shares) {
   extern __shared__ u32x4 hL[];
@@ -515,9 +534,9 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterArgs a, i
     }
     f32x4* turn = turns[wave];
     if (count <= 16)
-      expand<F16, IO, RB, 1>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
+      expand<F16, IO, RB, 1, INF>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
     else
-      expand<F16, IO, RB, 2>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
+      expand<F16, IO, RB, 2, INF>(a, t0, which, list, count, first, last, hL, pitch, back, turn);
   });
 }
 
@@ -591,12 +610,13 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
     const dim3 grid((unsigned)(groups * shares));
     // (weights of 32 ranks at a time: 64 leave a SIMD two waves, 91 against 85 µs where U·h takes
     // 5100 tokens of ranks 32 and 64 to 14336 channels)
-#define G2_EXPAND(IO)                                                                             \
-  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RB < 2 ? 1 : 2>), grid, dim3(256), lds, st, \
-                     a, pitch, (int)shares)
-    if (a.N % 8) G2_EXPAND(kRagged);
-    else if (streamed(a)) G2_EXPAND(kStream);
-    else G2_EXPAND(kPieces);
+#define G2_EXPAND(IO, RANKS, INF)                                                                 \
+  hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RANKS, INF>), grid, dim3(256), lds, st, a,  \
+                     pitch, (int)shares)
+    if (a.infinite) G2_EXPAND(kRagged, 1, true);
+    else if (a.N % 8) G2_EXPAND(kRagged, RB < 2 ? 1 : 2, false);
+    else if (streamed(a)) G2_EXPAND(kStream, RB < 2 ? 1 : 2, false);
+    else G2_EXPAND(kPieces, RB < 2 ? 1 : 2, false);
 #undef G2_EXPAND
     G2PTQ_LAUNCHED();
   }
@@ -627,8 +647,8 @@ extern "C" int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const 
                               int64_t ldx, const int32_t* index, int64_t T, const void* base,
                               int64_t ldb, void* out, int64_t ldo, void* ws, size_t ws_bytes) {
   G2PTQ_CHECK(set, "adapters: null set");
-  G2PTQ_CHECK(set->dtype == 0 || set->dtype == 1, "adapters: dtype code %d (bf16 or fp16)",
-              set->dtype);
+  const int dtype = set->dtype & ~G2PTQ_ADAPTERS_INFINITE;
+  G2PTQ_CHECK(dtype == 0 || dtype == 1, "adapters: dtype code %d (bf16 or fp16)", set->dtype);
   G2PTQ_CHECK(set->n >= 1 && set->n < (1ll << 31) && set->K >= 1 && set->K <= (1 << 20) &&
                   set->N >= 1 && set->N <= (1 << 20) && set->R >= 16 && set->R <= 512 &&
                   set->R % 16 == 0,
@@ -657,8 +677,9 @@ extern "C" int g2ptq_adapters(void* stream, const g2ptq_adapter_set* set, const 
   a.base = static_cast<const uint16_t*>(base), a.ldb = ldb;
   a.out = static_cast<uint16_t*>(out), a.ldo = ldo;
   a.flags = set->flags;
+  a.infinite = set->dtype & G2PTQ_ADAPTERS_INFINITE;
   a.odd = reinterpret_cast<uintptr_t>(x) % 4 || (ldx % 2 && T > 1);
   a.aligned = aligned16(base) && aligned16(out) && ldb % 8 == 0 && ldo % 8 == 0;
   hipStream_t st = as_stream(stream);
-  return set->dtype == 0 ? adapters_by_rank<false>(st, a) : adapters_by_rank<true>(st, a);
+  return dtype == 0 ? adapters_by_rank<false>(st, a) : adapters_by_rank<true>(st, a);
 }

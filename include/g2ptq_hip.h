@@ -559,7 +559,9 @@ int g2ptq_pages_release(void* stream, const g2ptq_page_tables* tables, const int
  * in pieces of 8 values as the products take them, K' and N' the next multiples of 64:
  *   down [n][R/16][K'/64][2][4][16][8]: rank 16b + m, column 64s + 16g + 8i + e at [b][s][i][g][m][e]
  *   up   [n][N'/64][R/16][4][2][16][8]: channel 64c + 16j + m, rank 16b + 8p + e at [c][b][j][p][m][e]
- * rank (n, 1 to R) and scale (n).  flags: one int32. */
+ * rank (n, 1 to R) and scale (n).  flags: one int32.  dtype has the bit G2PTQ_ADAPTERS_INFINITE
+ * too where up holds an infinity: without it such a weight's products may be NaN. */
+#define G2PTQ_ADAPTERS_INFINITE 4
 typedef struct g2ptq_adapter_set {
   const void* down;
   const void* up;

@@ -266,6 +266,39 @@ def test_nan_and_infinities_stay_in_their_tokens(dev):
     s.own.check()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("ranks,N", [([16, 5], 70), ([20, 33], 264), ([64, 80], 130), ([200, 16], 65)])
+def test_infinite_and_nan_weights(dev, dtype, ranks, N):
+    """Weights that are infinite or NaN: rows are what the formula makes of them, in their own
+    channels and their own adapter's tokens."""
+    K, T = 100, 90
+    clean = Set(dev, ranks, N, K, dtype)
+    s = Set(dev, ranks, N, K, dtype)
+    inf, nan = float("inf"), float("nan")
+    s.up[0][3, 1], s.up[0][40, ranks[0] - 1], s.up[0][N - 1, 0], s.up[0][5, 2] = inf, -inf, inf, nan
+    s.up[0][7, 0], s.up[0][7, 1] = inf, -inf
+    s.up[0][9, 0], s.up[0][9, 1] = -inf, -inf
+    from g2ptq_amd import LowRankAdapters
+    s.own = LowRankAdapters([d.to(dev) for d in s.down], [u.to(dev) for u in s.up], scale=s.scale)
+    x, base = s.x(T), s.base(T)
+    x[4, 2], x[5] = inf, 0
+    for index in (s.index(T, "random"), torch.zeros(T, dtype=torch.int32)):
+        index[4:6] = 0
+        y = s.own(x.to(dev), index.to(dev), base=base.to(dev)).cpu()
+        whole = clean.own(x.to(dev), index.to(dev), base=base.to(dev)).cpu()
+        touched = torch.zeros(T, N, dtype=torch.bool)
+        touched[(index == 0)[:, None] & torch.tensor([c in (3, 5, 7, 9, 40, N - 1)
+                                                      for c in range(N)])[None]] = True
+        assert_bitexact(y[~touched], whole[~touched], "others")
+        for t in (index == 0).nonzero()[:, 0].tolist():
+            h = x[t].double() @ s.down[0].double().T
+            # (rounded as the kernel holds it, an infinity or a zero is one of the formula's)
+            ref = base[t].double() + s.scale[0] * (s.up[0].double() @ h)
+            for c in (3, 5, 7, 9, 40, N - 1):
+                a, b = float(y[t, c]), float(ref[c])
+                assert a == b or (a != a and b != b), (t, c, a, b)
+
+
 def test_an_index_of_no_adapter_is_flagged(dev):
     s = Set(dev, [16, 8], 40, 50, torch.bfloat16)
     x, base = s.x(100), s.base(100)

@@ -304,3 +304,12 @@ def test_a_check_of_page_tables_names_all_that_was_met():
         for kind in ("a row outside", "no free page"):
             assert (kind in said) == (kind in kinds), said
         t.check()
+
+
+def test_adapter_sets_say_whether_a_weight_is_infinite(lib):
+    """The dtype's bit of its own passes the checks beside both types, and nothing else does."""
+    for dtype, bad in ((4, False), (5, False), (6, True), (8, True), (12, True)):
+        a = ctypes.byref(adapters(dtype=dtype))
+        # (no tokens: no launch)
+        status = lib.g2ptq_adapters(None, a, FAKE, 64, FAKE, 0, FAKE, 64, FAKE, 64, FAKE, 1 << 20)
+        assert status == (-1 if bad else 0), dtype
