@@ -215,6 +215,13 @@ __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int whi
       products(s[u]);
     }
   }
+  if (U > 1 && step < whole) {
+    Step s;
+    fetch(s, (int64_t)step * 64);
+    if (ODD) shift(s);
+    products(s);
+    step += each;
+  }
   // the last columns
   for (; step * 64 < a.Kp; step += each) {
     const int64_t k = (int64_t)step * 64;
