@@ -351,6 +351,7 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
                                         float* back) {
   const float scale = a.scale[which];
   const int rank = a.rank[which], pieces = (rank + 15) / 16 * 2;
+  constexpr float most = F16 ? 65504.f : 0x1.fep127f;
   const int shift = pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3, lanes = 1 << shift;
   for (int i = threadIdx.x; (i & ~255) < count << shift; i += 256) {
     const int t = i >> shift, l = i & (lanes - 1);
@@ -382,9 +383,11 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& a, int64_t t0, int wh
         // (beside an infinity or a NaN finite terms do not count, and fp16 has no room for them)
         if (F16 && infinite && fabsf(f) < __builtin_inff())
           f = INF && f != 0.f ? copysignf(1.f, f) : 0.f;
-        const uint16_t q = narrow<F16>(f);
-        const float left = f - widen<F16>(q);
-        const uint16_t u = narrow<F16>(fabsf(left) < __builtin_inff() ? left : 0.f);
+        // (what is above the type's largest number goes into what is left out, infinities and NaN
+        // too; infinite weights meet the rounding alone, which has to keep those)
+        const bool all = INF && !(fabsf(f) < __builtin_inff());
+        const uint16_t q = narrow<F16>(all ? f : __builtin_amdgcn_fmed3f(f, -most, most));
+        const uint16_t u = narrow<F16>(all ? 0.f : f - widen<F16>(q));
         if (j & 1) hi[j >> 1] |= (uint32_t)q << 16, lo[j >> 1] |= (uint32_t)u << 16;
         else hi[j >> 1] = q, lo[j >> 1] = u;
       }

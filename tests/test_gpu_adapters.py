@@ -299,6 +299,23 @@ def test_infinite_and_nan_weights(dev, dtype, ranks, N):
                 assert a == b or (a != a and b != b), (t, c, a, b)
 
 
+def test_inner_values_next_to_the_largest(dev):
+    """An h between the largest bf16 and the largest fp32 is no infinity."""
+    from g2ptq_amd import LowRankAdapters
+    top = torch.finfo(torch.bfloat16).max
+    down = torch.zeros(3, 40, dtype=torch.bfloat16)
+    down[:, 0], down[0, 1], down[1, 1], down[2, 1] = top, 2.0 ** 119, 1.5 * 2.0 ** 119, -2.0 ** 119
+    down[1] *= -1
+    up = torch.zeros(20, 3, dtype=torch.bfloat16)
+    up[:3] = torch.eye(3) * 2.0 ** -20
+    x = torch.ones(2, 40, dtype=torch.bfloat16)
+    y = LowRankAdapters([down.to(dev)], [up.to(dev)])(x.to(dev), torch.zeros(2, dtype=torch.int32,
+                                                                            device=dev))
+    ref = x.double() @ down.double().T @ up.double().T
+    # (all sums are exact: h has 8 bits more than bf16, and the result is rounded once)
+    assert_bitexact(y, ref.bfloat16(), "result")
+
+
 def test_an_index_of_no_adapter_is_flagged(dev):
     s = Set(dev, [16, 8], 40, 50, torch.bfloat16)
     x, base = s.x(100), s.base(100)
