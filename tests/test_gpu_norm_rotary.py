@@ -500,3 +500,62 @@ def test_rotary_past_32_bits(dev):
     assert not bool(out[:1000].any()) and not bool(out[-1000:-1].any())
     del q, out
     torch.cuda.empty_cache()
+
+
+def test_rotary_past_the_first_launch(dev):
+    """One token a workgroup and more tokens than a launch has: the last ones lie in the second."""
+    from g2ptq_amd import Rotary
+    T, H = (1 << 23) + 3, 160
+    for layout in ("half", "interleaved"):
+        rotary = Rotary(2, layout=layout)
+        q = _x(3, H, 2, dtype=torch.bfloat16, seed=7)
+        k = _x(3, 1, 2, dtype=torch.bfloat16, seed=8)
+        # (inputs of one token for all but the last three; an output of 5 GB)
+        p = torch.zeros(T, dtype=torch.int64, device=dev)
+        p[-3:] = torch.tensor([5, 1 << 33, -7], device=dev)
+        wide = torch.zeros(T, 1, 2, dtype=torch.bfloat16, device=dev)
+        wide[-3:] = k.to(dev)
+        out, kout = rotary(wide.expand(T, H, 2), wide, p)
+        _check_rotary(rotary, out[-3:], k.expand(3, H, 2), p[-3:].cpu())
+        _check_rotary(rotary, kout[-3:], k, p[-3:].cpu())
+        assert not bool(out[-1000:-3].any()) and not bool(out[:1000].any())
+        assert not bool(kout[:-3].any())
+        del out, kout
+        torch.cuda.empty_cache()
+        got, _ = rotary(q.to(dev), None, p[-3:])
+        _check_rotary(rotary, got, q, p[-3:].cpu())
+
+
+@pytest.mark.parametrize("what", ["rms_norm", "rms_norm_quantize", "dequantize_tokens", "rotary",
+                                  "adapters"])
+def test_tangents_are_refused(dev, what):
+    """A tangent raises, in every argument that may carry one, and the primal alone is served."""
+    from torch.autograd import forward_ad
+
+    from g2ptq_amd import LowRankAdapters, Rotary, dequantize_tokens, rms_norm, rms_norm_quantize
+    x = torch.randn(3, 64, generator=gen(1)).to(dev)
+    w, codes = torch.ones(64, device=dev), torch.ones(3, 64, dtype=torch.int8, device=dev)
+    p, index = torch.arange(3, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    half = x.half()
+    set_ = LowRankAdapters([half[:2].contiguous()], [half[:, :2].contiguous()])
+    rotary = Rotary(64)
+    y = torch.zeros(3, 3, dtype=torch.float16, device=dev)
+    calls = {
+        "rms_norm": [(lambda a: rms_norm(a, w), x), (lambda a: rms_norm(x, a), w),
+                     (lambda a: rms_norm(x, w, residual=a), x)],
+        "rms_norm_quantize": [(lambda a: rms_norm_quantize(a, w), x),
+                              (lambda a: rms_norm_quantize(x, w, residual=a), x)],
+        "dequantize_tokens": [(lambda a: dequantize_tokens(codes, a), w[:3]),
+                              (lambda a: dequantize_tokens(codes, w[:3], a), w[:3])],
+        "rotary": [(lambda a: rotary(a, x[:, None], p), x[:, None]),
+                   (lambda a: rotary(x[:, None], a, p), x[:, None]),
+                   (lambda a: rotary(a, None, p), x[:, None])],
+        "adapters": [(lambda a: set_(a, index), half), (lambda a: set_(half, index, base=a), y),
+                     (lambda a: set_.add_(y.clone(), a, index), half)]}[what]
+    for call, t in calls:
+        with forward_ad.dual_level():
+            call(t)
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="tangent|forward-mode"):
+                call(dual)
+            call(forward_ad.unpack_dual(dual).primal)
