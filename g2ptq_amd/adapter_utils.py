@@ -25,8 +25,12 @@ MAX_RANK, MAX_FEATURES = 512, 1 << 20
 class LowRankAdapters:
     """``down``: n tensors (rank_i, in_features), ``up``: n tensors (out_features, rank_i), all
     bf16 or all fp16 on one GPU, ranks of 1 to 512; ``scale``: a number, or one per adapter.
-    They are copied once into the layout of the kernels.  Equal calls give equal bits; the order in
-    which a token's products are summed in fp32 goes by the call's number of tokens."""
+    They are copied once into the layout of the kernels, which gives every adapter the set's
+    largest rank: memory is n times that rank, 16 at least.  A set does not change: other adapters
+    are another set, and a graph that was captured with the old one needs it kept.
+
+    Equal calls give equal bits.  The order in which a token's products are summed in fp32 goes by
+    the call's number of tokens, not by which tokens they are."""
 
     def __init__(self, down, up, scale=1.0):
         down, up = list(down), list(up)
@@ -70,7 +74,7 @@ class LowRankAdapters:
                 d[i, :r, :self.in_features] = down[i]
                 u[i, :self.out_features, :r] = up[i]
             # (a rare set: kernels of its own look after these weights)
-            infinite = bool(torch.stack([t.isinf().any() for t in up]).any())
+            infinite = bool(u.isinf().any())
             # the order in which the kernels' lanes take 16 bytes each: down by 16 ranks and 64
             # columns (2 × 4 × 16 pieces: half of 16 columns, 16 columns, rank), up by 64 channels
             # and 16 ranks (4 × 2 × 16: 16 channels, half of the ranks, channel)
