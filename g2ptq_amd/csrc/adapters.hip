@@ -12,11 +12,13 @@
 // every lane (no sort, no launch of its own); each is multiplied with its own tokens only.
 //
 // Bound by memory where tokens are many: MI355X, under the profiler, 5100 tokens of eight
-// requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 16–20 µs (its 42 MB of
-// tokens at a copy's rate 8), U·h 78–85 (292 MB of rows in and out: 57; a launch that only copies
-// them through the same mapping takes some 70).  By latency where they are few: 48 tokens with
-// 32 adapters of rank 16, 4096 × 4096, 3.8–4.1 and 6.0–6.5 µs: index, adapter, operands and sums
-// follow each other through memory.
+// requests with four adapters of ranks 32 and 64, 4096 to 14336: D·x 16–18 µs (its 42 MB of
+// tokens at a copy's rate 8), U·h 77–83 (292 MB of rows in and out: 57; a launch that only copies
+// them through the same mapping takes some 70).  Every share of the channels reads h's shares of K
+// again, 42 MB there.  By latency where tokens are few: 48 with 32 adapters of rank 16, 4096 × 4096,
+// 3.7–4.1 and 6.3–6.6 µs: index, adapter, operands and sums follow each other through memory.  By
+// the adapters' weights where tokens take turns at many of them: every window reads its own again
+// (2048 tokens of 40 adapters of rank 16, 4096 × 4096: 71 µs for 12 of bytes).
 #include <algorithm>
 #include <type_traits>
 
@@ -73,7 +75,7 @@ __device__ __forceinline__ uint16_t narrow(float v) {
 }
 
 // Eight values from p on, at any address: sixteen bytes are one instruction wherever they lie
-// (MI355X, 2048 tokens of rank 64, 4097 × 4097: 43 µs, 73 a value at a time).
+// (MI355X, 2048 tokens of rank 64, 4097 × 4097: 37 µs, 39 with a load and a store a value).
 __device__ __forceinline__ u32x4 piece(const uint16_t* p) {
   u32x4 v;
   __builtin_memcpy(&v, p, 16);
@@ -142,8 +144,8 @@ __device__ __forceinline__ int32_t index_of_lane(const AdapterArgs& a, int64_t t
 // have no part in.  U steps' loads are under way together.
 // ODD: rows may start between two 32-bit words.  There the memory takes a load of sixteen bytes
 // apart, so the words are loaded that hold the values (two bytes before the first and behind the
-// last share theirs and are shifted out).  MI355X, 777 tokens of rank 20 from 2047 columns: 11 µs,
-// 17 without; 2048 tokens of rank 64 from 4097: 14 and 21.
+// last share theirs and are shifted out).  MI355X, both launches, 777 tokens of rank 20, 2047 to 2751:
+// 20.4 µs, 23.2 without; 2048 tokens of rank 64, 4097 × 4097: 36.7 and 43.5.
 template <bool F16, int RB, int TB, bool ODD>
 __device__ __forceinline__ void shrink(const AdapterArgs& a, int64_t t0, int which, int64_t r0,
                                        int blocks, const uint8_t* list, int count,
@@ -555,8 +557,9 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // Workgroups of a window: one for every token of a single window (each may have its own adapter),
 // one for every adapter of a few, fewer where windows fill the chip and mostly hold one.
 // MI355X, 4096 × 4096, windows · slots up to 1024 against 512: 8192 tokens of four requests of
-// rank 16 54 and 60 µs, of rank 64 73 and 69, 2048 tokens of 40 adapters in any order 69 and 73;
-// one slot: 64 tokens of 32 adapters 56 against 11, 1024 of four requests 18 and 20.
+// rank 16 46 and 54 µs, of rank 64 66 and 66, of 40 adapters of rank 16 in any order 235 and 286,
+// 2048 of those 71 and 72; against one slot: 64 tokens of 32 adapters 9.7 and 86, 1024 of four
+// requests 14.1 and 14.1, but 64 of a single adapter 12.7 and 10.9.
 int slots_of(int64_t T, int64_t n) {
   const int64_t windows = cdiv(T, kWindow);
   if (windows == 1) return (int)T;
@@ -571,23 +574,23 @@ int64_t busy_of(int64_t T, int64_t n) {
 }
 
 // Shares of K: enough workgroups for the chip where there are few, 128 columns a wave at least.
-// MI355X, 4096 × 4096, with and without: 64 tokens of 32 adapters 11 and 15 µs, 256 tokens 11 and
-// 19, 2048 of rank 64 37 and 55.  Up to 1024 workgroups instead of 256: 8192 of rank 64 73
-// against 69 (the second product reads every share).
+// MI355X, 4096 × 4096, with and without: 64 tokens of 32 adapters 9.7 and 11.0 µs, 256 tokens of
+// eight 10.3 and 16.9, 2048 of rank 64 29 and 46.  Up to 1024 workgroups instead of 256: 8192 of
+// rank 64 73 against 66 (the second product reads every share), 2048 29 and 29.
 int parts_of(int64_t T, int64_t K, int64_t n) {
   int p = 1;
   while (p < 8 && busy_of(T, n) * p < 256 && cdiv(K, 64) >= p * 8) p *= 2;
   return p;
 }
 // Shares of the channels: 256 each where windows are few.  MI355X, against the power of two below:
-// 1800 tokens of five adapters of rank 64 to 2560 channels 27.7 and 33.4 µs, 200 of eight of rank
-// 16 to 11008 14.7 and 16.4; with more workgroups, busy or not, 1000 tokens to 11008 22.3 and
-// 21.0, 64 of eight adapters 11.0 and 10.1.  Otherwise a power of two, so that an XCD, which takes
-// every eighth workgroup, has the same shares of all windows and keeps their weights in its L2.
-// Each prepares h again, so that they are fewer where windows may hold many adapters.  MI355X,
-// 4096 × 4096, against six shares in the order of windows: 8192 tokens of four requests of rank 16
-// 46.4 and 50.7 µs, of rank 64 66 and 71, 2048 of rank 64 31 and 35; eight shares against four:
-// 2048 of 40 adapters in any order 82 and 70, 1024 of four requests 16.6 and 21.8.
+// 1800 tokens of five adapters of rank 64 to 2560 channels 27.1 and 32.6 µs, 200 of eight of rank
+// 16 to 11008 12.1 and 13.2; against up to 2048 busy workgroups instead of 512, 1000 tokens to
+// 11008 19.6 and 20.9, 64 of eight adapters 10.9 and 10.6.  Otherwise a power of two, so that an
+// XCD, which takes every eighth workgroup, has the same shares of all windows and keeps their
+// weights in its L2.  Each prepares h again, so that they are fewer where windows may hold many
+// adapters.  MI355X, 4096 × 4096, against six shares in the order of windows: 8192 tokens of four
+// requests of rank 16 46.3 and 47.7 µs, of rank 64 66 and 68, 2048 of rank 64 29 and 32; against
+// twice as many shares: 2048 of 40 adapters in any order 70 and 82, 512 of 32 of rank 32 33 and 39.
 int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
   const int64_t rounds = cdiv(N, 256), windows = cdiv(T, kWindow);
   const int64_t mixed = std::min<int64_t>(windows * std::min<int64_t>(n, kWindow) / 4, 128);
@@ -599,7 +602,7 @@ int64_t channel_shares(int64_t T, int64_t N, int64_t n) {
 }
 
 // Rows that no cache will hold are kept out of the caches.  MI355X, 5100 tokens × 14336 channels
-// (292 MB in and out), rank 64: 92 µs, 96 without (x stays cached too: D·x 21 and 24 µs).
+// (292 MB in and out), rank 64, both launches: 100 µs, 104 without (x stays cached too).
 bool streamed(const AdapterArgs& a) { return a.aligned && a.T * a.N >= 1 << 26; }
 
 template <bool F16, int RB>
@@ -618,8 +621,8 @@ int launch_adapters(hipStream_t st, AdapterArgs& a) {
 #undef G2_SHRINK
     G2PTQ_LAUNCHED();
     const dim3 grid((unsigned)(groups * shares));
-    // (weights of 32 ranks at a time: 64 leave a SIMD two waves, 91 against 85 µs where U·h takes
-    // 5100 tokens of ranks 32 and 64 to 14336 channels)
+    // (weights of 32 ranks at a time: 64 leave a SIMD fewer waves.  Both launches: 2048 tokens of
+    // rank 64, 4096 × 4096, 29.3 and 30.2 µs; 5100 tokens of rank 64 to 14336 channels 100 and 96)
 #define G2_EXPAND(IO, RANKS, INF)                                                                 \
   hipLaunchKernelGGL((adapter_expand_kernel<F16, IO, RANKS, INF>), grid, dim3(256), lds, st, a,  \
                      pitch, (int)shares)

@@ -63,8 +63,10 @@ __device__ __forceinline__ void row_range(Range<SYM>& r, float (*lds)[3]) {
 // L lanes walk a row, eight values at a time: V pieces kept in registers, or read again
 // for each use (V = 0).  Q: 0 y alone, 1 symmetric codes, 2 asymmetric ones.  Bound by the bytes:
 // MI355X, under the profiler, 8192 × 4096 bf16 with residual to codes and sum 53–55 µs (235 MB,
-// 4.3 TB/s), 262144 heads of 128 26.5–28.5 µs (134 MB, 4.9 TB/s); one row of 4096 4.2–4.5 µs, the
-// latencies of a launch, the loads and two reductions.
+// 4.3 TB/s), 262144 heads of 128 27–29 µs (134 MB, 4.9 TB/s); one row of 4096 4.1–4.5 µs, the
+// latencies of a launch, the loads and two reductions.  These stay bare where a row is few bytes for
+// its workgroup, to codes without a residual most: replayed, 8192 × 4096 28.8 µs (101 MB, 3.5 TB/s),
+// 4096 × 4099 25.4 (50 MB), 2048 × 8192 18.4 (50 MB), 1024 × 16384, read three times, 26 (50 MB).
 template <int DT, int Q, int L, int V>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
   constexpr bool SYM = Q != 2;
@@ -239,9 +241,9 @@ int launch_norm(hipStream_t st, NormArgs& a) {
 // those that four waves hold need barriers.  MI355X, bf16 with residual, against a workgroup a
 // row: 16384 × 512 13.3 and 21.1 µs, 8192 × 1000 11.9 and 16.2 (64 × 1000 4.5 and 3.4); against a
 // wave a row: 8192 × 2048 23.1 and 26.0, 8192 × 4096 57 and 97.  Rows of 8193 values and more are
-// read again for each use where there are many: 2048 × 16384 60 µs, 74 with eight pieces in
-// registers, 1024 × 9000 18.9 and 21.6, but 512 × 16384 20.9 and 16.2, 64 rows 11.9 and 9.4, of
-// codes 17.0 and 10.8; 2048 × 8192 24.9 with four in registers and 30.3 read again.
+// read again for each use where there are many: 2048 × 16384 61 µs, 71 with eight pieces in
+// registers, 1024 × 9000 18.4 and 21.5, but 512 × 16384 19.8 and 16.1, 64 rows 11.6 and 9.4, to
+// codes 16.7 and 10.8; 2048 × 8192 24.4 with four in registers and 29.8 read again.
 template <int DT, int Q>
 int norm_by_size(hipStream_t st, NormArgs& a) {
   if (a.C <= 64) return launch_norm<DT, Q, 8, 1>(st, a);
